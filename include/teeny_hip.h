@@ -509,6 +509,88 @@ teeny_status teeny_attention_backward(const void *q, const void *k, const void *
 teeny_status teeny_attention_backward_workspace_size(int64_t batch, int64_t q_heads, int64_t n_ctx_q,
                                                      size_t *bytes);
 
+/* ── 8-bit paged K/V cache ────────────────────────────────────────────────
+ * Serving one step of a ragged batch: a plan of the step's pages, the write
+ * of its K and V, and the attention of its queries over the cache.  No
+ * counterpart in the reference, whose attention reads dense K and V
+ * (flash_attn2.rs:18-21); codes are teeny-quant's symmetric int8
+ * (quant/affine.rs:55-148) with one group per (page, head).
+ *
+ * The cache is num_pages pages of page_size tokens (16, 32, 64 or 128):
+ *   k_cache  int8 [num_pages, kv_heads, page_size, head_dim]
+ *   v_cache  int8 [num_pages, kv_heads, head_dim, page_size]  (transposed)
+ *   k_scale, v_scale  fp32 [num_pages, kv_heads], value = code * scale
+ * Token t of sequence b lies in page block_table[b][t / page_size], at offset
+ * t % page_size; its slot is page * page_size + offset.  block_table is int32
+ * [batch, max_pages].  Page numbers, slots and lengths are read on the device
+ * and checked there: what names no page of the cache is no token.
+ *
+ * The plan.  Request b has seq_lens[b] cached tokens and adds new_lens[b] (0:
+ * none; negative: it has ended, and its pages go back).  free_list int32
+ * [num_pages] is a stack of free pages, free_count[0] of them.  Returned
+ * pages are pushed first, in request and row order; then each request with
+ * new tokens takes what its row still needs, in request order from the top of
+ * the stack, and its row of block_table gets them.  A request is refused, with
+ * all of its tokens, if its row or the step would be too long (max_pages;
+ * n_tokens) or if the pages that it and the requests before it need exceed
+ * those there are.  Outputs:
+ *   q_starts [batch + 1]  first row of each request's tokens (refused or not;
+ *                         at most n_tokens)
+ *   slots, positions [n_tokens]  of each row; -1 for refused tokens and for
+ *                         rows past the last request
+ *   context_lens [batch]  tokens cached after the step
+ *   granted [batch]       tokens granted (new_lens[b] or 0)
+ *   free_after [1]        free pages left
+ * context_lens may be seq_lens, granted may be new_lens and free_after may be
+ * free_count: the plan then updates them in place (with a second launch where
+ * n_tokens is over 256).  At most 4096 requests.  The request order alone
+ * decides every result. */
+teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_lens, int32_t *block_table,
+                                 int32_t *free_list, const int32_t *free_count, int32_t *q_starts, int32_t *slots,
+                                 int32_t *positions, int32_t *context_lens, int32_t *granted, int32_t *free_after,
+                                 int64_t batch, int64_t max_pages, int64_t num_pages, int64_t page_size,
+                                 int64_t n_tokens, teeny_stream stream);
+
+/* The write: k, v bf16 [n_tokens, kv_heads, head_dim] (rows k_stride and
+ * v_stride elements apart, multiples of 8) into the slots (negative: the token
+ * is skipped).  A page's scale becomes max(scale, amax / 127) over its tokens,
+ * codes that it held become rint(code * scale / new scale), new ones
+ * rint(x / new scale).  A write that begins at a page's first slot forgets what
+ * the page held, so pages are used again without clearing.  A page and head
+ * that meets an infinity or NaN holds NaN (codes 0 under that scale) until then.
+ * A page's new tokens are consecutive rows at consecutive slots, as the plan
+ * lays them out; a call that names a page in two places, or a slot twice, is
+ * out of contract (the page's contents are then unspecified).  head_dim 64 or
+ * 128; 16-byte aligned tensors. */
+teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *slots, int8_t *k_cache, int8_t *v_cache,
+                                  float *k_scale, float *v_scale, int64_t n_tokens, int64_t kv_heads, int64_t head_dim,
+                                  int64_t num_pages, int64_t page_size, int64_t k_stride, int64_t v_stride,
+                                  teeny_stream stream);
+
+/* Attention of q bf16 [n_tokens, q_heads, head_dim] (rows q_stride elements
+ * apart, a multiple of 8) over the cache, o bf16 [n_tokens, q_heads, head_dim]
+ * dense.  Sequence b's queries are rows q_starts[b] .. q_starts[b + 1] - 1 (NULL:
+ * one query per sequence), the last tokens of its context_lens[b]; with
+ * `causal` query i of len sees the first context - len + 1 + i tokens, else
+ * all.  Heads grouped as teeny_attention_forward.  l (fp32 [n_tokens, q_heads],
+ * may be NULL) is the logsumexp of the scaled scores.  A query that sees no
+ * token gives 0 and -inf; rows past the last sequence are left as they were.
+ * fp32 scores, probabilities rounded to bf16 (times the V scale) for the second
+ * product, fp32 sums.  Scales must not be negative.  max_q_len and max_context
+ * (queries and tokens of the longest sequence) choose how the work is cut;
+ * longer sequences are computed all the same.  With a stream workspace of
+ * teeny_kv_cache_attention_workspace_size bytes a sequence's tokens are shared
+ * out over the device.  head_dim 64 or 128; 16-byte aligned tensors. */
+teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scale,
+                                      const float *v_scale, const int32_t *block_table, const int32_t *context_lens,
+                                      const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,
+                                      int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                      int64_t page_size, int64_t max_pages, int64_t max_q_len, int64_t max_context,
+                                      int64_t q_stride, float softmax_scale, int32_t causal, teeny_stream stream);
+teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                     int64_t head_dim, int64_t max_q_len, int64_t max_context,
+                                                     size_t *bytes);
+
 /* ── int8 affine quantization (teeny-quant) ───────────────────────────────
  * Reference: quantize_affine(tensor, data, shape, granularity, symmetric,
  * bits) and dequantize_affine, utilities/teeny-quant/src/quant/affine.rs
@@ -595,6 +677,31 @@ teeny_status teeny_linear_workspace_size(int64_t M, int64_t N, int64_t K, teeny_
 teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, const float *scale,
                                         const float *bias, void *y, int64_t M, int64_t N,
                                         int64_t K, teeny_activation act, teeny_stream stream);
+
+/* W4A16 linear: y[m,n] = act(sum_g scale[n,g] sum_{k in g} x[m,k] (q[n,k] -
+ * zero_point[n,g]) + bias[n]), g = k / group_size: linear_forward on
+ * dequantize_affine's weights (affine.rs:151-161) for teeny-quant's 4-bit output
+ * with TEENY_GROUP granularity along axis 1.  x bf16 [M,K], scale fp32 and
+ * zero_point int32 (NULL: symmetric) [N, ceil(K / group_size)] as
+ * teeny_quantize_affine writes them, bias fp32 [N] or NULL, y bf16 [M,N].
+ * qweight is teeny_pack_int4's, N rows of ceil(K / 128) * 64 bytes.  group_size
+ * 32, 64 or a multiple of 128; K a multiple of 8; x and qweight 16-byte aligned.
+ * The codes multiply x in fp32-accumulated products and the scale multiplies
+ * their fp32 sum.  From 65 rows on, with a stream workspace of
+ * teeny_w4a16_linear_workspace_size bytes, the weights are first written there
+ * as bf16 (scale applied in fp32, rounded once) for the matrix-core tiles of
+ * linear_forward. */
+teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, const float *scale,
+                                        const int32_t *zero_point, const float *bias, void *y, int64_t M, int64_t N,
+                                        int64_t K, int64_t group_size, teeny_activation act, teeny_stream stream);
+teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t group_size, size_t *bytes);
+
+/* int8 codes [N,K] (teeny_quantize_affine's with bits = 4; the low four bits
+ * count, -8..7) -> the packed rows that teeny_w4a16_linear_forward reads: chunks
+ * of 128 k's, 64 bytes each (a row's last chunk filled up with zero codes).  In
+ * a chunk the 32-bit word 4 g + c holds k = 32 c + 8 g + 0..7, code + 8 in the
+ * nibbles 0, 4, 1, 5, 2, 6, 3, 7 in this order. */
+teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t K, teeny_stream stream);
 
 /* W8A16 conv2d, NHWC bf16 activations, int8 weights [C_OUT,KH,KW,C_IN/G]
  * with per-output-channel fp32 scale, fp32 bias or NULL, bf16 output:
@@ -693,7 +800,8 @@ teeny_status teeny_checkpoint_load_w8a16(teeny_checkpoint ckpt, const char *weig
  * layer_norm_forward_inference, rms_norm_forward, conv2d_forward,
  * conv2d_bias_forward, flash_attention2_forward (HEAD_DIM[, CAUSAL]),
  * linear_forward, and for the reference's TODO lowering arms
- * multi_head_attention_forward, w8a16_linear_forward, w8a16_conv2d_forward,
+ * multi_head_attention_forward, w8a16_linear_forward, w4a16_linear_forward,
+ * w8a16_conv2d_forward,
  * quantize_affine and dequantize_affine (dims as TEENY_ARG_I64). */
 typedef enum teeny_arg_kind {
   TEENY_ARG_PTR = 0,

@@ -201,6 +201,22 @@ extern "C" teeny_status teeny_dispatch(const char *entry_point, const int64_t *c
                                       static_cast<teeny_activation>(cg[1]), stream);
   }
 
+  // w4a16_linear_forward<USE_BIAS, ACT, GROUP_SIZE>(x, qweight, scale, zero_point,
+  // bias, y, M, N, K): the same targets with teeny-quant's 4-bit group weights;
+  // zero_point null for a symmetric scheme.
+  if (name_is(entry_point, "w4a16_linear_forward")) {
+    TEENY_REQUIRE(n_cg == 3, TEENY_ERR_INVALID_ARGUMENT,
+                  "w4a16_linear_forward: expects const generics USE_BIAS, ACT, GROUP_SIZE");
+    void *x = r.ptr("x_ptr"), *q = r.ptr("qweight_ptr"), *sc = r.ptr("scale_ptr"), *z = r.ptr("zero_point_ptr"),
+         *b = r.ptr("bias_ptr"), *y = r.ptr("y_ptr");
+    int64_t M = r.i32("M"), N = r.i32("N"), K = r.i32("K");
+    if (r.done() != TEENY_OK) return r.st;
+    TEENY_REQUIRE(dtype == TEENY_BF16, TEENY_ERR_UNSUPPORTED_DTYPE, "w4a16_linear_forward: dtype must be BF16");
+    return teeny_w4a16_linear_forward(x, static_cast<const int8_t *>(q), static_cast<const float *>(sc),
+                                      static_cast<const int32_t *>(z), cg[0] ? static_cast<const float *>(b) : nullptr,
+                                      y, M, N, K, cg[2], static_cast<teeny_activation>(cg[1]), stream);
+  }
+
   // w8a16_conv2d_forward<KH,KW,SH,SW,PH,PW,G,BLOCK_OW,USE_BIAS,ACT>(x, qweight,
   // scale, bias, y, B, C_IN, C_OUT, H, W, OH, OW): Op::QLinearConv /
   // Op::ConvInteger (TODO arms, graph/mod.rs:2595-2601) on NHWC bf16

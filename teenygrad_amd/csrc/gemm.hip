@@ -17,6 +17,7 @@
 #include "gemm_core.hpp"
 #include "gemm_f32.hpp"
 #include "gemm_skinny.hpp"
+#include "gemm_w4.hpp"
 
 namespace teeny {
 
@@ -304,6 +305,103 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
     if (st != TEENY_OK) return st;
   }
   return after_launch("w8a16_linear_forward", s);
+}
+
+// The rows from which a bf16 copy of the weights and the matrix-core tiles are
+// the better way, given room for the copy.
+static bool w4_as_bf16(int64_t M, int64_t K) { return M > 64 && K % 8 == 0; }
+static size_t w4_copy_bytes(int64_t N, int64_t K) { return (static_cast<size_t>(N) * K * 2 + 255) / 256 * 256; }
+
+static teeny_status w4_sizes(const char *nm, int64_t M, int64_t N, int64_t K, int64_t group_size) {
+  const std::string at = std::string(nm) + ": ";
+  TEENY_REQUIRE(M >= 0 && N >= 0 && K >= 0, TEENY_ERR_SHAPE_MISMATCH, at + "negative size");
+  TEENY_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= 0x7fffff80, TEENY_ERR_SHAPE_MISMATCH,
+                at + "size exceeds 2^31-1");
+  TEENY_REQUIRE(group_size == 32 || group_size == 64 || (group_size > 0 && group_size % 128 == 0),
+                TEENY_ERR_INVALID_GROUP_SIZE, at + "group_size must be 32, 64 or a multiple of 128");
+  TEENY_REQUIRE(K % 8 == 0, TEENY_ERR_SHAPE_MISMATCH, at + "K must be a multiple of 8");
+  return TEENY_OK;
+}
+
+teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t K, teeny_stream stream) {
+  TEENY_REQUIRE(N >= 0 && K >= 0, TEENY_ERR_SHAPE_MISMATCH, "pack_int4: negative size");
+  TEENY_REQUIRE(N <= 0x7fffffff && K <= 0x7fffff80, TEENY_ERR_SHAPE_MISMATCH, "pack_int4: size exceeds 2^31-1");
+  if (N == 0 || K == 0) return TEENY_OK;
+  TEENY_REQUIRE(q != nullptr && packed != nullptr, TEENY_ERR_NULL_POINTER, "pack_int4: q/packed");
+  TEENY_REQUIRE(aligned(packed, 16), TEENY_ERR_MISALIGNED, "pack_int4: packed must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t per_row = cdiv(K, 128) * 16, rows = std::max<int64_t>(1, (int64_t{1} << 30) / per_row);
+  for (int64_t n0 = 0; n0 < N; n0 += rows) {  // launches of at most 2^30 threads
+    const int64_t words = std::min(rows, N - n0) * per_row;
+    hipLaunchKernelGGL(w4_pack, dim3(static_cast<unsigned>(cdiv(words, 256))), dim3(256), 0, s, q + n0 * K,
+                       reinterpret_cast<uint32_t *>(packed) + n0 * per_row, words, static_cast<int>(K));
+  }
+  return after_launch("pack_int4", s);
+}
+
+teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, const float *scale,
+                                        const int32_t *zero_point, const float *bias, void *y, int64_t M, int64_t N,
+                                        int64_t K, int64_t group_size, teeny_activation act, teeny_stream stream) {
+  const char *nm = "w4a16_linear_forward";
+  const teeny_status st = w4_sizes(nm, M, N, K, group_size);
+  if (st != TEENY_OK) return st;
+  TEENY_REQUIRE(act >= TEENY_ACT_NONE && act <= TEENY_ACT_SILU, TEENY_ERR_INVALID_ARGUMENT,
+                "w4a16_linear_forward: unknown activation");
+  if (M == 0 || N == 0) return TEENY_OK;
+  TEENY_REQUIRE(y != nullptr && (K == 0 || (x != nullptr && qweight != nullptr && scale != nullptr)),
+                TEENY_ERR_NULL_POINTER, "w4a16_linear_forward: x/qweight/scale/y");
+  TEENY_REQUIRE(aligned(x, 16) && aligned(qweight, 16), TEENY_ERR_MISALIGNED,
+                "w4a16_linear_forward: x and qweight must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  W4Args p{static_cast<const bf16 *>(x), qweight, scale, zero_point, bias, static_cast<bf16 *>(y), static_cast<int>(M),
+           static_cast<int>(N), static_cast<int>(K), static_cast<int>(cdiv(K, group_size)),
+           static_cast<int>(std::min<int64_t>(group_size, int64_t{1} << 30)), act};
+  const Scratch scr = stream_scratch(s);
+  const size_t copy = w4_copy_bytes(N, K);
+  if (w4_as_bf16(M, K) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {
+    bf16 *wb = static_cast<bf16 *>(scr.ptr);
+    const int64_t per_row = K / 8, rows = std::max<int64_t>(1, (int64_t{1} << 30) / per_row);
+    for (int64_t n0 = 0; n0 < N; n0 += rows) {
+      const int64_t words = std::min(rows, N - n0) * per_row;
+      W4Args c = p;
+      c.w = p.w + n0 * cdiv(K, 128) * 64;
+      c.scale = p.scale + n0 * p.groups;
+      if (p.zero) c.zero = p.zero + n0 * p.groups;
+      auto kern = p.zero ? w4_unpack<true> : w4_unpack<false>;
+      hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(cdiv(words, 256))), dim3(256), 0, s, c, wb + n0 * K, words);
+    }
+    const GemmParams gp = plain_params(x, K, wb, K, y, N, nullptr, bias, nullptr, M, N, K);
+    launch_gemm_mfma<false, kAPlain>(gp, act, s, Scratch{static_cast<char *>(scr.ptr) + copy, scr.bytes - copy});
+  } else {
+    // 2^31 threads a launch at most, and 65535 workgroups along y
+    const int64_t cols = int64_t{1} << 25, most = 65535 * 16;
+    for (int64_t m0 = 0; m0 < M; m0 += most)
+      for (int64_t n0 = 0; n0 < N; n0 += cols) {
+        W4Args c = p;
+        c.x = p.x + m0 * K;
+        c.y = p.y + m0 * N + n0;
+        c.M = static_cast<int>(std::min(most, M - m0));
+        c.N = static_cast<int>(std::min(cols, N - n0));
+        c.ldy = N;
+        c.w = p.w + n0 * cdiv(K, 128) * 64;
+        c.scale = p.scale + n0 * p.groups;
+        if (p.zero) c.zero = p.zero + n0 * p.groups;
+        if (p.bias) c.bias = p.bias + n0;
+        launch_gemm_w4(c, s);
+      }
+  }
+  return after_launch(nm, s);
+}
+
+teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t group_size, size_t *bytes) {
+  TEENY_REQUIRE(bytes != nullptr, TEENY_ERR_NULL_POINTER, "w4a16_linear_workspace_size: bytes");
+  *bytes = 0;
+  const teeny_status st = w4_sizes("w4a16_linear_workspace_size", M, N, K, group_size);
+  if (st != TEENY_OK) return st;
+  if (M == 0 || N == 0 || K == 0 || !w4_as_bf16(M, K)) return TEENY_OK;
+  const GemmParams p = plain_params(nullptr, K, nullptr, K, nullptr, N, nullptr, nullptr, nullptr, M, N, K);
+  *bytes = w4_copy_bytes(N, K) + gemm_scratch_bytes<false, kAPlain>(p);
+  return TEENY_OK;
 }
 
 // linear_backward's MFMA plan: the gradients of a 1x1 convolution over M

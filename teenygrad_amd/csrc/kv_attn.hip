@@ -1,0 +1,541 @@
+// Attention over the 8-bit paged K/V cache (kv_cache.hip), bf16 queries.
+//
+//   s = softmax_scale ks[page] (q . kq),  o = sum softmax(s) vs[page] vq
+//
+// for ragged batches: sequence b's queries are rows q_starts[b] ..
+// q_starts[b + 1] - 1 of q [tokens, q_heads, D], the last tokens of its
+// context.  No counterpart in the reference (flash_attn2.rs:52-158 reads
+// dense K and V); grouped heads as teeny_attention_forward.
+//
+// Bound: for few queries by reading the cache once, for many by the products.
+// The query rows that share a K/V head (its query heads times the sequence's
+// queries) are the columns of v_mfma_f32_16x16x32_bf16: S^T = K Q^T, then
+// O^T += V^T P^T.  A wave takes 64 tokens a time, 16 to each of its four lane
+// groups: the score tiles' rows are dealt out so that lane group g's results
+// are tokens 16 g .. 16 g + 15 of one query, which is one page (pages are
+// whole multiples of 16): one K scale and one V scale per lane and round, and
+// the probabilities are the next product's operand in the registers they were
+// made in.  K's rows and V^T's rows then come straight from memory, 16 bytes
+// a lane in whole 64-byte pieces, each byte to one lane: no LDS and no barrier
+// in the loop.  Codes go to bf16 (exact) in registers, scales are applied in
+// fp32: K's to the scores, V's to the probability before its rounding to bf16
+// (the one rounding on the way; the row sum takes the unrounded probability).
+#include "mfma.hpp"
+
+namespace teeny {
+
+int kv_page_shift(int64_t page_size);
+
+struct KvAttnArgs {
+  const bf16 *q;
+  int64_t q_stride;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const int32_t *table, *ctx, *starts;
+  bf16 *o;
+  float *l;
+  float *part;      // [unit][split][row][D] fp32, then (at ml_off) [unit][split][row][2]; null: one split
+  int64_t ml_off;
+  int batch, tokens, heads, kv_heads, group, pages, shift, width;
+  int blocks;       // row blocks of a head, over all sequences
+  int splits, chunk;  // chunk: tokens per split (a multiple of a workgroup's round)
+  float scale_log2;
+  int causal;
+};
+
+// A head's row block: sequence b has blocks floor(q_starts[b] group / RB) + b
+// on, at least as many as its rows need (whatever the lengths, at most
+// tokens group / RB + batch over all).
+struct KvRows {
+  int b, row0, rows, len, first, ctx;  // rows: of the sequence and head; len: its queries; first: its first token's row
+};
+
+template <int RB>
+__device__ __forceinline__ bool kv_rows(const KvAttnArgs &p, int u, KvRows &r) {
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int i) { return min(max(p.starts ? p.starts[i] : i, 0), p.tokens); };
+  auto block = [&](int i) { return static_cast<int>(static_cast<int64_t>(start(i)) * p.group / RB) + i; };
+  int b = -1;  // the last sequence whose blocks begin at or before u
+  for (int i = 0; i < p.batch; i += 64) {
+    const uint64_t m = __ballot(i + lane < p.batch && block(min(i + lane, p.batch - 1)) <= u);
+    if (m == 0) break;
+    b = i + 63 - __builtin_clzll(m);
+  }
+  if (b < 0) return false;
+  r.b = b;
+  r.first = start(b);
+  r.len = start(b + 1) - r.first;
+  r.rows = r.len * p.group;
+  r.row0 = (u - block(b)) * RB;
+  r.ctx = min(max(p.ctx[b], 0), p.width << p.shift);
+  return r.len > 0 && r.row0 < r.rows;
+}
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Eight int8 codes as bf16.
+__device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t word = (j < 2 ? lo : hi) >> (16 * (j & 1));
+    const bf16x2 pr = cvt_pk_bf16(static_cast<float>(static_cast<int8_t>(word & 0xffu)),
+                                  static_cast<float>(static_cast<int8_t>((word >> 8) & 0xffu)));
+    r[2 * j] = pr[0];
+    r[2 * j + 1] = pr[1];
+  }
+  return r;
+}
+
+// The same value in the four lanes l % 16, l % 16 + 16, ..: their maximum or sum.
+template <typename F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+  v = f(v, __shfl_xor(v, 16, 64));
+  return f(v, __shfl_xor(v, 32, 64));
+}
+
+// NQ: 16-row column blocks per wave; WK: waves that share a workgroup's rows
+// (and its tokens, 64 a time), 4 / WK row blocks.
+template <int D, int NQ, int WK>
+__global__ __launch_bounds__(256) void kv_attn(KvAttnArgs p) {
+  constexpr int WR = 4 / WK, WROWS = 16 * NQ, RB = WROWS * WR;
+  constexpr int NC = D / 32, ND = D / 16, NL = D / 64;  // k-steps of the scores, d blocks, 16-byte pieces of a K row
+  constexpr int LD = D + 4;
+  __shared__ __attribute__((aligned(16))) float red[WK > 1 ? WK * WROWS * LD : 1];
+  __shared__ float ml[2][WK][WROWS];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wr = w / WK, wk = w % WK;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = id % p.splits, unit = id / p.splits;
+  const int head = unit / p.blocks, u = unit - head * p.blocks;
+  KvRows r;
+  if (!kv_rows<RB>(p, u, r)) return;
+  // row i of the sequence: query i / group, head i % group of the K/V head's; it sees seen(i) tokens
+  auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
+  const int last = min(r.row0 + RB, r.rows) - 1;
+  const int k_end = seen(last);
+  // the last split takes what lies past the longest context that the caller expected
+  const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
+  if (split > 0 && kb >= k_end) return;
+  const int base = r.row0 + wr * WROWS;  // the wave's rows
+  const bool idle = WK == 1 && base >= r.rows;
+  if (WK == 1 && idle) return;
+
+  const float sc0 = fabsf(p.scale_log2);
+  const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
+  bf16x8 qf[NQ][NC];
+  int vis[NQ];
+  int64_t out_row[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = min(base + 16 * n + c, r.rows - 1), t = row / p.group;
+    vis[n] = seen(row);
+    const int h = head * p.group + row - t * p.group;
+    out_row[n] = static_cast<int64_t>(r.first + t) * p.heads + h;
+    const bf16 *at = p.q + (r.first + t) * p.q_stride + h * D;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      u32x4 raw = *reinterpret_cast<const u32x4 *>(at + (i >> 1) * 64 + g * 16 + (i & 1) * 8);
+      raw ^= qsign;
+      qf[n][i] = __builtin_bit_cast(bf16x8, raw);
+    }
+  }
+  // all of the wave's rows see the tokens below it
+  const int all_see = seen(min(base, r.rows - 1));
+  const int w_end = min(ke, seen(min(base + WROWS, r.rows) - 1));
+
+  f32x4 acc[NQ][ND];
+  float m_run[NQ], l_run[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m_run[n] = -INFINITY;
+    l_run[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
+  const int page_mask = (1 << p.shift) - 1;
+  const int kg = c >> 2;  // the lane group whose tokens the lane's K rows are
+  struct Pages {
+    int k, v;  // pages of the lane's K rows and V columns, -1: none
+  };
+  auto page_at = [&](int t) {
+    if (t >= k_end) return -1;
+    const int pg = row[t >> p.shift];
+    return pg >= 0 && pg < p.pages ? pg : -1;
+  };
+  auto load_pages = [&](int t0) { return Pages{page_at(t0 + 16 * kg), page_at(t0 + 16 * g)}; };
+  u32x4 kr[4][NL], vr[ND];
+  float ksc = 0.0f, vsc = 0.0f;
+  bool none = false;
+  auto load_k = [&](int t0, Pages pg) {
+    const int64_t at = (static_cast<int64_t>(max(pg.k, 0)) * p.kv_heads + head) << p.shift;
+    const int8_t *src = p.kc + (at + ((t0 + 16 * kg) & page_mask) + (c & 3)) * D + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NL; ++j) kr[i][j] = *reinterpret_cast<const u32x4 *>(src + 4 * i * D + 64 * j);
+  };
+  auto load_v = [&](int t0, Pages pg) {
+    const int64_t unit_at = static_cast<int64_t>(max(pg.v, 0)) * p.kv_heads + head;
+    const int8_t *src = p.vc + (unit_at * D << p.shift) + (c << p.shift) + ((t0 + 16 * g) & page_mask);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vr[d] = *reinterpret_cast<const u32x4 *>(src + (16 * d << p.shift));
+    ksc = p.ks[unit_at];
+    vsc = p.vs[unit_at];
+    none = pg.v < 0;
+  };
+
+  int t0 = kb + 64 * wk;
+  constexpr int STEP = 64 * WK;
+  if (t0 < w_end) {
+    Pages pg = load_pages(t0);
+    load_k(t0, pg);
+    load_v(t0, pg);
+    pg = load_pages(t0 + STEP);
+    for (; t0 < w_end; t0 += STEP) {
+      f32x4 s[NQ][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const bf16x8 a = codes8(kr[i][j >> 1][2 * (j & 1)], kr[i][j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][i] = mfma16(a, qf[n][j], s[n][i]);
+        }
+      }
+      const bool more = t0 + STEP < w_end;
+      // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too; NaN stays
+      const float sc = __builtin_elementwise_maximum(sc0 * ksc, 1.17549435e-38f), vmul = vsc;
+      const bool hidden = none;
+      if (more) load_k(t0 + STEP, pg);
+      const bool masks = t0 + 64 > all_see || __any(hidden);
+      const int at = t0 + 16 * g;  // the lane's first token
+      bf16x8 pb[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        float scn = sc;
+        if (masks) {
+          if (hidden || at >= vis[n]) scn = 1.17549435e-38f;  // the scale of a page that the row does not see may be anything
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (hidden || at + 4 * i + v >= vis[n]) s[n][i][v] = -INFINITY;
+        }
+        float mx = s[n][0][0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) mx = __builtin_elementwise_maximum(mx, s[n][i][v]);
+        mx = over_groups(mx * scn, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+        if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
+          const float m_new = fmaxf(m_run[n], mx);
+          const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
+          l_run[n] *= alpha;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
+          m_run[n] = m_new;
+        }
+        const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i][v], scn, neg_m));
+            l_run[n] += e;
+            s[n][i][v] = e * vmul;
+          }
+        if (masks) {  // a hidden token's V scale may be anything
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (hidden || at + 4 * i + v >= vis[n]) s[n][i][v] = 0.0f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              const bf16x2 pr = cvt_pk_bf16(s[n][2 * h + i][2 * v], s[n][2 * h + i][2 * v + 1]);
+              pb[n][h][4 * i + 2 * v] = pr[0];
+              pb[n][h][4 * i + 2 * v + 1] = pr[1];
+            }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bf16x8 a = codes8(vr[d][2 * h], vr[d][2 * h + 1]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) acc[n][d] = mfma16(a, pb[n][h], acc[n][d]);
+        }
+      if (more) {
+        load_v(t0 + STEP, pg);
+        pg = load_pages(t0 + 2 * STEP);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) l_run[n] = over_groups(l_run[n], [](float a, float b) { return a + b; });
+
+  const bool whole = p.part == nullptr;
+  const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB;  // part rows of this (unit, split)
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int at = wr * WROWS + 16 * n + c;
+      if (r.row0 + at >= r.rows) continue;
+      const float mul = whole ? (l_run[n] == 0.0f ? 0.0f : 1.0f / l_run[n]) : 1.0f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        if (whole) {
+          bf16x4 o4;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(acc[n][d][v] * mul);
+          *reinterpret_cast<bf16x4 *>(p.o + out_row[n] * D + 16 * d + 4 * g) = o4;
+        } else {
+          *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + 16 * d + 4 * g) = acc[n][d];
+        }
+      }
+      if (g == 0 && !whole) {
+        p.part[p.ml_off + (slot + at) * 2] = m_run[n];
+        p.part[p.ml_off + (slot + at) * 2 + 1] = l_run[n];
+      } else if (g == 0 && p.l != nullptr) {
+        p.l[out_row[n]] = (m_run[n] + log2f(l_run[n])) * 0.6931471805599453f;
+      }
+    }
+  } else {
+    // the waves' parts: a common max, then the sum of their outputs in wave order
+    if (g == 0) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        ml[0][wk][16 * n + c] = m_run[n];
+        ml[1][wk][16 * n + c] = l_run[n];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int at = 16 * n + c;
+      float m = ml[0][0][at], l = 0.0f;
+#pragma unroll
+      for (int i = 1; i < WK; ++i) m = fmaxf(m, ml[0][i][at]);
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < WK; ++i) l += ml[1][i][at] * __builtin_amdgcn_exp2f(ml[0][i][at] - ref);
+      const float mul = __builtin_amdgcn_exp2f(m_run[n] - ref) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        *reinterpret_cast<f32x4 *>(red + (wk * WROWS + at) * LD + 16 * d + 4 * g) = acc[n][d] * mul;
+      if (wk == 0 && g == 0 && r.row0 + at < r.rows) {
+        if (!whole) {
+          p.part[p.ml_off + (slot + at) * 2] = m;
+          p.part[p.ml_off + (slot + at) * 2 + 1] = l;
+        } else if (p.l != nullptr) {
+          p.l[out_row[n]] = (m + log2f(l)) * 0.6931471805599453f;
+        }
+      }
+    }
+    __syncthreads();
+    const int rows = min(WROWS, r.rows - r.row0);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+      const int at = i / (D / 4), d = 4 * (i % (D / 4));
+      f32x4 o = *reinterpret_cast<const f32x4 *>(red + at * LD + d);
+#pragma unroll
+      for (int k = 1; k < WK; ++k) o += *reinterpret_cast<const f32x4 *>(red + (k * WROWS + at) * LD + d);
+      if (whole) {
+        const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
+        bf16x4 o4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(o[v]);
+        *reinterpret_cast<bf16x4 *>(p.o + (static_cast<int64_t>(r.first + t) * p.heads + h) * D + d) = o4;
+      } else {
+        *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + d) = o;
+      }
+    }
+  }
+}
+
+// One wave per row: the splits' parts, in split order.
+template <int D, int RB>
+__global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
+  constexpr int V = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int unit = static_cast<int>(wave / RB), at = static_cast<int>(wave % RB);
+  const int head = unit / p.blocks;
+  if (head >= p.kv_heads) return;
+  KvRows r;
+  if (!kv_rows<RB>(p, unit - head * p.blocks, r) || r.row0 + at >= r.rows) return;
+  const int last = min(r.row0 + RB, r.rows) - 1;
+  const int k_end = p.causal ? min(max(r.ctx - r.len + 1 + last / p.group, 0), r.ctx) : r.ctx;
+  const int n = min(p.splits, max(1, (k_end - 1) / p.chunk + 1));
+  const int64_t slot = static_cast<int64_t>(unit) * p.splits * RB + at;
+  const float *ml = p.part + p.ml_off;
+  float m = -INFINITY;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, ml[(slot + i * RB) * 2]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, o[V] = {};
+  for (int i = 0; i < n; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[(slot + i * RB) * 2] - ref);
+    l += ml[(slot + i * RB) * 2 + 1] * f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = __builtin_fmaf(p.part[(slot + i * RB) * D + lane * V + j], f, o[j]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
+  const int64_t row = static_cast<int64_t>(r.first + t) * p.heads + h;
+#pragma unroll
+  for (int j = 0; j < V; ++j) p.o[row * D + lane * V + j] = static_cast<bf16>(o[j] * inv);
+  if (p.l != nullptr && lane == 0) p.l[row] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// ── which form, and how many splits ─────────────────────────────────────────
+struct KvAttnPlan {
+  int nq = 1, wk = 4, rb = 16;
+  int64_t blocks = 0;
+  int splits = 1, chunk = 0;
+  size_t bytes = 0;
+};
+
+static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
+                               int64_t max_q, int64_t max_ctx, size_t scratch) {
+  KvAttnPlan pl;
+  const int64_t group = heads / kv_heads, rows = group * max_q;
+  if (rows > 64) pl.nq = 2, pl.wk = 1, pl.rb = 128;
+  else if (rows > 16) pl.nq = 2, pl.wk = 4, pl.rb = 32;
+  pl.blocks = tokens * group / pl.rb + batch;
+  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = 64 * pl.wk;
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(4 * cus / std::max<int64_t>(units, 1), max_ctx / 512));
+  auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
+  if (size(splits) > scratch) splits = 1;
+  pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), splits), step) * step);
+  pl.splits = static_cast<int>(cdiv(std::max<int64_t>(max_ctx, 1), pl.chunk));
+  pl.bytes = size(pl.splits);
+  return pl;
+}
+
+template <int D, int NQ, int WK>
+static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_t s) {
+  constexpr int RB = 16 * NQ * (4 / WK);
+  const int64_t units = pl.blocks * p.kv_heads;
+  hipLaunchKernelGGL((kv_attn<D, NQ, WK>), dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+  if (pl.splits > 1)
+    hipLaunchKernelGGL((kv_attn_combine<D, RB>), dim3(static_cast<unsigned>(cdiv(units * RB, 4))), dim3(256), 0, s, p);
+}
+
+template <int D>
+static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_t s) {
+  if (pl.wk == 1) launch_kv_attn<D, 2, 1>(pl, p, s);
+  else if (pl.nq == 2) launch_kv_attn<D, 2, 4>(pl, p, s);
+  else launch_kv_attn<D, 1, 4>(pl, p, s);
+}
+
+static teeny_status kv_attn_sizes(const char *nm, int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t max_q_len, int64_t max_context) {
+  const std::string at = std::string(nm) + ": ";
+  TEENY_REQUIRE(n_tokens >= 0 && batch >= 0 && q_heads >= 0 && kv_heads >= 0 && max_q_len >= 0 && max_context >= 0,
+                TEENY_ERR_SHAPE_MISMATCH, at + "negative size");
+  TEENY_REQUIRE(head_dim == 64 || head_dim == 128, TEENY_ERR_UNSUPPORTED, at + "head_dim must be 64 or 128");
+  TEENY_REQUIRE(kv_heads > 0 ? q_heads % kv_heads == 0 : q_heads == 0, TEENY_ERR_SHAPE_MISMATCH,
+                at + "q_heads must be a multiple of kv_heads");
+  TEENY_REQUIRE(n_tokens <= 0x7fffffff && batch < 0x7fffffff && max_context <= 0x7fffffff - 4096 &&
+                    q_heads <= 65535 && n_tokens * q_heads <= 0x7fffffff && batch * q_heads <= 0x7fffffff,
+                TEENY_ERR_SHAPE_MISMATCH, at + "tokens * q_heads, batch * q_heads or max_context exceed 2^31-1");
+  return TEENY_OK;
+}
+
+}  // namespace teeny
+
+using namespace teeny;
+
+extern "C" {
+
+teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scale,
+                                      const float *v_scale, const int32_t *block_table, const int32_t *context_lens,
+                                      const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,
+                                      int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                      int64_t page_size, int64_t max_pages, int64_t max_q_len, int64_t max_context,
+                                      int64_t q_stride, float softmax_scale, int32_t causal, teeny_stream stream) {
+  const char *nm = "kv_cache_attention";
+  teeny_status st = kv_attn_sizes(nm, n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context);
+  if (st != TEENY_OK) return st;
+  const int shift = kv_page_shift(page_size);
+  TEENY_REQUIRE(shift > 0, TEENY_ERR_UNSUPPORTED, "kv_cache_attention: page_size must be 16, 32, 64 or 128");
+  TEENY_REQUIRE(num_pages >= 0 && max_pages >= 0 && num_pages <= 0x7fffffff / page_size &&
+                    max_pages <= (0x7fffffff - 4096) / page_size,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_attention: num_pages or max_pages out of range");
+  TEENY_REQUIRE(q_starts != nullptr || n_tokens == batch, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_attention: without q_starts there is one query per sequence");
+  if (n_tokens == 0 || batch == 0 || q_heads == 0) return TEENY_OK;
+  TEENY_REQUIRE(q != nullptr && o != nullptr && context_lens != nullptr, TEENY_ERR_NULL_POINTER,
+                "kv_cache_attention: q/o/context_lens");
+  TEENY_REQUIRE((max_pages == 0 || block_table != nullptr) &&
+                    (num_pages == 0 || (k_cache != nullptr && v_cache != nullptr && k_scale != nullptr && v_scale != nullptr)),
+                TEENY_ERR_NULL_POINTER, "kv_cache_attention: block_table/cache/scale");
+  TEENY_REQUIRE(q_stride >= q_heads * head_dim, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_attention: token stride below q_heads * head_dim");
+  TEENY_REQUIRE(aligned(q, 16) && aligned(o, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && q_stride % 8 == 0,
+                TEENY_ERR_MISALIGNED, "kv_cache_attention: 16-byte aligned tensors and token stride");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const Scratch scr = stream_scratch(s);
+  max_context = std::min(std::max<int64_t>(max_context, 1), std::max<int64_t>(max_pages * page_size, 1));
+  const KvAttnPlan pl =
+      kv_attn_plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, scr.ptr ? scr.bytes : 0);
+  const int64_t units = pl.blocks * kv_heads;
+  TEENY_REQUIRE(units * pl.splits < (int64_t{1} << 31) / 256 && units * pl.rb < (int64_t{1} << 31) / 64,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_attention: too many rows for a launch");
+  KvAttnArgs p{};
+  p.q = static_cast<const bf16 *>(q);
+  p.q_stride = q_stride;
+  p.kc = k_cache;
+  p.vc = v_cache;
+  p.ks = k_scale;
+  p.vs = v_scale;
+  p.table = block_table;
+  p.ctx = context_lens;
+  p.starts = q_starts;
+  p.o = static_cast<bf16 *>(o);
+  p.l = l;
+  p.part = pl.splits > 1 ? static_cast<float *>(scr.ptr) : nullptr;
+  p.ml_off = units * pl.splits * pl.rb * head_dim;
+  p.batch = static_cast<int>(batch);
+  p.tokens = static_cast<int>(n_tokens);
+  p.heads = static_cast<int>(q_heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = static_cast<int>(q_heads / kv_heads);
+  p.pages = static_cast<int>(num_pages);
+  p.shift = shift;
+  p.width = num_pages > 0 ? static_cast<int>(max_pages) : 0;
+  p.blocks = static_cast<int>(pl.blocks);
+  p.splits = pl.splits;
+  p.chunk = pl.chunk;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.causal = causal != 0;
+  if (head_dim == 64) launch_kv_attn<64>(pl, p, s);
+  else launch_kv_attn<128>(pl, p, s);
+  return after_launch(nm, s);
+}
+
+teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                     int64_t head_dim, int64_t max_q_len, int64_t max_context,
+                                                     size_t *bytes) {
+  const char *nm = "kv_cache_attention_workspace_size";
+  TEENY_REQUIRE(bytes != nullptr, TEENY_ERR_NULL_POINTER, "kv_cache_attention_workspace_size: bytes");
+  *bytes = 0;
+  teeny_status st = kv_attn_sizes(nm, n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context);
+  if (st != TEENY_OK) return st;
+  if (n_tokens == 0 || batch == 0 || q_heads == 0) return TEENY_OK;
+  *bytes = kv_attn_plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, SIZE_MAX).bytes;
+  return TEENY_OK;
+}
+
+}  // extern "C"

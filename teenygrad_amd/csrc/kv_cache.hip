@@ -1,0 +1,451 @@
+// The 8-bit paged K/V cache: a step's plan (pages, slots) and its writes.
+//
+// No counterpart in the reference, whose attention reads dense K and V
+// (kernels/teeny-kernels/src/nn/attention/flash_attn2.rs:18-21); the codes
+// follow teeny-quant's symmetric int8 (utilities/teeny-quant/src/quant/
+// affine.rs:55-148: scale = amax / 127, zero point 0), with one group per
+// (page, head) and ties to even.
+//
+// Pages: K [pages, heads, page_size, D], V transposed [pages, heads, D,
+// page_size]: kv_attn.hip multiplies both straight from memory, and V^T's
+// operand wants consecutive tokens of one d.
+#include "mfma.hpp"
+
+namespace teeny {
+
+// ── plan ────────────────────────────────────────────────────────────────────
+//
+// The sums over requests (tokens, pages given back, pages needed) are prefix
+// sums; everything else follows from them without a further dependency: page
+// k of a step is entry avail - 1 - k of the free stack with the returned pages
+// on top, and an entry at or above the old count is found in its request's
+// row of the table.  So every workgroup does the sums for itself (a few KB
+// that come from L2), and then its share of the tokens and pages: one launch.
+// Bound by latency: two rounds of loads and the scans.
+
+constexpr int kPlanThreads = 256, kPlanMost = 4096;
+
+struct KvPlanArgs {
+  const int32_t *new_lens, *seq_lens;
+  int32_t *table, *free_list;
+  const int32_t *free_count;
+  int32_t *q_starts, *slots, *positions, *context_lens, *granted, *free_after;
+  int batch, width, pages, shift, tokens;
+  int state, work;  // what this launch does: the per-request outputs; tokens, pages and the table
+};
+
+// Sums that saturate: lengths come from the caller and may be anything.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_add_sat(uint32_t v) {
+  return __builtin_elementwise_add_sat(
+      v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xf, false)));
+}
+// Inclusive prefix sum over a wave: within rows of 16 (row_shr), then the rows' totals.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add_sat<0x111, 0xf>(v);
+  v = dpp_add_sat<0x112, 0xf>(v);
+  v = dpp_add_sat<0x114, 0xf>(v);
+  v = dpp_add_sat<0x118, 0xf>(v);
+  v = dpp_add_sat<0x142, 0xa>(v);
+  v = dpp_add_sat<0x143, 0xc>(v);
+  return v;
+}
+
+// Smallest i with cum[i] > x (cum ascending, cum[n - 1] > x).
+__device__ __forceinline__ int upper(const uint32_t *cum, int n, uint32_t x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] > x) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void kv_plan(KvPlanArgs p) {
+  constexpr int WAVES = kPlanThreads / 64;
+  __shared__ uint32_t ends[kPlanMost], backs[kPlanMost], needs[kPlanMost];  // inclusive sums
+  __shared__ uint32_t part[2][WAVES], given_pages;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t room = static_cast<int64_t>(p.width) << p.shift;  // tokens of a table row
+  auto pages_of = [&](int64_t n) { return static_cast<uint32_t>((n + (1 << p.shift) - 1) >> p.shift); };
+  // inclusive prefix sums of two values over the workgroup, behind the carries
+  auto scan2 = [&](uint32_t &a, uint32_t &b, uint32_t &ca, uint32_t &cb) {
+    a = wave_scan(a);
+    b = wave_scan(b);
+    __syncthreads();
+    if (lane == 63) part[0][w] = a, part[1][w] = b;
+    __syncthreads();
+    uint32_t sa = ca, sb = cb;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      if (i == w) {
+        a = __builtin_elementwise_add_sat(a, sa);
+        b = __builtin_elementwise_add_sat(b, sb);
+      }
+      sa = __builtin_elementwise_add_sat(sa, part[0][i]);
+      sb = __builtin_elementwise_add_sat(sb, part[1][i]);
+    }
+    ca = sa;
+    cb = sb;
+  };
+  if (tid == 0) given_pages = 0;
+  uint32_t all_tokens = 0, all_back = 0, all_need = 0, none = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int nw = b < p.batch ? p.new_lens[b] : 0;
+    const int64_t seq = b < p.batch ? p.seq_lens[b] : 0;
+    uint32_t add = nw > 0 ? nw : 0;
+    uint32_t back = nw < 0 ? pages_of(min(max(seq, int64_t{0}), room)) : 0;
+    scan2(add, back, all_tokens, all_back);
+    const bool fits = nw > 0 && seq >= 0 && seq + nw <= room && add <= static_cast<uint32_t>(p.tokens);
+    uint32_t need = fits ? pages_of(seq + nw) - pages_of(seq) : 0, zero = 0;
+    scan2(need, zero, all_need, none);
+    if (b < p.batch) ends[b] = add, backs[b] = back, needs[b] = need;
+  }
+  __syncthreads();
+  const uint32_t held = min(max(p.free_count[0], 0), p.pages);
+  const uint32_t avail = min(held + min(all_back, static_cast<uint32_t>(p.pages)), static_cast<uint32_t>(p.pages));
+  // whether request b gets its pages, and how many it needs
+  auto need_of = [&](int b, int nw, int64_t seq) -> uint32_t {
+    const bool fits = nw > 0 && seq >= 0 && seq + nw <= room && ends[b] <= static_cast<uint32_t>(p.tokens);
+    return fits ? pages_of(seq + nw) - pages_of(seq) : 0;
+  };
+  auto gets = [&](int b, int nw, int64_t seq) {
+    const bool fits = nw > 0 && seq >= 0 && seq + nw <= room && ends[b] <= static_cast<uint32_t>(p.tokens);
+    return fits && (needs[b] <= avail || need_of(b, nw, seq) == 0);
+  };
+  // what the granted requests take together: the largest sum that the pool covers
+  uint32_t most = 0;
+  for (int b = tid; b < p.batch; b += kPlanThreads)
+    if (needs[b] <= avail) most = max(most, needs[b]);
+  if (most > 0) atomicMax(&given_pages, most);
+  __syncthreads();
+  const uint32_t taken = given_pages;
+
+  // entry i < avail of the stack with the returned pages on top
+  auto entry = [&](uint32_t i) -> int32_t {
+    if (i < held) return p.free_list[i];
+    const uint32_t r = i - held;
+    const int b = upper(backs, p.batch, r);
+    return p.table[static_cast<int64_t>(b) * p.width + (r - (b > 0 ? backs[b - 1] : 0))];
+  };
+  const int step = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
+  if (p.work) {
+    for (int t = first; t < p.tokens; t += step) {
+      int32_t slot = -1, pos = -1;
+      if (static_cast<uint32_t>(t) < all_tokens) {
+        const int b = upper(ends, p.batch, t);
+        const int nw = p.new_lens[b];
+        const int64_t seq = p.seq_lens[b];
+        if (gets(b, nw, seq)) {
+          pos = static_cast<int32_t>(seq) + t - static_cast<int32_t>(b > 0 ? ends[b - 1] : 0);
+          const uint32_t at = static_cast<uint32_t>(pos) >> p.shift, had = pages_of(seq);
+          const int32_t page = at < had ? p.table[static_cast<int64_t>(b) * p.width + at]
+                                        : entry(avail - 1 - ((b > 0 ? needs[b - 1] : 0) + at - had));
+          // a page that is none (a table that was never filled) takes no token
+          if (page >= 0 && page < p.pages) slot = (page << p.shift) + (pos & ((1 << p.shift) - 1));
+        }
+      }
+      p.slots[t] = slot;
+      p.positions[t] = pos;
+    }
+    for (uint32_t k = first; k < taken; k += step) {
+      const int b = upper(needs, p.batch, k);
+      const uint32_t had = pages_of(p.seq_lens[b]);
+      p.table[static_cast<int64_t>(b) * p.width + had + (k - (b > 0 ? needs[b - 1] : 0))] = entry(avail - 1 - k);
+    }
+    for (uint32_t r = first; r < avail - held; r += step) p.free_list[held + r] = entry(held + r);
+  }
+  if (p.state && blockIdx.x == 0) {
+    // the outputs may be the inputs themselves: everything above has been read
+    __syncthreads();
+    for (int b = tid; b < p.batch; b += kPlanThreads) {
+      const int nw = p.new_lens[b], seq = p.seq_lens[b];
+      const int got = gets(b, nw, seq) ? nw : 0;
+      p.q_starts[b + 1] = static_cast<int32_t>(min(ends[b], static_cast<uint32_t>(p.tokens)));
+      p.granted[b] = got;
+      p.context_lens[b] = nw < 0 ? 0 : seq + got;
+    }
+    if (tid == 0) {
+      p.q_starts[0] = 0;
+      p.free_after[0] = static_cast<int32_t>(avail - taken);
+    }
+  }
+}
+
+// ── write ───────────────────────────────────────────────────────────────────
+//
+// s' = max(s, amax / 127) over a page's old and new tokens, old codes q ->
+// rint(q s / s'), new ones rint(x / s').  A page's new tokens are a run of
+// consecutive slots; the run's first token finds itself from the slots, and
+// a team of page_size / 16 waves does the page of one head and one cache, 16
+// tokens a wave, held in registers between the two passes over them.  A page
+// that a run begins at its first slot forgets its old scale.  Bound by
+// reading the tokens and writing the codes, and by latency for few tokens.
+
+struct KvWriteArgs {
+  const bf16 *k, *v;
+  int64_t k_stride, v_stride;
+  const int32_t *slots;
+  int8_t *kc, *vc;
+  float *ks, *vs;
+  int tokens, heads, pages, shift, chunk;
+};
+
+// Codes of x and of an old code under the scale s; 0 where s is 0 or not finite.
+__device__ __forceinline__ int kv_code(float x, float s, bool fine) {
+  return fine ? static_cast<int>(__builtin_rintf(fminf(fmaxf(x / s, -127.0f), 127.0f))) : 0;
+}
+__device__ __forceinline__ int kv_recode(int q, float ratio, bool fine) {
+  return fine ? static_cast<int>(__builtin_rintf(static_cast<float>(q) * ratio)) : 0;
+}
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+}
+__device__ __forceinline__ int byte_of(uint32_t word, int i) {
+  return static_cast<int8_t>((word >> (8 * i)) & 0xffu);
+}
+
+// D: head size; WPP: waves per page (page_size / 16); blockIdx.y: head, blockIdx.z: K or V.
+template <int D, int WPP>
+__global__ __launch_bounds__(64 * (WPP > 4 ? WPP : 4)) void kv_write(KvWriteArgs p) {
+  constexpr int TEAMS = WPP > 4 ? 1 : 4 / WPP, PAGE = 16 * WPP;
+  __shared__ uint32_t big[TEAMS][WPP];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, team = w / WPP, part = w % WPP;
+  const int head = blockIdx.y;
+  const bool is_v = blockIdx.z == 1;
+  const int t0 = blockIdx.x * p.chunk;
+  const int limit = p.pages << p.shift;  // slots of the cache, below 2^31
+
+  // the runs that begin in this chunk of at most 64 tokens
+  bool leads = false;
+  {
+    const int t = t0 + lane;
+    if (lane < p.chunk && t < p.tokens) {
+      const int s = p.slots[t], before = t > 0 ? p.slots[t - 1] : -2;
+      leads = s >= 0 && s < limit && (s % PAGE == 0 || s != before + 1);
+    }
+  }
+  uint64_t runs = __ballot(leads);
+  const int rounds = (__popcll(runs) + TEAMS - 1) / TEAMS;
+  for (int skip = 0; skip < team; ++skip) runs &= runs - 1;
+  for (int round = 0; round < rounds; ++round) {
+    const bool live = runs != 0;
+    const int first = live ? t0 + __builtin_ctzll(runs) : 0;
+#pragma unroll
+    for (int skip = 0; skip < TEAMS; ++skip) runs &= runs - 1;
+    const int slot = live ? p.slots[first] : 0;
+    const int page = slot / PAGE, old = slot % PAGE;
+    int n = 0;  // the run's length
+    if (live) {
+      for (int i = 0; i < PAGE; i += 64) {
+        const int at = i + lane;
+        const bool in = at < PAGE - old && first + at < p.tokens && p.slots[first + at] == slot + at;
+        const uint64_t same = __ballot(in);
+        const int more = same == ~0ull ? 64 : __builtin_ctzll(~same);
+        n += more;
+        if (more < 64) break;
+      }
+    }
+    const int64_t unit = static_cast<int64_t>(page) * p.heads + head;
+    float *scale_at = (is_v ? p.vs : p.ks) + unit;
+    const float before = live && old > 0 ? *scale_at : 0.0f;
+    // offsets of this wave's 16 tokens: [lo, hi) are new
+    const int base = 16 * part, lo = max(old - base, 0), hi = min(old + n - base, 16);
+    const bool news = live && hi > lo;
+    uint32_t mx = 0;  // the largest magnitude as bf16 bits: ordered like the values, NaN above all
+    constexpr int VPR = D / 8, RPI = 64 / VPR, NK = 16 / RPI;  // K: lanes per row, rows per round
+    u32x4 kr[NK];
+    uint32_t vr[16];
+    constexpr int DPL = D / 64;  // V: d's per lane
+    if (news && !is_v) {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const int o = i * RPI + lane / VPR;
+        kr[i] = u32x4{0u, 0u, 0u, 0u};
+        if (o >= lo && o < hi)
+          kr[i] = *reinterpret_cast<const u32x4 *>(p.k + (first + base + o - old) * p.k_stride + head * D + 8 * (lane % VPR));
+      }
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = max(mx, max(kr[i][j] & 0x7fffu, (kr[i][j] >> 16) & 0x7fffu));
+    } else if (news) {
+#pragma unroll
+      for (int o = 0; o < 16; ++o) {
+        vr[o] = 0;
+        if (o >= lo && o < hi) {
+          const bf16 *at = p.v + (first + base + o - old) * p.v_stride + head * D + DPL * lane;
+          if constexpr (DPL == 2) vr[o] = *reinterpret_cast<const uint32_t *>(at);
+          else vr[o] = *reinterpret_cast<const uint16_t *>(at);
+        }
+      }
+#pragma unroll
+      for (int o = 0; o < 16; ++o) mx = max(mx, max(vr[o] & 0x7fffu, (vr[o] >> 16) & 0x7fffu));
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), off, 64)));
+    if constexpr (WPP > 1) {
+      if (lane == 0) big[team][part] = mx;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < WPP; ++i) mx = max(mx, big[team][i]);
+      __syncthreads();  // before the next round's values
+    }
+    if (!live) continue;
+    const float scale = __builtin_elementwise_maximum(before, __uint_as_float(mx << 16) / 127.0f);
+    const bool fine = scale > 0.0f && scale < INFINITY;
+    const float ratio = fine ? before / scale : 1.0f;
+    const bool again = old > base && scale != before;  // old codes here, under another scale (also NaN)
+    if (!is_v) {
+      if (news || again) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const int o = i * RPI + lane / VPR;
+          u32x2 *at = reinterpret_cast<u32x2 *>(p.kc + unit * (PAGE * D) + (base + o) * D + 8 * (lane % VPR));
+          u32x2 c;
+          if (o >= lo && o < hi && news) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              int q[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t word = kr[i][2 * j + (e >> 1)];
+                q[e] = kv_code(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), scale, fine);
+              }
+              c[j] = pack4(q[0], q[1], q[2], q[3]);
+            }
+            *at = c;
+          } else if (o < lo && again) {
+            c = *at;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              c[j] = pack4(kv_recode(byte_of(c[j], 0), ratio, fine), kv_recode(byte_of(c[j], 1), ratio, fine),
+                           kv_recode(byte_of(c[j], 2), ratio, fine), kv_recode(byte_of(c[j], 3), ratio, fine));
+            *at = c;
+          }
+        }
+      }
+    } else if (news || again) {
+      const bool whole = lo == 0 && hi == 16 && news;
+#pragma unroll
+      for (int dd = 0; dd < DPL; ++dd) {
+        u32x4 *at = reinterpret_cast<u32x4 *>(p.vc + unit * (PAGE * D) + (DPL * lane + dd) * PAGE + base);
+        u32x4 c = u32x4{0u, 0u, 0u, 0u};
+        if (!whole) c = *at;  // the other tokens' bytes stay
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t word = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int o = 4 * j + e;
+            int q = byte_of(c[j], e);
+            if (news && o >= lo && o < hi) q = kv_code(__uint_as_float(dd ? vr[o] & 0xffff0000u : vr[o] << 16), scale, fine);
+            else if (again && o < lo) q = kv_recode(q, ratio, fine);
+            word |= (static_cast<uint32_t>(q) & 0xffu) << (8 * e);
+          }
+          c[j] = word;
+        }
+        *at = c;
+      }
+    }
+    if (part == 0 && lane == 0) *scale_at = scale;
+  }
+}
+
+template <int D>
+static void launch_kv_write(const KvWriteArgs &p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(cdiv(p.tokens, p.chunk)), static_cast<unsigned>(p.heads), 2);
+  switch (p.shift) {
+    case 4: hipLaunchKernelGGL((kv_write<D, 1>), grid, dim3(256), 0, s, p); break;
+    case 5: hipLaunchKernelGGL((kv_write<D, 2>), grid, dim3(256), 0, s, p); break;
+    case 6: hipLaunchKernelGGL((kv_write<D, 4>), grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL((kv_write<D, 8>), grid, dim3(512), 0, s, p); break;
+  }
+}
+
+int kv_page_shift(int64_t page_size) {
+  return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : page_size == 128 ? 7 : -1;
+}
+
+}  // namespace teeny
+
+using namespace teeny;
+
+extern "C" {
+
+teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_lens, int32_t *block_table,
+                                 int32_t *free_list, const int32_t *free_count, int32_t *q_starts, int32_t *slots,
+                                 int32_t *positions, int32_t *context_lens, int32_t *granted, int32_t *free_after,
+                                 int64_t batch, int64_t max_pages, int64_t num_pages, int64_t page_size,
+                                 int64_t n_tokens, teeny_stream stream) {
+  const char *nm = "kv_cache_plan";
+  TEENY_REQUIRE(batch >= 0 && max_pages >= 0 && num_pages >= 0 && n_tokens >= 0, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_plan: negative size");
+  TEENY_REQUIRE(batch <= kPlanMost, TEENY_ERR_SHAPE_MISMATCH, "kv_cache_plan: more than 4096 requests");
+  const int shift = kv_page_shift(page_size);
+  TEENY_REQUIRE(shift > 0, TEENY_ERR_UNSUPPORTED, "kv_cache_plan: page_size must be 16, 32, 64 or 128");
+  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && max_pages <= 0x7fffffff / page_size && n_tokens <= 0x7fffffff,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_plan: slots, a row's tokens or the step's tokens exceed 2^31-1");
+  TEENY_REQUIRE(q_starts != nullptr && free_count != nullptr && free_after != nullptr, TEENY_ERR_NULL_POINTER,
+                "kv_cache_plan: q_starts/free_count/free_after");
+  TEENY_REQUIRE(batch == 0 || (new_lens != nullptr && seq_lens != nullptr && context_lens != nullptr && granted != nullptr),
+                TEENY_ERR_NULL_POINTER, "kv_cache_plan: new_lens/seq_lens/context_lens/granted");
+  TEENY_REQUIRE((batch == 0 || max_pages == 0 || block_table != nullptr) && (num_pages == 0 || free_list != nullptr),
+                TEENY_ERR_NULL_POINTER, "kv_cache_plan: block_table/free_list");
+  TEENY_REQUIRE(n_tokens == 0 || (slots != nullptr && positions != nullptr), TEENY_ERR_NULL_POINTER,
+                "kv_cache_plan: slots/positions");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  KvPlanArgs p{new_lens, seq_lens, block_table, free_list, free_count, q_starts, slots, positions, context_lens, granted,
+               free_after, static_cast<int>(batch), static_cast<int>(max_pages), static_cast<int>(num_pages), shift,
+               static_cast<int>(n_tokens), 1, 1};
+  const unsigned grid =
+      static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(cdiv(n_tokens, kPlanThreads), device_cu_count())));
+  // outputs in place of inputs that other workgroups still read: a launch of their own
+  const bool in_place = context_lens == seq_lens || context_lens == new_lens || granted == new_lens ||
+                        granted == seq_lens || free_after == free_count;
+  if (grid > 1 && in_place) {
+    p.state = 0;
+    hipLaunchKernelGGL(kv_plan, dim3(grid), dim3(kPlanThreads), 0, s, p);
+    p.state = 1;
+    p.work = 0;
+    hipLaunchKernelGGL(kv_plan, dim3(1), dim3(kPlanThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(kv_plan, dim3(grid), dim3(kPlanThreads), 0, s, p);
+  }
+  return after_launch(nm, s);
+}
+
+teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *slots, int8_t *k_cache, int8_t *v_cache,
+                                  float *k_scale, float *v_scale, int64_t n_tokens, int64_t kv_heads, int64_t head_dim,
+                                  int64_t num_pages, int64_t page_size, int64_t k_stride, int64_t v_stride,
+                                  teeny_stream stream) {
+  const char *nm = "kv_cache_write";
+  TEENY_REQUIRE(n_tokens >= 0 && kv_heads >= 0 && num_pages >= 0, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_write: negative size");
+  TEENY_REQUIRE(head_dim == 64 || head_dim == 128, TEENY_ERR_UNSUPPORTED, "kv_cache_write: head_dim must be 64 or 128");
+  const int shift = kv_page_shift(page_size);
+  TEENY_REQUIRE(shift > 0, TEENY_ERR_UNSUPPORTED, "kv_cache_write: page_size must be 16, 32, 64 or 128");
+  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && n_tokens <= 0x7fffffff && kv_heads <= 65535,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_write: slots or tokens exceed 2^31-1, or kv_heads 65535");
+  if (n_tokens == 0 || kv_heads == 0 || num_pages == 0) return TEENY_OK;
+  TEENY_REQUIRE(k != nullptr && v != nullptr && slots != nullptr && k_cache != nullptr && v_cache != nullptr &&
+                    k_scale != nullptr && v_scale != nullptr,
+                TEENY_ERR_NULL_POINTER, "kv_cache_write: k/v/slots/cache/scale");
+  TEENY_REQUIRE(k_stride >= kv_heads * head_dim && v_stride >= kv_heads * head_dim, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_write: token strides below kv_heads * head_dim");
+  TEENY_REQUIRE(aligned(k, 16) && aligned(v, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && k_stride % 8 == 0 &&
+                    v_stride % 8 == 0,
+                TEENY_ERR_MISALIGNED, "kv_cache_write: 16-byte aligned tensors and token strides");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  KvWriteArgs p{static_cast<const bf16 *>(k), static_cast<const bf16 *>(v), k_stride, v_stride, slots, k_cache, v_cache,
+                k_scale, v_scale, static_cast<int>(n_tokens), static_cast<int>(kv_heads), static_cast<int>(num_pages),
+                shift, 4};
+  p.chunk = n_tokens <= 1024 ? 4 : 16;
+  if (head_dim == 64) launch_kv_write<64>(p, s);
+  else launch_kv_write<128>(p, s);
+  return after_launch(nm, s);
+}
+
+}  // extern "C"

@@ -27,7 +27,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import check, lib
-from .dtypes import DType, bf16, f32, from_any, i8
+from .dtypes import DType, bf16, f32, from_any, i8, i32
 from .runtime import Buffer, Stream, _h
 
 # ── ArgVisitor (core/teeny-core/src/device/program.rs:22-46) ────────────────
@@ -664,6 +664,51 @@ class W8A16LinearRuntimeOp(RuntimeOp):
         visitor.visit_ptr(params[0])
         visitor.visit_ptr(params[1])
         visitor.visit_ptr(params[2] if self.use_bias else None)
+        visitor.visit_ptr(output)
+        for v in (m, n, k):
+            visitor.visit_i32(v)
+
+    def grid(self, output_shape):
+        return (-(-int(output_shape[0]) // 256) * -(-int(output_shape[1]) // 256), 1, 1)
+
+
+class W4A16LinearRuntimeOp(RuntimeOp):
+    """Lowering of Op::QLinearMatMul / Op::MatMulInteger (TODO arms, kernels/
+    teeny-kernels/src/graph/mod.rs:2595-2601) for teeny-quant's 4-bit group
+    weights: linear_forward (nn/mlp/linear.rs:20-116) on dequantize_affine's
+    weights.  Input x bf16 [M, K]; params qweight (``pack_int4``'s rows), scale
+    fp32 [N, groups] (and zero_point int32 [N, groups], bias fp32 [N]); const
+    generics USE_BIAS, ACT, GROUP_SIZE; args (x, qweight, scale, zero_point,
+    bias, y, M, N, K)."""
+
+    name = "w4a16_linear_forward"
+
+    def __init__(self, group_size: int, use_zero_point: bool = False, use_bias: bool = False, act: Optional[str] = None):
+        self.group_size = int(group_size)
+        self.use_zero_point, self.use_bias = bool(use_zero_point), bool(use_bias)
+        self.act = ACTS[act]
+
+    def const_generics(self):
+        return (int(self.use_bias), self.act, self.group_size)
+
+    def param_shapes(self, input_shapes, output_shape):
+        k, n = int(input_shapes[0][1]), int(output_shape[1])
+        groups = [n, -(-k // self.group_size)]
+        return ([[n, -(-k // 128) * 64], groups] + ([groups] if self.use_zero_point else []) +
+                ([[n]] if self.use_bias else []))
+
+    def param_names(self):
+        return (("qweight", "scale") + (("zero_point",) if self.use_zero_point else ()) +
+                (("bias",) if self.use_bias else ()))
+
+    def pack_args(self, inputs, params, output, output_shape, output_row_stride, visitor):
+        m, n = int(output_shape[0]), int(output_shape[1])
+        k = int(inputs[0][1][1])
+        visitor.visit_ptr(inputs[0][0])
+        visitor.visit_ptr(params[0])
+        visitor.visit_ptr(params[1])
+        visitor.visit_ptr(params[2] if self.use_zero_point else None)
+        visitor.visit_ptr(params[-1] if self.use_bias else None)
         visitor.visit_ptr(output)
         for v in (m, n, k):
             visitor.visit_i32(v)
@@ -1326,6 +1371,107 @@ def attention_backward_workspace_size(batch: int, q_heads: int, n_ctx_q: int) ->
     return int(out.value)
 
 
+def kv_cache_dims(k_cache_shape, v_cache_shape, k_scale_shape, v_scale_shape) -> Tuple[int, int, int, int]:
+    """-> (pages, kv_heads, page_size, head_dim) of a cache: K [pages, kv_heads, page_size, head_dim], V
+    [pages, kv_heads, head_dim, page_size], scales [pages, kv_heads]."""
+    _need(len(k_cache_shape) == 4 and len(v_cache_shape) == 4, "kv_cache: k_cache and v_cache must be 4-D")
+    pages, heads, size, d = k_cache_shape
+    if tuple(v_cache_shape) != (pages, heads, d, size):
+        raise ValueError(f"kv_cache: v_cache must be {[pages, heads, d, size]}, is {list(v_cache_shape)}")
+    if tuple(k_scale_shape) != (pages, heads) or tuple(v_scale_shape) != (pages, heads):
+        raise ValueError(f"kv_cache: scales must be {[pages, heads]}")
+    return pages, heads, size, d
+
+
+def _need_cache(k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer):
+    _need(k_cache.dtype == i8 and v_cache.dtype == i8 and k_scale.dtype == f32 and v_scale.dtype == f32,
+          "kv_cache: codes int8, scales fp32")
+    return kv_cache_dims(k_cache.shape, v_cache.shape, k_scale.shape, v_scale.shape)
+
+
+def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_list: Buffer, free_count: Buffer,
+                  page_size: int, n_tokens: Optional[int] = None, slots: Optional[Buffer] = None,
+                  positions: Optional[Buffer] = None, q_starts: Optional[Buffer] = None,
+                  context_lens: Optional[Buffer] = None, granted: Optional[Buffer] = None,
+                  free_after: Optional[Buffer] = None, stream: Optional[Stream] = None):
+    """A step's pages: requests of seq_lens cached tokens add new_lens ones (negative: the request has ended), pages go
+    back to and come from the stack free_list[:free_count], block_table [batch, max_pages] is filled in.  Returns
+    (slots, positions, q_starts, context_lens, granted, free_after), int32; n_tokens rows of slots and positions (with
+    `slots` given: as many as it has).  context_lens=seq_lens, granted=new_lens and free_after=free_count update in
+    place.  A request that does not fit is refused as a whole: granted 0, slots -1."""
+    b = new_lens.numel
+    _need(len(block_table.shape) == 2 and block_table.shape[0] == b and seq_lens.numel == b,
+          "kv_cache_plan: new_lens and seq_lens [batch], block_table [batch, max_pages]")
+    _need(free_count.numel == 1, "kv_cache_plan: free_count has one element")
+    _need(all(t.dtype == i32 for t in (new_lens, seq_lens, block_table, free_list, free_count)),
+          "kv_cache_plan: int32 buffers")
+    _need(slots is not None or n_tokens is not None, "kv_cache_plan: n_tokens or slots")
+    t = slots.numel if n_tokens is None else int(n_tokens)
+    slots, positions = _out(new_lens, slots, (t,)), _out(new_lens, positions, (t,))
+    q_starts = _out(new_lens, q_starts, (b + 1,))
+    context_lens, granted = _out(new_lens, context_lens, (b,)), _out(new_lens, granted, (b,))
+    free_after = _out(new_lens, free_after, (1,))
+    check(lib.teeny_kv_cache_plan(new_lens.ptr, seq_lens.ptr, block_table.ptr, free_list.ptr, free_count.ptr,
+                                  q_starts.ptr, slots.ptr, positions.ptr, context_lens.ptr, granted.ptr, free_after.ptr,
+                                  b, block_table.shape[1], free_list.numel, page_size, t, _h(stream)))
+    return slots, positions, q_starts, context_lens, granted, free_after
+
+
+def kv_cache_write(k: Buffer, v: Buffer, slots: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer,
+                   v_scale: Buffer, stream: Optional[Stream] = None) -> None:
+    """Tokens k, v bf16 [n_tokens, kv_heads, head_dim] into the 8-bit cache at `slots` (int32; negative: skipped).  The
+    pages' codes and scales are updated in place; a page's new tokens are consecutive rows and slots."""
+    pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
+    t = slots.numel
+    if not (tuple(k.shape) == (t, heads, d) and tuple(v.shape) == (t, heads, d)):
+        raise ValueError(f"kv_cache_write: k and v must be {[t, heads, d]}")
+    _need(k.dtype == bf16 and v.dtype == bf16 and slots.dtype == i32, "kv_cache_write: k/v bf16, slots int32")
+    check(lib.teeny_kv_cache_write(k.ptr, v.ptr, slots.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, t, heads,
+                                   d, pages, size, heads * d, heads * d, _h(stream)))
+
+
+def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer,
+                       block_table: Buffer, context_lens: Buffer, q_starts: Optional[Buffer] = None,
+                       max_q_len: Optional[int] = None, max_context: Optional[int] = None,
+                       softmax_scale: Optional[float] = None, causal: bool = True, o: Optional[Buffer] = None,
+                       lse: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
+    """Attention of q bf16 [n_tokens, q_heads, head_dim] over the 8-bit cache -> o like q.  Sequence b's queries are rows
+    q_starts[b] .. q_starts[b + 1] - 1 (None: one each), the last of its context_lens[b] tokens.  max_q_len and
+    max_context (host numbers; default: as much as the buffers allow) choose how the work is cut, not the result."""
+    pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
+    _need(len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16, "kv_cache_attention: q bf16 [n_tokens, q_heads, D]")
+    t, hq, _ = q.shape
+    b = context_lens.numel
+    _need(heads > 0 and hq % heads == 0, "kv_cache_attention: q_heads % kv_heads != 0")
+    _need(len(block_table.shape) == 2 and block_table.shape[0] == b, "kv_cache_attention: block_table [batch, max_pages]")
+    if not (t == b if q_starts is None else q_starts.numel == b + 1):
+        raise ValueError(f"kv_cache_attention: q_starts [{b + 1}], or one query for each of the {b} sequences")
+    _need(block_table.dtype == i32 and context_lens.dtype == i32 and (q_starts is None or q_starts.dtype == i32),
+          "kv_cache_attention: block_table, context_lens and q_starts are int32")
+    _need(lse is None or (lse.numel == t * hq and lse.dtype == f32), "kv_cache_attention: lse fp32 [n_tokens, q_heads]")
+    if max_q_len is None:
+        max_q_len = 1 if q_starts is None else t
+    if max_context is None:
+        max_context = block_table.shape[1] * size
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else softmax_scale
+    o = _out(q, o)
+    check(lib.teeny_kv_cache_attention(q.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, block_table.ptr,
+                                       context_lens.ptr, q_starts.ptr if q_starts is not None else None, o.ptr,
+                                       lse.ptr if lse is not None else None, t, b, hq, heads, d, pages, size,
+                                       block_table.shape[1], max_q_len, max_context, hq * d, scale, int(bool(causal)),
+                                       _h(stream)))
+    return o
+
+
+def kv_cache_attention_workspace_size(n_tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                                      max_q_len: int, max_context: int) -> int:
+    """Stream workspace bytes that let ``kv_cache_attention`` share a sequence's tokens out over the device."""
+    out = ctypes.c_size_t(0)
+    check(lib.teeny_kv_cache_attention_workspace_size(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len,
+                                                      max_context, ctypes.byref(out)))
+    return int(out.value)
+
+
 GRANULARITY = {"tensor": _lib.PER_TENSOR, "channel": _lib.PER_CHANNEL, "group": _lib.GROUP}
 
 
@@ -1418,6 +1564,58 @@ def w8a16_linear(x: Buffer, qweight: Buffer, scale: Buffer, bias: Optional[Buffe
                                          bias.ptr if bias is not None else None, y.ptr, m, n, k,
                                          ACTS[act], _h(stream)))
     return y
+
+
+def pack_int4(q: Buffer, out: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
+    """int8 codes [N, K] of ``quantize_affine(..., bits=4)`` -> the packed rows
+    [N, ceil(K / 128) * 64] that ``w4a16_linear`` reads."""
+    _need(len(q.shape) == 2 and q.dtype == i8, "pack_int4: q must be int8 [N, K]")
+    n, k = q.shape
+    out = _out(q, out, (n, -(-k // 128) * 64), i8)
+    check(lib.teeny_pack_int4(q.ptr, out.ptr, n, k, _h(stream)))
+    return out
+
+
+def w4a16_dims(x_shape, q_shape, scale_shape, group_size, zero_shape=None, bias_shape=None) -> Tuple[int, int, int]:
+    _need(len(x_shape) == 2 and len(q_shape) == 2, "w4a16: x and qweight must be 2-D")
+    m, k = x_shape
+    n = q_shape[0]
+    if not (group_size in (32, 64) or (group_size > 0 and group_size % 128 == 0)):
+        raise ValueError(f"w4a16: group_size must be 32, 64 or a multiple of 128, is {group_size}")
+    if q_shape[1] != -(-k // 128) * 64:
+        raise ValueError(f"w4a16: qweight must be pack_int4's [{n}, {-(-k // 128) * 64}], is {list(q_shape)}")
+    groups = n * -(-k // group_size)
+    if _prod(scale_shape) != groups or (zero_shape is not None and _prod(zero_shape) != groups):
+        raise ValueError(f"w4a16: scale/zero_point must have N x groups = {groups} elements")
+    if not (bias_shape is None or _prod(bias_shape) == n):
+        raise ValueError(f"w4a16: bias must have {n} elements")
+    return int(m), int(n), int(k)
+
+
+def w4a16_linear(x: Buffer, qweight: Buffer, scale: Buffer, group_size: int, zero_point: Optional[Buffer] = None,
+                 bias: Optional[Buffer] = None, act: Optional[str] = None, y: Optional[Buffer] = None,
+                 stream: Optional[Stream] = None) -> Buffer:
+    """act(x W^T + bias) with W[n, k] = scale[n, g] (q[n, k] - zero_point[n, g]), g = k // group_size: x bf16
+    [M, K], qweight from ``pack_int4``, scale fp32 and zero_point int32 (None: symmetric) as ``quantize_affine(...,
+    "group", axis=1, group_size=group_size, bits=4)`` gives them, bias fp32 [N]."""
+    m, n, k = w4a16_dims(x.shape, qweight.shape, scale.shape, group_size,
+                         zero_point.shape if zero_point is not None else None, bias.shape if bias is not None else None)
+    _need(x.dtype == bf16 and qweight.dtype == i8 and scale.dtype == f32 and (bias is None or bias.dtype == f32) and
+          (zero_point is None or zero_point.dtype == i32),
+          "w4a16_linear: x bf16, qweight int8, scale/bias fp32, zero_point int32")
+    y = _out(x, y, (m, n), bf16)
+    check(lib.teeny_w4a16_linear_forward(x.ptr, qweight.ptr, scale.ptr,
+                                         zero_point.ptr if zero_point is not None else None,
+                                         bias.ptr if bias is not None else None, y.ptr, m, n, k, group_size, ACTS[act],
+                                         _h(stream)))
+    return y
+
+
+def w4a16_linear_workspace_size(m: int, n: int, k: int, group_size: int) -> int:
+    """Stream workspace bytes that let ``w4a16_linear`` take its fastest plan."""
+    out = ctypes.c_size_t(0)
+    check(lib.teeny_w4a16_linear_workspace_size(m, n, k, group_size, ctypes.byref(out)))
+    return int(out.value)
 
 
 def w8a16_conv2d(x: Buffer, qweight: Buffer, scale: Buffer, bias: Optional[Buffer] = None,
