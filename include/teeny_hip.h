@@ -685,12 +685,13 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
  * zero_point int32 (NULL: symmetric) [N, ceil(K / group_size)] as
  * teeny_quantize_affine writes them, bias fp32 [N] or NULL, y bf16 [M,N].
  * qweight is teeny_pack_int4's, N rows of ceil(K / 128) * 64 bytes.  group_size
- * 32, 64 or a multiple of 128; K a multiple of 8; x and qweight 16-byte aligned.
+ * 32, 64 or a multiple of 128; K a multiple of 8 below 2^23; x and qweight
+ * 16-byte aligned.
  * The codes multiply x in fp32-accumulated products and the scale multiplies
- * their fp32 sum.  From 65 rows on, with a stream workspace of
- * teeny_w4a16_linear_workspace_size bytes, the weights are first written there
- * as bf16 (scale applied in fp32, rounded once) for the matrix-core tiles of
- * linear_forward. */
+ * their fp32 sum.  For many rows, with a stream workspace of
+ * teeny_w4a16_linear_workspace_size bytes (0: never for this shape), the weights
+ * are first written there as bf16 (scale applied in fp32, rounded once) for the
+ * matrix-core tiles of linear_forward. */
 teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, const float *scale,
                                         const int32_t *zero_point, const float *bias, void *y, int64_t M, int64_t N,
                                         int64_t K, int64_t group_size, teeny_activation act, teeny_stream stream);

@@ -307,16 +307,19 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
   return after_launch("w8a16_linear_forward", s);
 }
 
-// The rows from which a bf16 copy of the weights and the matrix-core tiles are
-// the better way, given room for the copy.
-static bool w4_as_bf16(int64_t M, int64_t K) { return M > 64 && K % 8 == 0; }
+// Whether a bf16 copy of the weights and the matrix-core tiles are the better
+// way, given room for the copy.  us, streamed / through the copy: 128 x 11008 x
+// 4096 47 / 49, 192 x 11008 x 4096 68 / 61, 192 x 4096 x 4096 31 / 35, 256 x 4096
+// x 4096 41 / 34, 192 x 5504 x 2048 29 / 34, 256 x 5504 x 2048 34 / 34, 512 x 1024
+// x 4096 18 / 24, 512 x 11008 x 4096 166 / 87.
+static bool w4_as_bf16(int64_t M, int64_t N) { return M > 160 && M * N >= (int64_t{1} << 20); }
 static size_t w4_copy_bytes(int64_t N, int64_t K) { return (static_cast<size_t>(N) * K * 2 + 255) / 256 * 256; }
 
 static teeny_status w4_sizes(const char *nm, int64_t M, int64_t N, int64_t K, int64_t group_size) {
   const std::string at = std::string(nm) + ": ";
   TEENY_REQUIRE(M >= 0 && N >= 0 && K >= 0, TEENY_ERR_SHAPE_MISMATCH, at + "negative size");
-  TEENY_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= 0x7fffff80, TEENY_ERR_SHAPE_MISMATCH,
-                at + "size exceeds 2^31-1");
+  TEENY_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K < (1 << 23), TEENY_ERR_SHAPE_MISMATCH,
+                at + "M or N exceeds 2^31-1, or K 2^23-1");
   TEENY_REQUIRE(group_size == 32 || group_size == 64 || (group_size > 0 && group_size % 128 == 0),
                 TEENY_ERR_INVALID_GROUP_SIZE, at + "group_size must be 32, 64 or a multiple of 128");
   TEENY_REQUIRE(K % 8 == 0, TEENY_ERR_SHAPE_MISMATCH, at + "K must be a multiple of 8");
@@ -325,7 +328,8 @@ static teeny_status w4_sizes(const char *nm, int64_t M, int64_t N, int64_t K, in
 
 teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t K, teeny_stream stream) {
   TEENY_REQUIRE(N >= 0 && K >= 0, TEENY_ERR_SHAPE_MISMATCH, "pack_int4: negative size");
-  TEENY_REQUIRE(N <= 0x7fffffff && K <= 0x7fffff80, TEENY_ERR_SHAPE_MISMATCH, "pack_int4: size exceeds 2^31-1");
+  TEENY_REQUIRE(N <= 0x7fffffff && K < (1 << 23), TEENY_ERR_SHAPE_MISMATCH,
+                "pack_int4: N exceeds 2^31-1, or K 2^23-1");
   if (N == 0 || K == 0) return TEENY_OK;
   TEENY_REQUIRE(q != nullptr && packed != nullptr, TEENY_ERR_NULL_POINTER, "pack_int4: q/packed");
   TEENY_REQUIRE(aligned(packed, 16), TEENY_ERR_MISALIGNED, "pack_int4: packed must be 16-byte aligned");
@@ -358,7 +362,7 @@ teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, co
            static_cast<int>(std::min<int64_t>(group_size, int64_t{1} << 30)), act};
   const Scratch scr = stream_scratch(s);
   const size_t copy = w4_copy_bytes(N, K);
-  if (w4_as_bf16(M, K) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {
+  if (w4_as_bf16(M, N) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {
     bf16 *wb = static_cast<bf16 *>(scr.ptr);
     const int64_t per_row = K / 8, rows = std::max<int64_t>(1, (int64_t{1} << 30) / per_row);
     for (int64_t n0 = 0; n0 < N; n0 += rows) {
@@ -398,7 +402,7 @@ teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, 
   *bytes = 0;
   const teeny_status st = w4_sizes("w4a16_linear_workspace_size", M, N, K, group_size);
   if (st != TEENY_OK) return st;
-  if (M == 0 || N == 0 || K == 0 || !w4_as_bf16(M, K)) return TEENY_OK;
+  if (M == 0 || N == 0 || K == 0 || !w4_as_bf16(M, N)) return TEENY_OK;
   const GemmParams p = plain_params(nullptr, K, nullptr, K, nullptr, N, nullptr, nullptr, nullptr, M, N, K);
   *bytes = w4_copy_bytes(N, K) + gemm_scratch_bytes<false, kAPlain>(p);
   return TEENY_OK;

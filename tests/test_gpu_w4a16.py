@@ -46,7 +46,7 @@ def test_pack(dev, n, k):
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize("zero", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (1, 1, 8), (2, 33, 264), (16, 100, 1024), (17, 48, 520), (33, 70, 2048), (64, 31, 384),
-                                   (65, 40, 256), (200, 17, 136)])
+                                   (65, 40, 256), (200, 17, 136), (4, 20, 8200), (7, 40, 8192), (13, 17, 8456), (5, 100, 640), (130, 1100, 256), (64, 8200, 128)])
 def test_linear(dev, m, n, k, group, zero):
     rng = np.random.default_rng(m + 3 * n + k + group)
     c = case(rng, m, n, k, group, zero)
@@ -63,7 +63,9 @@ def test_linear_epilogue(dev, m, act):
 
 
 @pytest.mark.parametrize("m,n,k,group,zero,act", [(65, 40, 256, 32, True, None), (100, 256, 512, 128, False, "silu"),
-                                                  (300, 1000, 1032, 64, True, "gelu"), (513, 264, 2048, 256, False, None)])
+                                                  (300, 1000, 1032, 64, True, "gelu"), (513, 264, 2048, 256, False, None),
+                                                  (1050, 1000, 1032, 64, True, "silu"), (200, 5300, 256, 32, False, None),
+                                                  (4100, 264, 512, 512, True, None)])
 def test_linear_copy(dev, m, n, k, group, zero, act):
     """Many rows with a workspace: the weights as bf16, each rounded once."""
     rng = np.random.default_rng(m + k)
@@ -121,13 +123,13 @@ def test_runtime_op(dev):
 def test_linear_in_a_graph(dev):
     """Both forms captured once and replayed over new inputs, eager work of another stream between."""
     rng = np.random.default_rng(41)
-    for m in (4, 130):
-        x, codes, scale, zp, bias = case(rng, m, 96, 512, 64, False)
+    for m, n in ((4, 96), (1030, 1024)):
+        x, codes, scale, zp, bias = case(rng, m, n, 512, 64, False)
         s = Stream.create()
-        xb, y = dev.buffer(bf16, (m, 512)), dev.buffer(bf16, (m, 96))
+        xb, y = dev.buffer(bf16, (m, 512)), dev.buffer(bf16, (m, n))
         w, sc, bb = K.pack_int4(dev.upload(codes)), dev.upload(scale), dev.upload(bias)
         dev.synchronize()
-        with stream_workspace(dev, K.w4a16_linear_workspace_size(m, 96, 512, 64), s):
+        with stream_workspace(dev, K.w4a16_linear_workspace_size(m, n, 512, 64), s):
             s.begin_capture()
             K.w4a16_linear(xb, w, sc, 64, bias=bb, y=y, stream=s)
             graph = s.end_capture()
