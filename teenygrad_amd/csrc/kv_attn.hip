@@ -364,6 +364,238 @@ __global__ __launch_bounds__(256) void kv_attn(KvAttnArgs p) {
   }
 }
 
+// Many query rows (prompts in pieces): bound by the products, and next by
+// turning codes into operands, which in kv_attn every wave does for itself.
+// Here a workgroup of four waves, 32 rows each, turns a tile of 64 tokens once:
+// its lanes read 16 codes each of K and of V per D / 64, and write the bf16
+// operands of v_mfma_f32_32x32x16_bf16 to LDS in the order in which lanes take
+// them up, 1 KiB a product, so that writes and reads are without conflicts.  The
+// codes of the tile after next are in flight meanwhile; one barrier a tile, two
+// tiles in LDS, two workgroups on a CU, whose products and exponentials overlap.
+// Rows of the scores are dealt out as in kv_attn: lane half g's results of a
+// block of 32 tokens are tokens 16 g .. 16 g + 15 of one query, one page.
+template <int D>
+__global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
+  constexpr int RB = 128, NS = D / 16, ND = D / 32, NU = D / 64, FR = 2 * NS + 4 * ND;
+  __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = id % p.splits, unit = id / p.splits;
+  const int head = unit / p.blocks, u = unit - head * p.blocks;
+  KvRows r;
+  if (!kv_rows<RB>(p, u, r)) return;
+  auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
+  const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
+  const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
+  if (split > 0 && kb >= k_end) return;
+  const int base = r.row0 + 32 * w;  // the wave's rows; past r.rows it only helps to turn the tiles
+
+  const float sc0 = fabsf(p.scale_log2);
+  const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+  const int my = min(base + c, r.rows - 1), qt = my / p.group, qh = head * p.group + my - qt * p.group;
+  const int64_t out_row = static_cast<int64_t>(r.first + qt) * p.heads + qh;
+  const int vis = seen(my), all_see = seen(min(base, r.rows - 1));
+  const int w_end = base < r.rows ? min(ke, seen(min(base + 32, r.rows) - 1)) : 0;
+  bf16x8 qf[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    u32x4 raw = *reinterpret_cast<const u32x4 *>(p.q + (r.first + qt) * p.q_stride + qh * D + (i >> 1) * 32 + g * 16 + (i & 1) * 8);
+    raw ^= qsign;
+    qf[i] = __builtin_bit_cast(bf16x8, raw);
+  }
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = zero16();
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  // The wave's share of a tile: K rows of block w / 2 (D = 128: 64 bytes of each row in two pieces), and V rows of
+  // d block w, tokens of both blocks (D = 64: of d block w / 2 and block w % 2).
+  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
+  const int page_mask = (1 << p.shift) - 1;
+  const int k_tok = 32 * (w >> 1) + 16 * ((c >> 2) & 1), k_in = 4 * (c >> 3) + (c & 3);  // token of the lane's K row
+  const int v_d = 32 * (D == 128 ? w : w >> 1) + c;
+  auto v_block = [&](int i) { return D == 128 ? i : w & 1; };
+  auto page_at = [&](int t) {
+    if (t >= ke) return -1;
+    const int pg = row[t >> p.shift];
+    return pg >= 0 && pg < p.pages ? pg : -1;
+  };
+  struct Pages {
+    int k, v[2];  // of the lane's K row; of tokens 16 g .. of both blocks
+  };
+  auto load_pages = [&](int t0) {
+    return Pages{page_at(t0 + k_tok), {page_at(t0 + 16 * g), page_at(t0 + 32 + 16 * g)}};
+  };
+  u32x4 kr[NU], vr[NU];
+  float ks_next[2], vs_next[2];
+  bool none_next[2];
+  auto load_codes = [&](int t0, const Pages &pg) {
+    const int64_t k_at = (static_cast<int64_t>(max(pg.k, 0)) * p.kv_heads + head) << p.shift;
+    const int8_t *k_src = p.kc + (k_at + ((t0 + k_tok) & page_mask) + k_in) * D + 16 * g + (D == 128 ? 64 : 32) * (w & 1);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) kr[i] = *reinterpret_cast<const u32x4 *>(k_src + 32 * i);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int b = v_block(i);
+      const int64_t v_at = static_cast<int64_t>(max(b ? pg.v[1] : pg.v[0], 0)) * p.kv_heads + head;
+      vr[i] = *reinterpret_cast<const u32x4 *>(p.vc + ((v_at * D + v_d) << p.shift) + ((t0 + 32 * b + 16 * g) & page_mask));
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t at = static_cast<int64_t>(max(pg.v[b], 0)) * p.kv_heads + head;
+      ks_next[b] = p.ks[at];
+      vs_next[b] = p.vs[at];
+      none_next[b] = pg.v[b] < 0;
+    }
+  };
+  auto turn = [&](u32x4 *to) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int step = 2 * (NU * (w & 1) + i), at = (w >> 1) * NS + step;
+      to[at * 64 + lane] = __builtin_bit_cast(u32x4, codes8(kr[i][0], kr[i][1]));
+      to[(at + 1) * 64 + lane] = __builtin_bit_cast(u32x4, codes8(kr[i][2], kr[i][3]));
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int at = 2 * NS + ((D == 128 ? w : w >> 1) * 2 + v_block(i)) * 2;
+      to[at * 64 + lane] = __builtin_bit_cast(u32x4, codes8(vr[i][0], vr[i][1]));
+      to[(at + 1) * 64 + lane] = __builtin_bit_cast(u32x4, codes8(vr[i][2], vr[i][3]));
+    }
+  };
+
+  Pages pg;
+  int buf = 0;
+  float ksc[2], vsc[2];
+  bool none[2];
+  auto take = [&]() {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) ksc[b] = ks_next[b], vsc[b] = vs_next[b], none[b] = none_next[b];
+  };
+  if (kb < ke) {
+    pg = load_pages(kb);
+    load_codes(kb, pg);
+    pg = load_pages(kb + 64);
+    turn(frag[0]);
+    take();
+    if (kb + 64 < ke) {
+      load_codes(kb + 64, pg);
+      pg = load_pages(kb + 128);
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t0 = kb; t0 < ke; t0 += 64) {
+    const u32x4 *now = frag[buf];
+    const float sc1[2] = {__builtin_elementwise_maximum(sc0 * ksc[0], 1.17549435e-38f),
+                          __builtin_elementwise_maximum(sc0 * ksc[1], 1.17549435e-38f)};
+    const float vm[2] = {vsc[0], vsc[1]};
+    const bool hidden[2] = {none[0], none[1]};
+    if (t0 + 64 < ke) {
+      turn(frag[buf ^ 1]);
+      take();
+      if (t0 + 128 < ke) {
+        load_codes(t0 + 128, pg);
+        pg = load_pages(t0 + 192);
+      }
+    }
+    if (t0 < w_end) {
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = zero16();
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[b] = mfma32x32x16(__builtin_bit_cast(bf16x8, now[(b * NS + i) * 64 + lane]), qf[i], s[b]);
+      }
+      const bool masks = t0 + 64 > all_see || __any(hidden[0] || hidden[1]);
+      float sc[2] = {sc1[0], sc1[1]};
+      if (masks) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int at = t0 + 32 * b + 16 * g;
+          if (hidden[b] || at >= vis) sc[b] = 1.17549435e-38f;  // the scale of a page that the row does not see may be anything
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (hidden[b] || at + v >= vis) s[b][v] = -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float x = s[b][0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) x = __builtin_elementwise_maximum(x, s[b][v]);
+        mx = __builtin_elementwise_maximum(mx, x * sc[b]);
+      }
+      mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+      if (__any(mx > m_run + 8.0f)) {  // rescaled rarely: p <= 2^8
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+        m_run = m_new;
+      }
+      const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+      bf16x8 pb[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][v], sc[b], neg_m));
+          l_run += e;
+          s[b][v] = e * vm[b];
+        }
+        if (masks) {  // a hidden token's V scale may be anything
+          const int at = t0 + 32 * b + 16 * g;
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (hidden[b] || at + v >= vis) s[b][v] = 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+          const bf16x2 pr = cvt_pk_bf16(s[b][v], s[b][v + 1]);
+          pb[b][v >> 3][v & 7] = pr[0];
+          pb[b][v >> 3][(v & 7) + 1] = pr[1];
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, now[(2 * NS + (d * 2 + b) * 2 + h) * 64 + lane]), pb[b][h], acc[d]);
+    }
+    buf ^= 1;
+    __syncthreads();
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (base + c >= r.rows) return;
+  const bool whole = p.part == nullptr;
+  const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB + 32 * w + c;
+  const float mul = whole ? (l_run == 0.0f ? 0.0f : 1.0f / l_run) : 1.0f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int at = 32 * d + 8 * a + 4 * g;
+      if (whole) {
+        bf16x4 o4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(acc[d][4 * a + v] * mul);
+        *reinterpret_cast<bf16x4 *>(p.o + out_row * D + at) = o4;
+      } else {
+        *reinterpret_cast<f32x4 *>(p.part + slot * D + at) = f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+      }
+    }
+  if (g == 0 && !whole) {
+    p.part[p.ml_off + slot * 2] = m_run;
+    p.part[p.ml_off + slot * 2 + 1] = l_run;
+  } else if (g == 0 && p.l != nullptr) {
+    p.l[out_row] = (m_run + log2f(l_run)) * 0.6931471805599453f;
+  }
+}
+
 // One wave per row: the splits' parts, in split order.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
@@ -400,6 +632,7 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
 
 // ── which form, and how many splits ─────────────────────────────────────────
 struct KvAttnPlan {
+  bool tile = false;
   int nq = 1, wk = 4, rb = 16;
   int64_t blocks = 0;
   int splits = 1, chunk = 0;
@@ -410,10 +643,10 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
                                int64_t max_q, int64_t max_ctx, size_t scratch) {
   KvAttnPlan pl;
   const int64_t group = heads / kv_heads, rows = group * max_q;
-  if (rows > 64) pl.nq = 2, pl.wk = 1, pl.rb = 128;
+  if (rows > 64) pl.tile = true, pl.rb = 128;
   else if (rows > 16) pl.nq = 2, pl.wk = 4, pl.rb = 32;
   pl.blocks = tokens * group / pl.rb + batch;
-  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = 64 * pl.wk;
+  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = pl.tile ? 64 : 64 * pl.wk;
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(4 * cus / std::max<int64_t>(units, 1), max_ctx / 512));
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   if (size(splits) > scratch) splits = 1;
@@ -434,7 +667,12 @@ static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_
 
 template <int D>
 static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_t s) {
-  if (pl.wk == 1) launch_kv_attn<D, 2, 1>(pl, p, s);
+  if (pl.tile) {
+    const int64_t units = pl.blocks * p.kv_heads;
+    hipLaunchKernelGGL(kv_attn_tile<D>, dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+    if (pl.splits > 1)
+      hipLaunchKernelGGL((kv_attn_combine<D, 128>), dim3(static_cast<unsigned>(cdiv(units * 128, 4))), dim3(256), 0, s, p);
+  }
   else if (pl.nq == 2) launch_kv_attn<D, 2, 4>(pl, p, s);
   else launch_kv_attn<D, 1, 4>(pl, p, s);
 }
