@@ -152,4 +152,21 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Inclusive prefix sum over a wave, saturating at 2^32 - 1 (all lanes active):
+// within rows of 16 (row_shr), then the rows' totals.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_add_sat(uint32_t v) {
+  return __builtin_elementwise_add_sat(
+      v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add_sat<0x111, 0xf>(v);
+  v = dpp_add_sat<0x112, 0xf>(v);
+  v = dpp_add_sat<0x114, 0xf>(v);
+  v = dpp_add_sat<0x118, 0xf>(v);
+  v = dpp_add_sat<0x142, 0xa>(v);
+  v = dpp_add_sat<0x143, 0xc>(v);
+  return v;
+}
+
 }  // namespace teeny

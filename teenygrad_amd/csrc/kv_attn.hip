@@ -71,6 +71,49 @@ __device__ __forceinline__ bool kv_rows(const KvAttnArgs &p, int u, KvRows &r) {
   return r.len > 0 && r.row0 < r.rows;
 }
 
+// The same blocks in order of their work, the longest first, for up to 64
+// sequences: a later, longer block would run on alone when the others are done.
+// Lane b counts its sequence's blocks that see more than T tokens; the count over
+// all sequences is above u for T up to the block's own, found by bisection.
+template <int RB>
+__device__ __forceinline__ bool kv_rows_sorted(const KvAttnArgs &p, int u, KvRows &r) {
+  if (p.batch > 64) return kv_rows<RB>(p, u, r);
+  const int lane = threadIdx.x & 63, b = min(lane, p.batch - 1);
+  auto start = [&](int i) { return min(max(p.starts ? p.starts[i] : i, 0), p.tokens); };
+  const int first = start(b), len = lane < p.batch ? max(start(b + 1) - first, 0) : 0;
+  const int rows = len * p.group, nb = (rows + RB - 1) / RB;
+  const int ctx = min(max(p.ctx[b], 0), p.width << p.shift);
+  // blocks (from the last one down) whose last row sees more than 64 tau - 1 tokens
+  auto count = [&](int tau) -> uint32_t {
+    if (tau == 0) return nb;
+    const int t = 64 * tau - 1;
+    if (ctx <= t) return 0;
+    if (!p.causal) return nb;
+    // block nb - 1 - i, i > 0, ends with row (nb - i) RB - 1, whose query sees ctx - len + 1 + row / group tokens
+    const int64_t need = (static_cast<int64_t>(t) - ctx + len) * p.group + 1;
+    return need <= 1 ? nb : max(1, nb - static_cast<int>((need + RB - 1) / RB) + 1);
+  };
+  auto total = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(v)), 63)); };
+  if (total(nb) <= static_cast<uint32_t>(u)) return false;
+  int lo = 0, hi = (p.width << p.shift) / 64 + 1;  // total(count(lo)) > u >= total(count(hi)) = 0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (total(count(mid)) > static_cast<uint32_t>(u)) lo = mid;
+    else hi = mid;
+  }
+  const uint32_t above = count(hi), here = count(lo) - above, upto = wave_scan(here);
+  const uint32_t at = u - total(above);
+  const int owner = __builtin_ctzll(__ballot(upto > at));
+  auto from = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+  r.b = owner;
+  r.first = from(first);
+  r.len = from(len);
+  r.rows = from(rows);
+  r.ctx = from(ctx);
+  r.row0 = (from(nb) - 1 - static_cast<int>(from(above) + at - (from(upto) - from(here)))) * RB;
+  return true;
+}
+
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -383,7 +426,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   const int split = id % p.splits, unit = id / p.splits;
   const int head = unit / p.blocks, u = unit - head * p.blocks;
   KvRows r;
-  if (!kv_rows<RB>(p, u, r)) return;
+  if (!kv_rows_sorted<RB>(p, u, r)) return;
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
   const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
   const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
@@ -606,7 +649,8 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
   const int head = unit / p.blocks;
   if (head >= p.kv_heads) return;
   KvRows r;
-  if (!kv_rows<RB>(p, unit - head * p.blocks, r) || r.row0 + at >= r.rows) return;
+  const bool found = RB == 128 ? kv_rows_sorted<RB>(p, unit - head * p.blocks, r) : kv_rows<RB>(p, unit - head * p.blocks, r);
+  if (!found || r.row0 + at >= r.rows) return;
   const int last = min(r.row0 + RB, r.rows) - 1;
   const int k_end = p.causal ? min(max(r.ctx - r.len + 1 + last / p.group, 0), r.ctx) : r.ctx;
   const int n = min(p.splits, max(1, (k_end - 1) / p.chunk + 1));

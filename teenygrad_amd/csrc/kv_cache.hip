@@ -34,23 +34,6 @@ struct KvPlanArgs {
   int state, work;  // what this launch does: the per-request outputs; tokens, pages and the table
 };
 
-// Sums that saturate: lengths come from the caller and may be anything.
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ uint32_t dpp_add_sat(uint32_t v) {
-  return __builtin_elementwise_add_sat(
-      v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xf, false)));
-}
-// Inclusive prefix sum over a wave: within rows of 16 (row_shr), then the rows' totals.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v = dpp_add_sat<0x111, 0xf>(v);
-  v = dpp_add_sat<0x112, 0xf>(v);
-  v = dpp_add_sat<0x114, 0xf>(v);
-  v = dpp_add_sat<0x118, 0xf>(v);
-  v = dpp_add_sat<0x142, 0xa>(v);
-  v = dpp_add_sat<0x143, 0xc>(v);
-  return v;
-}
-
 // Smallest i with cum[i] > x (cum ascending, cum[n - 1] > x).
 __device__ __forceinline__ int upper(const uint32_t *cum, int n, uint32_t x) {
   int lo = 0, hi = n - 1;
@@ -69,7 +52,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan(KvPlanArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t room = static_cast<int64_t>(p.width) << p.shift;  // tokens of a table row
   auto pages_of = [&](int64_t n) { return static_cast<uint32_t>((n + (1 << p.shift) - 1) >> p.shift); };
-  // inclusive prefix sums of two values over the workgroup, behind the carries
+  // inclusive prefix sums of two values over the workgroup, behind the carries (lengths come from the caller and may
+  // be anything: sums saturate)
   auto scan2 = [&](uint32_t &a, uint32_t &b, uint32_t &ca, uint32_t &cb) {
     a = wave_scan(a);
     b = wave_scan(b);
