@@ -421,7 +421,7 @@ template <int D>
 __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   constexpr int RB = 128, NS = D / 16, ND = D / 32, NU = D / 64, FR = 2 * NS + 4 * ND;
   __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int split = id % p.splits, unit = id / p.splits;
   const int head = unit / p.blocks, u = unit - head * p.blocks;
@@ -452,43 +452,47 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   float m_run = -INFINITY, l_run = 0.0f;
 
   // The wave's share of a tile: K rows of block w / 2 (D = 128: 64 bytes of each row in two pieces), and V rows of
-  // d block w, tokens of both blocks (D = 64: of d block w / 2 and block w % 2).
+  // d block w, tokens of both blocks (D = 64: of d block w / 2 and block w % 2).  The four pages of a tile are one
+  // load for the wave; what follows from them is the same for all lanes and is worked out in scalar registers.
   const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
-  const int page_mask = (1 << p.shift) - 1;
-  const int k_tok = 32 * (w >> 1) + 16 * ((c >> 2) & 1), k_in = 4 * (c >> 3) + (c & 3);  // token of the lane's K row
-  const int v_d = 32 * (D == 128 ? w : w >> 1) + c;
+  const int page_mask = (1 << p.shift) - 1, wb = w >> 1;
+  const bool k_odd = (c >> 2) & 1, g_odd = g;
+  const int k_lane = (4 * (c >> 3) + (c & 3)) * D + 16 * g + (D == 128 ? 64 : 32) * (w & 1);
+  const int v_lane = (32 * (D == 128 ? w : wb) + c) << p.shift;
   auto v_block = [&](int i) { return D == 128 ? i : w & 1; };
-  auto page_at = [&](int t) {
-    if (t >= ke) return -1;
-    const int pg = row[t >> p.shift];
-    return pg >= 0 && pg < p.pages ? pg : -1;
-  };
-  struct Pages {
-    int k, v[2];  // of the lane's K row; of tokens 16 g .. of both blocks
-  };
-  auto load_pages = [&](int t0) {
-    return Pages{page_at(t0 + k_tok), {page_at(t0 + 16 * g), page_at(t0 + 32 + 16 * g)}};
-  };
+  // lane l: the page of tokens 16 (l % 4) .. of a tile
+  auto load_pages = [&](int t0) { return row[min(t0 + 16 * (lane & 3), k_end - 1) >> p.shift]; };
   u32x4 kr[NU], vr[NU];
   float ks_next[2], vs_next[2];
   bool none_next[2];
-  auto load_codes = [&](int t0, const Pages &pg) {
-    const int64_t k_at = (static_cast<int64_t>(max(pg.k, 0)) * p.kv_heads + head) << p.shift;
-    const int8_t *k_src = p.kc + (k_at + ((t0 + k_tok) & page_mask) + k_in) * D + 16 * g + (D == 128 ? 64 : 32) * (w & 1);
+  auto load_codes = [&](int t0, int pg) {
+    uint32_t at[4];  // (page, head) index: below 2^29
+    int in[4];       // offset in the page
+    bool there[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int page = __builtin_amdgcn_readlane(pg, j), t = t0 + 16 * j;
+      there[j] = page >= 0 && page < p.pages && t < ke;
+      at[j] = static_cast<uint32_t>(there[j] ? page : 0) * p.kv_heads + head;
+      in[j] = t & page_mask;
+    }
+    auto pick = [&](bool odd, int64_t x, int64_t y) { return odd ? y : x; };
+    auto k_off = [&](int j) { return ((static_cast<int64_t>(at[j]) << p.shift) + in[j]) * D; };
+    auto v_off = [&](int j) { return (static_cast<int64_t>(at[j]) * D << p.shift) + in[j]; };
+    const int8_t *k_src = p.kc + (pick(k_odd, wb ? k_off(2) : k_off(0), wb ? k_off(3) : k_off(1)) + k_lane);
 #pragma unroll
     for (int i = 0; i < NU; ++i) kr[i] = *reinterpret_cast<const u32x4 *>(k_src + 32 * i);
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int b = v_block(i);
-      const int64_t v_at = static_cast<int64_t>(max(b ? pg.v[1] : pg.v[0], 0)) * p.kv_heads + head;
-      vr[i] = *reinterpret_cast<const u32x4 *>(p.vc + ((v_at * D + v_d) << p.shift) + ((t0 + 32 * b + 16 * g) & page_mask));
+      const int v = v_block(i);
+      vr[i] = *reinterpret_cast<const u32x4 *>(p.vc + (pick(g_odd, v ? v_off(2) : v_off(0), v ? v_off(3) : v_off(1)) + v_lane));
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int64_t at = static_cast<int64_t>(max(pg.v[b], 0)) * p.kv_heads + head;
-      ks_next[b] = p.ks[at];
-      vs_next[b] = p.vs[at];
-      none_next[b] = pg.v[b] < 0;
+      const uint32_t i = g_odd ? at[2 * b + 1] : at[2 * b];
+      ks_next[b] = p.ks[i];
+      vs_next[b] = p.vs[i];
+      none_next[b] = g_odd ? !there[2 * b + 1] : !there[2 * b];
     }
   };
   auto turn = [&](u32x4 *to) {
@@ -506,8 +510,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
     }
   };
 
-  Pages pg;
-  int buf = 0;
+  int pg = 0, buf = 0;
   float ksc[2], vsc[2];
   bool none[2];
   auto take = [&]() {
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
     const u32x4 *now = frag[buf];
     const float sc1[2] = {__builtin_elementwise_maximum(sc0 * ksc[0], 1.17549435e-38f),
                           __builtin_elementwise_maximum(sc0 * ksc[1], 1.17549435e-38f)};
-    const float vm[2] = {vsc[0], vsc[1]};
+    float vm[2] = {vsc[0], vsc[1]};
     const bool hidden[2] = {none[0], none[1]};
     if (t0 + 64 < ke) {
       turn(frag[buf ^ 1]);
@@ -542,12 +545,22 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
       }
     }
     if (t0 < w_end) {
-      f32x16 s[2];
+      // operands are read LA products ahead, V's first ones before the exponentials; the order is kept as written
+      constexpr int LA = 4, W = LA + 1;
+      u32x4 win[W];
+      auto read = [&](int i) __attribute__((always_inline)) {
+        const int j = i - 2 * NS;  // scores: both blocks in turn; outputs: the d blocks in turn
+        const int at = i < 2 * NS ? (i & 1) * NS + (i >> 1) : 2 * NS + (j % ND) * 4 + j / ND;
+        win[i % W] = now[at * 64 + lane];
+      };
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        s[b] = zero16();
+      for (int i = 0; i < LA; ++i) read(i);
+      f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-        for (int i = 0; i < NS; ++i) s[b] = mfma32x32x16(__builtin_bit_cast(bf16x8, now[(b * NS + i) * 64 + lane]), qf[i], s[b]);
+      for (int i = 0; i < 2 * NS; ++i) {
+        read(i + LA);
+        s[i & 1] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), qf[i >> 1], s[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       const bool masks = t0 + 64 > all_see || __any(hidden[0] || hidden[1]);
       float sc[2] = {sc1[0], sc1[1]};
@@ -580,19 +593,38 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
       }
       const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
       bf16x8 pb[2][2];
+      // p vs[page] as exp2(s - m + log2 vs), where every scale of the wave has a logarithm (one multiplication less a
+      // score; the sum is divided by the scale again); what is hidden takes the scale 1
+      bool plain = true;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
+        if (masks && (hidden[b] || t0 + 32 * b + 16 * g >= vis)) vm[b] = 1.0f;
+        plain = plain && vm[b] > 1e-30f && vm[b] < 1e30f;
+      }
+      plain = __all(plain);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][v], sc[b], neg_m));
-          l_run += e;
-          s[b][v] = e * vm[b];
-        }
-        if (masks) {  // a hidden token's V scale may be anything
-          const int at = t0 + 32 * b + 16 * g;
+      for (int b = 0; b < 2; ++b) {
+        if (plain) {
+          const float off = neg_m + __builtin_amdgcn_logf(vm[b]);
+          float sum = 0.0f;
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (hidden[b] || at + v >= vis) s[b][v] = 0.0f;
+          for (int v = 0; v < 16; ++v) {
+            s[b][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][v], sc[b], off));
+            sum += s[b][v];
+          }
+          l_run = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vm[b]), l_run);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][v], sc[b], neg_m));
+            l_run += e;
+            s[b][v] = e * vm[b];
+          }
+          if (masks) {  // a hidden token of a page that the row sees in part: its scale may be infinite
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+              if (hidden[b] || t0 + 32 * b + 16 * g + v >= vis) s[b][v] = 0.0f;
+          }
         }
 #pragma unroll
         for (int v = 0; v < 16; v += 2) {
@@ -601,13 +633,14 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
           pb[b][v >> 3][(v & 7) + 1] = pr[1];
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, now[(2 * NS + (d * 2 + b) * 2 + h) * 64 + lane]), pb[b][h], acc[d]);
+      for (int j = 0; j < 4 * ND; ++j) {
+        const int i = 2 * NS + j, d = j % ND, bh = j / ND;
+        if (j + LA < 4 * ND) read(i + LA);
+        acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), pb[bh >> 1][bh & 1], acc[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     buf ^= 1;
     __syncthreads();
@@ -755,6 +788,8 @@ teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, cons
   TEENY_REQUIRE(num_pages >= 0 && max_pages >= 0 && num_pages <= 0x7fffffff / page_size &&
                     max_pages <= (0x7fffffff - 4096) / page_size,
                 TEENY_ERR_SHAPE_MISMATCH, "kv_cache_attention: num_pages or max_pages out of range");
+  TEENY_REQUIRE(num_pages * kv_heads < (int64_t{1} << 29), TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_attention: num_pages * kv_heads must be below 2^29");
   TEENY_REQUIRE(q_starts != nullptr || n_tokens == batch, TEENY_ERR_SHAPE_MISMATCH,
                 "kv_cache_attention: without q_starts there is one query per sequence");
   if (n_tokens == 0 || batch == 0 || q_heads == 0) return TEENY_OK;
