@@ -54,20 +54,25 @@ template <int RB>
 __device__ __forceinline__ bool kv_rows(const KvAttnArgs &p, int u, KvRows &r) {
   const int lane = threadIdx.x & 63;
   auto start = [&](int i) { return min(max(p.starts ? p.starts[i] : i, 0), p.tokens); };
-  auto block = [&](int i) { return static_cast<int>(static_cast<int64_t>(start(i)) * p.group / RB) + i; };
-  int b = -1;  // the last sequence whose blocks begin at or before u
+  int found = -1, first = 0, end = 0, ctx = 0;  // of the last sequence whose blocks begin at or before u
   for (int i = 0; i < p.batch; i += 64) {
-    const uint64_t m = __ballot(i + lane < p.batch && block(min(i + lane, p.batch - 1)) <= u);
+    const int b = min(i + lane, p.batch - 1), s0 = start(b), s1 = start(b + 1), n = p.ctx[b];
+    const int block = static_cast<int>(static_cast<int64_t>(s0) * p.group / RB) + b;
+    const uint64_t m = __ballot(i + lane < p.batch && block <= u);
     if (m == 0) break;
-    b = i + 63 - __builtin_clzll(m);
+    const int at = 63 - __builtin_clzll(m);
+    found = i + at;
+    first = __builtin_amdgcn_readlane(s0, at);
+    end = __builtin_amdgcn_readlane(s1, at);
+    ctx = __builtin_amdgcn_readlane(n, at);
   }
-  if (b < 0) return false;
-  r.b = b;
-  r.first = start(b);
-  r.len = start(b + 1) - r.first;
+  if (found < 0) return false;
+  r.b = found;
+  r.first = first;
+  r.len = end - first;
   r.rows = r.len * p.group;
-  r.row0 = (u - block(b)) * RB;
-  r.ctx = min(max(p.ctx[b], 0), p.width << p.shift);
+  r.row0 = (u - static_cast<int>(static_cast<int64_t>(first) * p.group / RB) - found) * RB;
+  r.ctx = min(max(ctx, 0), p.width << p.shift);
   return r.len > 0 && r.row0 < r.rows;
 }
 
@@ -118,8 +123,10 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight int8 codes as bf16.
+// Eight int8 codes as bf16.  The words are opaque here, or the compiler carries
+// a loop's loads on as single bytes, a register each.
 __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
+  asm("" : "+v"(lo), "+v"(hi));
   bf16x8 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -139,32 +146,69 @@ __device__ __forceinline__ float over_groups(float v, F f) {
   return f(v, __shfl_xor(v, 32, 64));
 }
 
-// NQ: 16-row column blocks per wave; WK: waves that share a workgroup's rows
-// (and its tokens, 64 a time), 4 / WK row blocks.
-template <int D, int NQ, int WK>
-__global__ __launch_bounds__(256) void kv_attn(KvAttnArgs p) {
-  constexpr int WR = 4 / WK, WROWS = 16 * NQ, RB = WROWS * WR;
+// NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
+template <int D, int NQ>
+__global__ __launch_bounds__(256, NQ == 1 && D == 64 ? 4 : 2) void kv_attn(KvAttnArgs p) {
+  constexpr int WK = 4, WROWS = 16 * NQ, RB = WROWS;
   constexpr int NC = D / 32, ND = D / 16, NL = D / 64;  // k-steps of the scores, d blocks, 16-byte pieces of a K row
   constexpr int LD = D + 4;
-  __shared__ __attribute__((aligned(16))) float red[WK > 1 ? WK * WROWS * LD : 1];
+  __shared__ __attribute__((aligned(16))) float red[WK * WROWS * LD];
   __shared__ float ml[2][WK][WROWS];
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int wr = w / WK, wk = w % WK;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int split = id % p.splits, unit = id / p.splits;
-  const int head = unit / p.blocks, u = unit - head * p.blocks;
+  const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
+  const int split = in_head / p.blocks, u = in_head - split * p.blocks, unit = head * p.blocks + u;
   KvRows r;
   if (!kv_rows<RB>(p, u, r)) return;
   // row i of the sequence: query i / group, head i % group of the K/V head's; it sees seen(i) tokens
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
-  const int last = min(r.row0 + RB, r.rows) - 1;
-  const int k_end = seen(last);
+  const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
   // the last split takes what lies past the longest context that the caller expected
   const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
   if (split > 0 && kb >= k_end) return;
-  const int base = r.row0 + wr * WROWS;  // the wave's rows
-  const bool idle = WK == 1 && base >= r.rows;
-  if (WK == 1 && idle) return;
+
+  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
+  const int page_mask = (1 << p.shift) - 1;
+  struct Pages {
+    int k, v;  // pages of the lane's K rows and V columns, -1: none
+  };
+  auto page_at = [&](int t) {
+    const int pg = row[min(t, k_end - 1) >> p.shift];
+    return t < k_end && pg >= 0 && pg < p.pages ? pg : -1;
+  };
+  auto load_pages = [&](int t0) { return Pages{page_at(t0 + 16 * (c >> 2)), page_at(t0 + 16 * g)}; };
+  u32x4 kr[4][NL], vr[ND];
+  float ksc = 0.0f, vsc = 0.0f;
+  bool none = false;
+  auto load_k = [&](int t0, Pages pg) {
+    const int64_t at = (static_cast<int64_t>(max(pg.k, 0)) * p.kv_heads + head) << p.shift;
+    const int8_t *src = p.kc + (at + ((t0 + 16 * (c >> 2)) & page_mask) + (c & 3)) * D + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NL; ++j) kr[i][j] = *reinterpret_cast<const u32x4 *>(src + 4 * i * D + 64 * j);
+  };
+  auto load_v = [&](int t0, Pages pg) {
+    const int64_t unit_at = static_cast<int64_t>(max(pg.v, 0)) * p.kv_heads + head;
+    const int8_t *src = p.vc + (((unit_at * D + c) << p.shift) + ((t0 + 16 * g) & page_mask));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      vr[d] = *reinterpret_cast<const u32x4 *>(src);
+      src += 16 << p.shift;
+    }
+    ksc = p.ks[unit_at];
+    vsc = p.vs[unit_at];
+    none = pg.v < 0;
+  };
+  constexpr int STEP = 64 * WK;
+  int t0 = kb + 64 * w;
+  Pages pg;
+  if (t0 < ke) {
+    pg = load_pages(t0);
+    load_k(t0, pg);
+    load_v(t0, pg);
+    pg = load_pages(t0 + STEP);
+  }
 
   const float sc0 = fabsf(p.scale_log2);
   const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
@@ -173,21 +217,19 @@ __global__ __launch_bounds__(256) void kv_attn(KvAttnArgs p) {
   int64_t out_row[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int row = min(base + 16 * n + c, r.rows - 1), t = row / p.group;
-    vis[n] = seen(row);
-    const int h = head * p.group + row - t * p.group;
+    const int i = min(r.row0 + 16 * n + c, r.rows - 1), t = i / p.group;
+    vis[n] = p.causal ? min(max(r.ctx - r.len + 1 + t, 0), r.ctx) : r.ctx;
+    const int h = head * p.group + i - t * p.group;
     out_row[n] = static_cast<int64_t>(r.first + t) * p.heads + h;
     const bf16 *at = p.q + (r.first + t) * p.q_stride + h * D;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      u32x4 raw = *reinterpret_cast<const u32x4 *>(at + (i >> 1) * 64 + g * 16 + (i & 1) * 8);
+    for (int j = 0; j < NC; ++j) {
+      u32x4 raw = *reinterpret_cast<const u32x4 *>(at + (j >> 1) * 64 + g * 16 + (j & 1) * 8);
       raw ^= qsign;
-      qf[n][i] = __builtin_bit_cast(bf16x8, raw);
+      qf[n][j] = __builtin_bit_cast(bf16x8, raw);
     }
   }
-  // all of the wave's rows see the tokens below it
-  const int all_see = seen(min(base, r.rows - 1));
-  const int w_end = min(ke, seen(min(base + WROWS, r.rows) - 1));
+  const int all_see = seen(r.row0);  // all rows see the tokens below it
 
   f32x4 acc[NQ][ND];
   float m_run[NQ], l_run[NQ];
@@ -198,211 +240,130 @@ __global__ __launch_bounds__(256) void kv_attn(KvAttnArgs p) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-
-  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
-  const int page_mask = (1 << p.shift) - 1;
-  const int kg = c >> 2;  // the lane group whose tokens the lane's K rows are
-  struct Pages {
-    int k, v;  // pages of the lane's K rows and V columns, -1: none
-  };
-  auto page_at = [&](int t) {
-    if (t >= k_end) return -1;
-    const int pg = row[t >> p.shift];
-    return pg >= 0 && pg < p.pages ? pg : -1;
-  };
-  auto load_pages = [&](int t0) { return Pages{page_at(t0 + 16 * kg), page_at(t0 + 16 * g)}; };
-  u32x4 kr[4][NL], vr[ND];
-  float ksc = 0.0f, vsc = 0.0f;
-  bool none = false;
-  auto load_k = [&](int t0, Pages pg) {
-    const int64_t at = (static_cast<int64_t>(max(pg.k, 0)) * p.kv_heads + head) << p.shift;
-    const int8_t *src = p.kc + (at + ((t0 + 16 * kg) & page_mask) + (c & 3)) * D + 16 * g;
+#pragma unroll 1
+  for (; t0 < ke; t0 += STEP) {
+    f32x4 s[NQ][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j < NL; ++j) kr[i][j] = *reinterpret_cast<const u32x4 *>(src + 4 * i * D + 64 * j);
-  };
-  auto load_v = [&](int t0, Pages pg) {
-    const int64_t unit_at = static_cast<int64_t>(max(pg.v, 0)) * p.kv_heads + head;
-    const int8_t *src = p.vc + (unit_at * D << p.shift) + (c << p.shift) + ((t0 + 16 * g) & page_mask);
+      for (int n = 0; n < NQ; ++n) s[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int d = 0; d < ND; ++d) vr[d] = *reinterpret_cast<const u32x4 *>(src + (16 * d << p.shift));
-    ksc = p.ks[unit_at];
-    vsc = p.vs[unit_at];
-    none = pg.v < 0;
-  };
-
-  int t0 = kb + 64 * wk;
-  constexpr int STEP = 64 * WK;
-  if (t0 < w_end) {
-    Pages pg = load_pages(t0);
-    load_k(t0, pg);
-    load_v(t0, pg);
-    pg = load_pages(t0 + STEP);
-    for (; t0 < w_end; t0 += STEP) {
-      f32x4 s[NQ][4];
+      for (int j = 0; j < NC; ++j) {
+        const bf16x8 a = codes8(kr[i][j >> 1][2 * (j & 1)], kr[i][j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) s[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const bf16x8 a = codes8(kr[i][j >> 1][2 * (j & 1)], kr[i][j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[n][i] = mfma16(a, qf[n][j], s[n][i]);
-        }
+        for (int n = 0; n < NQ; ++n) s[n][i] = mfma16(a, qf[n][j], s[n][i]);
       }
-      const bool more = t0 + STEP < w_end;
-      // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too; NaN stays
-      const float sc = __builtin_elementwise_maximum(sc0 * ksc, 1.17549435e-38f), vmul = vsc;
-      const bool hidden = none;
-      if (more) load_k(t0 + STEP, pg);
-      const bool masks = t0 + 64 > all_see || __any(hidden);
-      const int at = t0 + 16 * g;  // the lane's first token
-      bf16x8 pb[NQ][2];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const bool more = t0 + STEP < ke;
+    // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too; NaN stays
+    const float sc = __builtin_elementwise_maximum(sc0 * ksc, 1.17549435e-38f), vmul = vsc;
+    const bool hidden = none;
+    if (more) load_k(t0 + STEP, pg);
+    const bool masks = t0 + 64 > all_see || __any(hidden);
+    const int at = t0 + 16 * g;  // the lane's first token
+    bf16x8 pb[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float scn = sc;
-        if (masks) {
-          if (hidden || at >= vis[n]) scn = 1.17549435e-38f;  // the scale of a page that the row does not see may be anything
+    for (int n = 0; n < NQ; ++n) {
+      float scn = sc;
+      if (masks) {
+        if (hidden || at >= vis[n]) scn = 1.17549435e-38f;  // the scale of a page that the row does not see may be anything
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 16; ++i)
+          if (hidden || at + i >= vis[n]) s[n][i >> 2][i & 3] = -INFINITY;
+      }
+      float mx = s[n][0][0];
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (hidden || at + 4 * i + v >= vis[n]) s[n][i][v] = -INFINITY;
-        }
-        float mx = s[n][0][0];
+      for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
+      mx = over_groups(mx * scn, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
+        const float m_new = fmaxf(m_run[n], mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
+        l_run[n] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
+        m_run[n] = m_new;
+      }
+      const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) mx = __builtin_elementwise_maximum(mx, s[n][i][v]);
-        mx = over_groups(mx * scn, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
-        if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
-          const float m_new = fmaxf(m_run[n], mx);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
-          l_run[n] *= alpha;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
-          m_run[n] = m_new;
-        }
-        const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i][v], scn, neg_m));
-            l_run[n] += e;
-            s[n][i][v] = e * vmul;
-          }
-        if (masks) {  // a hidden token's V scale may be anything
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (hidden || at + 4 * i + v >= vis[n]) s[n][i][v] = 0.0f;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              const bf16x2 pr = cvt_pk_bf16(s[n][2 * h + i][2 * v], s[n][2 * h + i][2 * v + 1]);
-              pb[n][h][4 * i + 2 * v] = pr[0];
-              pb[n][h][4 * i + 2 * v + 1] = pr[1];
-            }
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], scn, neg_m));
+        l_run[n] += e;
+        s[n][i >> 2][i & 3] = masks && (hidden || at + i >= vis[n]) ? 0.0f : e * vmul;  // a hidden token's V scale may be anything
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bf16x8 a = codes8(vr[d][2 * h], vr[d][2 * h + 1]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) acc[n][d] = mfma16(a, pb[n][h], acc[n][d]);
-        }
-      if (more) {
-        load_v(t0 + STEP, pg);
-        pg = load_pages(t0 + 2 * STEP);
+      for (int i = 0; i < 16; i += 2) {
+        const bf16x2 pr = cvt_pk_bf16(s[n][i >> 2][i & 3], s[n][i >> 2][(i & 3) + 1]);
+        pb[n][i >> 3][i & 7] = pr[0];
+        pb[n][i >> 3][(i & 7) + 1] = pr[1];
       }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bf16x8 a = codes8(vr[d][2 * h], vr[d][2 * h + 1]);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) acc[n][d] = mfma16(a, pb[n][h], acc[n][d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (more) {
+      load_v(t0 + STEP, pg);
+      pg = load_pages(t0 + 2 * STEP);
     }
   }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) l_run[n] = over_groups(l_run[n], [](float a, float b) { return a + b; });
 
+  // the waves' parts: a common max, then the sum of their outputs in wave order
   const bool whole = p.part == nullptr;
   const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB;  // part rows of this (unit, split)
-  if constexpr (WK == 1) {
+  if (g == 0) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int at = wr * WROWS + 16 * n + c;
-      if (r.row0 + at >= r.rows) continue;
-      const float mul = whole ? (l_run[n] == 0.0f ? 0.0f : 1.0f / l_run[n]) : 1.0f;
+      ml[0][w][16 * n + c] = m_run[n];
+      ml[1][w][16 * n + c] = l_run[n];
+    }
+  }
+  __syncthreads();
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        if (whole) {
-          bf16x4 o4;
+  for (int n = 0; n < NQ; ++n) {
+    const int at = 16 * n + c;
+    float m = ml[0][0][at], l = 0.0f;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(acc[n][d][v] * mul);
-          *reinterpret_cast<bf16x4 *>(p.o + out_row[n] * D + 16 * d + 4 * g) = o4;
-        } else {
-          *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + 16 * d + 4 * g) = acc[n][d];
-        }
-      }
-      if (g == 0 && !whole) {
-        p.part[p.ml_off + (slot + at) * 2] = m_run[n];
-        p.part[p.ml_off + (slot + at) * 2 + 1] = l_run[n];
-      } else if (g == 0 && p.l != nullptr) {
-        p.l[out_row[n]] = (m_run[n] + log2f(l_run[n])) * 0.6931471805599453f;
+    for (int i = 1; i < WK; ++i) m = fmaxf(m, ml[0][i][at]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) l += ml[1][i][at] * __builtin_amdgcn_exp2f(ml[0][i][at] - ref);
+    const float mul = __builtin_amdgcn_exp2f(m_run[n] - ref) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<f32x4 *>(red + (w * WROWS + at) * LD + 16 * d + 4 * g) = acc[n][d] * mul;
+    if (w == 0 && g == 0 && r.row0 + at < r.rows) {
+      if (!whole) {
+        p.part[p.ml_off + (slot + at) * 2] = m;
+        p.part[p.ml_off + (slot + at) * 2 + 1] = l;
+      } else if (p.l != nullptr) {
+        p.l[out_row[n]] = (m + log2f(l)) * 0.6931471805599453f;
       }
     }
-  } else {
-    // the waves' parts: a common max, then the sum of their outputs in wave order
-    if (g == 0) {
+  }
+  __syncthreads();
+  const int rows = min(WROWS, r.rows - r.row0);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int at = i / (D / 4), d = 4 * (i % (D / 4));
+    f32x4 o = *reinterpret_cast<const f32x4 *>(red + at * LD + d);
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        ml[0][wk][16 * n + c] = m_run[n];
-        ml[1][wk][16 * n + c] = l_run[n];
-      }
-    }
-    __syncthreads();
+    for (int k = 1; k < WK; ++k) o += *reinterpret_cast<const f32x4 *>(red + (k * WROWS + at) * LD + d);
+    if (whole) {
+      const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
+      bf16x4 o4;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int at = 16 * n + c;
-      float m = ml[0][0][at], l = 0.0f;
-#pragma unroll
-      for (int i = 1; i < WK; ++i) m = fmaxf(m, ml[0][i][at]);
-      const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int i = 0; i < WK; ++i) l += ml[1][i][at] * __builtin_amdgcn_exp2f(ml[0][i][at] - ref);
-      const float mul = __builtin_amdgcn_exp2f(m_run[n] - ref) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-        *reinterpret_cast<f32x4 *>(red + (wk * WROWS + at) * LD + 16 * d + 4 * g) = acc[n][d] * mul;
-      if (wk == 0 && g == 0 && r.row0 + at < r.rows) {
-        if (!whole) {
-          p.part[p.ml_off + (slot + at) * 2] = m;
-          p.part[p.ml_off + (slot + at) * 2 + 1] = l;
-        } else if (p.l != nullptr) {
-          p.l[out_row[n]] = (m + log2f(l)) * 0.6931471805599453f;
-        }
-      }
-    }
-    __syncthreads();
-    const int rows = min(WROWS, r.rows - r.row0);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-      const int at = i / (D / 4), d = 4 * (i % (D / 4));
-      f32x4 o = *reinterpret_cast<const f32x4 *>(red + at * LD + d);
-#pragma unroll
-      for (int k = 1; k < WK; ++k) o += *reinterpret_cast<const f32x4 *>(red + (k * WROWS + at) * LD + d);
-      if (whole) {
-        const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
-        bf16x4 o4;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(o[v]);
-        *reinterpret_cast<bf16x4 *>(p.o + (static_cast<int64_t>(r.first + t) * p.heads + h) * D + d) = o4;
-      } else {
-        *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + d) = o;
-      }
+      for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(o[v]);
+      *reinterpret_cast<bf16x4 *>(p.o + (static_cast<int64_t>(r.first + t) * p.heads + h) * D + d) = o4;
+    } else {
+      *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + d) = o;
     }
   }
 }
@@ -423,8 +384,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int split = id % p.splits, unit = id / p.splits;
-  const int head = unit / p.blocks, u = unit - head * p.blocks;
+  const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
+  const int split = in_head / p.blocks, u = in_head - split * p.blocks, unit = head * p.blocks + u;
   KvRows r;
   if (!kv_rows_sorted<RB>(p, u, r)) return;
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
@@ -648,7 +609,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   l_run += __shfl_xor(l_run, 32, 64);
   if (base + c >= r.rows) return;
   const bool whole = p.part == nullptr;
-  const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB + 32 * w + c;
+  // (the block's own number, not its place in the order)
+  const int block = head * p.blocks + static_cast<int>(static_cast<int64_t>(r.first) * p.group / RB) + r.b + r.row0 / RB;
+  const int64_t slot = (static_cast<int64_t>(block) * p.splits + split) * RB + 32 * w + c;
   const float mul = whole ? (l_run == 0.0f ? 0.0f : 1.0f / l_run) : 1.0f;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -672,45 +635,71 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   }
 }
 
-// One wave per row: the splits' parts, in split order.
+// One wave per row of the output: the splits' parts, in split order.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
   constexpr int V = D / 64;
+  typedef float fv __attribute__((ext_vector_type(V)));
   const int lane = threadIdx.x & 63;
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int unit = static_cast<int>(wave / RB), at = static_cast<int>(wave % RB);
-  const int head = unit / p.blocks;
-  if (head >= p.kv_heads) return;
-  KvRows r;
-  const bool found = RB == 128 ? kv_rows_sorted<RB>(p, unit - head * p.blocks, r) : kv_rows<RB>(p, unit - head * p.blocks, r);
-  if (!found || r.row0 + at >= r.rows) return;
-  const int last = min(r.row0 + RB, r.rows) - 1;
-  const int k_end = p.causal ? min(max(r.ctx - r.len + 1 + last / p.group, 0), r.ctx) : r.ctx;
+  const uint32_t row = blockIdx.x * 4u + (threadIdx.x >> 6);  // below 2^31
+  const int t = row / p.heads, h = static_cast<int>(row - static_cast<uint32_t>(t) * p.heads), head = h / p.group;
+  if (t >= p.tokens) return;
+  // the row's sequence, and its place among the sequence's rows
+  int b = -1, first = 0, end = 0, ctx = 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    const int at = min(i + lane, p.batch - 1), s0 = p.starts ? p.starts[at] : at, s1 = p.starts ? p.starts[at + 1] : at + 1;
+    const int n = p.ctx[at];
+    const uint64_t m = __ballot(i + lane < p.batch && s0 <= t && t < s1);
+    if (m == 0) continue;
+    const int from = __builtin_ctzll(m);
+    b = i + from;
+    first = max(__builtin_amdgcn_readlane(s0, from), 0);
+    end = min(__builtin_amdgcn_readlane(s1, from), p.tokens);
+    ctx = min(max(__builtin_amdgcn_readlane(n, from), 0), p.width << p.shift);
+    break;
+  }
+  if (b < 0) return;
+  const int i = (t - first) * p.group + h - head * p.group, len = end - first;
+  const int last = min(i / RB * RB + RB, len * p.group) - 1;
+  const int k_end = p.causal ? min(max(ctx - len + 1 + last / p.group, 0), ctx) : ctx;
   const int n = min(p.splits, max(1, (k_end - 1) / p.chunk + 1));
-  const int64_t slot = static_cast<int64_t>(unit) * p.splits * RB + at;
+  const int unit = head * p.blocks + static_cast<int>(static_cast<int64_t>(first) * p.group / RB) + b + i / RB;
+  const int64_t slot = static_cast<int64_t>(unit) * p.splits * RB + i % RB;
   const float *ml = p.part + p.ml_off;
   float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, ml[(slot + i * RB) * 2]);
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, ml[(slot + static_cast<int64_t>(s) * RB) * 2]);
+  m = wave_max(m);
   const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, o[V] = {};
-  for (int i = 0; i < n; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[(slot + i * RB) * 2] - ref);
-    l += ml[(slot + i * RB) * 2 + 1] * f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = __builtin_fmaf(p.part[(slot + i * RB) * D + lane * V + j], f, o[j]);
+  float l = 0.0f;
+  fv o = {};
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const int64_t at = slot + static_cast<int64_t>(s) * RB;
+    const float f = __builtin_amdgcn_exp2f(ml[at * 2] - ref);
+    l += ml[at * 2 + 1] * f;
+    o += *reinterpret_cast<const fv *>(p.part + at * D + lane * V) * f;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
-  const int64_t row = static_cast<int64_t>(r.first + t) * p.heads + h;
 #pragma unroll
-  for (int j = 0; j < V; ++j) p.o[row * D + lane * V + j] = static_cast<bf16>(o[j] * inv);
+  for (int j = 0; j < V; ++j) p.o[static_cast<int64_t>(row) * D + lane * V + j] = static_cast<bf16>(o[j] * inv);
   if (p.l != nullptr && lane == 0) p.l[row] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ── which form, and how many splits ─────────────────────────────────────────
+// Few rows take kv_attn, more than 64 a sequence the shared tiles.  Splits fill
+// the device with two workgroups to a CU, of 256 tokens each at least (512 where
+// there are many: a second launch, 2 us, and a workgroup's start and end, 4 us,
+// which no other work hides), and cut contexts that may differ much in length.
+// us by splits: 16 x 4000 tokens, 8 K/V heads of 128, one query, 1 / 2 / 4 / 6 / 8
+// 48 / 44 / 35 / 38 / 39; 1 x 16000 1 / 8 / 16 / 32 145 / 28 / 20 / 19; 64 x 2048 1
+// / 2 / 3 56 / 63 / 66; 64 x 90 to 8000 1 / 2 / 3 / 4 / 8 132 / 130 / 119 / 127 /
+// 132; 24 x 1000 of 64 1 / 2 12 / 14.  Shared tiles: 1 x 64 queries x 16000 1 / 8 /
+// 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads of 64, 1 / 4 / 8 / 16 145 / 49
+// / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242 / 180 / 139 / 160; 4 x 700 x 1100
+// to 4100 1 / 2 162 / 200.
 struct KvAttnPlan {
   bool tile = false;
-  int nq = 1, wk = 4, rb = 16;
+  int nq = 1, rb = 16;
   int64_t blocks = 0;
   int splits = 1, chunk = 0;
   size_t bytes = 0;
@@ -721,10 +710,15 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   KvAttnPlan pl;
   const int64_t group = heads / kv_heads, rows = group * max_q;
   if (rows > 64) pl.tile = true, pl.rb = 128;
-  else if (rows > 16) pl.nq = 2, pl.wk = 4, pl.rb = 32;
+  else if (rows > 16) pl.nq = 2, pl.rb = 32;
   pl.blocks = tokens * group / pl.rb + batch;
-  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = pl.tile ? 64 : 64 * pl.wk;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(4 * cus / std::max<int64_t>(units, 1), max_ctx / 512));
+  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = pl.tile ? 64 : 256;
+  // workgroups with work, unsplit: at most the row blocks of every sequence
+  const int64_t busy = std::max<int64_t>(1, std::min(pl.blocks, batch * cdiv(std::max<int64_t>(rows, 1), pl.rb)) * kv_heads);
+  const int64_t least = pl.tile ? (busy < 32 ? 256 : 768) : busy < 64 ? 256 : 512;
+  int64_t splits = std::min(2 * cus / busy, max_ctx / least);
+  if (!pl.tile || busy < 2 * cus) splits = std::max(splits, max_ctx / 2560);
+  splits = std::max<int64_t>(1, splits);
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   if (size(splits) > scratch) splits = 1;
   pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), splits), step) * step);
@@ -733,25 +727,25 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   return pl;
 }
 
-template <int D, int NQ, int WK>
+template <int D, int NQ>
 static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_t s) {
-  constexpr int RB = 16 * NQ * (4 / WK);
-  const int64_t units = pl.blocks * p.kv_heads;
-  hipLaunchKernelGGL((kv_attn<D, NQ, WK>), dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+  constexpr int RB = 16 * NQ;
+  const int64_t units = pl.blocks * p.kv_heads, rows = static_cast<int64_t>(p.tokens) * p.heads;
+  hipLaunchKernelGGL((kv_attn<D, NQ>), dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
   if (pl.splits > 1)
-    hipLaunchKernelGGL((kv_attn_combine<D, RB>), dim3(static_cast<unsigned>(cdiv(units * RB, 4))), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((kv_attn_combine<D, RB>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
 }
 
 template <int D>
 static void launch_kv_attn(const KvAttnPlan &pl, const KvAttnArgs &p, hipStream_t s) {
   if (pl.tile) {
-    const int64_t units = pl.blocks * p.kv_heads;
+    const int64_t units = pl.blocks * p.kv_heads, rows = static_cast<int64_t>(p.tokens) * p.heads;
     hipLaunchKernelGGL(kv_attn_tile<D>, dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
     if (pl.splits > 1)
-      hipLaunchKernelGGL((kv_attn_combine<D, 128>), dim3(static_cast<unsigned>(cdiv(units * 128, 4))), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((kv_attn_combine<D, 128>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
   }
-  else if (pl.nq == 2) launch_kv_attn<D, 2, 4>(pl, p, s);
-  else launch_kv_attn<D, 1, 4>(pl, p, s);
+  else if (pl.nq == 2) launch_kv_attn<D, 2>(pl, p, s);
+  else launch_kv_attn<D, 1>(pl, p, s);
 }
 
 static teeny_status kv_attn_sizes(const char *nm, int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
