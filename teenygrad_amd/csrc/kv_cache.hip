@@ -166,7 +166,9 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan(KvPlanArgs p) {
 // a team of page_size / 16 waves does the page of one head and one cache, 16
 // tokens a wave, held in registers between the two passes over them.  A page
 // that a run begins at its first slot forgets its old scale.  Bound by
-// reading the tokens and writing the codes, and by latency for few tokens.
+// reading the tokens and writing the codes, and by latency for few tokens:
+// 5 x 1600 tokens of 8 heads of 128 take 13.8 us (49 MB, 3.6 TB/s; 20.0 with
+// a division of its own for each code), 64 requests' single tokens 5.1 us.
 
 struct KvWriteArgs {
   const bf16 *k, *v;
@@ -174,18 +176,39 @@ struct KvWriteArgs {
   const int32_t *slots;
   int8_t *kc, *vc;
   float *ks, *vs;
-  int tokens, heads, pages, shift, chunk;
+  int tokens, heads, pages, shift, share;  // share: workgroups to 64 tokens, a head and a cache
 };
 
-// Codes of x and of an old code under the scale s; 0 where s is 0 or not finite.
-__device__ __forceinline__ int kv_code(float x, float s, bool fine) {
-  return fine ? static_cast<int>(__builtin_rintf(fminf(fmaxf(x / s, -127.0f), 127.0f))) : 0;
+// bits[i]: a word whose low byte is rint(x[i] / s), in -127..127, the quotient
+// rounded to fp32 first as division does: x inv, inv the rounded reciprocal, and
+// two corrections by the exact remainder, the last of which rounds correctly
+// (Markstein, 1990).  Adding 1.5 * 2^23 rounds to an integer and leaves it in the
+// low bits.  tiny: s and x were scaled up from where fp32 has fewer bits, and s
+// may be too small for its largest x.
+template <int N>
+__device__ __forceinline__ void kv_codes(float (&x)[N], float s, float inv, bool tiny, uint32_t (&bits)[N]) {
+  if (tiny)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= 0x1p100f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float t = x[i] * inv;
+    t = __builtin_fmaf(__builtin_fmaf(-t, s, x[i]), inv, t);
+    x[i] = __builtin_fmaf(__builtin_fmaf(-t, s, x[i]), inv, t);
+  }
+  if (tiny)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fminf(fmaxf(x[i], -127.0f), 127.0f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) bits[i] = __float_as_uint(x[i] + 12582912.0f);
 }
-__device__ __forceinline__ int kv_recode(int q, float ratio, bool fine) {
-  return fine ? static_cast<int>(__builtin_rintf(static_cast<float>(q) * ratio)) : 0;
+// An old code under a larger scale: ratio = old scale / new scale.
+__device__ __forceinline__ int kv_recode(int q, float ratio) {
+  return static_cast<int>(__builtin_rintf(static_cast<float>(q) * ratio));
 }
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
 }
 __device__ __forceinline__ int byte_of(uint32_t word, int i) {
   return static_cast<int8_t>((word >> (8 * i)) & 0xffu);
@@ -195,143 +218,159 @@ __device__ __forceinline__ int byte_of(uint32_t word, int i) {
 template <int D, int WPP>
 __global__ __launch_bounds__(64 * (WPP > 4 ? WPP : 4)) void kv_write(KvWriteArgs p) {
   constexpr int TEAMS = WPP > 4 ? 1 : 4 / WPP, PAGE = 16 * WPP;
-  __shared__ uint32_t big[TEAMS][WPP];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, team = w / WPP, part = w % WPP;
-  const int head = blockIdx.y;
+  __shared__ uint32_t big[2][TEAMS][WPP];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int team = w / WPP, part = w % WPP, head = blockIdx.y;
   const bool is_v = blockIdx.z == 1;
-  const int t0 = blockIdx.x * p.chunk;
+  // worker by worker, so that those without a run, the later ones, are not always the same XCD's
+  const int chunks = (p.tokens + 63) / 64, worker = blockIdx.x / chunks, t0 = (blockIdx.x - worker * chunks) * 64;
   const int limit = p.pages << p.shift;  // slots of the cache, below 2^31
 
-  // the runs that begin in this chunk of at most 64 tokens
-  bool leads = false;
-  {
-    const int t = t0 + lane;
-    if (lane < p.chunk && t < p.tokens) {
-      const int s = p.slots[t], before = t > 0 ? p.slots[t - 1] : -2;
-      leads = s >= 0 && s < limit && (s % PAGE == 0 || s != before + 1);
-    }
-  }
-  uint64_t runs = __ballot(leads);
-  const int rounds = (__popcll(runs) + TEAMS - 1) / TEAMS;
-  for (int skip = 0; skip < team; ++skip) runs &= runs - 1;
-  for (int round = 0; round < rounds; ++round) {
-    const bool live = runs != 0;
-    const int first = live ? t0 + __builtin_ctzll(runs) : 0;
-#pragma unroll
-    for (int skip = 0; skip < TEAMS; ++skip) runs &= runs - 1;
-    const int slot = live ? p.slots[first] : 0;
+  // 64 tokens' slots and the runs that begin among them, dealt out to the workers' teams in turn
+  const int mine = t0 + lane < p.tokens ? p.slots[t0 + lane] : -1;
+  int before = __shfl_up(mine, 1, 64);
+  if (lane == 0) before = t0 > 0 ? p.slots[t0 - 1] : -2;
+  const bool leads = mine >= 0 && mine < limit && (mine % PAGE == 0 || mine != before + 1);
+  const uint64_t runs = __ballot(leads);
+  const int rank = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(runs >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(runs), 0));
+  const int stride = p.share * TEAMS, count = __popcll(runs);
+  for (int round = 0, turn = worker * TEAMS; turn < count; ++round, turn += stride) {
+    const uint64_t own = __ballot(leads && rank == turn + team);
+    const bool live = own != 0;
+    const int at0 = live ? __builtin_ctzll(own) : 0, first = t0 + at0;
+    const int slot = live ? __builtin_amdgcn_readlane(mine, at0) : 0;
     const int page = slot / PAGE, old = slot % PAGE;
     int n = 0;  // the run's length
     if (live) {
-      for (int i = 0; i < PAGE; i += 64) {
-        const int at = i + lane;
-        const bool in = at < PAGE - old && first + at < p.tokens && p.slots[first + at] == slot + at;
-        const uint64_t same = __ballot(in);
-        const int more = same == ~0ull ? 64 : __builtin_ctzll(~same);
-        n += more;
-        if (more < 64) break;
+      const uint64_t in = __ballot(lane >= at0 && lane - at0 < PAGE - old && mine == slot + lane - at0) >> at0;
+      n = in == ~0ull ? 64 : __builtin_ctzll(~in);
+      // past the slots at hand
+      while (n < PAGE - old && at0 + n >= 64) {
+        const int at = n + lane;
+        const uint64_t more = __ballot(at < PAGE - old && first + at < p.tokens && p.slots[first + at] == slot + at);
+        const int m = more == ~0ull ? 64 : __builtin_ctzll(~more);
+        n += m;
+        if (m < 64) break;
       }
     }
     const int64_t unit = static_cast<int64_t>(page) * p.heads + head;
     float *scale_at = (is_v ? p.vs : p.ks) + unit;
-    const float before = live && old > 0 ? *scale_at : 0.0f;
+    const float scale0 = live && old > 0 ? *scale_at : 0.0f;
     // offsets of this wave's 16 tokens: [lo, hi) are new
     const int base = 16 * part, lo = max(old - base, 0), hi = min(old + n - base, 16);
-    const bool news = live && hi > lo;
+    const bool news = live && hi > lo, whole = lo == 0 && hi == 16;
     uint32_t mx = 0;  // the largest magnitude as bf16 bits: ordered like the values, NaN above all
     constexpr int VPR = D / 8, RPI = 64 / VPR, NK = 16 / RPI;  // K: lanes per row, rows per round
-    u32x4 kr[NK];
+    constexpr int DPL = D / 64;                                // V: d's per lane
+    u32x4 kr[NK], vc[DPL];
     uint32_t vr[16];
-    constexpr int DPL = D / 64;  // V: d's per lane
+    u32x4 *v_at = reinterpret_cast<u32x4 *>(p.vc + unit * (PAGE * D) + DPL * lane * PAGE + base);
+    // (outside of [lo, hi) the nearest new token once more: it changes no maximum)
     if (news && !is_v) {
+      const bf16 *src = p.k + (first + base - old) * p.k_stride + head * D + 8 * (lane % VPR);
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const int o = i * RPI + lane / VPR;
-        kr[i] = u32x4{0u, 0u, 0u, 0u};
-        if (o >= lo && o < hi)
-          kr[i] = *reinterpret_cast<const u32x4 *>(p.k + (first + base + o - old) * p.k_stride + head * D + 8 * (lane % VPR));
-      }
+      for (int i = 0; i < NK; ++i)
+        kr[i] = *reinterpret_cast<const u32x4 *>(src + min(max(i * RPI + lane / VPR, lo), hi - 1) * p.k_stride);
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = max(mx, max(kr[i][j] & 0x7fffu, (kr[i][j] >> 16) & 0x7fffu));
-    } else if (news) {
+    } else if (live && is_v) {
+      // bytes of other tokens stay as they are (or take the new scale)
+      if (!whole)
 #pragma unroll
-      for (int o = 0; o < 16; ++o) {
-        vr[o] = 0;
-        if (o >= lo && o < hi) {
-          const bf16 *at = p.v + (first + base + o - old) * p.v_stride + head * D + DPL * lane;
+        for (int dd = 0; dd < DPL; ++dd) vc[dd] = v_at[dd * (PAGE / 16)];
+      if (news) {
+        const bf16 *src = p.v + (first + base - old) * p.v_stride + head * D + DPL * lane;
+#pragma unroll
+        for (int o = 0; o < 16; ++o) {
+          const bf16 *at = src + min(max(o, lo), hi - 1) * p.v_stride;
           if constexpr (DPL == 2) vr[o] = *reinterpret_cast<const uint32_t *>(at);
           else vr[o] = *reinterpret_cast<const uint16_t *>(at);
         }
-      }
 #pragma unroll
-      for (int o = 0; o < 16; ++o) mx = max(mx, max(vr[o] & 0x7fffu, (vr[o] >> 16) & 0x7fffu));
+        for (int o = 0; o < 16; ++o) mx = max(mx, max(vr[o] & 0x7fffu, (vr[o] >> 16) & 0x7fffu));
+      }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), off, 64)));
-    if constexpr (WPP > 1) {
-      if (lane == 0) big[team][part] = mx;
+    if constexpr (WPP > 1) {  // two sets in turn: a wave writes the next one at most before the last reads this one
+      if (lane == 0) big[round & 1][team][part] = mx;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < WPP; ++i) mx = max(mx, big[team][i]);
-      __syncthreads();  // before the next round's values
+      for (int i = 0; i < WPP; ++i) mx = max(mx, big[round & 1][team][i]);
     }
     if (!live) continue;
-    const float scale = __builtin_elementwise_maximum(before, __uint_as_float(mx << 16) / 127.0f);
-    const bool fine = scale > 0.0f && scale < INFINITY;
-    const float ratio = fine ? before / scale : 1.0f;
-    const bool again = old > base && scale != before;  // old codes here, under another scale (also NaN)
+    const float scale = __builtin_elementwise_maximum(scale0, __uint_as_float(mx << 16) / 127.0f);
+    const bool fine = scale > 0.0f && scale < INFINITY;  // else every code is 0
+    const bool tiny = scale < 1e-30f;
+    const float div = tiny ? scale * 0x1p100f : scale, inv = fine ? 1.0f / div : 0.0f, ratio = fine ? scale0 / scale : 0.0f;
+    const bool again = old > base && scale != scale0;  // old codes here, under another scale (also NaN)
     if (!is_v) {
       if (news || again) {
+        u32x2 *at = reinterpret_cast<u32x2 *>(p.kc + unit * (PAGE * D) + (base + lane / VPR) * D + 8 * (lane % VPR));
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
           const int o = i * RPI + lane / VPR;
-          u32x2 *at = reinterpret_cast<u32x2 *>(p.kc + unit * (PAGE * D) + (base + o) * D + 8 * (lane % VPR));
           u32x2 c;
-          if (o >= lo && o < hi && news) {
+          if (news && o >= lo && o < hi) {
+            float x[8];
+            uint32_t q[8];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              int q[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t word = kr[i][2 * j + (e >> 1)];
-                q[e] = kv_code(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), scale, fine);
-              }
-              c[j] = pack4(q[0], q[1], q[2], q[3]);
+            for (int j = 0; j < 4; ++j) {
+              x[2 * j] = __uint_as_float(kr[i][j] << 16);
+              x[2 * j + 1] = __uint_as_float(kr[i][j] & 0xffff0000u);
             }
-            *at = c;
-          } else if (o < lo && again) {
-            c = *at;
+            kv_codes(x, div, inv, tiny, q);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) c[j] = fine ? pack4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]) : 0u;
+            at[i * (RPI * D / 8)] = c;
+          } else if (again && o < lo) {
+            c = at[i * (RPI * D / 8)];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              c[j] = pack4(kv_recode(byte_of(c[j], 0), ratio, fine), kv_recode(byte_of(c[j], 1), ratio, fine),
-                           kv_recode(byte_of(c[j], 2), ratio, fine), kv_recode(byte_of(c[j], 3), ratio, fine));
-            *at = c;
+              c[j] = pack4(kv_recode(byte_of(c[j], 0), ratio), kv_recode(byte_of(c[j], 1), ratio),
+                           kv_recode(byte_of(c[j], 2), ratio), kv_recode(byte_of(c[j], 3), ratio));
+            at[i * (RPI * D / 8)] = c;
           }
         }
       }
     } else if (news || again) {
-      const bool whole = lo == 0 && hi == 16 && news;
+      auto below = [](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; };
+      uint32_t fresh[4];  // bytes of the new tokens
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fresh[j] = below(hi - 4 * j) & ~below(lo - 4 * j);
 #pragma unroll
       for (int dd = 0; dd < DPL; ++dd) {
-        u32x4 *at = reinterpret_cast<u32x4 *>(p.vc + unit * (PAGE * D) + (DPL * lane + dd) * PAGE + base);
         u32x4 c = u32x4{0u, 0u, 0u, 0u};
-        if (!whole) c = *at;  // the other tokens' bytes stay
+        if (!whole) {
+          c = vc[dd];
+          if (again) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t word = 0;
+            for (int j = 0; j < 4; ++j) {
+              uint32_t word = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int o = 4 * j + e;
-            int q = byte_of(c[j], e);
-            if (news && o >= lo && o < hi) q = kv_code(__uint_as_float(dd ? vr[o] & 0xffff0000u : vr[o] << 16), scale, fine);
-            else if (again && o < lo) q = kv_recode(q, ratio, fine);
-            word |= (static_cast<uint32_t>(q) & 0xffu) << (8 * e);
+              for (int e = 0; e < 4; ++e) {
+                const int q = byte_of(c[j], e);
+                word |= (static_cast<uint32_t>(4 * j + e < lo ? kv_recode(q, ratio) : q) & 0xffu) << (8 * e);
+              }
+              c[j] = word;
+            }
           }
-          c[j] = word;
         }
-        *at = c;
+        if (news) {
+          float x[16];
+          uint32_t q[16];
+#pragma unroll
+          for (int o = 0; o < 16; ++o) x[o] = __uint_as_float(dd ? vr[o] & 0xffff0000u : vr[o] << 16);
+          kv_codes(x, div, inv, tiny, q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t word = fine ? pack4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]) : 0u;
+            c[j] = whole ? word : (c[j] & ~fresh[j]) | (word & fresh[j]);
+          }
+        }
+        v_at[dd * (PAGE / 16)] = c;
       }
     }
     if (part == 0 && lane == 0) *scale_at = scale;
@@ -340,7 +379,7 @@ __global__ __launch_bounds__(64 * (WPP > 4 ? WPP : 4)) void kv_write(KvWriteArgs
 
 template <int D>
 static void launch_kv_write(const KvWriteArgs &p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(cdiv(p.tokens, p.chunk)), static_cast<unsigned>(p.heads), 2);
+  const dim3 grid(static_cast<unsigned>(cdiv(p.tokens, 64) * p.share), static_cast<unsigned>(p.heads), 2);
   switch (p.shift) {
     case 4: hipLaunchKernelGGL((kv_write<D, 1>), grid, dim3(256), 0, s, p); break;
     case 5: hipLaunchKernelGGL((kv_write<D, 2>), grid, dim3(256), 0, s, p); break;
@@ -370,8 +409,8 @@ teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_len
   TEENY_REQUIRE(batch <= kPlanMost, TEENY_ERR_SHAPE_MISMATCH, "kv_cache_plan: more than 4096 requests");
   const int shift = kv_page_shift(page_size);
   TEENY_REQUIRE(shift > 0, TEENY_ERR_UNSUPPORTED, "kv_cache_plan: page_size must be 16, 32, 64 or 128");
-  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && max_pages <= 0x7fffffff / page_size && n_tokens <= 0x7fffffff,
-                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_plan: slots, a row's tokens or the step's tokens exceed 2^31-1");
+  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && max_pages <= 0x7fffffff / page_size && n_tokens <= 1 << 30,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_plan: slots or a row's tokens exceed 2^31-1, or the step's tokens 2^30");
   TEENY_REQUIRE(q_starts != nullptr && free_count != nullptr && free_after != nullptr, TEENY_ERR_NULL_POINTER,
                 "kv_cache_plan: q_starts/free_count/free_after");
   TEENY_REQUIRE(batch == 0 || (new_lens != nullptr && seq_lens != nullptr && context_lens != nullptr && granted != nullptr),
@@ -411,8 +450,9 @@ teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *s
   TEENY_REQUIRE(head_dim == 64 || head_dim == 128, TEENY_ERR_UNSUPPORTED, "kv_cache_write: head_dim must be 64 or 128");
   const int shift = kv_page_shift(page_size);
   TEENY_REQUIRE(shift > 0, TEENY_ERR_UNSUPPORTED, "kv_cache_write: page_size must be 16, 32, 64 or 128");
-  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && n_tokens <= 0x7fffffff && kv_heads <= 65535,
-                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_write: slots or tokens exceed 2^31-1, or kv_heads 65535");
+  // (a launch has less than 2^32 threads: 2^27 / 64 * 2 workgroups of 512 at most)
+  TEENY_REQUIRE(num_pages <= 0x7fffffff / page_size && n_tokens <= 1 << 27 && kv_heads <= 65535,
+                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_write: slots exceed 2^31-1, tokens 2^27 or kv_heads 65535");
   if (n_tokens == 0 || kv_heads == 0 || num_pages == 0) return TEENY_OK;
   TEENY_REQUIRE(k != nullptr && v != nullptr && slots != nullptr && k_cache != nullptr && v_cache != nullptr &&
                     k_scale != nullptr && v_scale != nullptr,
@@ -425,8 +465,12 @@ teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *s
   hipStream_t s = static_cast<hipStream_t>(stream);
   KvWriteArgs p{static_cast<const bf16 *>(k), static_cast<const bf16 *>(v), k_stride, v_stride, slots, k_cache, v_cache,
                 k_scale, v_scale, static_cast<int>(n_tokens), static_cast<int>(kv_heads), static_cast<int>(num_pages),
-                shift, 4};
-  p.chunk = n_tokens <= 1024 ? 4 : 16;
+                shift,
+                // 64 tokens are between one page and 64 of them, which only the device knows.  8 heads of 128, us with
+                // 1 / 2 / 4 / 8 / 16 workgroups: 5 prompts of 1600 tokens 15.6 / 14.6 / 16.4 / 19.5 / 25.8, one of 500
+                // 6.5 / 5.4 / 5.3 / 6.2 / 6.8; single tokens of 64 requests (pages of 16) 34 / 18 / 10.4 / 6.3 / 5.7, of
+                // 500 36 / 20 / 12.8 / 10.0 / 10.1, of 2000 (heads of 64) 36 / 25 / 24 / 23 / 24
+                n_tokens <= 256 ? 16 : n_tokens <= 1024 ? 8 : 2};
   if (head_dim == 64) launch_kv_write<64>(p, s);
   else launch_kv_write<128>(p, s);
   return after_launch(nm, s);

@@ -183,6 +183,20 @@ def test_write_special_values(dev, page):
     assert np.isfinite(again[2][last]).all() and np.isfinite(again[3][last]).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_write_over_all_exponents(dev, d):
+    """Codes are rint of the fp32 quotient exactly: pages of every magnitude that bf16 has, and quotients at a half."""
+    rng = np.random.default_rng(d)
+    exps = np.arange(-133, 128)  # 2^-133: the smallest bf16 number
+    x, slots, *cache = write_case(rng, [0] * len(exps), [7] * len(exps), 1, d, 16)
+    for n in "kv":
+        m = np.ldexp(rng.uniform(-1, 1, x[n].shape), np.repeat(exps, 7)[:, None, None])
+        m[3::7] = np.sign(m[3::7]) * np.ldexp((rng.integers(0, 127, m[3::7].shape) + 0.5) / 127, np.repeat(exps, 1)[:, None, None])
+        m[0::7, 0, 0] = np.ldexp(1.0, exps)  # the largest: the half steps above are halves of its scale
+        x[n] = from_bf16(to_bf16(m.astype(np.float32)))
+    check_write(dev, x, slots, *cache)
+
+
 def test_write_token_strides(dev):
     """K and V as parts of one projection's rows: strides over the C entry point."""
     rng = np.random.default_rng(9)

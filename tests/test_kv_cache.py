@@ -32,7 +32,7 @@ def plan_args(**kw):
     (dict(batch=4097), _lib.ERR_SHAPE_MISMATCH), (dict(page_size=0), _lib.ERR_UNSUPPORTED),
     (dict(page_size=24), _lib.ERR_UNSUPPORTED), (dict(page_size=256), _lib.ERR_UNSUPPORTED),
     (dict(num_pages=BIG // 16), _lib.ERR_SHAPE_MISMATCH), (dict(max_pages=BIG // 16), _lib.ERR_SHAPE_MISMATCH),
-    (dict(n_tokens=BIG), _lib.ERR_SHAPE_MISMATCH),
+    (dict(n_tokens=BIG), _lib.ERR_SHAPE_MISMATCH), (dict(n_tokens=(1 << 30) + 1), _lib.ERR_SHAPE_MISMATCH),
     *[(dict([(n, None)]), _lib.ERR_NULL_POINTER) for n in (
         "new_lens", "seq_lens", "block_table", "free_list", "free_count", "q_starts", "slots", "positions",
         "context_lens", "granted", "free_after")]])
@@ -52,7 +52,8 @@ def write_args(**kw):
     (dict(num_pages=-1), _lib.ERR_SHAPE_MISMATCH), (dict(head_dim=96), _lib.ERR_UNSUPPORTED),
     (dict(head_dim=0), _lib.ERR_UNSUPPORTED), (dict(page_size=8), _lib.ERR_UNSUPPORTED),
     (dict(num_pages=BIG // 16), _lib.ERR_SHAPE_MISMATCH), (dict(kv_heads=65536, k_stride=1 << 24, v_stride=1 << 24), _lib.ERR_SHAPE_MISMATCH),
-    (dict(n_tokens=BIG), _lib.ERR_SHAPE_MISMATCH), (dict(k_stride=255), _lib.ERR_SHAPE_MISMATCH),
+    (dict(n_tokens=BIG), _lib.ERR_SHAPE_MISMATCH), (dict(n_tokens=(1 << 27) + 1), _lib.ERR_SHAPE_MISMATCH),
+    (dict(k_stride=255), _lib.ERR_SHAPE_MISMATCH),
     (dict(v_stride=128), _lib.ERR_SHAPE_MISMATCH), (dict(k_stride=260), _lib.ERR_MISALIGNED),
     (dict(v_stride=257), _lib.ERR_MISALIGNED), (dict(k=FAKE_ODD), _lib.ERR_MISALIGNED),
     (dict(v=FAKE_ODD), _lib.ERR_MISALIGNED), (dict(k_cache=FAKE_ODD), _lib.ERR_MISALIGNED),
