@@ -915,6 +915,14 @@ def _out(like: Buffer, out: Optional[Buffer], shape=None, dtype=None) -> Buffer:
     return Buffer(dtype, shape)
 
 
+def _types(*pairs) -> bool:
+    """Whether each buffer (or None) has its dtype: nearly always the very object, which needs no comparison."""
+    for buf, dtype in pairs:
+        if buf is not None and buf.dtype is not dtype and buf.dtype != dtype:
+            return False
+    return True
+
+
 # Shape rules of each entry point, as pure functions of buffer shapes (so the
 # rules are testable without a device).  Every wrapper below checks its
 # buffers with these before calling the C ABI, which cannot see allocation
@@ -1374,19 +1382,29 @@ def attention_backward_workspace_size(batch: int, q_heads: int, n_ctx_q: int) ->
 def kv_cache_dims(k_cache_shape, v_cache_shape, k_scale_shape, v_scale_shape) -> Tuple[int, int, int, int]:
     """-> (pages, kv_heads, page_size, head_dim) of a cache: K [pages, kv_heads, page_size, head_dim], V
     [pages, kv_heads, head_dim, page_size], scales [pages, kv_heads]."""
-    _need(len(k_cache_shape) == 4 and len(v_cache_shape) == 4, "kv_cache: k_cache and v_cache must be 4-D")
+    if not len(k_cache_shape) == len(v_cache_shape) == 4:
+        raise ValueError("kv_cache: k_cache and v_cache must be 4-D")
     pages, heads, size, d = k_cache_shape
-    if tuple(v_cache_shape) != (pages, heads, d, size):
+    if v_cache_shape != (pages, heads, d, size):
         raise ValueError(f"kv_cache: v_cache must be {[pages, heads, d, size]}, is {list(v_cache_shape)}")
-    if tuple(k_scale_shape) != (pages, heads) or tuple(v_scale_shape) != (pages, heads):
+    if not k_scale_shape == v_scale_shape == (pages, heads):
         raise ValueError(f"kv_cache: scales must be {[pages, heads]}")
     return pages, heads, size, d
 
 
 def _need_cache(k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer):
-    _need(k_cache.dtype == i8 and v_cache.dtype == i8 and k_scale.dtype == f32 and v_scale.dtype == f32,
-          "kv_cache: codes int8, scales fp32")
+    if not _types((k_cache, i8), (v_cache, i8), (k_scale, f32), (v_scale, f32)):
+        raise ValueError("kv_cache: codes int8, scales fp32")
     return kv_cache_dims(k_cache.shape, v_cache.shape, k_scale.shape, v_scale.shape)
+
+
+def _ints(buf: Optional[Buffer], n: int, what: str) -> Buffer:
+    """An int32 buffer of n elements: `buf`, checked, or a new one."""
+    if buf is None:
+        return Buffer(i32, (n,))
+    if buf.numel != n or (buf.dtype is not i32 and buf.dtype != i32):
+        raise ValueError(f"kv_cache: {what} must be int32 with {n} elements, is {buf.dtype.name} with {buf.numel}")
+    return buf
 
 
 def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_list: Buffer, free_count: Buffer,
@@ -1400,17 +1418,17 @@ def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_
     `slots` given: as many as it has).  context_lens=seq_lens, granted=new_lens and free_after=free_count update in
     place.  A request that does not fit is refused as a whole: granted 0, slots -1."""
     b = new_lens.numel
-    _need(len(block_table.shape) == 2 and block_table.shape[0] == b and seq_lens.numel == b,
-          "kv_cache_plan: new_lens and seq_lens [batch], block_table [batch, max_pages]")
-    _need(free_count.numel == 1, "kv_cache_plan: free_count has one element")
-    _need(all(t.dtype == i32 for t in (new_lens, seq_lens, block_table, free_list, free_count)),
-          "kv_cache_plan: int32 buffers")
+    if len(block_table.shape) != 2 or block_table.shape[0] != b or block_table.dtype != i32:
+        raise ValueError(f"kv_cache_plan: block_table must be int32 [{b}, max_pages]")
+    if not (seq_lens.numel == b and free_count.numel == 1 and
+            _types((new_lens, i32), (seq_lens, i32), (free_list, i32), (free_count, i32))):
+        raise ValueError(f"kv_cache_plan: new_lens and seq_lens [{b}], free_list and free_count [1], int32")
     _need(slots is not None or n_tokens is not None, "kv_cache_plan: n_tokens or slots")
     t = slots.numel if n_tokens is None else int(n_tokens)
-    slots, positions = _out(new_lens, slots, (t,)), _out(new_lens, positions, (t,))
-    q_starts = _out(new_lens, q_starts, (b + 1,))
-    context_lens, granted = _out(new_lens, context_lens, (b,)), _out(new_lens, granted, (b,))
-    free_after = _out(new_lens, free_after, (1,))
+    slots, positions = _ints(slots, t, "slots"), _ints(positions, t, "positions")
+    q_starts = _ints(q_starts, b + 1, "q_starts")
+    context_lens, granted = _ints(context_lens, b, "context_lens"), _ints(granted, b, "granted")
+    free_after = _ints(free_after, 1, "free_after")
     check(lib.teeny_kv_cache_plan(new_lens.ptr, seq_lens.ptr, block_table.ptr, free_list.ptr, free_count.ptr,
                                   q_starts.ptr, slots.ptr, positions.ptr, context_lens.ptr, granted.ptr, free_after.ptr,
                                   b, block_table.shape[1], free_list.numel, page_size, t, _h(stream)))
@@ -1423,9 +1441,10 @@ def kv_cache_write(k: Buffer, v: Buffer, slots: Buffer, k_cache: Buffer, v_cache
     pages' codes and scales are updated in place; a page's new tokens are consecutive rows and slots."""
     pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
     t = slots.numel
-    if not (tuple(k.shape) == (t, heads, d) and tuple(v.shape) == (t, heads, d)):
+    if not k.shape == v.shape == (t, heads, d):
         raise ValueError(f"kv_cache_write: k and v must be {[t, heads, d]}")
-    _need(k.dtype == bf16 and v.dtype == bf16 and slots.dtype == i32, "kv_cache_write: k/v bf16, slots int32")
+    if not _types((k, bf16), (v, bf16), (slots, i32)):
+        raise ValueError("kv_cache_write: k/v bf16, slots int32")
     check(lib.teeny_kv_cache_write(k.ptr, v.ptr, slots.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, t, heads,
                                    d, pages, size, heads * d, heads * d, _h(stream)))
 
@@ -1439,21 +1458,25 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     q_starts[b] .. q_starts[b + 1] - 1 (None: one each), the last of its context_lens[b] tokens.  max_q_len and
     max_context (host numbers; default: as much as the buffers allow) choose how the work is cut, not the result."""
     pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
-    _need(len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16, "kv_cache_attention: q bf16 [n_tokens, q_heads, D]")
+    if not (len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16):
+        raise ValueError("kv_cache_attention: q bf16 [n_tokens, q_heads, head_dim]")
     t, hq, _ = q.shape
     b = context_lens.numel
-    _need(heads > 0 and hq % heads == 0, "kv_cache_attention: q_heads % kv_heads != 0")
-    _need(len(block_table.shape) == 2 and block_table.shape[0] == b, "kv_cache_attention: block_table [batch, max_pages]")
-    if not (t == b if q_starts is None else q_starts.numel == b + 1):
-        raise ValueError(f"kv_cache_attention: q_starts [{b + 1}], or one query for each of the {b} sequences")
-    _need(block_table.dtype == i32 and context_lens.dtype == i32 and (q_starts is None or q_starts.dtype == i32),
-          "kv_cache_attention: block_table, context_lens and q_starts are int32")
-    _need(lse is None or (lse.numel == t * hq and lse.dtype == f32), "kv_cache_attention: lse fp32 [n_tokens, q_heads]")
+    if heads == 0 or hq % heads:
+        raise ValueError("kv_cache_attention: q_heads % kv_heads != 0")
+    if not (len(block_table.shape) == 2 and block_table.shape[0] == b and _types((block_table, i32), (context_lens, i32))):
+        raise ValueError(f"kv_cache_attention: block_table [{b}, max_pages] and context_lens [{b}], int32")
+    if q_starts is not None:
+        _ints(q_starts, b + 1, "q_starts")
+    elif t != b:
+        raise ValueError(f"kv_cache_attention: q_starts, or one query for each of the {b} sequences")
+    if not (lse is None or (lse.numel == t * hq and lse.dtype == f32)):
+        raise ValueError("kv_cache_attention: lse fp32 [n_tokens, q_heads]")
     if max_q_len is None:
         max_q_len = 1 if q_starts is None else t
     if max_context is None:
         max_context = block_table.shape[1] * size
-    scale = 1.0 / math.sqrt(d) if softmax_scale is None else softmax_scale
+    scale = d ** -0.5 if softmax_scale is None else softmax_scale
     o = _out(q, o)
     check(lib.teeny_kv_cache_attention(q.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, block_table.ptr,
                                        context_lens.ptr, q_starts.ptr if q_starts is not None else None, o.ptr,
@@ -1600,9 +1623,8 @@ def w4a16_linear(x: Buffer, qweight: Buffer, scale: Buffer, group_size: int, zer
     "group", axis=1, group_size=group_size, bits=4)`` gives them, bias fp32 [N]."""
     m, n, k = w4a16_dims(x.shape, qweight.shape, scale.shape, group_size,
                          zero_point.shape if zero_point is not None else None, bias.shape if bias is not None else None)
-    _need(x.dtype == bf16 and qweight.dtype == i8 and scale.dtype == f32 and (bias is None or bias.dtype == f32) and
-          (zero_point is None or zero_point.dtype == i32),
-          "w4a16_linear: x bf16, qweight int8, scale/bias fp32, zero_point int32")
+    if not _types((x, bf16), (qweight, i8), (scale, f32), (bias, f32), (zero_point, i32)):
+        raise ValueError("w4a16_linear: x bf16, qweight int8, scale/bias fp32, zero_point int32")
     y = _out(x, y, (m, n), bf16)
     check(lib.teeny_w4a16_linear_forward(x.ptr, qweight.ptr, scale.ptr,
                                          zero_point.ptr if zero_point is not None else None,
