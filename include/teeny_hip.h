@@ -543,8 +543,8 @@ teeny_status teeny_attention_backward_workspace_size(int64_t batch, int64_t q_he
  *   free_after [1]        free pages left
  * context_lens may be seq_lens, granted may be new_lens and free_after may be
  * free_count: the plan then updates them in place (with a second launch where
- * n_tokens is over 256).  At most 4096 requests and 2^30 rows.  The request
- * order alone decides every result. */
+ * n_tokens is over 256, or 1024 for more than 256 requests).  At most 4096
+ * requests and 2^30 rows.  The request order alone decides every result. */
 teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_lens, int32_t *block_table,
                                  int32_t *free_list, const int32_t *free_count, int32_t *q_starts, int32_t *slots,
                                  int32_t *positions, int32_t *context_lens, int32_t *granted, int32_t *free_after,
