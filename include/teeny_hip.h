@@ -580,7 +580,8 @@ teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *s
  * (queries and tokens of the longest sequence) choose how the work is cut;
  * longer sequences are computed all the same.  With a stream workspace of
  * teeny_kv_cache_attention_workspace_size bytes a sequence's tokens are shared
- * out over the device.  head_dim 64 or 128; 16-byte aligned tensors. */
+ * out over the device.  head_dim 64 or 128; 16-byte aligned tensors; num_pages *
+ * kv_heads below 2^29, (n_tokens * q_heads + 128 * batch * kv_heads) below 2^25. */
 teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scale,
                                       const float *v_scale, const int32_t *block_table, const int32_t *context_lens,
                                       const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,

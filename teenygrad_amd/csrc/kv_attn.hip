@@ -702,7 +702,7 @@ struct KvAttnPlan {
   int nq = 1, rb = 16;
   int64_t blocks = 0;
   int splits = 1, chunk = 0;
-  size_t bytes = 0;
+  size_t bytes = 0, most = 0;  // of workspace: used; enough for this and any smaller max_context
 };
 
 static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
@@ -720,10 +720,14 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   if (!pl.tile || busy < 2 * cus) splits = std::max(splits, max_ctx / 2560);
   splits = std::max<int64_t>(1, splits);
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
-  if (size(splits) > scratch) splits = 1;
-  pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), splits), step) * step);
-  pl.splits = static_cast<int>(cdiv(std::max<int64_t>(max_ctx, 1), pl.chunk));
-  pl.bytes = size(pl.splits);
+  auto cut = [&](int64_t n) {
+    pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), n), step) * step);
+    pl.splits = static_cast<int>(cdiv(std::max<int64_t>(max_ctx, 1), pl.chunk));
+    pl.bytes = size(pl.splits);
+  };
+  cut(splits);
+  pl.most = size(splits);
+  if (pl.bytes > scratch) cut(1);
   return pl;
 }
 
@@ -845,7 +849,7 @@ teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t b
   teeny_status st = kv_attn_sizes(nm, n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context);
   if (st != TEENY_OK) return st;
   if (n_tokens == 0 || batch == 0 || q_heads == 0) return TEENY_OK;
-  *bytes = kv_attn_plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, SIZE_MAX).bytes;
+  *bytes = kv_attn_plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, SIZE_MAX).most;
   return TEENY_OK;
 }
 

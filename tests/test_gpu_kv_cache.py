@@ -12,7 +12,7 @@ from teenygrad_amd import _lib
 from teenygrad_amd import kernels as K
 from teenygrad_amd._lib import check, lib
 from teenygrad_amd.dtypes import bf16, from_bf16, to_bf16
-from teenygrad_amd.runtime import Stream
+from teenygrad_amd.runtime import NULL_STREAM, Stream
 
 pytestmark = pytest.mark.gpu
 
@@ -285,6 +285,53 @@ def test_attention_splits(dev, ctx, new, hq, hkv, causal):
             check_attn(c, run_attn(dev, c, causal=causal, hint=hint), causal=causal)
         with stream_workspace(dev, 1024):  # too small: none is used
             check_attn(c, run_attn(dev, c, causal=causal, hint=hint), causal=causal)
+
+
+@pytest.mark.parametrize("ctx,new", [(2000, 1), (2000, 7), (4500, 40)])
+def test_attention_workspace_size(dev, ctx, new):
+    """The size that is asked for is enough: the results are those of any larger workspace."""
+    c = attn_case(np.random.default_rng(ctx + new), [ctx], [new], 8, 2, 64, 16)
+    c["table"] = c["table"][:, :kv.pages_of(ctx, 16)]
+    size = K.kv_cache_attention_workspace_size(new, 1, 8, 2, 64, new, 1 << 15)
+    assert 0 < size < 32 << 20
+    got = []
+    for n, hint in ((K.kv_cache_attention_workspace_size(new, 1, 8, 2, 64, new, ctx), ctx), (size, 1 << 15), (64 << 20, 1 << 15)):
+        ws = dev.upload(np.full(n, 77, np.int8))
+        NULL_STREAM.set_workspace(ws)
+        try:
+            got.append(run_attn(dev, c, hint=(new, hint)))
+        finally:
+            NULL_STREAM.set_workspace(None)
+        assert (ws.to_host() != 77).any()  # it was used
+    for o, lse in got[1:]:
+        np.testing.assert_array_equal(o, got[0][0])
+        np.testing.assert_array_equal(lse, got[0][1])
+    check_attn(c, got[0])
+
+
+@pytest.mark.parametrize("new", [1, 5, 20])
+def test_attention_of_many_sequences(dev, new):
+    """More sequences than lanes: one, a few and many query rows, some sequences without any, with and without splits."""
+    rng = np.random.default_rng(70 + new)
+    lens = rng.integers(0, 200, 150)
+    lens[[3, 77, 149]] = 1500, 0, 2000
+    c = attn_case(rng, [int(n) for n in lens], [int(n) for n in rng.integers(new == 1, new + 1, 150)], 8, 2, 64, 16)
+    t, hint = int(c["starts"][-1]), (new, 2000)
+    check_attn(c, run_attn(dev, c, hint=hint, pad=2))
+    with stream_workspace(dev, K.kv_cache_attention_workspace_size(t + 2, 150, 8, 2, 64, *hint)):
+        check_attn(c, run_attn(dev, c, hint=hint, pad=2))
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_attention_rows_of_no_sequence(dev, new):
+    """Rows before the first sequence stay as they were, as those past the last one do."""
+    rng = np.random.default_rng(new)
+    c = attn_case(rng, [70, 200], [new, new], 8, 2, 128, 32)
+    before = 5
+    moved = dict(c, starts=c["starts"] + before, q=np.concatenate([np.ones((before, 8, 128), np.float32), c["q"]]))
+    o, lse = run_attn(dev, moved, hint=(new, 200), pad=1)
+    assert (o[:before] == 123.0).all() and (lse[:before] == 55.0).all()
+    check_attn(c, (o[before:], lse[before:]))
 
 
 def test_attention_not_causal(dev):
