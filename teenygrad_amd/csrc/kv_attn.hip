@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256, NQ == 1 && D == 64 ? 4 : 2) void kv_attn(KvAtt
   for (int n = 0; n < NQ; ++n) l_run[n] = over_groups(l_run[n], [](float a, float b) { return a + b; });
 
   // the waves' parts: a common max, then the sum of their outputs in wave order
-  const bool whole = p.part == nullptr;
+  const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
   const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB;  // part rows of this (unit, split)
   if (g == 0) {
 #pragma unroll
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   }
   l_run += __shfl_xor(l_run, 32, 64);
   if (base + c >= r.rows) return;
-  const bool whole = p.part == nullptr;
+  const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
   // (the block's own number, not its place in the order)
   const int block = head * p.blocks + static_cast<int>(static_cast<int64_t>(r.first) * p.group / RB) + r.b + r.row0 / RB;
   const int64_t slot = (static_cast<int64_t>(block) * p.splits + split) * RB + 32 * w + c;
@@ -662,7 +662,8 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
   const int i = (t - first) * p.group + h - head * p.group, len = end - first;
   const int last = min(i / RB * RB + RB, len * p.group) - 1;
   const int k_end = p.causal ? min(max(ctx - len + 1 + last / p.group, 0), ctx) : ctx;
-  const int n = min(p.splits, max(1, (k_end - 1) / p.chunk + 1));
+  if (k_end <= p.chunk) return;  // the one split that saw the row wrote its output
+  const int n = min(p.splits, (k_end - 1) / p.chunk + 1);
   const int unit = head * p.blocks + static_cast<int>(static_cast<int64_t>(first) * p.group / RB) + b + i / RB;
   const int64_t slot = static_cast<int64_t>(unit) * p.splits * RB + i % RB;
   const float *ml = p.part + p.ml_off;
