@@ -37,43 +37,48 @@ struct KvAttnArgs {
   float *part;      // [unit][split][row][D] fp32, then (at ml_off) [unit][split][row][2]; null: one split
   int64_t ml_off;
   int batch, tokens, heads, kv_heads, group, pages, shift, width;
-  int blocks;       // row blocks of a head, over all sequences
+  int blocks;       // row blocks of a head, over all sequences, at most
+  int walk;         // of these, as many as the caller's lengths stand for
   int splits, chunk;  // chunk: tokens per split (a multiple of a workgroup's round)
   float scale_log2;
   int causal;
 };
 
-// A head's row block: sequence b has blocks floor(q_starts[b] group / RB) + b
-// on, at least as many as its rows need (whatever the lengths, at most
-// tokens group / RB + batch over all).
+// A head's row block.  Its number, and so its place in the workspace, is
+// floor(q_starts[b] group / RB) + b + its place in sequence b: distinct, and below
+// tokens group / RB + batch, whatever the lengths.
 struct KvRows {
   int b, row0, rows, len, first, ctx;  // rows: of the sequence and head; len: its queries; first: its first token's row
+  template <int RB>
+  __device__ __forceinline__ int number(const KvAttnArgs &p) const {
+    return static_cast<int>(static_cast<int64_t>(first) * p.group / RB) + b + row0 / RB;
+  }
 };
 
+// The u-th block that there is, in the order of the sequences.
 template <int RB>
-__device__ __forceinline__ bool kv_rows(const KvAttnArgs &p, int u, KvRows &r) {
+__device__ __forceinline__ bool kv_rows(const KvAttnArgs &p, uint32_t u, KvRows &r) {
   const int lane = threadIdx.x & 63;
   auto start = [&](int i) { return min(max(p.starts ? p.starts[i] : i, 0), p.tokens); };
-  int found = -1, first = 0, end = 0, ctx = 0;  // of the last sequence whose blocks begin at or before u
+  uint32_t before = 0;
   for (int i = 0; i < p.batch; i += 64) {
-    const int b = min(i + lane, p.batch - 1), s0 = start(b), s1 = start(b + 1), n = p.ctx[b];
-    const int block = static_cast<int>(static_cast<int64_t>(s0) * p.group / RB) + b;
-    const uint64_t m = __ballot(i + lane < p.batch && block <= u);
-    if (m == 0) break;
-    const int at = 63 - __builtin_clzll(m);
-    found = i + at;
-    first = __builtin_amdgcn_readlane(s0, at);
-    end = __builtin_amdgcn_readlane(s1, at);
-    ctx = __builtin_amdgcn_readlane(n, at);
+    const int b = min(i + lane, p.batch - 1), first = start(b), len = start(b + 1) - first, ctx = p.ctx[b];
+    const uint32_t nb = i + lane < p.batch && len > 0 ? (len * p.group + RB - 1) / RB : 0, upto = wave_scan(nb);
+    const uint32_t here = __builtin_amdgcn_readlane(upto, 63);
+    if (u - before < here) {
+      const int at = __builtin_ctzll(__ballot(upto > u - before));
+      auto from = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      r.b = i + at;
+      r.first = from(first);
+      r.len = from(len);
+      r.rows = r.len * p.group;
+      r.row0 = static_cast<int>(u - before - from(upto - nb)) * RB;
+      r.ctx = min(max(from(ctx), 0), p.width << p.shift);
+      return true;
+    }
+    before += here;
   }
-  if (found < 0) return false;
-  r.b = found;
-  r.first = first;
-  r.len = end - first;
-  r.rows = r.len * p.group;
-  r.row0 = (u - static_cast<int>(static_cast<int64_t>(first) * p.group / RB) - found) * RB;
-  r.ctx = min(max(ctx, 0), p.width << p.shift);
-  return r.len > 0 && r.row0 < r.rows;
+  return false;
 }
 
 // The same blocks in order of their work, the longest first, for up to 64
@@ -155,11 +160,13 @@ __global__ __launch_bounds__(256, NQ == 1 && D == 64 ? 4 : 2) void kv_attn(KvAtt
   __shared__ __attribute__((aligned(16))) float red[WK * WROWS * LD];
   __shared__ float ml[2][WK][WROWS];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
-  const int split = in_head / p.blocks, u = in_head - split * p.blocks, unit = head * p.blocks + u;
+  // the blocks that the caller's lengths stand for come first, then those that there may be beyond, mostly none
+  const int per_block = p.splits * p.kv_heads, first = p.walk * per_block;
+  const bool beyond = static_cast<int>(blockIdx.x) >= first;
+  const int id = beyond ? blockIdx.x - first : xcd_remap(blockIdx.x, first), of = beyond ? p.blocks - p.walk : p.walk;
+  const int head = id / (p.splits * of), in_head = id - head * (p.splits * of), split = in_head / of;
   KvRows r;
-  if (!kv_rows<RB>(p, u, r)) return;
+  if (!kv_rows<RB>(p, in_head - split * of + (beyond ? p.walk : 0), r)) return;
   // row i of the sequence: query i / group, head i % group of the K/V head's; it sees seen(i) tokens
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
   const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
@@ -318,7 +325,8 @@ __global__ __launch_bounds__(256, NQ == 1 && D == 64 ? 4 : 2) void kv_attn(KvAtt
 
   // the waves' parts: a common max, then the sum of their outputs in wave order
   const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
-  const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * RB;  // part rows of this (unit, split)
+  const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
+  const int64_t slot = (unit * p.splits + split) * RB;  // part rows of this (unit, split)
   if (g == 0) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -385,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
-  const int split = in_head / p.blocks, u = in_head - split * p.blocks, unit = head * p.blocks + u;
+  const int split = in_head / p.blocks, u = in_head - split * p.blocks;
   KvRows r;
   if (!kv_rows_sorted<RB>(p, u, r)) return;
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
@@ -609,9 +617,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   l_run += __shfl_xor(l_run, 32, 64);
   if (base + c >= r.rows) return;
   const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
-  // (the block's own number, not its place in the order)
-  const int block = head * p.blocks + static_cast<int>(static_cast<int64_t>(r.first) * p.group / RB) + r.b + r.row0 / RB;
-  const int64_t slot = (static_cast<int64_t>(block) * p.splits + split) * RB + 32 * w + c;
+  const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
+  const int64_t slot = (unit * p.splits + split) * RB + 32 * w + c;
   const float mul = whole ? (l_run == 0.0f ? 0.0f : 1.0f / l_run) : 1.0f;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -673,12 +680,23 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   fv o = {};
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const int64_t at = slot + static_cast<int64_t>(s) * RB;
-    const float f = __builtin_amdgcn_exp2f(ml[at * 2] - ref);
-    l += ml[at * 2 + 1] * f;
-    o += *reinterpret_cast<const fv *>(p.part + at * D + lane * V) * f;
+  for (int s0 = 0; s0 < n; s0 += 64) {  // a lane's factor is of split s0 + lane
+    float f = 0.0f, ls = 0.0f;
+    if (s0 + lane < n) {
+      const float *of = ml + (slot + static_cast<int64_t>(s0 + lane) * RB) * 2;
+      f = __builtin_amdgcn_exp2f(of[0] - ref);
+      ls = of[1] * f;
+    }
+    l += wave_sum(ls);
+    const int here = min(n - s0, 64);
+    const float *at = p.part + (slot + static_cast<int64_t>(s0) * RB) * D + lane * V;
+    for (int s = 0; s < here; s += 8) {  // eight loads in flight; past the last split its part again, times 0
+      fv x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const fv *>(at + static_cast<int64_t>(min(s + j, here - 1)) * (RB * D));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o += x[j] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + j));
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -687,21 +705,24 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
 }
 
 // ── which form, and how many splits ─────────────────────────────────────────
-// Few rows take kv_attn, more than 64 a sequence the shared tiles.  Splits fill
-// the device with two workgroups to a CU, of 256 tokens each at least (512 where
-// there are many: a second launch, 2 us, and a workgroup's start and end, 4 us,
-// which no other work hides), and cut contexts that may differ much in length.
-// us by splits: 16 x 4000 tokens, 8 K/V heads of 128, one query, 1 / 2 / 4 / 6 / 8
-// 48 / 44 / 35 / 38 / 39; 1 x 16000 1 / 8 / 16 / 32 145 / 28 / 20 / 19; 64 x 2048 1
-// / 2 / 3 56 / 63 / 66; 64 x 90 to 8000 1 / 2 / 3 / 4 / 8 132 / 130 / 119 / 127 /
-// 132; 24 x 1000 of 64 1 / 2 12 / 14.  Shared tiles: 1 x 64 queries x 16000 1 / 8 /
-// 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads of 64, 1 / 4 / 8 / 16 145 / 49
-// / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242 / 180 / 139 / 160; 4 x 700 x 1100
-// to 4100 1 / 2 162 / 200.
+// Few rows take kv_attn, more than 64 a sequence the shared tiles.  kv_attn's
+// splits give a workgroup one round of 256 tokens where they leave CUs free (a
+// round is 1.9 us of dependent work, a row's other parts 0.04 us each), two rounds
+// where the device is busier, from three rounds on; more workgroups than two to a
+// CU (one where there are few: their parts count) only where contexts may differ
+// much in length.  us by splits, 8 K/V heads of 128, one query: 1 x 600 1 / 3 10.6 /
+// 9.9; 1 x 2000 1 / 4 / 8 20 / 12.5 / 10.7; 1 x 30000 16 / 32 / 64 28 / 21.7 / 23.3;
+// 4 x 2000 4 / 8 13.4 / 12.1; 8 x 1000 1 / 2 / 4 14.4 / 13.7 / 12.3; 8 x 4000 4 / 6 /
+// 8 20.9 / 22.4 / 20.4; 16 x 1000 1 / 2 / 4 14.6 / 15.8 / 15.4; 16 x 4000 2 / 4 / 8 33 /
+// 33 / 36; 32 x 2000 1 / 2 28.8 / 33.3, but 32 x 100 to 8000 1 / 2 / 3 83 / 71 / 65; 64
+// x 90 to 8000 1 / 2 / 3 / 4 116 / 126 / 112 / 117.  Shared tiles: 1 x 64 queries x
+// 16000 1 / 8 / 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads of 64, 1 / 4 / 8 /
+// 16 145 / 49 / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242 / 180 / 139 / 160; 4 x
+// 700 x 1100 to 4100 1 / 2 160 / 193.
 struct KvAttnPlan {
   bool tile = false;
   int nq = 1, rb = 16;
-  int64_t blocks = 0;
+  int64_t blocks = 0, walk = 0;  // row blocks of a head at most; as the lengths have it
   int splits = 1, chunk = 0;
   size_t bytes = 0, most = 0;  // of workspace: used; enough for this and any smaller max_context
 };
@@ -713,12 +734,14 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   if (rows > 64) pl.tile = true, pl.rb = 128;
   else if (rows > 16) pl.nq = 2, pl.rb = 32;
   pl.blocks = tokens * group / pl.rb + batch;
+  pl.walk = std::max<int64_t>(1, std::min(pl.blocks, batch * cdiv(std::max<int64_t>(rows, 1), pl.rb)));
   const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = pl.tile ? 64 : 256;
-  // workgroups with work, unsplit: at most the row blocks of every sequence
-  const int64_t busy = std::max<int64_t>(1, std::min(pl.blocks, batch * cdiv(std::max<int64_t>(rows, 1), pl.rb)) * kv_heads);
-  const int64_t least = pl.tile ? (busy < 32 ? 256 : 768) : busy < 64 ? 256 : 512;
-  int64_t splits = std::min(2 * cus / busy, max_ctx / least);
-  if (!pl.tile || busy < 2 * cus) splits = std::max(splits, max_ctx / 2560);
+  const int64_t busy = pl.walk * kv_heads;  // workgroups with work, unsplit
+  const int64_t least = pl.tile ? (busy < 32 ? 256 : 768) : busy <= 64 ? 256 : 512;
+  int64_t splits = 1;
+  if (pl.tile) splits = std::min(2 * cus / busy, max_ctx / least);
+  else if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
+  if (pl.tile ? busy < 2 * cus : busy >= 32) splits = std::max(splits, max_ctx / 2560);
   splits = std::max<int64_t>(1, splits);
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   auto cut = [&](int64_t n) {
@@ -832,6 +855,7 @@ teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, cons
   p.shift = shift;
   p.width = num_pages > 0 ? static_cast<int>(max_pages) : 0;
   p.blocks = static_cast<int>(pl.blocks);
+  p.walk = static_cast<int>(pl.walk);
   p.splits = pl.splits;
   p.chunk = pl.chunk;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
