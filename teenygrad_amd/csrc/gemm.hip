@@ -308,11 +308,13 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
 }
 
 // Whether a bf16 copy of the weights and the matrix-core tiles are the better
-// way, given room for the copy.  us, streamed / through the copy: 128 x 11008 x
-// 4096 47 / 49, 192 x 11008 x 4096 68 / 61, 192 x 4096 x 4096 31 / 35, 256 x 4096
-// x 4096 41 / 34, 192 x 5504 x 2048 29 / 34, 256 x 5504 x 2048 34 / 34, 512 x 1024
-// x 4096 18 / 24, 512 x 11008 x 4096 166 / 87.
-static bool w4_as_bf16(int64_t M, int64_t N) { return M > 160 && M * N >= (int64_t{1} << 20); }
+// way, given room for the copy.  us, streamed / through the copy: 192 x 11008 x
+// 4096 58 / 63, 256 x 11008 x 4096 72 / 63, 256 x 4096 x 11008 79 / 66, 256 x 4096 x
+// 4096 32 / 37, 384 x 4096 x 4096 43 / 44, 400 x 5504 x 2048 36 / 40, 512 x 5504 x
+// 2048 44 / 40, 512 x 1024 x 4096 18 / 25, 800 x 1024 x 4096 32 / 24.
+static bool w4_as_bf16(int64_t M, int64_t N, int64_t K) {
+  return (M > 160 && static_cast<double>(M) * N * K > 9.2e9) || (M > 448 && M * N >= int64_t{3} << 18);
+}
 static size_t w4_copy_bytes(int64_t N, int64_t K) { return (static_cast<size_t>(N) * K * 2 + 255) / 256 * 256; }
 
 static teeny_status w4_sizes(const char *nm, int64_t M, int64_t N, int64_t K, int64_t group_size) {
@@ -362,7 +364,7 @@ teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, co
            static_cast<int>(std::min<int64_t>(group_size, int64_t{1} << 30)), act};
   const Scratch scr = stream_scratch(s);
   const size_t copy = w4_copy_bytes(N, K);
-  if (w4_as_bf16(M, N) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {
+  if (w4_as_bf16(M, N, K) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {
     bf16 *wb = static_cast<bf16 *>(scr.ptr);
     const int64_t per_row = K / 8, rows = std::max<int64_t>(1, (int64_t{1} << 30) / per_row);
     for (int64_t n0 = 0; n0 < N; n0 += rows) {
@@ -402,7 +404,7 @@ teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, 
   *bytes = 0;
   const teeny_status st = w4_sizes("w4a16_linear_workspace_size", M, N, K, group_size);
   if (st != TEENY_OK) return st;
-  if (M == 0 || N == 0 || K == 0 || !w4_as_bf16(M, N)) return TEENY_OK;
+  if (M == 0 || N == 0 || K == 0 || !w4_as_bf16(M, N, K)) return TEENY_OK;
   const GemmParams p = plain_params(nullptr, K, nullptr, K, nullptr, N, nullptr, nullptr, nullptr, M, N, K);
   *bytes = w4_copy_bytes(N, K) + gemm_scratch_bytes<false, kAPlain>(p);
   return TEENY_OK;

@@ -289,12 +289,17 @@ inline void launch_w4_form(const W4Args &p, hipStream_t s) {
 }
 
 // Rows of x and blocks of columns per workgroup, and waves along K.  In us, the
-// weights through 6 sets of operands.  Sixteen waves pay once each has several
-// rounds: 8 x 4096 x 11008 11.0 / 9.2, 16 x 2048 x 8192 9.5 / 8.5, but 8 x 4096
-// x 4096 7.0 / 8.3.  Past 16 rows two column blocks share what is read of x, and
-// 32 rows a workgroup (over 16) the weights, where enough workgroups are left:
-// 64 x 11008 x 4096 26.3 / 24.5, 128 x 4096 x 4096 18.3 / 16.4, 250 x 1024 x 4096
-// 12.8 / 10.1, but 32 x 4096 x 4096 6.9 / 8.9 and 50 x 5504 x 2048 10.7 / 12.3.
+// weights through 4 to 6 sets of operands.  Sixteen waves pay once each has several
+// rounds: 8 x 4096 x 11008 11.0 / 9.2, 16 x 2048 x 8192 9.5 / 8.5, but 8 x 4096 x
+// 4096 7.0 / 8.3.  Past 16 rows two column blocks share what is read of x, and the
+// number of workgroups decides.  Registers let two of eight waves onto a CU, one
+// with 32 rows, and a second turn costs the most: 16 rows while that is one a CU,
+// else 32 while that is; beyond, workgroups of four waves, of which four or two
+// (32 rows) fit.  16 rows / 32 / 16 of four waves / 32 of four: 32 x 4096 x 4096
+// 7.1 / 9.1 / 9.4 / 11.6, 32 x 5504 x 2048 8.1 / 6.9 / 8.3 / 7.7, 64 x 4096 x 4096
+// 10.8 / 9.5 / 12.1 / 11.8, 50 x 5504 x 2048 10.8 / 12.5 / 10.0 / 10.3, 32 x 11008 x
+// 4096 15.2 / 17.1 / 15.6 / 16.3, 64 x 7000 x 4096 19.9 / 18.1 / 20.1 / 17.1, 64 x
+// 11008 x 4096 26.3 / 25.0 / 27.1 / 21.2, 150 x 11008 x 4096 56 / 56 / 56 / 44.
 inline void launch_gemm_w4(const W4Args &p, hipStream_t s) {
   const bool deep = p.K >= 8192;
   if (p.M <= 16) {
@@ -302,9 +307,11 @@ inline void launch_gemm_w4(const W4Args &p, hipStream_t s) {
     else if (p.M <= 8) deep ? launch_w4_form<8, 1, 16, 1>(p, s) : launch_w4_form<8, 1, 8, 1>(p, s);
     else deep ? launch_w4_form<16, 1, 16, 1>(p, s) : launch_w4_form<16, 1, 8, 1>(p, s);
   } else {
-    const int64_t wgs = cdiv(p.N, 32) * cdiv(p.M, 32), cus = device_cu_count();
-    if (wgs >= 2 * cus || (wgs >= cus && p.K >= 4096)) launch_w4_form<32, 2, 8, 1>(p, s);
-    else launch_w4_form<16, 2, 8, 1>(p, s);
+    const int64_t cols = cdiv(p.N, 32), wgs = cols * cdiv(p.M, 32), cus = device_cu_count();
+    if (cols * cdiv(p.M, 16) <= cus) launch_w4_form<16, 2, 8, 1>(p, s);
+    else if (wgs <= cus) launch_w4_form<32, 2, 8, 1>(p, s);
+    else if (2 * wgs <= 3 * cus) launch_w4_form<16, 2, 4, 1>(p, s);
+    else launch_w4_form<32, 2, 4, 1>(p, s);
   }
 }
 

@@ -46,7 +46,7 @@ def test_pack(dev, n, k):
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize("zero", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (1, 1, 8), (2, 33, 264), (16, 100, 1024), (17, 48, 520), (33, 70, 2048), (64, 31, 384),
-                                   (65, 40, 256), (200, 17, 136), (4, 20, 8200), (7, 40, 8192), (13, 17, 8456), (5, 100, 640), (130, 1100, 256), (64, 8200, 128)])
+                                   (65, 40, 256), (200, 17, 136), (4, 20, 8200), (7, 40, 8192), (13, 17, 8456), (5, 100, 640), (130, 1100, 256), (64, 8200, 128), (40, 4200, 200)])
 def test_linear(dev, m, n, k, group, zero):
     rng = np.random.default_rng(m + 3 * n + k + group)
     c = case(rng, m, n, k, group, zero)
@@ -65,7 +65,8 @@ def test_linear_epilogue(dev, m, act):
 @pytest.mark.parametrize("m,n,k,group,zero,act", [(65, 40, 256, 32, True, None), (100, 256, 512, 128, False, "silu"),
                                                   (300, 1000, 1032, 64, True, "gelu"), (513, 264, 2048, 256, False, None),
                                                   (1050, 1000, 1032, 64, True, "silu"), (200, 5300, 256, 32, False, None),
-                                                  (4100, 264, 512, 512, True, None)])
+                                                  (4100, 264, 512, 512, True, None), (460, 1720, 136, 128, True, None),
+                                                  (500, 2000, 264, 32, False, "relu")])
 def test_linear_copy(dev, m, n, k, group, zero, act):
     """Many rows with a workspace: the weights as bf16, each rounded once."""
     rng = np.random.default_rng(m + k)
