@@ -291,7 +291,9 @@ inline void launch_w4_form(const W4Args &p, hipStream_t s) {
 // Rows of x and blocks of columns per workgroup, and waves along K.  In us, the
 // weights through 4 to 6 sets of operands.  Sixteen waves pay once each has several
 // rounds: 8 x 4096 x 11008 11.0 / 9.2, 16 x 2048 x 8192 9.5 / 8.5, but 8 x 4096 x
-// 4096 7.0 / 8.3.  Past 16 rows two column blocks share what is read of x, and the
+// 4096 7.0 / 8.3.  Nine rows and more with over three workgroups of 16 columns to
+// a CU take 32 columns each: 16 x 16000 x 4096 13.4 / 11.9, but 16 x 11008 x 4096 10.6
+// / 10.9 and 8 x 16000 x 4096 11.4 / 11.6.  Past 16 rows two column blocks share what is read of x, and the
 // number of workgroups decides.  Registers let two of eight waves onto a CU, one
 // with 32 rows, and a second turn costs the most: 16 rows while that is one a CU,
 // else 32 while that is; beyond, workgroups of four waves, of which four or two
@@ -302,12 +304,14 @@ inline void launch_w4_form(const W4Args &p, hipStream_t s) {
 // 11008 x 4096 26.3 / 25.0 / 27.1 / 21.2, 150 x 11008 x 4096 56 / 56 / 56 / 44.
 inline void launch_gemm_w4(const W4Args &p, hipStream_t s) {
   const bool deep = p.K >= 8192;
+  const int64_t cols = cdiv(p.N, 32), cus = device_cu_count();
   if (p.M <= 16) {
     if (p.M <= 4) deep ? launch_w4_form<4, 1, 16, 2>(p, s) : launch_w4_form<4, 1, 8, 2>(p, s);
     else if (p.M <= 8) deep ? launch_w4_form<8, 1, 16, 1>(p, s) : launch_w4_form<8, 1, 8, 1>(p, s);
-    else deep ? launch_w4_form<16, 1, 16, 1>(p, s) : launch_w4_form<16, 1, 8, 1>(p, s);
+    else if (deep) launch_w4_form<16, 1, 16, 1>(p, s);
+    else cols * 2 > 3 * cus ? launch_w4_form<16, 2, 8, 1>(p, s) : launch_w4_form<16, 1, 8, 1>(p, s);
   } else {
-    const int64_t cols = cdiv(p.N, 32), wgs = cols * cdiv(p.M, 32), cus = device_cu_count();
+    const int64_t wgs = cols * cdiv(p.M, 32);
     if (cols * cdiv(p.M, 16) <= cus) launch_w4_form<16, 2, 8, 1>(p, s);
     else if (wgs <= cus) launch_w4_form<32, 2, 8, 1>(p, s);
     else if (2 * wgs <= 3 * cus) launch_w4_form<16, 2, 4, 1>(p, s);

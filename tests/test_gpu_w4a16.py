@@ -46,7 +46,7 @@ def test_pack(dev, n, k):
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize("zero", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (1, 1, 8), (2, 33, 264), (16, 100, 1024), (17, 48, 520), (33, 70, 2048), (64, 31, 384),
-                                   (65, 40, 256), (200, 17, 136), (4, 20, 8200), (7, 40, 8192), (13, 17, 8456), (5, 100, 640), (130, 1100, 256), (64, 8200, 128), (40, 4200, 200)])
+                                   (65, 40, 256), (200, 17, 136), (4, 20, 8200), (7, 40, 8192), (13, 17, 8456), (5, 100, 640), (130, 1100, 256), (64, 8200, 128), (40, 4200, 200), (11, 12300, 128)])
 def test_linear(dev, m, n, k, group, zero):
     rng = np.random.default_rng(m + 3 * n + k + group)
     c = case(rng, m, n, k, group, zero)
