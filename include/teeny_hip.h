@@ -152,14 +152,17 @@ teeny_status teeny_hip_stream_sync(teeny_stream stream);
  * operator scratch; ptr NULL or bytes 0 detaches.  Operators never allocate:
  * the paths that need scratch -- split-K partial sums for GEMM and conv grids
  * too small to fill the device, the space-to-depth copy of stride-2 NHWC
- * convs whose C_IN is not a multiple of 8, and the bf16 copy of the int8
- * weights of W8A16 3x3 convs that run on the band-tiled kernel -- run only
- * when the stream's
- * workspace is large enough (sizes from teeny_linear_workspace_size and
- * teeny_conv2d_workspace_size), and otherwise the operator takes a path that
+ * convs whose C_IN is not a multiple of 8, the bf16 copy of the int8
+ * weights of W8A16 3x3 convs that run on the band-tiled kernel, that of 4-bit
+ * weights for many rows, and the parts of attention over the paged cache -- run
+ * only when the stream's workspace is large enough (sizes from
+ * teeny_linear_workspace_size, teeny_conv2d_workspace_size and the other
+ * teeny_*_workspace_size), and otherwise the operator takes a path that
  * needs none.  Work on one stream runs in order, so every operator on it may
  * share the buffer; the buffer must outlive the work enqueued while it is
- * attached.  Destroying the stream detaches it.  Reference counterpart: none
+ * attached.  A captured graph keeps using the workspace that its stream had
+ * then: graphs and streams that share one must not run side by side.
+ * Destroying the stream detaches it.  Reference counterpart: none
  * (the reference's ops use no scratch; this mirrors cublasSetWorkspace). */
 teeny_status teeny_hip_stream_set_workspace(teeny_stream stream, void *ptr, size_t bytes);
 teeny_status teeny_hip_event_create(teeny_event *event);
@@ -689,7 +692,8 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
  * 32, 64 or a multiple of 128; K a multiple of 8 below 2^23; x and qweight
  * 16-byte aligned.
  * The codes multiply x in fp32-accumulated products and the scale multiplies
- * their fp32 sum.  For many rows, with a stream workspace of
+ * their fp32 sum, with 1.5 + zero_point / 16 times the sum of x over the group
+ * taken off: a row of x with an infinity gives NaN.  For many rows, with a stream workspace of
  * teeny_w4a16_linear_workspace_size bytes (0: never for this shape), the weights
  * are first written there as bf16 (scale applied in fp32, rounded once) for the
  * matrix-core tiles of linear_forward. */

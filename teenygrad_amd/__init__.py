@@ -1,6 +1,8 @@
 """teenygrad_amd — MI355X (gfx950) HIP implementation of teeny-kernels' forward
 operators (conv2d, flash attention, LayerNorm/RMSNorm, ReLU/GELU/SiLU) and
-teeny-quant's int8 affine quantization with W8A16 linear and conv.
+teeny-quant's int8 affine quantization with W8A16 linear and conv, and the
+operators of a quantized decode step: an 8-bit paged K/V cache (plan, write,
+attention) and linear layers with 4-bit weights.
 
 The compute lives in libteeny_hip.so (C ABI: include/teeny_hip.h); this
 package is the host-side mirror of the reference's runtime and RuntimeOp

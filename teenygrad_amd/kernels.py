@@ -15,7 +15,7 @@ Two layers:
 * Functions (``relu``, ``layer_norm``, ``conv2d``, ``flash_attention`` ...)
   call the typed entry points of include/teeny_hip.h directly on
   ``Buffer`` objects, with this library's extensions (bf16, NHWC, causal,
-  fused activations, W8A16).
+  fused activations, W8A16, W4A16, the 8-bit paged K/V cache).
 """
 from __future__ import annotations
 
