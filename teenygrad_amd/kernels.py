@@ -1456,7 +1456,8 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
                        lse: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
     """Attention of q bf16 [n_tokens, q_heads, head_dim] over the 8-bit cache -> o like q.  Sequence b's queries are rows
     q_starts[b] .. q_starts[b + 1] - 1 (None: one each), the last of its context_lens[b] tokens.  max_q_len and
-    max_context (host numbers; default: as much as the buffers allow) choose how the work is cut, not the result."""
+    max_context (host numbers; default: the mean of the queries, and a whole row of the table) choose how the work is
+    cut, not the result."""
     pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
     if not (len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16):
         raise ValueError("kv_cache_attention: q bf16 [n_tokens, q_heads, head_dim]")
@@ -1473,7 +1474,7 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     if not (lse is None or (lse.numel == t * hq and lse.dtype == f32)):
         raise ValueError("kv_cache_attention: lse fp32 [n_tokens, q_heads]")
     if max_q_len is None:
-        max_q_len = 1 if q_starts is None else t
+        max_q_len = -(-t // max(b, 1))
     if max_context is None:
         max_context = block_table.shape[1] * size
     scale = d ** -0.5 if softmax_scale is None else softmax_scale

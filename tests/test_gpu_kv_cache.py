@@ -309,16 +309,16 @@ def test_attention_workspace_size(dev, ctx, new):
     check_attn(c, got[0])
 
 
-@pytest.mark.parametrize("new", [1, 5, 20])
-def test_attention_of_many_sequences(dev, new):
+@pytest.mark.parametrize("new,batch", [(1, 150), (5, 150), (20, 150), (1, 300), (5, 300), (20, 300), (1, 4500)])
+def test_attention_of_many_sequences(dev, new, batch):
     """More sequences than lanes: one, a few and many query rows, some sequences without any, with and without splits."""
     rng = np.random.default_rng(70 + new)
-    lens = rng.integers(0, 200, 150)
-    lens[[3, 77, 149]] = 1500, 0, 2000
-    c = attn_case(rng, [int(n) for n in lens], [int(n) for n in rng.integers(new == 1, new + 1, 150)], 8, 2, 64, 16)
+    lens = rng.integers(0, 200 if batch < 1000 else 30, batch)
+    lens[[3, 77, batch - 1]] = 1500, 0, 2000
+    c = attn_case(rng, [int(n) for n in lens], [int(n) for n in rng.integers(new == 1, new + 1, batch)], 8, 2, 64, 16)
     t, hint = int(c["starts"][-1]), (new, 2000)
     check_attn(c, run_attn(dev, c, hint=hint, pad=2))
-    with stream_workspace(dev, K.kv_cache_attention_workspace_size(t + 2, 150, 8, 2, 64, *hint)):
+    with stream_workspace(dev, K.kv_cache_attention_workspace_size(t + 2, batch, 8, 2, 64, *hint)):
         check_attn(c, run_attn(dev, c, hint=hint, pad=2))
 
 
