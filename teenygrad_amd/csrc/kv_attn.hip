@@ -745,7 +745,10 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
 // x 90 to 8000 1 / 2 / 3 / 4 116 / 126 / 112 / 117.  Shared tiles: 1 x 64 queries x
 // 16000 1 / 8 / 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads of 64, 1 / 4 / 8 /
 // 16 145 / 49 / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242 / 180 / 139 / 160; 4 x
-// 700 x 1100 to 4100 1 / 2 160 / 193.
+// 700 x 1100 to 4100 1 / 2 160 / 193.  Several sequences on a busy device get half as
+// many again, since contexts seldom are of one length: 16 x 40 x 1000 to 6000 2 / 3 /
+// 4 133 / 101 / 125, of 4000 104 / 116 / 110; 20 x 40 x 300 to 4000 1 / 2 125 / 97, of
+// 2000 88 / 98.
 struct KvAttnPlan {
   bool tile = false;
   int nq = 1, rb = 16;
@@ -767,7 +770,7 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   const int64_t busy = there * kv_heads;  // workgroups with work, unsplit
   const int64_t least = pl.tile ? (busy < 32 ? 256 : 768) : busy <= 64 ? 256 : 512;
   int64_t splits = 1;
-  if (pl.tile) splits = std::min(2 * cus / busy, max_ctx / least);
+  if (pl.tile) splits = std::min((batch > 1 && 2 * busy > cus ? 3 : 2) * cus / busy, max_ctx / least);
   else if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
   if (pl.tile ? busy < 2 * cus : busy >= 32) splits = std::max(splits, max_ctx / 2560);
   splits = std::max<int64_t>(1, splits);
