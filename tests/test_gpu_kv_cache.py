@@ -504,6 +504,30 @@ def test_step_in_a_graph(dev):
         graph.destroy()
 
 
+def test_two_streams(dev):
+    """Calls on two streams at once, each with its own workspace: split attention, shared tiles and few rows."""
+    rng = np.random.default_rng(14)
+    streams = [Stream.create(), Stream.create()]
+    jobs = []
+    for i, (ctx, new) in enumerate([([3000, 40, 700], [1, 1, 1]), ([1500, 300], [60, 90]), ([900, 2100], [9, 5]), ([2500], [1])]):
+        c = attn_case(rng, ctx, new, 8, 2, 128, 16)
+        bufs = [dev.upload(to_bf16(c["q"]), bf16)] + [dev.upload(c[n]) for n in ("kc", "vc", "ks", "vs", "table")]
+        bufs += [ints(dev, c["ctx"]), ints(dev, c["starts"])]
+        t = c["q"].shape[0]
+        jobs.append((c, streams[i % 2], bufs, (max(new), max(ctx)), dev.buffer(bf16, c["q"].shape), dev.buffer("f32", (t, 8)),
+                     K.kv_cache_attention_workspace_size(t, len(ctx), 8, 2, 128, max(new), max(ctx))))
+    dev.synchronize()
+    most = max(j[-1] for j in jobs)
+    with stream_workspace(dev, most, streams[0]), stream_workspace(dev, most, streams[1]):
+        for _ in range(5):
+            for c, s, bufs, hint, o, lse, _ in jobs:
+                K.kv_cache_attention(*bufs, *hint, o=o, lse=lse, stream=s)
+        for s in streams:
+            s.synchronize()
+        for c, s, bufs, hint, o, lse, _ in jobs:
+            check_attn(c, (from_bf16(o.to_host()), lse.to_host()))
+
+
 def test_large_cache(dev):
     """Pages whose bytes lie past 2^32: the same tokens at the pool's start and end."""
     rng = np.random.default_rng(13)

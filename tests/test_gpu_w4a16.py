@@ -5,6 +5,8 @@ import pytest
 import kv_cases as kv
 from gpu_util import stream_workspace
 from teenygrad_amd import kernels as K
+from teenygrad_amd._lib import check as check_status
+from teenygrad_amd._lib import lib
 from teenygrad_amd.dtypes import bf16, from_bf16, to_bf16
 from teenygrad_amd.runtime import Stream
 
@@ -80,6 +82,14 @@ def test_linear_copy(dev, m, n, k, group, zero, act):
 def test_linear_of_nothing(dev):
     x, w = dev.buffer(bf16, (0, 128)), dev.buffer("i8", (16, 64))
     assert K.w4a16_linear(x, w, dev.buffer("f32", (16, 1)), 128).shape == (0, 16)
+
+
+def test_linear_without_k(dev):
+    """K = 0: the bias and the activation."""
+    bias = np.array([-1.0, 0.5, 3.0], np.float32)
+    y, b = dev.buffer(bf16, (2, 3)), dev.upload(bias)
+    check_status(lib.teeny_w4a16_linear_forward(None, None, None, None, b.ptr, y.ptr, 2, 3, 0, 128, K.ACTS["relu"], None))
+    np.testing.assert_array_equal(from_bf16(y.to_host()), np.tile(np.maximum(bias, 0), (2, 1)))
 
 
 def test_linear_ignores_what_pads_k(dev):
