@@ -916,11 +916,9 @@ def _out(like: Buffer, out: Optional[Buffer], shape=None, dtype=None) -> Buffer:
 
 
 def _types(*pairs) -> bool:
-    """Whether each buffer (or None) has its dtype: nearly always the very object, which needs no comparison."""
-    for buf, dtype in pairs:
-        if buf is not None and buf.dtype is not dtype and buf.dtype != dtype:
-            return False
-    return True
+    """Whether each buffer (or None) has its dtype.  (Callers whose kernels run for a few us look first whether it is
+    the very object, as it nearly always is.)"""
+    return all(buf is None or buf.dtype == dtype for buf, dtype in pairs)
 
 
 # Shape rules of each entry point, as pure functions of buffer shapes (so the
@@ -1393,8 +1391,8 @@ def kv_cache_dims(k_cache_shape, v_cache_shape, k_scale_shape, v_scale_shape) ->
 
 
 def _need_cache(k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer):
-    if not _types((k_cache, i8), (v_cache, i8), (k_scale, f32), (v_scale, f32)):
-        raise ValueError("kv_cache: codes int8, scales fp32")
+    if not (k_cache.dtype is v_cache.dtype is i8 and k_scale.dtype is v_scale.dtype is f32):
+        _need(_types((k_cache, i8), (v_cache, i8), (k_scale, f32), (v_scale, f32)), "kv_cache: codes int8, scales fp32")
     return kv_cache_dims(k_cache.shape, v_cache.shape, k_scale.shape, v_scale.shape)
 
 
@@ -1402,7 +1400,7 @@ def _ints(buf: Optional[Buffer], n: int, what: str) -> Buffer:
     """An int32 buffer of n elements: `buf`, checked, or a new one."""
     if buf is None:
         return Buffer(i32, (n,))
-    if buf.numel != n or (buf.dtype is not i32 and buf.dtype != i32):
+    if buf.numel != n or buf.dtype != i32:
         raise ValueError(f"kv_cache: {what} must be int32 with {n} elements, is {buf.dtype.name} with {buf.numel}")
     return buf
 
@@ -1418,17 +1416,29 @@ def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_
     `slots` given: as many as it has).  context_lens=seq_lens, granted=new_lens and free_after=free_count update in
     place.  A request that does not fit is refused as a whole: granted 0, slots -1."""
     b = new_lens.numel
-    if len(block_table.shape) != 2 or block_table.shape[0] != b or block_table.dtype != i32:
-        raise ValueError(f"kv_cache_plan: block_table must be int32 [{b}, max_pages]")
-    if not (seq_lens.numel == b and free_count.numel == 1 and
-            _types((new_lens, i32), (seq_lens, i32), (free_list, i32), (free_count, i32))):
-        raise ValueError(f"kv_cache_plan: new_lens and seq_lens [{b}], free_list and free_count [1], int32")
-    _need(slots is not None or n_tokens is not None, "kv_cache_plan: n_tokens or slots")
-    t = slots.numel if n_tokens is None else int(n_tokens)
-    slots, positions = _ints(slots, t, "slots"), _ints(positions, t, "positions")
-    q_starts = _ints(q_starts, b + 1, "q_starts")
-    context_lens, granted = _ints(context_lens, b, "context_lens"), _ints(granted, b, "granted")
-    free_after = _ints(free_after, 1, "free_after")
+    if len(block_table.shape) != 2 or block_table.shape[0] != b or seq_lens.numel != b or free_count.numel != 1:
+        raise ValueError(f"kv_cache_plan: block_table must be [{b}, max_pages], seq_lens [{b}], free_count [1]")
+    if not new_lens.dtype is seq_lens.dtype is block_table.dtype is free_list.dtype is free_count.dtype is i32:
+        _need(_types((new_lens, i32), (seq_lens, i32), (block_table, i32), (free_list, i32), (free_count, i32)),
+              "kv_cache_plan: new_lens, seq_lens, block_table, free_list and free_count must be int32")
+    if n_tokens is not None:
+        t = int(n_tokens)
+    elif slots is not None:
+        t = slots.numel
+    else:
+        raise ValueError("kv_cache_plan: n_tokens or slots")
+    if slots is None or slots.numel != t or slots.dtype is not i32:
+        slots = _ints(slots, t, "slots")
+    if positions is None or positions.numel != t or positions.dtype is not i32:
+        positions = _ints(positions, t, "positions")
+    if q_starts is None or q_starts.numel != b + 1 or q_starts.dtype is not i32:
+        q_starts = _ints(q_starts, b + 1, "q_starts")
+    if context_lens is None or context_lens.numel != b or context_lens.dtype is not i32:
+        context_lens = _ints(context_lens, b, "context_lens")
+    if granted is None or granted.numel != b or granted.dtype is not i32:
+        granted = _ints(granted, b, "granted")
+    if free_after is None or free_after.numel != 1 or free_after.dtype is not i32:
+        free_after = _ints(free_after, 1, "free_after")
     check(lib.teeny_kv_cache_plan(new_lens.ptr, seq_lens.ptr, block_table.ptr, free_list.ptr, free_count.ptr,
                                   q_starts.ptr, slots.ptr, positions.ptr, context_lens.ptr, granted.ptr, free_after.ptr,
                                   b, block_table.shape[1], free_list.numel, page_size, t, _h(stream)))
@@ -1443,8 +1453,8 @@ def kv_cache_write(k: Buffer, v: Buffer, slots: Buffer, k_cache: Buffer, v_cache
     t = slots.numel
     if not k.shape == v.shape == (t, heads, d):
         raise ValueError(f"kv_cache_write: k and v must be {[t, heads, d]}")
-    if not _types((k, bf16), (v, bf16), (slots, i32)):
-        raise ValueError("kv_cache_write: k/v bf16, slots int32")
+    if not (k.dtype is v.dtype is bf16 and slots.dtype is i32):
+        _need(_types((k, bf16), (v, bf16), (slots, i32)), "kv_cache_write: k/v bf16, slots int32")
     check(lib.teeny_kv_cache_write(k.ptr, v.ptr, slots.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, t, heads,
                                    d, pages, size, heads * d, heads * d, _h(stream)))
 
@@ -1465,10 +1475,13 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     b = context_lens.numel
     if heads == 0 or hq % heads:
         raise ValueError("kv_cache_attention: q_heads % kv_heads != 0")
-    if not (len(block_table.shape) == 2 and block_table.shape[0] == b and _types((block_table, i32), (context_lens, i32))):
-        raise ValueError(f"kv_cache_attention: block_table [{b}, max_pages] and context_lens [{b}], int32")
+    if len(block_table.shape) != 2 or block_table.shape[0] != b:
+        raise ValueError(f"kv_cache_attention: block_table must be [{b}, max_pages]")
+    if not block_table.dtype is context_lens.dtype is i32:
+        _need(_types((block_table, i32), (context_lens, i32)), "kv_cache_attention: block_table and context_lens must be int32")
     if q_starts is not None:
-        _ints(q_starts, b + 1, "q_starts")
+        if q_starts.numel != b + 1 or q_starts.dtype is not i32:
+            _ints(q_starts, b + 1, "q_starts")
     elif t != b:
         raise ValueError(f"kv_cache_attention: q_starts, or one query for each of the {b} sequences")
     if not (lse is None or (lse.numel == t * hq and lse.dtype == f32)):
@@ -1478,7 +1491,8 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     if max_context is None:
         max_context = block_table.shape[1] * size
     scale = d ** -0.5 if softmax_scale is None else softmax_scale
-    o = _out(q, o)
+    if o is None or o.numel != q.numel or o.dtype is not bf16:
+        o = _out(q, o)
     check(lib.teeny_kv_cache_attention(q.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, block_table.ptr,
                                        context_lens.ptr, q_starts.ptr if q_starts is not None else None, o.ptr,
                                        lse.ptr if lse is not None else None, t, b, hq, heads, d, pages, size,
@@ -1601,17 +1615,19 @@ def pack_int4(q: Buffer, out: Optional[Buffer] = None, stream: Optional[Stream] 
 
 
 def w4a16_dims(x_shape, q_shape, scale_shape, group_size, zero_shape=None, bias_shape=None) -> Tuple[int, int, int]:
-    _need(len(x_shape) == 2 and len(q_shape) == 2, "w4a16: x and qweight must be 2-D")
+    if len(x_shape) != 2 or len(q_shape) != 2:
+        raise ValueError("w4a16: x and qweight must be 2-D")
     m, k = x_shape
-    n = q_shape[0]
+    n, row = q_shape
     if not (group_size in (32, 64) or (group_size > 0 and group_size % 128 == 0)):
         raise ValueError(f"w4a16: group_size must be 32, 64 or a multiple of 128, is {group_size}")
-    if q_shape[1] != -(-k // 128) * 64:
+    if row != (k + 127) // 128 * 64:
         raise ValueError(f"w4a16: qweight must be pack_int4's [{n}, {-(-k // 128) * 64}], is {list(q_shape)}")
-    groups = n * -(-k // group_size)
-    if _prod(scale_shape) != groups or (zero_shape is not None and _prod(zero_shape) != groups):
-        raise ValueError(f"w4a16: scale/zero_point must have N x groups = {groups} elements")
-    if not (bias_shape is None or _prod(bias_shape) == n):
+    groups = (n, -(-k // group_size))
+    for shape in (scale_shape, zero_shape):
+        if shape is not None and shape != groups and _prod(shape) != _prod(groups):
+            raise ValueError(f"w4a16: scale/zero_point must have N x groups = {_prod(groups)} elements")
+    if not (bias_shape is None or bias_shape == (n,) or _prod(bias_shape) == n):
         raise ValueError(f"w4a16: bias must have {n} elements")
     return int(m), int(n), int(k)
 
@@ -1624,9 +1640,12 @@ def w4a16_linear(x: Buffer, qweight: Buffer, scale: Buffer, group_size: int, zer
     "group", axis=1, group_size=group_size, bits=4)`` gives them, bias fp32 [N]."""
     m, n, k = w4a16_dims(x.shape, qweight.shape, scale.shape, group_size,
                          zero_point.shape if zero_point is not None else None, bias.shape if bias is not None else None)
-    if not _types((x, bf16), (qweight, i8), (scale, f32), (bias, f32), (zero_point, i32)):
-        raise ValueError("w4a16_linear: x bf16, qweight int8, scale/bias fp32, zero_point int32")
-    y = _out(x, y, (m, n), bf16)
+    if not (x.dtype is bf16 and qweight.dtype is i8 and scale.dtype is f32 and
+            (bias is None or bias.dtype is f32) and (zero_point is None or zero_point.dtype is i32)):
+        _need(_types((x, bf16), (qweight, i8), (scale, f32), (bias, f32), (zero_point, i32)),
+              "w4a16_linear: x bf16, qweight int8, scale/bias fp32, zero_point int32")
+    if y is None or y.numel != m * n or y.dtype is not bf16:
+        y = _out(x, y, (m, n), bf16)
     check(lib.teeny_w4a16_linear_forward(x.ptr, qweight.ptr, scale.ptr,
                                          zero_point.ptr if zero_point is not None else None,
                                          bias.ptr if bias is not None else None, y.ptr, m, n, k, group_size, ACTS[act],
