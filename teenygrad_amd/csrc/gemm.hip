@@ -359,9 +359,9 @@ teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, co
   TEENY_REQUIRE(aligned(x, 16) && aligned(qweight, 16), TEENY_ERR_MISALIGNED,
                 "w4a16_linear_forward: x and qweight must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  group_size = std::min<int64_t>(group_size, int64_t{1} << 30);  // beyond K all the same
   W4Args p{static_cast<const bf16 *>(x), qweight, scale, zero_point, bias, static_cast<bf16 *>(y), static_cast<int>(M),
-           static_cast<int>(N), static_cast<int>(K), static_cast<int>(cdiv(K, group_size)),
-           static_cast<int>(std::min<int64_t>(group_size, int64_t{1} << 30)), act};
+           static_cast<int>(N), static_cast<int>(K), static_cast<int>(cdiv(K, group_size)), static_cast<int>(group_size), act};
   const Scratch scr = stream_scratch(s);
   const size_t copy = w4_copy_bytes(N, K);
   if (w4_as_bf16(M, N, K) && K > 0 && scr.ptr != nullptr && scr.bytes >= copy) {

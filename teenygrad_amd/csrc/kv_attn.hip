@@ -760,7 +760,7 @@ struct KvAttnPlan {
 static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D,
                                int64_t max_q, int64_t max_ctx, size_t scratch) {
   KvAttnPlan pl;
-  const int64_t group = heads / kv_heads, rows = group * max_q;
+  const int64_t group = heads / kv_heads, rows = group * std::min(max_q, tokens);
   if (rows > 64) pl.tile = true, pl.rb = 128;
   else if (rows > 16) pl.nq = 2, pl.rb = 32;
   pl.blocks = tokens * group / pl.rb + batch;

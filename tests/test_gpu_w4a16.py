@@ -84,6 +84,13 @@ def test_linear_of_nothing(dev):
     assert K.w4a16_linear(x, w, dev.buffer("f32", (16, 1)), 128).shape == (0, 16)
 
 
+@pytest.mark.parametrize("group", [384, 1 << 20, 1 << 40, (1 << 63) - 128])
+def test_linear_of_one_group(dev, group):
+    rng = np.random.default_rng(7)
+    c = case(rng, 5, 20, 264, 384, True)
+    check(run(dev, *c, group, None), *c, 384, None, False)
+
+
 def test_linear_without_k(dev):
     """K = 0: the bias and the activation."""
     bias = np.array([-1.0, 0.5, 3.0], np.float32)

@@ -107,6 +107,11 @@ def test_attention_workspace_refusals():
     expect(f(-4, 4, 8, 2, 128, 1, 128, ctypes.byref(n)), _lib.ERR_SHAPE_MISMATCH)
     assert n.value == 0
     assert f(0, 4, 8, 2, 128, 1, 128, ctypes.byref(n)) == _lib.OK and n.value == 0
+    sizes = []
+    for longest in (40, 1 << 40, (1 << 63) - 1):  # no sequence has more queries than there are rows
+        assert f(40, 2, 8, 2, 128, longest, 9000, ctypes.byref(n)) == _lib.OK
+        sizes.append(n.value)
+    assert sizes[0] > 0 and len(set(sizes)) == 1
 
 
 def w4_args(**kw):
