@@ -773,7 +773,8 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   if (pl.tile) splits = std::min((batch > 1 && 2 * busy > cus ? 3 : 2) * cus / busy, max_ctx / least);
   else if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
   if (pl.tile ? busy < 2 * cus : busy >= 32) splits = std::max(splits, max_ctx / 2560);
-  splits = std::max<int64_t>(1, splits);
+  // a launch has less than 2^31 threads (the limit of rows leaves room for four splits at least)
+  splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / 256 - 1) / units));
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   auto cut = [&](int64_t n) {
     pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), n), step) * step);
@@ -861,8 +862,8 @@ teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, cons
   const KvAttnPlan pl =
       kv_attn_plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, scr.ptr ? scr.bytes : 0);
   const int64_t units = pl.blocks * kv_heads;
-  TEENY_REQUIRE(units * pl.splits < (int64_t{1} << 31) / 256 && units * pl.rb < (int64_t{1} << 31) / 64,
-                TEENY_ERR_SHAPE_MISMATCH, "kv_cache_attention: too many rows for a launch");
+  TEENY_REQUIRE(units * pl.rb < (int64_t{1} << 31) / 64, TEENY_ERR_SHAPE_MISMATCH,
+                "kv_cache_attention: too many rows for a launch");
   KvAttnArgs p{};
   p.q = static_cast<const bf16 *>(q);
   p.q_stride = q_stride;

@@ -546,3 +546,17 @@ def test_large_cache(dev):
     assert np.isfinite(from_bf16(outs[0])).all() and from_bf16(outs[0]).any()
     for b in (kc, vc):
         b.free()
+
+
+def test_attention_of_the_largest_launch(dev):
+    """Short sequences of many heads under a very large max_context, with the workspace that it asks for (35 GB): as
+    many parts as a launch takes, nearly all of them empty."""
+    rng = np.random.default_rng(15)
+    batch, heads, d, most = 1024, 64, 64, 1 << 19
+    c = attn_case(rng, [int(n) for n in rng.integers(0, 40, batch)], [1] * batch, heads, heads, d, 16)
+    c["table"] = np.pad(c["table"], ((0, 0), (0, most // 16 - c["table"].shape[1])), constant_values=-1)
+    c["ctx"][7], c["table"][7, [300, 700, 1023]] = 1 << 14, [0, 1, 2]  # a few pages, far apart
+    size = K.kv_cache_attention_workspace_size(batch, batch, heads, heads, d, 1, most)
+    assert size > 1 << 35
+    with stream_workspace(dev, size):
+        check_attn(c, run_attn(dev, c, hint=(1, most)))

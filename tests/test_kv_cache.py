@@ -186,3 +186,18 @@ def test_plan_oracle():
     assert out["slots"].tolist() == [95, 32] + [112 + i for i in range(16)] + [64, -1]
     assert out["q_starts"].tolist() == [0, 2, 2, 19] and out["context_lens"].tolist() == [17, 0, 17]
     assert out["granted"].tolist() == [2, 0, 17] and out["free_after"].tolist() == [0]
+
+
+@pytest.mark.parametrize("batch,hq,hkv,d,longest,context", [(4096, 8, 8, 64, 1, 1 << 20), (2000, 32, 32, 128, 1, (1 << 31) - 5000),
+                                                            (3000, 16, 4, 64, 4, 1 << 26), (1, 8, 2, 128, 1, 1 << 30)])
+def test_attention_splits_fit_a_launch(batch, hq, hkv, d, longest, context):
+    """A large max_context asks for no more parts than a launch of 2^31 threads has workgroups for, in which case the
+    call would be refused."""
+    tokens, rows = batch * longest, hq // hkv * longest
+    block = 128 if rows > 64 else 32 if rows > 16 else 16
+    units = (tokens * (hq // hkv) // block + batch) * hkv
+    assert units * block < 1 << 25, "within the documented limit of rows"
+    n = ctypes.c_size_t(0)
+    assert lib.teeny_kv_cache_attention_workspace_size(tokens, batch, hq, hkv, d, longest, context, ctypes.byref(n)) == _lib.OK
+    splits = n.value // (units * block * (d + 2) * 4)
+    assert splits > 1 and units * splits < (1 << 31) // 256
