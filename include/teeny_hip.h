@@ -691,12 +691,16 @@ teeny_status teeny_w8a16_linear_forward(const void *x, const int8_t *qweight, co
  * qweight is teeny_pack_int4's, N rows of ceil(K / 128) * 64 bytes.  group_size
  * 32, 64 or a multiple of 128; K a multiple of 8 below 2^23; x and qweight
  * 16-byte aligned.
- * The codes multiply x in fp32-accumulated products and the scale multiplies
- * their fp32 sum, with 1.5 + zero_point / 16 times the sum of x over the group
- * taken off: a row of x with an infinity gives NaN.  For many rows, with a stream workspace of
+ * There are two forms.  Streaming: the codes multiply x in fp32-accumulated
+ * products and the scale multiplies their fp32 sum, with 1.5 + zero_point / 16
+ * times the sum of x over the group taken off; nothing is rounded but y.  A row
+ * of x with an infinity gives NaN there, also one whose sums over a group pass
+ * fp32.  Copy: for many rows, with a stream workspace of
  * teeny_w4a16_linear_workspace_size bytes (0: never for this shape), the weights
- * are first written there as bf16 (scale applied in fp32, rounded once) for the
- * matrix-core tiles of linear_forward. */
+ * are first written there as bf16 (scale applied in fp32, rounded once, which
+ * moves each product by up to 2^-8) for the matrix-core tiles of linear_forward;
+ * infinities of x follow the products.  In both, what a row of x holds reaches
+ * that row of y alone. */
 teeny_status teeny_w4a16_linear_forward(const void *x, const int8_t *qweight, const float *scale,
                                         const int32_t *zero_point, const float *bias, void *y, int64_t M, int64_t N,
                                         int64_t K, int64_t group_size, teeny_activation act, teeny_stream stream);

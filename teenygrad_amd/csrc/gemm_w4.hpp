@@ -11,6 +11,7 @@
 // point) times the sum of x over the group comes off behind the products; the
 // sum is one more product, with ones, in the accumulator's own layout.  The
 // scale multiplies the group's fp32 result: nothing is rounded before the output.
+// (An infinity in a row of x makes both sums infinite, and the row's outputs NaN.)
 #pragma once
 
 #include "mfma.hpp"

@@ -1637,7 +1637,8 @@ def w4a16_linear(x: Buffer, qweight: Buffer, scale: Buffer, group_size: int, zer
                  stream: Optional[Stream] = None) -> Buffer:
     """act(x W^T + bias) with W[n, k] = scale[n, g] (q[n, k] - zero_point[n, g]), g = k // group_size: x bf16
     [M, K], qweight from ``pack_int4``, scale fp32 and zero_point int32 (None: symmetric) as ``quantize_affine(...,
-    "group", axis=1, group_size=group_size, bits=4)`` gives them, bias fp32 [N]."""
+    "group", axis=1, group_size=group_size, bits=4)`` gives them, bias fp32 [N].  Only y is rounded, but for many rows
+    on a stream with a workspace of ``w4a16_linear_workspace_size``: there the weights are, to bf16."""
     m, n, k = w4a16_dims(x.shape, qweight.shape, scale.shape, group_size,
                          zero_point.shape if zero_point is not None else None, bias.shape if bias is not None else None)
     if not (x.dtype is bf16 and qweight.dtype is i8 and scale.dtype is f32 and

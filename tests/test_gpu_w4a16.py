@@ -159,3 +159,30 @@ def test_linear_in_a_graph(dev):
                 s.synchronize()
                 check(from_bf16(y.to_host()), x, codes, scale, None, bias, 64, None, m > 64)
             graph.destroy()
+
+
+@pytest.mark.parametrize("m", [5, 460])
+def test_linear_rows_that_are_not_finite(dev, m):
+    """An infinity or NaN stays in its row.  There the streaming form gives NaN, the one through the copy what the
+    products add up to."""
+    rng = np.random.default_rng(51)
+    n, k, group = 1720, 136, 128
+    x, *w = case(rng, m, n, k, group, True)
+    sound = np.setdiff1d(np.arange(m), [1, 3])
+    x[1, 130], x[3, 5] = np.nan, -np.inf
+
+    def check_rows(copy):
+        got = run(dev, x, *w, group, None)
+        assert np.isnan(got[1]).all()
+        check(got[sound], x[sound], *w, group, None, copy)
+        return got[3]
+
+    size = K.w4a16_linear_workspace_size(m, n, k, group)
+    assert (size > 0) == (m > 448)
+    with stream_workspace(dev, 256):
+        assert np.isnan(check_rows(False)).all()
+    if size:
+        with stream_workspace(dev, size):
+            got = check_rows(True)
+        sign = np.sign(w[0][:, 5] - w[2][:, 0])
+        np.testing.assert_array_equal(got, np.where(sign == 0, np.nan, -np.inf * np.where(sign == 0, 1, sign)))
