@@ -186,3 +186,46 @@ def test_linear_rows_that_are_not_finite(dev, m):
             got = check_rows(True)
         sign = np.sign(w[0][:, 5] - w[2][:, 0])
         np.testing.assert_array_equal(got, np.where(sign == 0, np.nan, -np.inf * np.where(sign == 0, 1, sign)))
+
+
+def check_some(got, c, rows, cols, group, act, copy):
+    """The chosen rows and columns: an output needs no other row of x or of the weights."""
+    x, codes, scale, zp, bias = c
+    part = x[rows], codes[cols], scale[cols], zp[cols] if zp is not None else None, bias[cols]
+    check(got[np.ix_(rows, cols)], *part, group, act, copy)
+
+
+@pytest.mark.parametrize("m,n,k,group,zero,act", [
+    (256, 1024, 36000, 128, True, "gelu"),  # K in slices, whose sums lie behind the copy
+    (200, 11501, 4096, 128, True, "silu"), (450, 1749, 520, 64, False, None),  # rows of y at odd offsets
+    (300, 8003, 4000, 32, False, "relu"), (4096, 4099, 1024, 64, True, "silu"), (4096, 4104, 1032, 32, False, "gelu"),
+    (500, 1600, 264, 256, True, None)])
+def test_linear_through_the_copy(dev, m, n, k, group, zero, act):
+    rng = np.random.default_rng(m + n + k)
+    c = case(rng, m, n, k, group, zero)
+    size = K.w4a16_linear_workspace_size(m, n, k, group)
+    assert size >= 2 * n * k, "this shape takes the copy"
+    assert (size > 2 * n * k + 256) == (k == 36000)
+    rows = np.unique(np.concatenate([np.arange(4), m - 1 - np.arange(4), rng.integers(0, m, 200)]))
+    with stream_workspace(dev, size):
+        check_some(run(dev, *c, group, act), c, rows, np.arange(n), group, act, True)
+
+
+def test_linear_of_a_million_rows(dev):
+    """More rows than a launch has workgroups for along one axis, in both forms."""
+    rng = np.random.default_rng(61)
+    m = 65535 * 16 + 17
+    c = case(rng, m, 8, 8, 32, True)
+    rows, cols = np.concatenate([np.arange(100), np.arange(65535 * 16 - 40, m)]), np.arange(8)
+    check_some(run(dev, *c, 32, None), c, rows, cols, 32, None, False)  # no workspace: 256 bytes would hold the copy
+    with stream_workspace(dev, K.w4a16_linear_workspace_size(m, 8, 8, 32)):
+        check_some(run(dev, *c, 32, None), c, rows, cols, 32, None, True)
+
+
+def test_linear_of_many_columns(dev):
+    """More columns than one launch takes."""
+    rng = np.random.default_rng(62)
+    n = (1 << 25) + 21
+    c = case(rng, 3, n, 8, 32, True)
+    cols = np.concatenate([np.arange(100), np.arange((1 << 25) - 40, n)])
+    check_some(run(dev, *c, 32, "relu"), c, np.arange(3), cols, 32, "relu", False)
