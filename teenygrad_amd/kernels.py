@@ -685,6 +685,7 @@ class W4A16LinearRuntimeOp(RuntimeOp):
 
     def __init__(self, group_size: int, use_zero_point: bool = False, use_bias: bool = False, act: Optional[str] = None):
         self.group_size = int(group_size)
+        _w4_group(self.group_size)
         self.use_zero_point, self.use_bias = bool(use_zero_point), bool(use_bias)
         self.act = ACTS[act]
 
@@ -1614,13 +1615,17 @@ def pack_int4(q: Buffer, out: Optional[Buffer] = None, stream: Optional[Stream] 
     return out
 
 
+def _w4_group(group_size: int) -> None:
+    if not (group_size in (32, 64) or (0 < group_size < 1 << 63 and group_size % 128 == 0)):
+        raise ValueError(f"w4a16: group_size must be 32, 64 or a multiple of 128 below 2^63, is {group_size}")
+
+
 def w4a16_dims(x_shape, q_shape, scale_shape, group_size, zero_shape=None, bias_shape=None) -> Tuple[int, int, int]:
     if len(x_shape) != 2 or len(q_shape) != 2:
         raise ValueError("w4a16: x and qweight must be 2-D")
     m, k = x_shape
     n, row = q_shape
-    if not (group_size in (32, 64) or (group_size > 0 and group_size % 128 == 0)):
-        raise ValueError(f"w4a16: group_size must be 32, 64 or a multiple of 128, is {group_size}")
+    _w4_group(group_size)
     if row != (k + 127) // 128 * 64:
         raise ValueError(f"w4a16: qweight must be pack_int4's [{n}, {-(-k // 128) * 64}], is {list(q_shape)}")
     groups = (n, -(-k // group_size))

@@ -201,3 +201,13 @@ def test_attention_splits_fit_a_launch(batch, hq, hkv, d, longest, context):
     assert lib.teeny_kv_cache_attention_workspace_size(tokens, batch, hq, hkv, d, longest, context, ctypes.byref(n)) == _lib.OK
     splits = n.value // (units * block * (d + 2) * 4)
     assert splits > 1 and units * splits < (1 << 31) // 256
+
+
+@pytest.mark.parametrize("group", [(1 << 63), (1 << 64) + 32, (1 << 64) + 128, 3 << 64])
+def test_w4_group_size_beyond_64_bits(group):
+    """Cut to 64 bits it would be another group size, whose scales the buffers do not hold."""
+    with pytest.raises(ValueError):
+        K.w4a16_dims((3, 264), (7, 192), (7, 1), group)
+    with pytest.raises(ValueError):
+        K.W4A16LinearRuntimeOp(group)
+    assert K.w4a16_dims((3, 264), (7, 192), (7, 1), (1 << 63) - 128) == (3, 7, 264)
