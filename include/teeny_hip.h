@@ -557,9 +557,11 @@ teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_len
 /* The write: k, v bf16 [n_tokens, kv_heads, head_dim] (rows k_stride and
  * v_stride elements apart, multiples of 8) into the slots (negative: the token
  * is skipped).  A page's scale becomes max(scale, amax / 127) over its tokens,
- * codes that it held become rint(code * scale / new scale), new ones
- * rint(x / new scale).  A write that begins at a page's first slot forgets what
- * the page held, so pages are used again without clearing.  A page and head
+ * codes of the tokens before the new ones become rint(code * scale / new scale),
+ * new ones rint(x / new scale).  A write that begins at a page's first slot
+ * forgets what the page held, so pages are used again without clearing.  One
+ * that begins further on ends the sequence there: codes behind the new tokens
+ * stay as they are and are worth nothing under the new scale.  A page and head
  * that meets an infinity or NaN holds NaN (codes 0 under that scale) until then.
  * A page's new tokens are consecutive rows at consecutive slots, as the plan
  * lays them out; a call that names a page in two places, or a slot twice, is

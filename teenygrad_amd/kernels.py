@@ -1449,7 +1449,8 @@ def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_
 def kv_cache_write(k: Buffer, v: Buffer, slots: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer,
                    v_scale: Buffer, stream: Optional[Stream] = None) -> None:
     """Tokens k, v bf16 [n_tokens, kv_heads, head_dim] into the 8-bit cache at `slots` (int32; negative: skipped).  The
-    pages' codes and scales are updated in place; a page's new tokens are consecutive rows and slots."""
+    pages' codes and scales are updated in place; a page's new tokens are consecutive rows and slots, and what the page
+    held behind them counts no longer."""
     pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
     t = slots.numel
     if not k.shape == v.shape == (t, heads, d):

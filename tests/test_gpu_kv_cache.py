@@ -560,3 +560,30 @@ def test_attention_of_the_largest_launch(dev):
     assert size > 1 << 35
     with stream_workspace(dev, size):
         check_attn(c, run_attn(dev, c, hint=(1, most)))
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("d", [64, 128])
+def test_write_over_refused_tokens(dev, page, d):
+    """Drafts are written, some are refused, and others take their slots: what is before them takes the page's scale,
+    what is behind them keeps its codes, and attention over the tokens that count reads none of it."""
+    rng = np.random.default_rng(page + d)
+    heads, slots = 2, np.arange(page, 2 * page - 2, dtype=np.int32)  # the second page, but for two slots
+    cache = [np.zeros((2, heads, page, d), np.int8), np.zeros((2, heads, d, page), np.int8)] + [np.zeros((2, heads), np.float32)] * 2
+
+    def tokens(n, most):
+        return {m: from_bf16(to_bf16((most * rng.uniform(-1, 1, (n, heads, d))).astype(np.float32))) for m in "kv"}
+
+    first, second = tokens(len(slots), 1.0), tokens(3, 9.0)
+    cache = check_write(dev, first, slots, *cache)
+    after = check_write(dev, second, slots[5:8], *cache)
+    assert (after[2][1] > 5 * cache[2][1]).all()  # a larger scale
+    np.testing.assert_array_equal(after[0][1, :, 8:], cache[0][1, :, 8:])
+    np.testing.assert_array_equal(after[1][1, :, :, 8:], cache[1][1, :, :, 8:])
+    for codes, scale, name in ((after[0][1], after[2][1], "k"), (after[1][1].transpose(0, 2, 1), after[3][1], "v")):
+        want = np.concatenate([first[name][:5], second[name]]).transpose(1, 0, 2)
+        # half a step of the old scale, at most a fifth of the new one, and half of the new one
+        assert (np.abs(codes[:, :8] * scale[:, None, None] - want) <= 0.61 * scale[:, None, None]).all()
+    c = dict(q=from_bf16(to_bf16(rng.standard_normal((1, heads, d)).astype(np.float32))), kc=after[0], vc=after[1], ks=after[2], vs=after[3],
+             table=np.array([[1]], np.int32), ctx=np.array([8], np.int32), starts=np.array([0, 1], np.int32))
+    check_attn(c, run_attn(dev, c, hint=(1, page)))
