@@ -535,8 +535,12 @@ teeny_status teeny_attention_backward_workspace_size(int64_t batch, int64_t q_he
  * new tokens takes what its row still needs, in request order from the top of
  * the stack, and its row of block_table gets them.  A request is refused, with
  * all of its tokens, if its row or the step would be too long (max_pages;
- * n_tokens) or if the pages that it and the requests before it need exceed
- * those there are.  Outputs:
+ * n_tokens) or if it needs pages and those that it and the requests before it
+ * need exceed those there are.  A request knows its pages by seq_lens alone: to
+ * take tokens back (drafts that were refused) the caller lowers seq_lens[b] and,
+ * before the next plan, puts the pages of the row from
+ * ceil(seq_lens[b] / page_size) on back on the stack itself (free_list[
+ * free_count[0]++]); they are lost to the pool otherwise.  Outputs:
  *   q_starts [batch + 1]  first row of each request's tokens (refused or not;
  *                         at most n_tokens)
  *   slots, positions [n_tokens]  of each row; -1 for refused tokens and for

@@ -1415,7 +1415,8 @@ def kv_cache_plan(new_lens: Buffer, seq_lens: Buffer, block_table: Buffer, free_
     back to and come from the stack free_list[:free_count], block_table [batch, max_pages] is filled in.  Returns
     (slots, positions, q_starts, context_lens, granted, free_after), int32; n_tokens rows of slots and positions (with
     `slots` given: as many as it has).  context_lens=seq_lens, granted=new_lens and free_after=free_count update in
-    place.  A request that does not fit is refused as a whole: granted 0, slots -1."""
+    place.  A request that does not fit is refused as a whole: granted 0, slots -1.  Who lowers seq_lens to take tokens back
+    puts the row's pages past the new end back on the stack before the next plan."""
     b = new_lens.numel
     if len(block_table.shape) != 2 or block_table.shape[0] != b or seq_lens.numel != b or free_count.numel != 1:
         raise ValueError(f"kv_cache_plan: block_table must be [{b}, max_pages], seq_lens [{b}], free_count [1]")

@@ -587,3 +587,30 @@ def test_write_over_refused_tokens(dev, page, d):
     c = dict(q=from_bf16(to_bf16(rng.standard_normal((1, heads, d)).astype(np.float32))), kc=after[0], vc=after[1], ks=after[2], vs=after[3],
              table=np.array([[1]], np.int32), ctx=np.array([8], np.int32), starts=np.array([0, 1], np.int32))
     check_attn(c, run_attn(dev, c, hint=(1, page)))
+
+
+def test_plan_after_refused_tokens(dev):
+    """Five drafts a step, some taken back: within a page nothing else is to do, pages past the new end go back on the
+    stack, and over many steps none is lost or held twice."""
+    rng = np.random.default_rng(16)
+    batch, page, width, pages = 6, 16, 20, 100
+    table, stack, count, seq = np.full((batch, width), -1, np.int32), rng.permutation(pages).astype(np.int32), pages, np.zeros(batch, np.int32)
+    for step in range(60):
+        new = np.where(seq > 250, -1, np.where(seq == 0, rng.integers(1, 40, batch), 5)).astype(np.int32)
+        bufs = [ints(dev, new), ints(dev, seq), dev.upload(table), ints(dev, stack), ints(dev, [count])]
+        slots, _, starts, context, granted, left = [b.to_host() for b in K.kv_cache_plan(*bufs, page, n_tokens=int(new.clip(0).sum()))]
+        ref, table, stack = kv.plan(new, seq, table, stack, count, page, len(slots))
+        np.testing.assert_array_equal(granted, new.clip(0))
+        for name, got in (("slots", slots), ("context_lens", context), ("free_after", left)):
+            np.testing.assert_array_equal(got, ref[name], err_msg=name)
+        np.testing.assert_array_equal(bufs[2].to_host(), table)
+        seq, count = context, int(left[0])
+        back = np.where(new == 5, rng.integers(0, 6, batch), 0)
+        for b in range(batch):
+            for i in range(kv.pages_of(seq[b] - back[b], page), kv.pages_of(seq[b], page)):
+                stack[count] = table[b, i]
+                count += 1
+        seq = (seq - back).astype(np.int32)
+        held = [table[b, i] for b in range(batch) for i in range(kv.pages_of(seq[b], page))]
+        assert sorted(held + stack[:count].tolist()) == list(range(pages))
+    assert step == 59 and (seq > 0).any()
