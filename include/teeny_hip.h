@@ -565,10 +565,15 @@ teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_len
  * new ones rint(x / new scale).  A write that begins at a page's first slot
  * forgets what the page held, so pages are used again without clearing.  One
  * that begins further on ends the sequence there: codes behind the new tokens
- * stay as they are and are worth nothing under the new scale.  A page and head
- * that meets an infinity or NaN holds NaN (codes 0 under that scale) until then.
- * A page's new tokens are consecutive rows at consecutive slots, as the plan
- * lays them out; a call that names a page in two places, or a slot twice, is
+ * stay as they are and are worth nothing under the new scale.  Each growth of a
+ * scale rounds the older codes again: a token is off by at most half the sum of
+ * the scales that its page and head have had from its own write on, so by half a
+ * step in a page written at once.  (Normal values, pages of 16 / 128: rms error
+ * 0.0084 / 0.0095 written at once, 0.0104 / 0.0125 token by token.  Magnitudes
+ * that creep up by 0.4 % a token are the worst: 7 / 50 steps for the first one.)
+ * A page and head that meets an infinity or NaN holds NaN (codes 0 under that
+ * scale) until it is begun anew.  A page's new tokens are consecutive rows at
+ * consecutive slots, as the plan lays them out; a call that names a page in two places, or a slot twice, is
  * out of contract (the page's contents are then unspecified).  head_dim 64 or
  * 128; at most 2^27 tokens; 16-byte aligned tensors. */
 teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *slots, int8_t *k_cache, int8_t *v_cache,

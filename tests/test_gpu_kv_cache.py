@@ -614,3 +614,32 @@ def test_plan_after_refused_tokens(dev):
         held = [table[b, i] for b in range(batch) for i in range(kv.pages_of(seq[b], page))]
         assert sorted(held + stack[:count].tolist()) == list(range(pages))
     assert step == 59 and (seq > 0).any()
+
+
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("growth", ["none", "slow", "twice"])
+def test_write_rounds_at_every_growth(dev, page, growth):
+    """A page filled token by token.  A code is rounded when it is written and whenever its page's scale grows: a token is
+    off by at most half the sum of the scales that its page has had since."""
+    rng = np.random.default_rng(page)
+    heads, d = 2, 64
+    bufs = [dev.upload(a) for a in (np.zeros((1, heads, page, d), np.int8), np.zeros((1, heads, d, page), np.int8),
+                                    np.zeros((1, heads), np.float32), np.zeros((1, heads), np.float32))]
+    said = {n: np.zeros((heads, page, d)) for n in "kv"}
+    since = {n: np.zeros((heads, page)) for n in "kv"}  # the sum of the scales since the token was written
+    last = {n: np.zeros(heads) for n in "kv"}
+    for t in range(page):
+        most = 2.0 ** (t % 100 - 50) if growth == "twice" else 1.004 ** t if growth == "slow" else 1.0
+        x = {n: from_bf16(to_bf16((most * np.sign(rng.uniform(-1, 1, (1, heads, d))) * (rng.uniform(0, 1, (1, heads, d)) if growth == "none" else 1))
+                                  .astype(np.float32))) for n in "kv"}
+        K.kv_cache_write(dev.upload(to_bf16(x["k"]), bf16), dev.upload(to_bf16(x["v"]), bf16), ints(dev, [t]), *bufs)
+        kc, vc, ks, vs = [b.to_host()[0].astype(np.float64) for b in bufs]
+        for n, codes, scale in (("k", kc, ks), ("v", vc.transpose(0, 2, 1), vs)):
+            said[n][:, t] = x[n][0]
+            grown = scale > last[n]
+            since[n][:, :t] += np.where(grown, scale, 0)[:, None]
+            since[n][:, t] = scale
+            last[n] = scale
+            # (codes are at most 127: their fp32 quotients and ratios are off by less than 2^-15)
+            off = np.abs(codes[:, :t + 1] * scale[:, None, None] - said[n][:, :t + 1])
+            assert (off <= ((0.5 + 2.0 ** -15) * since[n][:, :t + 1])[..., None]).all()
