@@ -433,7 +433,10 @@ teeny_status teeny_kv_cache_plan(const int32_t *new_lens, const int32_t *seq_len
   KvPlanArgs p{new_lens, seq_lens, block_table, free_list, free_count, q_starts, slots, positions, context_lens, granted,
                free_after, static_cast<int>(batch), static_cast<int>(max_pages), static_cast<int>(num_pages), shift,
                static_cast<int>(n_tokens), 1, 1};
-  // threads for the requests' sums, workgroups for two items (tokens and pages) to a token
+  // Threads for the requests' sums, workgroups for two items (tokens and pages) to a token.  How many pages come back is
+  // on the device: where few tokens stand against many of them, one workgroup moves 1024 in 3 us, one round of searches
+  // and loads after the other (256 requests, 256 tokens, us with 0 / 20 / 200 requests that end with 500 pages each: 5 /
+  // 33 / 290).
   const int threads = batch > 256 ? 1024 : 256;
   const auto kern = batch > 256 ? kv_plan<1024> : kv_plan<256>;
   const unsigned grid = static_cast<unsigned>(

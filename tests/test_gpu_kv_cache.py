@@ -643,3 +643,27 @@ def test_write_rounds_at_every_growth(dev, page, growth):
             # (codes are at most 127: their fp32 quotients and ratios are off by less than 2^-15)
             off = np.abs(codes[:, :t + 1] * scale[:, None, None] - said[n][:, :t + 1])
             assert (off <= ((0.5 + 2.0 ** -15) * since[n][:, :t + 1])[..., None]).all()
+
+
+@pytest.mark.parametrize("batch,ended", [(40, 36), (256, 200), (400, 390)])
+def test_plan_of_many_endings(dev, batch, ended):
+    """A step of few tokens in which nearly all requests end, with long rows: their pages in request and row order."""
+    rng = np.random.default_rng(batch)
+    page, width = 16, 120
+    seq = rng.integers(60 * page, width * page - 1, batch).astype(np.int32)
+    new = np.ones(batch, np.int32)
+    new[rng.permutation(batch)[:ended]] = -1
+    table, pages, spare = make_table(rng, seq, page, width, extra=3)
+    stack = np.zeros(pages, np.int32)
+    stack[:len(spare)] = spare
+    tokens = batch - ended
+    ref, ref_table, ref_stack = kv.plan(new, seq, table, stack, len(spare), page, tokens)
+    for in_place in (False, True):
+        bufs = [ints(dev, new), ints(dev, seq), dev.upload(table), ints(dev, stack), ints(dev, [len(spare)])]
+        over = dict(context_lens=bufs[1], granted=bufs[0], free_after=bufs[4]) if in_place else {}
+        out = dict(zip(NAMES, K.kv_cache_plan(*bufs, page, n_tokens=tokens, **over)))
+        for n in NAMES:
+            np.testing.assert_array_equal(out[n].to_host(), ref[n], err_msg=n)
+        np.testing.assert_array_equal(bufs[2].to_host(), ref_table)
+        left = int(ref["free_after"][0])
+        np.testing.assert_array_equal(bufs[3].to_host()[:left], ref_stack[:left])
