@@ -1470,7 +1470,7 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     """Attention of q bf16 [n_tokens, q_heads, head_dim] over the 8-bit cache -> o like q.  Sequence b's queries are rows
     q_starts[b] .. q_starts[b + 1] - 1 (None: one each), the last of its context_lens[b] tokens.  max_q_len and
     max_context (host numbers; default: the mean of the queries, and a whole row of the table) choose how the work is
-    cut, not the result."""
+    cut, for all sequences alike, not the result: numbers near the true ones are the fast ones."""
     pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
     if not (len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16):
         raise ValueError("kv_cache_attention: q bf16 [n_tokens, q_heads, head_dim]")

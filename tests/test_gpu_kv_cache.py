@@ -667,3 +667,30 @@ def test_plan_of_many_endings(dev, batch, ended):
         np.testing.assert_array_equal(bufs[2].to_host(), ref_table)
         left = int(ref["free_after"][0])
         np.testing.assert_array_equal(bufs[3].to_host()[:left], ref_stack[:left])
+
+
+def test_attention_of_a_mixed_step(dev):
+    """Prompts and single tokens: in one call under either hint, and in a call each over its part of the sequences and the
+    whole of q and o."""
+    rng = np.random.default_rng(17)
+    ctx, new = [900, 260, 30, 1200, 77, 0, 515, 64, 700], [300, 130, 1, 1, 1, 1, 1, 1, 1]
+    hq, hkv, d, page = 8, 2, 128, 16
+    c = attn_case(rng, ctx, new, hq, hkv, d, page)
+    t, b = int(c["starts"][-1]), len(ctx)
+    size = max(K.kv_cache_attention_workspace_size(t, b, hq, hkv, d, n, 1200) for n in (300, 48, 1))
+    for hint in ((300, 1200), (1, 1200), None):
+        with stream_workspace(dev, size):
+            check_attn(c, run_attn(dev, c, hint=hint, pad=2))
+    bufs = [dev.upload(to_bf16(c["q"]), bf16)] + [dev.upload(c[n]) for n in ("kc", "vc", "ks", "vs", "table")]
+    lens, starts = ints(dev, c["ctx"]), ints(dev, c["starts"])
+    o, lse = dev.upload(to_bf16(np.full(c["q"].shape, 123.0, np.float32)), bf16), dev.upload(np.full((t, hq), 55.0, np.float32))
+    width = c["table"].shape[1]
+    with stream_workspace(dev, size):
+        for first, n, longest in ((0, 2, 300), (2, b - 2, 1)):
+            check(lib.teeny_kv_cache_attention(*[x.ptr for x in bufs[:5]], bufs[5].ptr + 4 * width * first, lens.ptr + 4 * first,
+                                               starts.ptr + 4 * first, o.ptr, lse.ptr, t, n, hq, hkv, d, c["kc"].shape[0], page, width, longest,
+                                               1200, hq * d, 1 / math.sqrt(d), 1, None))
+            got = from_bf16(o.to_host())
+            if first == 0:
+                assert (got[430:] == 123.0).all() and (got[:430] != 123.0).any()
+    check_attn(c, (got, lse.to_host()))
