@@ -248,8 +248,10 @@ __global__ __launch_bounds__(256) void w4_pack(const int8_t *q, uint32_t *out, i
   out[at] = v;
 }
 
-// Packed weights -> bf16 [N, K], rounded once; one word per thread.  11008 x 4096
-// take 21 us, 113 MB: the copy rate.
+// Packed weights -> bf16 [N, K], rounded once (group scales do not come out of the
+// tiles' sums over all of K): the rms error against 64 bits goes from 0.0017, the
+// output's own rounding, to 0.0023.  One word per thread.  11008 x 4096 take 21 us,
+// 113 MB: the copy rate.
 template <bool ZERO>
 __global__ __launch_bounds__(256) void w4_unpack(W4Args p, bf16 *out, int64_t words) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;

@@ -19,7 +19,10 @@
 // a lane in whole 64-byte pieces, each byte to one lane: no LDS and no barrier
 // in the loop.  Codes go to bf16 (exact) in registers, scales are applied in
 // fp32: K's to the scores, V's to the probability before its rounding to bf16
-// (the one rounding on the way; the row sum takes the unrounded probability).
+// (the one rounding on the way, since the second product's operands are bf16: two
+// bf16 parts would double that product; the row sum takes the unrounded
+// probability).  It takes the rms error against 64 bits from 0.0017, the output's
+// own rounding, to 0.0023.
 // 64 contexts of 90 to 8000 tokens, 8 K/V heads of 128 and one query each, take
 // 112 us (532 MB, 0.94 of the copy rate); one of 2000 tokens 10 us, where a wave's
 // round of dependent work is 1.9 us and every load is waited for.
@@ -422,6 +425,7 @@ __global__ __launch_bounds__(256, NQ == 1 && D == 64 ? 4 : 2) void kv_attn(KvAtt
 // block of 32 tokens are tokens 16 g .. 16 g + 15 of one query, one page.
 // 700 queries of 32 heads of 128 for each of four contexts of 1100 to 4100 tokens:
 // 144 us (319 with kv_attn), 647 TFLOP/s; 823 where contexts are of one length.
+// (Calls in a row; one after a pause takes 161.)
 template <int D>
 __global__ __launch_bounds__(256, 2) void kv_attn_tile(KvAttnArgs p) {
   constexpr int RB = 128, NS = D / 16, ND = D / 32, NU = D / 64, FR = 2 * NS + 4 * ND;
