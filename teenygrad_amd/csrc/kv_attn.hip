@@ -741,29 +741,31 @@ __global__ __launch_bounds__(256) void kv_attn_combine(KvAttnArgs p) {
 // round is 1.9 us of dependent work, a row's other parts 0.04 us each), two rounds
 // where the device is busier, from three rounds on; more workgroups than two to a
 // CU (one where there are few: their parts count) only where contexts may differ
-// much in length.  us by splits, 8 K/V heads of 128, one query: 1 x 600 1 / 3 10.6 /
-// 9.9; 1 x 2000 1 / 4 / 8 20 / 12.5 / 10.7; 1 x 30000 16 / 32 / 64 28 / 21.7 / 23.3;
-// 4 x 2000 4 / 8 13.4 / 12.1; 8 x 1000 1 / 2 / 4 14.4 / 13.7 / 12.3; 8 x 4000 4 / 6 /
-// 8 20.9 / 22.4 / 20.4; 16 x 1000 1 / 2 / 4 14.6 / 15.8 / 15.4; 16 x 4000 2 / 4 / 8 33 /
-// 33 / 36; 32 x 2000 1 / 2 28.8 / 33.3, but 32 x 100 to 8000 1 / 2 / 3 83 / 71 / 65; 64
-// x 90 to 8000 1 / 2 / 3 / 4 116 / 126 / 112 / 117.  Several long contexts, which may
-// differ, get a split for each 2560 tokens, so three from 7680 on: 64 x 90 to 12000 1 /
-// 3 / 4 / 5 172 / 162 / 167 / 164 (but 64 x 8000 187 / 195 / 196 / 201), 16 x 90 to 20000
-// 4 / 5 / 7 / 10 86 / 79 / 94 / 86, 4 x 1000 to 40000 6 / 8 / 10 / 15 59 / 48 / 55 / 43.  Two
-// never paid on two workgroups a CU (1 / 2 / 3: 64 x 90 to 5200 80 / 87 / 82, to 6400 96 /
-// 104 / 96, to 7600 113 / 120 / 112, 64 x 6400 151 / 158 / 160), but on four (128 x 90 to
-// 6400 184 / 177 / 177; on six 200 x 90 to 5200 216 / 219 / 225).  One sequence alone has
-// nothing to even out: 1 x 30000, 64 heads, 8 / 11 96 / 110, 1 x 60000, 32 heads, 16 / 23
-// 96 / 117.  Shared tiles: 1 x 64 queries x
-// 16000 1 / 8 / 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads of 64, 1 / 4 / 8 /
-// 16 145 / 49 / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242 / 180 / 139 / 160; 4 x
-// 700 x 1100 to 4100 1 / 2 160 / 193; with the split for 2560 tokens 15 x 100 x 300 to 6400
-// 1 / 2 / 3 197 / 167 / 183 (of 6400 255 / 286 / 290), 1 x 3000 x 16000, 16 heads of 64, 1 /
-// 3 / 6 / 10 453 / 375 / 363 / 383, 1 x 1900 x 6400 1 / 2 223 / 255, 1 x 1500 x 8000 1 / 3 281 /
-// 274.  Several sequences on a busy device get half as
-// many again, since contexts seldom are of one length: 16 x 40 x 1000 to 6000 2 / 3 /
-// 4 133 / 101 / 125, of 4000 104 / 116 / 110; 20 x 40 x 300 to 4000 1 / 2 125 / 97, of
-// 2000 88 / 98.
+// much in length.  us by splits, 8 K/V heads of 128, one query: 1 x 600 1 / 3 10.6
+// / 9.9; 1 x 2000 1 / 4 / 8 20 / 12.5 / 10.7; 1 x 30000 16 / 32 / 64 28 / 21.7 /
+// 23.3; 4 x 2000 4 / 8 13.4 / 12.1; 8 x 1000 1 / 2 / 4 14.4 / 13.7 / 12.3; 8 x 4000
+// 4 / 6 / 8 20.9 / 22.4 / 20.4; 16 x 1000 1 / 2 / 4 14.6 / 15.8 / 15.4; 16 x 4000 2
+// / 4 / 8 33 / 33 / 36; 32 x 2000 1 / 2 28.8 / 33.3, but 32 x 100 to 8000 1 / 2 / 3
+// 83 / 71 / 65; 64 x 90 to 8000 1 / 2 / 3 / 4 116 / 126 / 112 / 117.  Several long
+// contexts, which may differ, get a split for each 2560 tokens, so three from 7680
+// on: 64 x 90 to 12000 1 / 3 / 4 / 5 172 / 162 / 167 / 164 (but 64 x 8000 187 / 195
+// / 196 / 201), 16 x 90 to 20000 4 / 5 / 7 / 10 86 / 79 / 94 / 86, 4 x 1000 to
+// 40000 6 / 8 / 10 / 15 59 / 48 / 55 / 43.  Two do not pay where the unsplit call
+// just fills two workgroups a CU (1 / 2 / 3: 64 x 90 to 5200 80 / 87 / 82, to 6400
+// 96 / 104 / 96, to 7600 113 / 120 / 112, 64 x 6400 151 / 158 / 160, 56 x 90 to
+// 6400 90 / 95 / 90), but with fewer and with more (90 to 6400: 48 x 86 / 85 / 84,
+// 80 x 126 / 121 / 119, 96 x 150 / 144 / 139, 128 x 184 / 177 / 177; 200 x 90 to
+// 5200 216 / 219 / 225).  One sequence alone has nothing to even out: 1 x 30000, 64
+// heads, 8 / 11 96 / 110, 1 x 60000, 32 heads, 16 / 23 96 / 117.  Shared tiles: 1 x
+// 64 queries x 16000 1 / 8 / 16 / 32 488 / 76 / 60 / 52; 2 x 128 x 6000, 16 heads
+// of 64, 1 / 4 / 8 / 16 145 / 49 / 39 / 46; 8 x 100 x 300 to 8000 1 / 2 / 3 / 4 242
+// / 180 / 139 / 160; 4 x 700 x 1100 to 4100 1 / 2 160 / 193; with the split for
+// 2560 tokens 15 x 100 x 300 to 6400 1 / 2 / 3 197 / 167 / 183 (of 6400 255 / 286 /
+// 290), 1 x 3000 x 16000, 16 heads of 64, 1 / 3 / 6 / 10 453 / 375 / 363 / 383, 1 x
+// 1900 x 6400 1 / 2 223 / 255, 1 x 1500 x 8000 1 / 3 281 / 274.  Several sequences
+// on a busy device get half as many again, since contexts seldom are of one length:
+// 16 x 40 x 1000 to 6000 2 / 3 / 4 133 / 101 / 125, of 4000 104 / 116 / 110; 20 x
+// 40 x 300 to 4000 1 / 2 125 / 97, of 2000 88 / 98.
 struct KvAttnPlan {
   bool tile = false;
   int nq = 1, rb = 16;
@@ -788,7 +790,8 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   if (pl.tile) splits = std::min((batch > 1 && 2 * busy > cus ? 3 : 2) * cus / busy, max_ctx / least);
   else if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
   const int64_t pieces = max_ctx / 2560;
-  if (pl.tile ? busy < 2 * cus : busy >= 32 && batch > 1 && (pieces > 2 || busy >= 4 * cus)) splits = std::max(splits, pieces);
+  const bool two = pl.tile || 5 * busy <= 8 * cus || busy > 2 * cus;  // whether two splits may pay
+  if (pl.tile ? busy < 2 * cus : busy >= 32 && batch > 1 && (pieces > 2 || two)) splits = std::max(splits, pieces);
   // a launch has less than 2^31 threads (the limit of rows leaves room for four splits at least)
   splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / 256 - 1) / units));
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };

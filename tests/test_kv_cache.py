@@ -215,10 +215,11 @@ def test_w4_group_size_beyond_64_bits(group):
 
 @pytest.mark.parametrize("batch,hq,hkv,d,context,splits", [
     (64, 32, 8, 128, 5000, 1), (64, 32, 8, 128, 5200, 1), (64, 32, 8, 128, 7600, 1), (64, 32, 8, 128, 8000, 3), (128, 32, 8, 128, 6400, 2),
+    (48, 32, 8, 128, 6400, 2), (56, 32, 8, 128, 6400, 1), (80, 32, 8, 128, 6400, 2),
     (1, 64, 64, 128, 30000, 8), (1, 64, 32, 128, 60000, 16), (4, 32, 8, 128, 60000, 23)])
 def test_attention_splits_of_long_contexts(batch, hq, hkv, d, context, splits):
-    """Contexts that may differ in length get a split for each 2560 tokens, but not two of them where the unsplit call has two
-    workgroups a CU, and no more than the device holds where there is one sequence."""
+    """Contexts that may differ in length get a split for each 2560 tokens, but not two of them where the unsplit call just fills
+    two workgroups a CU, and no more than the device holds where there is one sequence."""
     n = ctypes.c_size_t(0)
     assert lib.teeny_kv_cache_attention_workspace_size(batch, batch, hq, hkv, d, 1, context, ctypes.byref(n)) == _lib.OK
     units = (batch * (hq // hkv) // 16 + batch) * hkv
