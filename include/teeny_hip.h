@@ -598,13 +598,14 @@ teeny_status teeny_kv_cache_write(const void *k, const void *v, const int32_t *s
  * all sequences of the call alike; longer ones are computed all the same.  With a
  * stream workspace of teeny_kv_cache_attention_workspace_size bytes for the same
  * hints a sequence's tokens are shared out over the device, with a smaller one
- * they are not.  Hints near the truth are the fast ones: one context of 2000 tokens
- * takes 11 us under a max_context of 2000 to 8000, 16 under 32768, 22 under
- * 131072 (32 / 8 heads of 128).  Prompts and single tokens are faster in calls of
- * their own, each over its part of q_starts, block_table and context_lens and the
- * whole q and o: 700 queries and 63 single tokens over up to 8000 tokens take 98 and
- * 114 us, together 253.  head_dim 64 or 128; 16-byte aligned tensors; num_pages *
- * kv_heads below 2^29, (n_tokens * q_heads + 128 * batch * kv_heads) below 2^25. */
+ * over as many workgroups as it has room for.  Hints near the truth are the fast
+ * ones: one context of 2000 tokens takes 11 us under a max_context of 2000 to
+ * 8000, 16 under 32768, 22 under 131072 (32 / 8 heads of 128).  Prompts and single
+ * tokens are faster in calls of their own, each over its part of q_starts,
+ * block_table and context_lens and the whole q and o: 700 queries and 63 single
+ * tokens over up to 8000 tokens take 98 and 114 us, together 253.  head_dim 64 or
+ * 128; 16-byte aligned tensors; num_pages * kv_heads below 2^29, (n_tokens *
+ * q_heads + 128 * batch * kv_heads) below 2^25. */
 teeny_status teeny_kv_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scale,
                                       const float *v_scale, const int32_t *block_table, const int32_t *context_lens,
                                       const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,

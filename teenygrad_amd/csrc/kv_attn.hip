@@ -802,7 +802,10 @@ static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int
   };
   cut(splits);
   pl.most = size(splits);
-  if (pl.bytes > scratch) cut(1);
+  if (pl.bytes > scratch) {  // as many parts as it holds
+    const int64_t fit = static_cast<int64_t>(scratch / (static_cast<size_t>(units) * pl.rb * (D + 2) * 4));
+    cut(std::max<int64_t>(1, fit == 2 && !two ? 1 : fit));
+  }
   return pl;
 }
 

@@ -694,3 +694,23 @@ def test_attention_of_a_mixed_step(dev):
             if first == 0:
                 assert (got[430:] == 123.0).all() and (got[:430] != 123.0).any()
     check_attn(c, (got, lse.to_host()))
+
+
+@pytest.mark.parametrize("ctx,new,hq,hkv", [([4500], 1, 8, 2), ([3000, 700], 7, 8, 2), ([9000, 60], 40, 4, 2)])
+@pytest.mark.parametrize("part", [0.9, 0.4])
+def test_attention_in_part_of_its_workspace(dev, ctx, new, hq, hkv, part):
+    """A workspace that does not hold all the parts that were planned holds fewer; nothing outside of it is written."""
+    c = attn_case(np.random.default_rng(ctx[0]), ctx, [new] * len(ctx), hq, hkv, 64, 16)
+    c["table"] = c["table"][:, :kv.pages_of(ctx[0], 16)]
+    size = K.kv_cache_attention_workspace_size(new * len(ctx), len(ctx), hq, hkv, 64, new, ctx[0])
+    assert size > 0
+    small = int(size * part) // 256 * 256
+    ws = dev.upload(np.full(size, 77, np.int8))
+    check(lib.teeny_hip_stream_set_workspace(None, ws.ptr, small))
+    try:
+        got = run_attn(dev, c, hint=(new, ctx[0]))
+    finally:
+        NULL_STREAM.set_workspace(None)
+    held = ws.to_host()
+    assert (held[:small] != 77).any() and (held[small:] == 77).all()
+    check_attn(c, got)
