@@ -616,6 +616,56 @@ teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t b
                                                      int64_t head_dim, int64_t max_q_len, int64_t max_context,
                                                      size_t *bytes);
 
+/* ── 4-bit paged K/V cache ────────────────────────────────────────────────
+ * Half the bytes of the 8-bit cache for the same plan (teeny_kv_cache_plan).  No
+ * counterpart in the reference.  A token of one head is held in groups of 64
+ * numbers (head_dim 64 or 128) with a bf16 scale each.  Of a group's numbers m is
+ * the one of largest magnitude (of two, the positive one): the scale is -m / 8
+ * rounded to five significant bits (nearest even; 0 where |m| < 2^-90, NaN where
+ * the group holds an infinity or NaN), a code rint(x / scale) in -8..7 (the fp32
+ * quotient).  A number is off by at most half a step, but one of the sign
+ * opposite to m's, above 7.5 steps, is held as 7: by at most 1.25 (normal values:
+ * rms error 0.095 of the standard deviation).  Layouts, bytes: k_cache
+ * [num_pages, kv_heads, page_size, head_dim / 2], of NG = head_dim / 64 groups the
+ * 32-bit word 2 NG g + 2 G + j of a token holds group G's numbers 16 g + 8 j +
+ * 0..7; v_cache [num_pages, kv_heads, page_size / 16, head_dim, 8], word h of a d
+ * holds tokens 8 h + 0..7 of the 16; code + 8 in a word's nibbles 0, 4, 1, 5, 2, 6,
+ * 3, 7 in this order; scales bf16 [num_pages, kv_heads, page_size, NG].
+ *
+ * The append: rows of q [n_tokens, q_heads, head_dim] and k, v [n_tokens, kv_heads,
+ * head_dim] (bf16, rows *_stride elements apart, multiples of 8) belong to tokens
+ * at `positions` (negative: the row is skipped).  Numbers i and i + rotary_dim / 2
+ * of a head of q and k (interleaved: 2 i and 2 i + 1) are rotated by the angle
+ * position * inv_freq[i] (fp32 [rotary_dim / 2]; the product, its cosine and sine
+ * in 64 bits), further numbers stay.  Rotated q goes to q_out (dense, rounded once;
+ * may be q where q is dense), k (rotated in 64 bits, rounded to fp32) and v into
+ * the slots (negative or beyond the cache: only q's row is written).  Other tokens
+ * of the page keep their codes.  The new tokens of 16 slots that begin at a
+ * multiple of 16 are consecutive rows at consecutive slots, as the plan lays them
+ * out; otherwise V's codes of those 16 are unspecified.  rotary_dim a multiple of
+ * 16 up to head_dim (0: no rotation, inv_freq may be NULL); at most 2^24 tokens;
+ * q_heads 0: no queries; 16-byte aligned tensors. */
+teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v, const int32_t *positions,
+                                    const int32_t *slots, const float *inv_freq, void *q_out, int8_t *k_cache,
+                                    int8_t *v_cache, void *k_scale, void *v_scale, int64_t n_tokens, int64_t q_heads,
+                                    int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t num_pages,
+                                    int64_t page_size, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                    int32_t interleaved, teeny_stream stream);
+
+/* Attention over the 4-bit cache: arguments, results, hints and workspace as
+ * teeny_kv_cache_attention's (its size: teeny_kv4_cache_attention_workspace_size).
+ * Scales may have either sign, and any bf16 value.  An infinity in a row of q
+ * gives NaN in that row and head.  Scales 4-byte aligned. */
+teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const void *k_scale,
+                                       const void *v_scale, const int32_t *block_table, const int32_t *context_lens,
+                                       const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,
+                                       int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                       int64_t page_size, int64_t max_pages, int64_t max_q_len, int64_t max_context,
+                                       int64_t q_stride, float softmax_scale, int32_t causal, teeny_stream stream);
+teeny_status teeny_kv4_cache_attention_workspace_size(int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                      int64_t head_dim, int64_t max_q_len, int64_t max_context,
+                                                      size_t *bytes);
+
 /* ── int8 affine quantization (teeny-quant) ───────────────────────────────
  * Reference: quantize_affine(tensor, data, shape, granularity, symmetric,
  * bits) and dequantize_affine, utilities/teeny-quant/src/quant/affine.rs
@@ -733,6 +783,21 @@ teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, 
  * a chunk the 32-bit word 4 g + c holds k = 32 c + 8 g + 0..7, code + 8 in the
  * nibbles 0, 4, 1, 5, 2, 6, 3, 7 in this order. */
 teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t K, teeny_stream stream);
+
+/* Low-rank adapters of many requests beside a linear layer that they share:
+ * out[m] = y[m] + scale[a] B[a] (A[a] x[m]) with a = adapters[m]; out[m] = y[m]
+ * where that is negative or num_adapters or more.  x bf16 [M,K], a bf16
+ * [num_adapters, rank, K], b bf16 [num_adapters, N, rank], scale fp32
+ * [num_adapters] or NULL (1), y (the shared layer's output) and out (which may be
+ * y) bf16 [M,N]; rows of x, y and out x_stride, y_stride and out_stride elements
+ * apart.  Rows of an adapter need not lie together, but are faster so.  fp32 sums,
+ * the rank's products held in two bf16 parts (2^-17) for the second product; out
+ * is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
+ * zeros); K a multiple of 8; x, a, b and x's rows 16-byte aligned. */
+teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, const int32_t *adapters, const float *scale,
+                               const void *y, void *out, int64_t M, int64_t N, int64_t K, int64_t rank,
+                               int64_t num_adapters, int64_t x_stride, int64_t y_stride, int64_t out_stride,
+                               teeny_stream stream);
 
 /* W8A16 conv2d, NHWC bf16 activations, int8 weights [C_OUT,KH,KW,C_IN/G]
  * with per-output-channel fp32 scale, fp32 bias or NULL, bf16 output:

@@ -164,6 +164,9 @@ _SIGS = {
     "teeny_kv_cache_write": (S, [P] * 7 + [c_int64] * 7 + [P]),
     "teeny_kv_cache_attention": (S, [P] * 10 + [c_int64] * 11 + [c_float, c_int32, P]),
     "teeny_kv_cache_attention_workspace_size": (S, [c_int64] * 7 + [POINTER(c_size_t)]),
+    "teeny_kv4_cache_append": (S, [P] * 11 + [c_int64] * 10 + [c_int32, P]),
+    "teeny_kv4_cache_attention": (S, [P] * 10 + [c_int64] * 11 + [c_float, c_int32, P]),
+    "teeny_kv4_cache_attention_workspace_size": (S, [c_int64] * 7 + [POINTER(c_size_t)]),
     "teeny_quant_num_groups": (S, [POINTER(c_int64), c_int32, c_int32, c_int32, c_int64, POINTER(c_int64)]),
     "teeny_quantize_affine": (S, [P, POINTER(c_int64), c_int32, c_int32, c_int32, c_int64, c_int32, c_int32, P, P, P, P, P]),
     "teeny_dequantize_affine": (S, [P, P, P, POINTER(c_int64), c_int32, c_int32, c_int32, c_int64, P, P]),
@@ -172,6 +175,7 @@ _SIGS = {
     "teeny_w4a16_linear_forward": (S, [P] * 6 + [c_int64] * 4 + [c_int32, P]),
     "teeny_w4a16_linear_workspace_size": (S, [c_int64] * 4 + [POINTER(c_size_t)]),
     "teeny_pack_int4": (S, [P, P, c_int64, c_int64, P]),
+    "teeny_adapter_add": (S, [P] * 7 + [c_int64] * 8 + [P]),
     "teeny_linear_workspace_size": (S, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),
     "teeny_linear_backward": (S, [P] * 6 + [c_int64] * 14 + [c_int32, P]),
     "teeny_linear_backward_workspace_size": (S, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),

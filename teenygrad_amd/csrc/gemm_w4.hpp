@@ -35,18 +35,6 @@ struct W4Args {
   int vec;               // a chunk's scales and zero points are aligned vectors
 };
 
-// code of position j (0..7) of a word: nibble w4_nibble(j)
-__host__ __device__ constexpr int w4_nibble(int j) { return (j & 1) * 4 + (j >> 1); }
-
-__device__ __forceinline__ bf16x8 w4_values(uint32_t word) {
-  u32x4 r;
-  r[0] = ((word << 3) & 0x00780078u) | 0x3F803F80u;
-  r[1] = ((word >> 1) & 0x00780078u) | 0x3F803F80u;
-  r[2] = ((word >> 5) & 0x00780078u) | 0x3F803F80u;
-  r[3] = ((word >> 9) & 0x00780078u) | 0x3F803F80u;
-  return __builtin_bit_cast(bf16x8, r);
-}
-
 // Bound on few rows: reading the weights once.  A workgroup owns 16 NB output
 // columns and up to XR rows of x (blockIdx.y); its KW waves share out the
 // chunks of K and meet in LDS in wave order.  The weights come straight from

@@ -1,0 +1,357 @@
+// Attention over the 4-bit paged K/V cache (kv4_cache.hip), bf16 queries.
+//
+//   s = softmax_scale sum_G ks[token, G] (q_G . kq_G),  o_G = sum softmax(s) vs[token, G] vq_G
+//
+// G: groups of 64 numbers of a head.  Ragged batches, grouped heads and the
+// dealing out of rows, tokens and splits as in kv_attn.hip; no counterpart in the
+// reference (flash_attn2.rs:52-158 reads dense K and V).
+//
+// A wave takes 64 tokens a time, 16 to each of its four lane groups, as the rows
+// of S^T = K Q^T and the k's of O^T += V^T P^T on v_mfma_f32_16x16x32_bf16: lane
+// group g's scores are tokens 16 g .. 16 g + 15 of one query, and the
+// probabilities are the next product's operand in the registers they were made
+// in.  The cache is laid out for this: a lane's 16 bytes are its operands of one
+// token's K row, or of two of V's d's over 16 tokens, so codes come straight from
+// memory, each byte to one lane: no LDS and no barrier in the loop.
+//
+// Codes become the bf16 values (24 + code) / 16 with two instructions a pair
+// (w4_values), exact.  The 24/16 too much is -1.5 times the sum of q, which the
+// scores start from, and -1.5 times the sum of the weighted probabilities, one more
+// product with a constant operand.  Scales are applied in fp32: K's to the group's
+// scores, V's to the probability before its rounding to bf16 (the one rounding on
+// the way, as in kv_attn).  Lane c of a group holds the scale of the group's token
+// c, and the multiplication fetches it across the 16 lanes (row_newbcast).
+#include "kv4.hpp"
+#include "kv_attn.hpp"
+
+namespace teeny {
+
+struct Kv4AttnArgs : KvAttnArgs {
+  const bf16 *ks, *vs;
+};
+
+// NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
+template <int D, int NQ>
+__global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
+  constexpr int WK = 4, WROWS = 16 * NQ, RB = WROWS;
+  constexpr int NC = D / 32, ND = D / 16, NG = D / 64, NV = D / 32;  // k-steps of the scores, d blocks, groups, V vectors
+  constexpr int LD = D + 4;
+  typedef uint32_t kvec __attribute__((ext_vector_type(2 * NG)));
+  typedef __bf16 svec __attribute__((ext_vector_type(NG)));
+  __shared__ __attribute__((aligned(16))) float red[WK * WROWS * LD];
+  __shared__ float ml[2][WK][WROWS];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  // the blocks that the caller's lengths stand for come first, then those that there may be beyond, mostly none
+  const int per_block = p.splits * p.kv_heads, first = p.walk * per_block;
+  const bool beyond = static_cast<int>(blockIdx.x) >= first;
+  const int id = beyond ? blockIdx.x - first : xcd_remap(blockIdx.x, first), of = beyond ? p.blocks - p.walk : p.walk;
+  const int head = id / (p.splits * of), in_head = id - head * (p.splits * of), split = in_head / of;
+  KvRows r;
+  if (!kv_rows<RB>(p, in_head - split * of + (beyond ? p.walk : 0), r)) return;
+  // row i of the sequence: query i / group, head i % group of the K/V head's; it sees seen(i) tokens
+  auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
+  const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
+  // the last split takes what lies past the longest context that the caller expected
+  const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
+  if (split > 0 && kb >= k_end) return;
+
+  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
+  const int page_mask = (1 << p.shift) - 1;
+  struct Pages {
+    int k, v;  // pages of the lane's K rows and V columns, -1: none
+  };
+  auto page_at = [&](int t) {
+    const int pg = row[min(t, k_end - 1) >> p.shift];
+    return t < k_end && pg >= 0 && pg < p.pages ? pg : -1;
+  };
+  auto load_pages = [&](int t0) { return Pages{page_at(t0 + 16 * (c >> 2)), page_at(t0 + 16 * g)}; };
+  // a page's tokens of this head, as tokens of the whole cache
+  auto token_at = [&](int page, int t) {
+    return ((static_cast<int64_t>(max(page, 0)) * p.kv_heads + head) << p.shift) + (t & page_mask);
+  };
+  kvec kr[4];
+  u32x4 vr[NV];
+  svec ks, vs;
+  bool none = false;
+  auto load_k = [&](int t0, Pages pg) {
+    const int8_t *src = p.kc + (token_at(pg.k, t0 + 16 * (c >> 2)) + (c & 3)) * (D / 2) + (D / 8) * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const kvec *>(src + 4 * i * (D / 2));
+  };
+  auto load_v = [&](int t0, Pages pg) {
+    const int64_t at = token_at(pg.v, t0 + 16 * g);
+    const int8_t *src = p.vc + at * (D / 2) + 16 * c;
+#pragma unroll
+    for (int a = 0; a < NV; ++a) vr[a] = *reinterpret_cast<const u32x4 *>(src + 256 * a);
+    ks = *reinterpret_cast<const svec *>(p.ks + (at + c) * NG);
+    vs = *reinterpret_cast<const svec *>(p.vs + (at + c) * NG);
+    none = pg.v < 0;
+  };
+  constexpr int STEP = 64 * WK;
+  int t0 = kb + 64 * w;
+  Pages pg;
+  if (t0 < ke) {
+    pg = load_pages(t0);
+    load_k(t0, pg);
+    load_v(t0, pg);
+    pg = load_pages(t0 + STEP);
+  }
+
+  const float sc0 = 16.0f * fabsf(p.scale_log2);  // 16: of w4_values
+  const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
+  const u32x4 off_bits = u32x4{0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};  // -1.5
+  const bf16x8 off = __builtin_bit_cast(bf16x8, off_bits);
+  bf16x8 qf[NQ][NC];
+  f32x4 q_off[NQ][NG];  // -1.5 sum of q over the group, in every row
+  int vis[NQ];
+  int64_t out_row[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = min(r.row0 + 16 * n + c, r.rows - 1), t = i / p.group;
+    vis[n] = p.causal ? min(max(r.ctx - r.len + 1 + t, 0), r.ctx) : r.ctx;
+    const int h = head * p.group + i - t * p.group;
+    out_row[n] = static_cast<int64_t>(r.first + t) * p.heads + h;
+    const bf16 *at = p.q + (r.first + t) * p.q_stride + h * D;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      u32x4 raw = *reinterpret_cast<const u32x4 *>(at + (j >> 1) * 64 + g * 16 + (j & 1) * 8);
+      raw ^= qsign;
+      qf[n][j] = __builtin_bit_cast(bf16x8, raw);
+    }
+#pragma unroll
+    for (int G = 0; G < NG; ++G) {
+      q_off[n][G] = mfma16(off, qf[n][2 * G], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      q_off[n][G] = mfma16(off, qf[n][2 * G + 1], q_off[n][G]);
+    }
+  }
+  const int all_see = seen(r.row0);  // all rows see the tokens below it
+
+  f32x4 acc[NQ][ND], p_off[NQ][NG];  // p_off: -1.5 sum of the weighted probabilities, in every row
+  float m_run[NQ], l_run[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m_run[n] = -INFINITY;
+    l_run[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int G = 0; G < NG; ++G) p_off[n][G] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+#pragma unroll 1
+  for (; t0 < ke; t0 += STEP) {
+    float ksc[NG], vsc[NG];  // of the lane group's token c
+#pragma unroll
+    for (int G = 0; G < NG; ++G) {
+      ksc[G] = static_cast<float>(ks[G]) * sc0;
+      vsc[G] = static_cast<float>(vs[G]);
+    }
+    f32x4 s[NQ][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        const bf16x8 a0 = w4_values(kr[i][2 * G]), a1 = w4_values(kr[i][2 * G + 1]);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const f32x4 x = mfma16(a1, qf[n][2 * G + 1], mfma16(a0, qf[n][2 * G], q_off[n][G]));
+          each16([&](auto t) {
+            constexpr int T = decltype(t)::value;
+            if (T >> 2 == i) {
+              const float sc = row_lane<T>(ksc[G]);
+              s[n][i][T & 3] = G == 0 ? x[T & 3] * sc : __builtin_fmaf(x[T & 3], sc, s[n][i][T & 3]);
+            }
+          });
+        }
+      }
+    }
+    const bool more = t0 + STEP < ke;
+    const bool hidden = none;
+    if (more) load_k(t0 + STEP, pg);
+    const bool masks = t0 + 64 > all_see || __any(hidden);
+    const int at = t0 + 16 * g;  // the lane's first token
+    bf16x8 pb[NQ][NG][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      if (masks) {  // also the scores of scales that may be anything
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (hidden || at + i >= vis[n]) s[n][i >> 2][i & 3] = -INFINITY;
+      }
+      float mx = s[n][0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
+      mx = over_groups(mx, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
+        const float m_new = fmaxf(m_run[n], mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
+        l_run[n] *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
+#pragma unroll
+        for (int G = 0; G < NG; ++G) p_off[n][G] *= alpha;
+        m_run[n] = m_new;
+      }
+      const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[n][i >> 2][i & 3] + neg_m);
+        l_run[n] += e;
+        s[n][i >> 2][i & 3] = e;
+      }
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        float v[16];
+        each16([&](auto t) {
+          constexpr int T = decltype(t)::value;
+          v[T] = s[n][T >> 2][T & 3] * row_lane<T>(vsc[G]);
+        });
+        if (masks) {  // a hidden token's V scale may be anything
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (hidden || at + i >= vis[n]) v[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const bf16x2 pr = cvt_pk_bf16(v[i], v[i + 1]);
+          pb[n][G][i >> 3][i & 7] = pr[0];
+          pb[n][G][i >> 3][(i & 7) + 1] = pr[1];
+        }
+      }
+    }
+#pragma unroll
+    for (int G = 0; G < NG; ++G)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) p_off[n][G] = mfma16(off, pb[n][G][h], p_off[n][G]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const bf16x8 a = w4_values(vr[2 * G + (d >> 1)][2 * (d & 1) + h]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) acc[n][4 * G + d] = mfma16(a, pb[n][G][h], acc[n][4 * G + d]);
+        }
+      }
+    if (more) {
+      load_v(t0 + STEP, pg);
+      pg = load_pages(t0 + 2 * STEP);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) l_run[n] = over_groups(l_run[n], [](float a, float b) { return a + b; });
+
+  // the waves' parts: a common max, then the sum of their outputs in wave order
+  const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
+  const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
+  const int64_t slot = (unit * p.splits + split) * RB;  // part rows of this (unit, split)
+  if (g == 0) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      ml[0][w][16 * n + c] = m_run[n];
+      ml[1][w][16 * n + c] = l_run[n];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int at = 16 * n + c;
+    float m = ml[0][0][at], l = 0.0f;
+#pragma unroll
+    for (int i = 1; i < WK; ++i) m = fmaxf(m, ml[0][i][at]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < WK; ++i) l += ml[1][i][at] * __builtin_amdgcn_exp2f(ml[0][i][at] - ref);
+    const float mul = 16.0f * __builtin_amdgcn_exp2f(m_run[n] - ref) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+    // blocks 2 a and 2 a + 1 hold the even and odd d's of 32 a ..: the lane's are eight consecutive ones
+#pragma unroll
+    for (int a = 0; a < NV; ++a) {
+      const f32x4 even = (acc[n][2 * a] + p_off[n][a >> 1]) * mul, odd = (acc[n][2 * a + 1] + p_off[n][a >> 1]) * mul;
+      float *to = red + (w * WROWS + at) * LD + 32 * a + 8 * g;
+      *reinterpret_cast<f32x4 *>(to) = f32x4{even[0], odd[0], even[1], odd[1]};
+      *reinterpret_cast<f32x4 *>(to + 4) = f32x4{even[2], odd[2], even[3], odd[3]};
+    }
+    if (w == 0 && g == 0 && r.row0 + at < r.rows) {
+      if (!whole) {
+        p.part[p.ml_off + (slot + at) * 2] = m;
+        p.part[p.ml_off + (slot + at) * 2 + 1] = l;
+      } else if (p.l != nullptr) {
+        p.l[out_row[n]] = (m + log2f(l)) * 0.6931471805599453f;
+      }
+    }
+  }
+  __syncthreads();
+  const int rows = min(WROWS, r.rows - r.row0);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int at = i / (D / 4), d = 4 * (i % (D / 4));
+    f32x4 o = *reinterpret_cast<const f32x4 *>(red + at * LD + d);
+#pragma unroll
+    for (int k = 1; k < WK; ++k) o += *reinterpret_cast<const f32x4 *>(red + (k * WROWS + at) * LD + d);
+    if (whole) {
+      const int t = (r.row0 + at) / p.group, h = head * p.group + (r.row0 + at) - t * p.group;
+      bf16x4 o4;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(o[v]);
+      *reinterpret_cast<bf16x4 *>(p.o + (static_cast<int64_t>(r.first + t) * p.heads + h) * D + d) = o4;
+    } else {
+      *reinterpret_cast<f32x4 *>(p.part + (slot + at) * D + d) = o;
+    }
+  }
+}
+
+static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
+                                int64_t max_ctx, size_t scratch) {
+  KvAttnPlan pl = kv_attn_plan(tokens, batch, heads, kv_heads, D, std::min<int64_t>(max_q, std::max<int64_t>(1, 64 * kv_heads / heads)), max_ctx, scratch);
+  return pl;
+}
+
+template <int D, int NQ>
+static void launch_kv4_attn(const KvAttnPlan &pl, const Kv4AttnArgs &p, hipStream_t s) {
+  constexpr int RB = 16 * NQ;
+  const int64_t units = pl.blocks * p.kv_heads, rows = static_cast<int64_t>(p.tokens) * p.heads;
+  hipLaunchKernelGGL((kv4_attn<D, NQ>), dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+  if (pl.splits > 1)
+    hipLaunchKernelGGL((kv_attn_combine<D, RB>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
+}
+
+template <int D>
+static void launch_kv4_attn(const KvAttnPlan &pl, const Kv4AttnArgs &p, hipStream_t s) {
+  if (pl.nq == 2) launch_kv4_attn<D, 2>(pl, p, s);
+  else launch_kv4_attn<D, 1>(pl, p, s);
+}
+
+}  // namespace teeny
+
+using namespace teeny;
+
+extern "C" {
+
+teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const void *k_scale,
+                                       const void *v_scale, const int32_t *block_table, const int32_t *context_lens,
+                                       const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,
+                                       int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                       int64_t page_size, int64_t max_pages, int64_t max_q_len, int64_t max_context,
+                                       int64_t q_stride, float softmax_scale, int32_t causal, teeny_stream stream) {
+  const char *nm = "kv4_cache_attention";
+  Kv4AttnArgs p{};
+  KvAttnPlan pl;
+  teeny_status st = kv_attn_open(nm, kv4_attn_plan, q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens,
+                                 q_starts, o, l, n_tokens, batch, q_heads, kv_heads, head_dim, num_pages, page_size,
+                                 max_pages, max_q_len, max_context, q_stride, softmax_scale, causal, stream, p, pl);
+  if (st != TEENY_OK || pl.blocks == 0) return st;
+  TEENY_REQUIRE(aligned(k_scale, 4) && aligned(v_scale, 4), TEENY_ERR_MISALIGNED,
+                "kv4_cache_attention: 4-byte aligned scales");
+  p.ks = static_cast<const bf16 *>(k_scale);
+  p.vs = static_cast<const bf16 *>(v_scale);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 64) launch_kv4_attn<64>(pl, p, s);
+  else launch_kv4_attn<128>(pl, p, s);
+  return after_launch(nm, s);
+}
+
+teeny_status teeny_kv4_cache_attention_workspace_size(int64_t n_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                      int64_t head_dim, int64_t max_q_len, int64_t max_context,
+                                                      size_t *bytes) {
+  return kv_attn_workspace("kv4_cache_attention_workspace_size", kv4_attn_plan, n_tokens, batch, q_heads, kv_heads, head_dim,
+                           max_q_len, max_context, bytes);
+}
+
+}  // extern "C"

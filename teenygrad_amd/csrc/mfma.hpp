@@ -161,4 +161,18 @@ __device__ __forceinline__ uint32_t pack_hi(uint32_t a, uint32_t b) {
   return (a >> 16) | (b & 0xffff0000u);
 }
 
+// Words of eight 4-bit codes (-8..7, held + 8): the operands of gemm_w4.hpp and
+// of the 4-bit cache.  Code j lies in nibble w4_nibble(j), so that a shift, an
+// AND and an OR give two neighbours as the bf16 values (16 + code + 8) / 16, exact.
+__host__ __device__ constexpr int w4_nibble(int j) { return (j & 1) * 4 + (j >> 1); }
+
+__device__ __forceinline__ bf16x8 w4_values(uint32_t word) {
+  u32x4 r;
+  r[0] = ((word << 3) & 0x00780078u) | 0x3F803F80u;
+  r[1] = ((word >> 1) & 0x00780078u) | 0x3F803F80u;
+  r[2] = ((word >> 5) & 0x00780078u) | 0x3F803F80u;
+  r[3] = ((word >> 9) & 0x00780078u) | 0x3F803F80u;
+  return __builtin_bit_cast(bf16x8, r);
+}
+
 }  // namespace teeny

@@ -1462,6 +1462,42 @@ def kv_cache_write(k: Buffer, v: Buffer, slots: Buffer, k_cache: Buffer, v_cache
                                    d, pages, size, heads * d, heads * d, _h(stream)))
 
 
+def _kv_attention(what: str, call, dims, q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer,
+                  block_table: Buffer, context_lens: Buffer, q_starts: Optional[Buffer], max_q_len: Optional[int],
+                  max_context: Optional[int], softmax_scale: Optional[float], causal: bool, o: Optional[Buffer],
+                  lse: Optional[Buffer], stream: Optional[Stream]) -> Buffer:
+    """``kv_cache_attention`` over a cache of either kind, of dims (pages, kv_heads, page_size, head_dim)."""
+    pages, heads, size, d = dims
+    if not (len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16):
+        raise ValueError(f"{what}: q bf16 [n_tokens, q_heads, head_dim]")
+    t, hq, _ = q.shape
+    b = context_lens.numel
+    if heads == 0 or hq % heads:
+        raise ValueError(f"{what}: q_heads % kv_heads != 0")
+    if len(block_table.shape) != 2 or block_table.shape[0] != b:
+        raise ValueError(f"{what}: block_table must be [{b}, max_pages]")
+    if not block_table.dtype is context_lens.dtype is i32:
+        _need(_types((block_table, i32), (context_lens, i32)), f"{what}: block_table and context_lens must be int32")
+    if q_starts is not None:
+        if q_starts.numel != b + 1 or q_starts.dtype is not i32:
+            _ints(q_starts, b + 1, "q_starts")
+    elif t != b:
+        raise ValueError(f"{what}: q_starts, or one query for each of the {b} sequences")
+    if not (lse is None or (lse.numel == t * hq and lse.dtype == f32)):
+        raise ValueError(f"{what}: lse fp32 [n_tokens, q_heads]")
+    if max_q_len is None:
+        max_q_len = -(-t // max(b, 1))
+    if max_context is None:
+        max_context = block_table.shape[1] * size
+    scale = d ** -0.5 if softmax_scale is None else softmax_scale
+    if o is None or o.numel != q.numel or o.dtype is not bf16:
+        o = _out(q, o)
+    check(call(q.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, block_table.ptr, context_lens.ptr,
+               q_starts.ptr if q_starts is not None else None, o.ptr, lse.ptr if lse is not None else None, t, b, hq, heads,
+               d, pages, size, block_table.shape[1], max_q_len, max_context, hq * d, scale, int(bool(causal)), _h(stream)))
+    return o
+
+
 def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer,
                        block_table: Buffer, context_lens: Buffer, q_starts: Optional[Buffer] = None,
                        max_q_len: Optional[int] = None, max_context: Optional[int] = None,
@@ -1471,37 +1507,9 @@ def kv_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buf
     q_starts[b] .. q_starts[b + 1] - 1 (None: one each), the last of its context_lens[b] tokens.  max_q_len and
     max_context (host numbers; default: the mean of the queries, and a whole row of the table) choose how the work is
     cut, for all sequences alike, not the result: numbers near the true ones are the fast ones."""
-    pages, heads, size, d = _need_cache(k_cache, v_cache, k_scale, v_scale)
-    if not (len(q.shape) == 3 and q.shape[2] == d and q.dtype == bf16):
-        raise ValueError("kv_cache_attention: q bf16 [n_tokens, q_heads, head_dim]")
-    t, hq, _ = q.shape
-    b = context_lens.numel
-    if heads == 0 or hq % heads:
-        raise ValueError("kv_cache_attention: q_heads % kv_heads != 0")
-    if len(block_table.shape) != 2 or block_table.shape[0] != b:
-        raise ValueError(f"kv_cache_attention: block_table must be [{b}, max_pages]")
-    if not block_table.dtype is context_lens.dtype is i32:
-        _need(_types((block_table, i32), (context_lens, i32)), "kv_cache_attention: block_table and context_lens must be int32")
-    if q_starts is not None:
-        if q_starts.numel != b + 1 or q_starts.dtype is not i32:
-            _ints(q_starts, b + 1, "q_starts")
-    elif t != b:
-        raise ValueError(f"kv_cache_attention: q_starts, or one query for each of the {b} sequences")
-    if not (lse is None or (lse.numel == t * hq and lse.dtype == f32)):
-        raise ValueError("kv_cache_attention: lse fp32 [n_tokens, q_heads]")
-    if max_q_len is None:
-        max_q_len = -(-t // max(b, 1))
-    if max_context is None:
-        max_context = block_table.shape[1] * size
-    scale = d ** -0.5 if softmax_scale is None else softmax_scale
-    if o is None or o.numel != q.numel or o.dtype is not bf16:
-        o = _out(q, o)
-    check(lib.teeny_kv_cache_attention(q.ptr, k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, block_table.ptr,
-                                       context_lens.ptr, q_starts.ptr if q_starts is not None else None, o.ptr,
-                                       lse.ptr if lse is not None else None, t, b, hq, heads, d, pages, size,
-                                       block_table.shape[1], max_q_len, max_context, hq * d, scale, int(bool(causal)),
-                                       _h(stream)))
-    return o
+    return _kv_attention("kv_cache_attention", lib.teeny_kv_cache_attention, _need_cache(k_cache, v_cache, k_scale, v_scale), q,
+                         k_cache, v_cache, k_scale, v_scale, block_table, context_lens, q_starts, max_q_len, max_context,
+                         softmax_scale, causal, o, lse, stream)
 
 
 def kv_cache_attention_workspace_size(n_tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
@@ -1510,6 +1518,81 @@ def kv_cache_attention_workspace_size(n_tokens: int, batch: int, q_heads: int, k
     out = ctypes.c_size_t(0)
     check(lib.teeny_kv_cache_attention_workspace_size(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len,
                                                       max_context, ctypes.byref(out)))
+    return int(out.value)
+
+
+def kv4_cache_dims(k_cache_shape, v_cache_shape, k_scale_shape, v_scale_shape) -> Tuple[int, int, int, int]:
+    """-> (pages, kv_heads, page_size, head_dim) of a 4-bit cache, in bytes: K [pages, kv_heads, page_size, head_dim / 2], V
+    [pages, kv_heads, page_size / 16, head_dim, 8], scales [pages, kv_heads, page_size, head_dim / 64]."""
+    if len(k_cache_shape) != 4:
+        raise ValueError("kv4_cache: k_cache must be 4-D")
+    pages, heads, size, row = k_cache_shape
+    d = 2 * row
+    if v_cache_shape != (pages, heads, size // 16, d, 8) or size % 16:
+        raise ValueError(f"kv4_cache: v_cache must be {[pages, heads, size // 16, d, 8]}, is {list(v_cache_shape)}")
+    if not k_scale_shape == v_scale_shape == (pages, heads, size, d // 64) or d % 64:
+        raise ValueError(f"kv4_cache: scales must be {[pages, heads, size, d // 64]}")
+    return pages, heads, size, d
+
+
+def _need_cache4(k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer):
+    if not (k_cache.dtype is v_cache.dtype is i8 and k_scale.dtype is v_scale.dtype is bf16):
+        _need(_types((k_cache, i8), (v_cache, i8), (k_scale, bf16), (v_scale, bf16)), "kv4_cache: codes int8, scales bf16")
+    return kv4_cache_dims(k_cache.shape, v_cache.shape, k_scale.shape, v_scale.shape)
+
+
+def kv4_cache_append(q: Optional[Buffer], k: Buffer, v: Buffer, positions: Buffer, slots: Buffer, inv_freq: Optional[Buffer],
+                     k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer, interleaved: bool = False,
+                     q_out: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Optional[Buffer]:
+    """A step's tokens: k, v bf16 [n_tokens, kv_heads, head_dim] into the 4-bit cache at `slots`, k and q (bf16 [n_tokens,
+    q_heads, head_dim], or None) rotated by `positions` times inv_freq (fp32 [rotary_dim / 2]; None: not rotated): numbers
+    i and i + rotary_dim / 2 of a head, or 2 i and 2 i + 1 (interleaved).  slots and positions as ``kv_cache_plan`` gives
+    them; a row of a negative position is skipped, one of a negative slot gives its q alone.  Returns the rotated q
+    (q_out, which may be q; a skipped row is left as it was)."""
+    pages, heads, size, d = _need_cache4(k_cache, v_cache, k_scale, v_scale)
+    t = slots.numel
+    if not k.shape == v.shape == (t, heads, d):
+        raise ValueError(f"kv4_cache_append: k and v must be {[t, heads, d]}")
+    if positions.numel != t:
+        raise ValueError(f"kv4_cache_append: positions must have {t} elements")
+    hq = 0
+    if q is not None:
+        if not (len(q.shape) == 3 and q.shape[0] == t and q.shape[2] == d):
+            raise ValueError(f"kv4_cache_append: q must be [{t}, q_heads, {d}]")
+        hq = q.shape[1]
+        if q_out is None or q_out.numel != q.numel or q_out.dtype is not bf16:
+            q_out = _out(q, q_out)
+    elif q_out is not None:
+        raise ValueError("kv4_cache_append: q_out without q")
+    if not (k.dtype is v.dtype is bf16 and positions.dtype is slots.dtype is i32 and (q is None or q.dtype is bf16) and
+            (inv_freq is None or inv_freq.dtype is f32)):
+        _need(_types((k, bf16), (v, bf16), (q, bf16), (positions, i32), (slots, i32), (inv_freq, f32)),
+              "kv4_cache_append: q/k/v bf16, positions and slots int32, inv_freq fp32")
+    check(lib.teeny_kv4_cache_append(q.ptr if q is not None else None, k.ptr, v.ptr, positions.ptr, slots.ptr,
+                                     inv_freq.ptr if inv_freq is not None else None, q_out.ptr if q is not None else None,
+                                     k_cache.ptr, v_cache.ptr, k_scale.ptr, v_scale.ptr, t, hq, heads, d,
+                                     2 * inv_freq.numel if inv_freq is not None else 0, pages, size, hq * d, heads * d,
+                                     heads * d, int(bool(interleaved)), _h(stream)))
+    return q_out
+
+
+def kv4_cache_attention(q: Buffer, k_cache: Buffer, v_cache: Buffer, k_scale: Buffer, v_scale: Buffer,
+                        block_table: Buffer, context_lens: Buffer, q_starts: Optional[Buffer] = None,
+                        max_q_len: Optional[int] = None, max_context: Optional[int] = None,
+                        softmax_scale: Optional[float] = None, causal: bool = True, o: Optional[Buffer] = None,
+                        lse: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
+    """``kv_cache_attention`` over the 4-bit cache: q, as ``kv4_cache_append`` returns it, and every other argument alike."""
+    return _kv_attention("kv4_cache_attention", lib.teeny_kv4_cache_attention, _need_cache4(k_cache, v_cache, k_scale, v_scale),
+                         q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, q_starts, max_q_len, max_context,
+                         softmax_scale, causal, o, lse, stream)
+
+
+def kv4_cache_attention_workspace_size(n_tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
+                                       max_q_len: int, max_context: int) -> int:
+    """Stream workspace bytes that let ``kv4_cache_attention`` share a sequence's tokens out over the device."""
+    out = ctypes.c_size_t(0)
+    check(lib.teeny_kv4_cache_attention_workspace_size(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len,
+                                                       max_context, ctypes.byref(out)))
     return int(out.value)
 
 
@@ -1666,6 +1749,39 @@ def w4a16_linear_workspace_size(m: int, n: int, k: int, group_size: int) -> int:
     out = ctypes.c_size_t(0)
     check(lib.teeny_w4a16_linear_workspace_size(m, n, k, group_size, ctypes.byref(out)))
     return int(out.value)
+
+
+def adapter_dims(x_shape, a_shape, b_shape, n_ids, y_shape, scale_shape=None) -> Tuple[int, int, int, int, int]:
+    """-> (M, N, K, rank, adapters) of x [M, K], a [adapters, rank, K], b [adapters, N, rank], y [M, N]."""
+    if not (len(x_shape) == len(y_shape) == 2 and len(a_shape) == len(b_shape) == 3):
+        raise ValueError("adapter_add: x and y must be 2-D, a and b 3-D")
+    m, k = x_shape
+    adapters, rank, _ = a_shape
+    n = y_shape[1]
+    if a_shape[2] != k or y_shape[0] != m or n_ids != m:
+        raise ValueError(f"adapter_add: a must be [adapters, rank, {k}], y [{m}, N], adapters [{m}]")
+    if b_shape != (adapters, n, rank):
+        raise ValueError(f"adapter_add: b must be {[adapters, n, rank]}, is {list(b_shape)}")
+    if scale_shape is not None and _prod(scale_shape) != adapters:
+        raise ValueError(f"adapter_add: scale must have {adapters} elements")
+    return m, n, k, rank, adapters
+
+
+def adapter_add(x: Buffer, a: Buffer, b: Buffer, adapters: Buffer, y: Buffer, scale: Optional[Buffer] = None,
+                out: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
+    """Low-rank adapters of many requests beside a linear layer that all share: out[m] = y[m] + scale[i] b[i] (a[i] x[m]),
+    i = adapters[m] (int32; negative: out[m] = y[m]).  x bf16 [M, K], y the shared layer's output on x, bf16 [M, N], a bf16
+    [adapters, rank, K], b bf16 [adapters, N, rank], scale fp32 [adapters] (None: 1).  out=y updates in place."""
+    m, n, k, rank, count = adapter_dims(x.shape, a.shape, b.shape, adapters.numel, y.shape,
+                                        scale.shape if scale is not None else None)
+    if not (x.dtype is a.dtype is b.dtype is y.dtype is bf16 and adapters.dtype is i32 and (scale is None or scale.dtype is f32)):
+        _need(_types((x, bf16), (a, bf16), (b, bf16), (y, bf16), (adapters, i32), (scale, f32)),
+              "adapter_add: x, a, b and y bf16, adapters int32, scale fp32")
+    if out is None or out.numel != m * n or out.dtype is not bf16:
+        out = _out(y, out)
+    check(lib.teeny_adapter_add(x.ptr, a.ptr, b.ptr, adapters.ptr, scale.ptr if scale is not None else None, y.ptr, out.ptr,
+                                m, n, k, rank, count, k, n, n, _h(stream)))
+    return out
 
 
 def w8a16_conv2d(x: Buffer, qweight: Buffer, scale: Buffer, bias: Optional[Buffer] = None,
