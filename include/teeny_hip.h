@@ -790,7 +790,9 @@ teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t
  * [num_adapters, rank, K], b bf16 [num_adapters, N, rank], scale fp32
  * [num_adapters] or NULL (1), y (the shared layer's output) and out (which may be
  * y) bf16 [M,N]; rows of x, y and out x_stride, y_stride and out_stride elements
- * apart.  Rows of an adapter need not lie together, but are faster so.  fp32 sums,
+ * apart.  With a stream workspace of teeny_adapter_add_workspace_size bytes the
+ * ranks' products are worked out once, shared out over the device; without it
+ * again by each workgroup.  Rows of an adapter need not lie together, but are faster so.  fp32 sums,
  * the rank's products held in two bf16 parts (2^-17) for the second product; out
  * is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
  * zeros); K a multiple of 8; x, a, b and x's rows 16-byte aligned. */
@@ -798,6 +800,7 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
                                const void *y, void *out, int64_t M, int64_t N, int64_t K, int64_t rank,
                                int64_t num_adapters, int64_t x_stride, int64_t y_stride, int64_t out_stride,
                                teeny_stream stream);
+teeny_status teeny_adapter_add_workspace_size(int64_t M, int64_t N, int64_t K, int64_t rank, size_t *bytes);
 
 /* W8A16 conv2d, NHWC bf16 activations, int8 weights [C_OUT,KH,KW,C_IN/G]
  * with per-output-channel fp32 scale, fp32 bias or NULL, bf16 output:

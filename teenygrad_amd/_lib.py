@@ -176,6 +176,7 @@ _SIGS = {
     "teeny_w4a16_linear_workspace_size": (S, [c_int64] * 4 + [POINTER(c_size_t)]),
     "teeny_pack_int4": (S, [P, P, c_int64, c_int64, P]),
     "teeny_adapter_add": (S, [P] * 7 + [c_int64] * 8 + [P]),
+    "teeny_adapter_add_workspace_size": (S, [c_int64] * 4 + [POINTER(c_size_t)]),
     "teeny_linear_workspace_size": (S, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),
     "teeny_linear_backward": (S, [P] * 6 + [c_int64] * 14 + [c_int32, P]),
     "teeny_linear_backward_workspace_size": (S, [c_int64, c_int64, c_int64, c_int32, POINTER(c_size_t)]),

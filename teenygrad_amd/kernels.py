@@ -1784,6 +1784,13 @@ def adapter_add(x: Buffer, a: Buffer, b: Buffer, adapters: Buffer, y: Buffer, sc
     return out
 
 
+def adapter_add_workspace_size(m: int, n: int, k: int, rank: int) -> int:
+    """Stream workspace bytes that let ``adapter_add`` work the ranks' products out once, shared out over the device."""
+    out = ctypes.c_size_t(0)
+    check(lib.teeny_adapter_add_workspace_size(m, n, k, rank, ctypes.byref(out)))
+    return int(out.value)
+
+
 def w8a16_conv2d(x: Buffer, qweight: Buffer, scale: Buffer, bias: Optional[Buffer] = None,
                  stride=(1, 1), padding=(0, 0), groups: int = 1, act: Optional[str] = None,
                  y: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:

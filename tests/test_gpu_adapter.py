@@ -1,4 +1,6 @@
 """Low-rank adapters of many requests on the GPU, against the plain form of kv4_cases.py."""
+import contextlib
+
 import numpy as np
 import pytest
 
@@ -45,8 +47,11 @@ def check_run(c, got, scale=True):
 
 
 def size_of(c):
-    return K.adapter_add_workspace_size(len(c["ids"]), c["y"].shape[1], c["x"].shape[1], c["a"].shape[1]) \
-        if hasattr(K, "adapter_add_workspace_size") else 256
+    return K.adapter_add_workspace_size(len(c["ids"]), c["y"].shape[1], c["x"].shape[1], c["a"].shape[1])
+
+
+def space_for(dev, c, space):
+    return stream_workspace(dev, size_of(c)) if space else contextlib.nullcontext()
 
 
 IDS = {
@@ -63,7 +68,7 @@ def test_adapters(dev, ids, rank, space):
     rng = np.random.default_rng(rank + len(ids))
     for n, k in ((4, 8), (100, 264), (333, 1032)):
         c = case(rng, IDS[ids], n, k, rank, 40 if ids == "each its own" else 4)
-        with stream_workspace(dev, size_of(c) if space else 0):
+        with space_for(dev, c, space):
             check_run(c, run(dev, c))
 
 
@@ -74,7 +79,7 @@ def test_larger(dev, m, n, k, rank, adapters, space):
     c = case(rng, np.sort(rng.integers(-1, adapters, m)) if m > 100 else rng.integers(-1, adapters, m), n, k, rank, adapters)
     if m == 1:
         c["ids"][:] = 1
-    with stream_workspace(dev, size_of(c) if space else 0):
+    with space_for(dev, c, space):
         check_run(c, run(dev, c))
         check_run(c, run(dev, c, scale=False), scale=False)
         check_run(c, run(dev, c, in_place=True))
@@ -88,7 +93,7 @@ def test_rows_are_apart(dev, space):
     clean = kv4.adapter(c["x"], c["a"], c["b"], c["ids"], c["scale"], c["y"])
     c["x"][2, 5], c["x"][4, 1], c["a"][2, 3, 7], c["b"][1, 11, 4] = np.nan, np.inf, np.inf, np.nan
     c["x"][3] = 1.0
-    with stream_workspace(dev, size_of(c) if space else 0):
+    with space_for(dev, c, space):
         got = run(dev, c)
     assert np.isnan(got[2]).all() and np.isnan(got[[1, 5], 11]).all() and np.isinf(got[3]).all()
     rows = np.ones(got.shape, bool)
@@ -108,7 +113,7 @@ def test_strides(dev, space):
         x[:, 8:56], y[:, first:first + n] = c["x"], c["y"]
         xb, yb, ob, a, b = (up(dev, z) for z in (x, y, out, c["a"], c["b"]))
         ids, s = dev.upload(c["ids"]), dev.upload(c["scale"])
-        with stream_workspace(dev, size_of(c) if space else 0):
+        with space_for(dev, c, space):
             check(lib.teeny_adapter_add(xb.ptr + 16, a.ptr, b.ptr, ids.ptr, s.ptr, yb.ptr + 2 * first, ob.ptr + 2 * first, m, n, 48, 8, 3,
                                         64, row, row + 4, None))
             got = from_bf16(ob.to_host())

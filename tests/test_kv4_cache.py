@@ -130,6 +130,18 @@ def test_adapter_refusals(kw, code):
     expect(lib.teeny_adapter_add(*adapter_args(**kw)), code)
 
 
+def test_adapter_workspace_refusals():
+    n = ctypes.c_size_t(7)
+    f = lib.teeny_adapter_add_workspace_size
+    expect(f(4, 32, 256, 16, None), _lib.ERR_NULL_POINTER)
+    expect(f(-4, 32, 256, 16, ctypes.byref(n)), _lib.ERR_SHAPE_MISMATCH)
+    expect(f(4, 32, 256, 20, ctypes.byref(n)), _lib.ERR_UNSUPPORTED)
+    expect(f(4, 32, BIG, 16, ctypes.byref(n)), _lib.ERR_SHAPE_MISMATCH)
+    assert n.value == 0
+    assert f(4, 32, 0, 16, ctypes.byref(n)) == _lib.OK and n.value == 0
+    assert f(4, 32, 256, 16, ctypes.byref(n)) == _lib.OK and n.value > 0
+
+
 def test_nothing_to_adapt():
     assert lib.teeny_adapter_add(*adapter_args(M=0, x=None, y=None, out=None, adapters=None)) == _lib.OK
     assert lib.teeny_adapter_add(*adapter_args(N=0, b=None)) == _lib.OK
