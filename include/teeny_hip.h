@@ -795,7 +795,8 @@ teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t
  * again by each workgroup.  Rows of an adapter need not lie together, but are faster so.  fp32 sums,
  * the rank's products held in two bf16 parts (2^-17) for the second product; out
  * is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
- * zeros); K a multiple of 8; x, a, b and x's rows 16-byte aligned. */
+ * zeros), N * rank below 2^30; K a multiple of 8 up to 2^22, x_stride up to 2^24; x,
+ * a, b and x's rows 16-byte aligned. */
 teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, const int32_t *adapters, const float *scale,
                                const void *y, void *out, int64_t M, int64_t N, int64_t K, int64_t rank,
                                int64_t num_adapters, int64_t x_stride, int64_t y_stride, int64_t out_stride,

@@ -19,10 +19,10 @@ struct AdapterArgs {
   const bf16 *y;
   bf16 *out;
   int64_t x_stride, y_stride, out_stride;
-  int M, N, K, rank, adapters, vec;  // vec: rows of y and out are aligned for eight numbers
+  int M, N, K, rank, adapters;
   int cols;                          // output columns of a workgroup
   float *part;                       // [splits][M][RP] products of the ranks, RP: the rank in whole tiles of 16
-  int splits, chunk, by_row;         // chunk: k's of a split; by_row: workgroups by rows, not by tiles of them
+  int splits, chunk, slots;          // chunk: k's of a split; slots: workgroups to a tile of rows, 0: one to each row
 };
 
 __device__ __forceinline__ f32x4 mfma_16x16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -33,91 +33,156 @@ __device__ __forceinline__ bf16x8 load8(const bf16 *p, bool there) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// 16 numbers of a row of the output from those of y and of the adapter.
-__device__ __forceinline__ void adapter_store(const AdapterArgs &p, int m, int n, const f32x4 (&add)[4]) {
+// A lane's numbers of 64 columns n ..: of a row m, the columns n + 8 g + 0..7 and 32 further on, two tiles each; so a
+// wave's access is 64 bytes of each row.  Rows may begin anywhere (global memory takes 16 bytes at any address).
+typedef u32x4 AdapterRow[2];
+__device__ __forceinline__ void adapter_load(const AdapterArgs &p, int m, int n, AdapterRow &v) {
   const bf16 *y = p.y + m * p.y_stride + n;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) __builtin_memcpy(&v[h], y + 32 * h, 16);
+}
+__device__ __forceinline__ void adapter_store(const AdapterArgs &p, int m, int n, const AdapterRow &v, const f32x4 (&add)[4]) {
   bf16 *out = p.out + m * p.out_stride + n;
-  if (p.vec && n + 16 <= p.N) {
-    bf16x8 v[2] = {*reinterpret_cast<const bf16x8 *>(y), *reinterpret_cast<const bf16x8 *>(y + 8)};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i >> 3][i & 7] = static_cast<bf16>(static_cast<float>(v[i >> 3][i & 7]) + add[i >> 2][i & 3]);
-    *reinterpret_cast<bf16x8 *>(out) = v[0];
-    *reinterpret_cast<bf16x8 *>(out + 8) = v[1];
-  } else {
+  for (int h = 0; h < 2; ++h) {
+    u32x4 o;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (n + i < p.N) out[i] = static_cast<bf16>(static_cast<float>(y[i]) + add[i >> 2][i & 3]);
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 &a = add[2 * h + (i >> 1)];
+      o[i] = __builtin_bit_cast(uint32_t, cvt_pk_bf16(__uint_as_float(v[h][i] << 16) + a[2 * (i & 1)],
+                                                      __uint_as_float(v[h][i] & 0xffff0000u) + a[2 * (i & 1) + 1]));
+    }
+    typedef u32x4 any __attribute__((aligned(2)));
+    // past the caches, which hold B (2000 rows x 11008 columns of rank 64: 36.0 -> 30.0 us)
+    __builtin_nontemporal_store(o, reinterpret_cast<any *>(out + 32 * h));
   }
 }
+// Where the 64 columns pass the last one: number by number; rows as offsets from m0's, so that the 16 addresses are one.
+__device__ __forceinline__ void adapter_edge(const AdapterArgs &p, int m0, int row, int n, const f32x4 (&add)[4]) {
+  const int extent = static_cast<int>(min(p.M - m0, 64) - 1);
+  const auto yr = buffer_rsrc(p.y + m0 * p.y_stride, static_cast<int>((extent * p.y_stride + p.N) * 2));
+  const auto outr = buffer_rsrc(p.out + m0 * p.out_stride, static_cast<int>((extent * p.out_stride + p.N) * 2));
+  const int y_at = static_cast<int>((row * p.y_stride + n) * 2), out_at = static_cast<int>((row * p.out_stride + n) * 2);
+  uint16_t v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b16(yr, y_at + 64 * (i >> 3) + 2 * (i & 7), 0, 0);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int at = 32 * (i >> 3) + (i & 7);
+    const bf16 o = static_cast<bf16>(__uint_as_float(static_cast<uint32_t>(v[i]) << 16) + add[i >> 2][i & 3]);
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, o), outr, n + at < p.N ? out_at + 2 * at : kOffNone, 0, 0);
+  }
+}
+// Columns n0 .. n1 - 1 of rows without an adapter, by the workgroup.
+__device__ __forceinline__ void adapter_copy(const AdapterArgs &p, int m0, uint64_t rows, int n0, int n1) {
+#pragma unroll 1
+  for (; rows != 0; rows &= rows - 1) {
+    const int m = m0 + __builtin_ctzll(rows);
+    const bf16 *y = p.y + m * p.y_stride;
+    bf16 *out = p.out + m * p.out_stride;
+#pragma unroll 1
+    for (int n = n0 + 8 * threadIdx.x; n < n1; n += 8 * 256) {
+      if (n + 8 <= n1) {
+        __builtin_memcpy(out + n, y + n, 16);
+      } else {
+#pragma unroll 1
+        for (int i = n; i < n1; ++i) out[i] = y[i];
+      }
+    }
+  }
+}
+__device__ __forceinline__ void adapter_add_row(const AdapterArgs &p, int m0, int row, int n, bool whole, const f32x4 (&add)[4]) {
+  if (whole) {
+    AdapterRow v;
+    adapter_load(p, m0 + row, n, v);
+    adapter_store(p, m0 + row, n, v, add);
+  } else {
+    adapter_edge(p, m0, row, n, add);
+  }
+}
+// The row of B that lane c holds for tile j of the columns n ..
+__device__ __forceinline__ int adapter_col(int n, int j, int c) { return n + 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3); }
 
-// The rows of one adapter among 16 MT rows: lane l's row l.
+// The rows of 16 MT ones that each adapter has: lane l's row l.  Either (slots 0) there is a workgroup for each row, which
+// takes the adapter of which the row is the first, or `slots` workgroups for each tile take its adapters in turn.
 template <int MT>
 struct AdapterRows {
   int m0, id;     // the first row; the lane's adapter (-1: none, -2: no row)
-  uint64_t left;  // rows that are still to be taken up, by the first of each adapter's
+  uint64_t left;  // rows whose adapters no workgroup has taken yet
+  int skip;       // adapters of other workgroups before the next one
   __device__ __forceinline__ AdapterRows(const AdapterArgs &p, int block) {
-    const int lane = threadIdx.x & 63;
-    m0 = p.by_row ? block & ~(16 * MT - 1) : block * 16 * MT;
+    // the first workgroups of all tiles, then the second ones, of which few may have anything to do: each XCD has its share
+    const int lane = threadIdx.x & 63, tiles = (p.M + 16 * MT - 1) / (16 * MT);
+    skip = p.slots == 0 ? 0 : block / tiles;
+    m0 = (p.slots == 0 ? block / (16 * MT) : block - skip * tiles) * 16 * MT;
     id = -2;
     if (lane < 16 * MT && m0 + lane < p.M) {
       id = p.ids[m0 + lane];
       if (id < 0 || id >= p.adapters) id = -1;
     }
     left = __ballot(id >= -1);
-    if (p.by_row) {
-      // the workgroup of an adapter's first row takes all of its rows
-      const int at = block - m0;
-      const uint64_t same = __ballot(id == __builtin_amdgcn_readlane(id, at));
-      left = __builtin_ctzll(same) == at ? same : 0;
+    if (p.slots == 0) {
+      const uint64_t same = __ballot(id == __builtin_amdgcn_readlane(id, block - m0));
+      left = __builtin_ctzll(same) == block - m0 ? same : 0;
     }
   }
-  // the next adapter; its rows
-  __device__ __forceinline__ int next(uint64_t &rows) {
-    const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    rows = __ballot(id == a);
-    left &= ~rows;
-    return a;
+  // whether there is another adapter for this workgroup; it and its rows
+  __device__ __forceinline__ bool next(const AdapterArgs &p, int &a, uint64_t &rows) {
+    while (left != 0) {
+      a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+      rows = __ballot(id == a);
+      left &= ~rows;
+      if (skip-- == 0) {
+        skip = p.slots - 1;
+        return true;
+      }
+    }
+    return false;
   }
 };
 
 // part[split] = A[a] x over the split's k's.  Four waves share them out in turn, 64 at
-// a time, and meet in LDS.  Rows of other adapters are multiplied too and not
+// a time, and meet in LDS; all of a wave's share is in flight at once (a k past the
+// split's end loads zeros).  Rows of other adapters are multiplied too and not
 // written; rows of A past the rank repeat the last one and are not read again.
 template <int RT, int MT>
 __global__ __launch_bounds__(256) void adapter_down(AdapterArgs p) {
-  constexpr int U = RT * MT >= 8 ? 1 : RT * MT >= 4 ? 2 : 4, RP = 16 * RT;
+  constexpr int U = RT * MT >= 8 ? 2 : 4, RP = 16 * RT;
   __shared__ __attribute__((aligned(16))) float sum[4][16 * MT][RP + 4];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
   AdapterRows<MT> rows(p, blockIdx.x);
   const int kb = blockIdx.y * p.chunk, ke = min(p.K, kb + p.chunk);
-  const bf16 *x[MT];
+  const int last = min(16 * MT, p.M - rows.m0) - 1;
+  const auto xr = buffer_rsrc(p.x + rows.m0 * p.x_stride, static_cast<int>((last * p.x_stride + p.K) * 2));
+  int x_at[MT], a_at[RT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x[t] = p.x + min(rows.m0 + 16 * t + c, p.M - 1) * p.x_stride + 8 * g;
-  while (rows.left != 0) {
-    uint64_t mine;
-    const int a = rows.next(mine);
+  for (int t = 0; t < MT; ++t) x_at[t] = static_cast<int>((min(16 * t + c, last) * p.x_stride + 8 * g) * 2);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) a_at[t] = (min(16 * t + c, p.rank - 1) * p.K + 8 * g) * 2;
+  int a;
+  uint64_t mine;
+  while (rows.next(p, a, mine)) {
     if (a < 0) continue;
-    const bf16 *ar[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) ar[t] = p.a + (static_cast<int64_t>(a) * p.rank + min(16 * t + c, p.rank - 1)) * p.K + 8 * g;
+    const auto ar = buffer_rsrc(p.a + static_cast<int64_t>(a) * p.rank * p.K, p.rank * p.K * 2);
     f32x4 acc[RT][MT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int t = 0; t < MT; ++t) acc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    int k = kb + 64 * w;
-    for (; k + 256 * (U - 1) + 64 <= ke; k += 256 * U) {
-      bf16x8 xf[U][2][MT], af[U][2][RT];
+    for (int k = kb + 64 * w; k < ke; k += 256 * U) {
+      u32x4 xf[U][2][MT], af[U][2][RT];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int at = k + 256 * u + 32 * h;
+          const bool in = at + 8 * g < ke;
 #pragma unroll
-          for (int r = 0; r < RT; ++r) af[u][h][r] = *reinterpret_cast<const bf16x8 *>(ar[r] + at);
+          for (int r = 0; r < RT; ++r) af[u][h][r] = buffer_load16(ar, in ? a_at[r] + 2 * at : kOffNone);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) xf[u][h][t] = *reinterpret_cast<const bf16x8 *>(x[t] + at);
+          for (int t = 0; t < MT; ++t) xf[u][h][t] = buffer_load16(xr, in ? x_at[t] + 2 * at : kOffNone);
         }
+      __builtin_amdgcn_sched_barrier(0);  // or products are moved up between the loads, to save registers
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -125,23 +190,9 @@ __global__ __launch_bounds__(256) void adapter_down(AdapterArgs p) {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[r][t] = mfma_16x16(af[u][h][r], xf[u][h][t], acc[r][t]);
+            for (int t = 0; t < MT; ++t)
+              acc[r][t] = mfma_16x16(__builtin_bit_cast(bf16x8, af[u][h][r]), __builtin_bit_cast(bf16x8, xf[u][h][t]), acc[r][t]);
     }
-    for (; k < ke; k += 256)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = k + 32 * h;
-        const bool in = at + 8 * g < ke;
-        bf16x8 xf[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) xf[t] = load8(x[t] + at, in);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const bf16x8 af = load8(ar[r] + at, in);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) acc[r][t] = mfma_16x16(af, xf[t], acc[r][t]);
-        }
-      }
     __syncthreads();  // the last adapter's sums have been read
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -159,70 +210,105 @@ __global__ __launch_bounds__(256) void adapter_down(AdapterArgs p) {
   }
 }
 
-// out = y + B[a] (scale part).  A wave takes 64 columns a time, 16 to each lane group:
-// 16 consecutive numbers of a row of the output are one lane's.  The ranks'
-// products are two bf16 parts of an fp32 number; at a rank of 16 or less both are
-// the k's of one product.
+// out = y + B[a] (scale part).  A wave takes 64 columns a time.  The ranks' products
+// are two bf16 parts of an fp32 number; at a rank of 16 or less both are the k's of
+// one product.  The next columns' operands are loaded as soon as this one's have
+// been multiplied, the first ones ahead of the ranks' sums.
 template <int RT, int MT>
-__global__ __launch_bounds__(256) void adapter_up(AdapterArgs p) {
+__global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT >= 4 || MT == 2 ? 3 : 4) void adapter_up(AdapterArgs p) {
   constexpr int RP = 16 * RT, KS = RT == 1 ? 1 : RT / 2, LH = (RT == 1 ? 32 : RP) + 8, PARTS = RT == 1 ? 1 : 2;
   __shared__ __attribute__((aligned(16))) bf16 hs[PARTS][16 * MT][LH];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
   AdapterRows<MT> rows(p, blockIdx.x);
   const int n0 = blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
-  while (rows.left != 0) {
-    uint64_t mine;
-    const int a = rows.next(mine);
-    if (a < 0) {
-      if (p.out == p.y) continue;
-      const f32x4 zero[4] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f},
-                             f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-      for (int n = n0 + 64 * w + 16 * g; n < n1; n += 256)
+  int a;
+  uint64_t mine;
+  while (rows.next(p, a, mine)) {
+    bool in[MT];  // the lane's rows
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-          if ((mine >> (16 * t + c)) & 1) adapter_store(p, rows.m0 + 16 * t + c, n, zero);
+    for (int t = 0; t < MT; ++t) in[t] = (mine >> (16 * t + c)) & 1;
+    if (a < 0) {
+      if (p.out != p.y) adapter_copy(p, rows.m0, mine, n0, n1);
       continue;
     }
-    const float scale = p.scale != nullptr ? p.scale[a] : 1.0f;
-    __syncthreads();  // the last adapter's products have been read
-    for (int i = tid; i < 16 * MT * RP; i += 256) {
-      const int m = i / RP, r = i - m * RP;
-      float h = 0.0f;
-      if (r < p.rank && ((mine >> m) & 1)) {
-        const float *at = p.part + static_cast<int64_t>(rows.m0 + m) * RP + r;
-        for (int s = 0; s < p.splits; ++s) h += at[static_cast<int64_t>(s) * p.M * RP];
-        h *= scale;
-      }
-      const bf16 hi = static_cast<bf16>(h);
-      const bf16 lo = fabsf(static_cast<float>(hi)) < INFINITY ? static_cast<bf16>(h - static_cast<float>(hi)) : static_cast<bf16>(0.0f);
-      hs[0][m][r] = hi;
-      if constexpr (RT == 1) hs[0][m][16 + r] = lo;
-      else hs[PARTS - 1][m][r] = lo;
-    }
-    __syncthreads();
-    const int r0 = RT == 1 ? 8 * (g & 1) : 8 * g;
-    const bf16 *b = p.b + static_cast<int64_t>(a) * p.N * p.rank;
-    for (int n = n0 + 64 * w; n < n1; n += 256) {
-      bf16x8 bf[4][KS];
+    int cc = c, gg = g;
+    asm volatile("" : "+v"(cc), "+v"(gg));
+    const auto br = buffer_rsrc(p.b + static_cast<int64_t>(a) * p.N * p.rank, p.N * p.rank * 2);
+    const int r0 = RT == 1 ? 8 * (gg & 1) : 8 * gg;
+    u32x4 b[4][KS];
+    AdapterRow y[MT];
+    uint32_t b_at[KS];  // zeros past the rank
+#pragma unroll
+    for (int k = 0; k < KS; ++k) b_at[k] = r0 + 32 * k < p.rank ? 2 * (r0 + 32 * k) : static_cast<uint32_t>(kOffNone);
+    auto load_b = [&](int n) __attribute__((always_inline)) {  // and past the columns
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          b[j][k] = buffer_load16(br, static_cast<int>(b_at[k] + 2 * static_cast<uint32_t>(adapter_col(n, j, cc) * p.rank)));
+    };
+    auto load_y = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        if (in[t]) adapter_load(p, rows.m0 + 16 * t + cc, n + 8 * gg, y[t]);
+    };
+    auto products = [&](int t, f32x4 (&o)[4]) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bf16 *at = b + static_cast<int64_t>(min(n + 16 * (c >> 2) + 4 * j + (c & 3), p.N - 1)) * p.rank + r0;
+        o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) bf[j][k] = load8(at + 32 * k, r0 + 32 * k < p.rank);
+        for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            o[j] = mfma_16x16(__builtin_bit_cast(bf16x8, b[j][k]),
+                              *reinterpret_cast<const bf16x8 *>(&hs[s][16 * t + cc][32 * k + 8 * gg]), o[j]);
       }
+    };
+    int n = n0 + 64 * w;
+    asm volatile("" : "+s"(n));  // or the loop over adapters carries every address along
+    const int n_whole = n1 - 63;  // below it all of 64 columns are there (a range that is not the last has whole ones)
+    if (n < n1) load_b(n);
+    if (n < n_whole) load_y(n);
+    const float scale = p.scale != nullptr ? p.scale[a] : 1.0f;
+    __syncthreads();  // the last adapter's products have been read
+    for (int i = tid; i < 4 * MT * RP; i += 256) {
+      const int row = i / (RP / 4), r = 4 * (i - row * (RP / 4));
+      f32x4 h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < p.rank && ((mine >> row) & 1)) {  // the rank is a multiple of 8
+        const float *at = p.part + static_cast<int64_t>(rows.m0 + row) * RP + r;
+        const int64_t next = static_cast<int64_t>(p.M) * RP;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) h += *reinterpret_cast<const f32x4 *>(at + s * next);
+        h *= scale;
+      }
+      bf16x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hi[e] = static_cast<bf16>(h[e]);
+        lo[e] = fabsf(static_cast<float>(hi[e])) < INFINITY ? static_cast<bf16>(h[e] - static_cast<float>(hi[e])) : static_cast<bf16>(0.0f);
+      }
+      *reinterpret_cast<bf16x4 *>(&hs[0][row][r]) = hi;
+      *reinterpret_cast<bf16x4 *>(RT == 1 ? &hs[0][row][16 + r] : &hs[PARTS - 1][row][r]) = lo;
+    }
+    __syncthreads();
+    for (; n < n_whole; n += 256) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         f32x4 o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int s = 0; s < PARTS; ++s)
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-              o[j] = mfma_16x16(bf[j][k], *reinterpret_cast<const bf16x8 *>(&hs[s][16 * t + c][32 * k + 8 * g]), o[j]);
+        products(t, o);
+        if (t == MT - 1 && n + 256 < n1) load_b(n + 256);
+        if (in[t]) {
+          adapter_store(p, rows.m0 + 16 * t + cc, n + 8 * gg, y[t], o);
+          if (n + 256 < n_whole) adapter_load(p, rows.m0 + 16 * t + cc, n + 256 + 8 * gg, y[t]);
         }
-        if ((mine >> (16 * t + c)) & 1) adapter_store(p, rows.m0 + 16 * t + c, n + 16 * g, o);
+      }
+    }
+    if (n < n1) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        f32x4 o[4];
+        products(t, o);
+        if (in[t]) adapter_edge(p, rows.m0, 16 * t + cc, n + 8 * gg, o);
       }
     }
   }
@@ -241,11 +327,7 @@ __global__ __launch_bounds__(256) void adapter_one(AdapterArgs p) {
   int id = m0 + c < p.M ? p.ids[row] : -1;
   if (id < 0 || id >= p.adapters) id = -1;
   const bool here = m0 + c < p.M;
-  const f32x4 zero[4] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f},
-                         f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-  // rows of no adapter
-  for (int n = n0 + 64 * w + 16 * g; n < n1; n += 256)
-    if (here && id < 0) adapter_store(p, row, n, zero);
+  if (p.out != p.y) adapter_copy(p, m0, __ballot(here && id < 0) & 0xffffu, n0, n1);
   uint64_t left = __ballot(id >= 0) & 0xffffu;
   while (left != 0) {
     const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
@@ -281,8 +363,8 @@ __global__ __launch_bounds__(256) void adapter_one(AdapterArgs p) {
       f32x4 o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[j] = zero[j];
-        const int col = n + 16 * (c >> 2) + 4 * j + (c & 3);
+        o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int col = adapter_col(n, j, c);
 #pragma unroll
         for (int k = 0; k < 16 * RT; k += 32) {
           const bf16x8 bf = load8(p.b + (static_cast<int64_t>(a) * p.N + col) * p.rank + k + 8 * g, col < p.N && k + 8 * g < p.rank);
@@ -290,43 +372,45 @@ __global__ __launch_bounds__(256) void adapter_one(AdapterArgs p) {
           for (int s = 0; s < 2; ++s) o[j] = mfma_16x16(bf, *reinterpret_cast<const bf16x8 *>(&hs[s][c][k + 8 * g]), o[j]);
         }
       }
-      if (mine && here) adapter_store(p, row, n + 16 * g, o);
+      if (mine && here) adapter_add_row(p, m0, row - m0, n + 8 * g, n + 64 <= p.N, o);
     }
   }
 }
 
 // ── which form ──────────────────────────────────────────────────────────────
 struct AdapterPlan {
-  int rt = 1, mt = 1, splits = 1, chunk = 0, cols = 0;
-  bool by_row = false;
+  int rt = 1, down = 1, up = 1, slots = 0, splits = 1, chunk = 0, cols = 0;  // down, up: 16-row tiles of a workgroup
   size_t bytes = 0;
 };
 
 static AdapterPlan adapter_plan(int64_t M, int64_t N, int64_t K, int64_t rank) {
   AdapterPlan pl;
+  const bool many = M > 256;
   pl.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
-  pl.by_row = M <= 256;
-  pl.mt = pl.by_row ? 1 : 2;
-  const int64_t units = pl.by_row ? M : cdiv(M, 16 * pl.mt);
-  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), cdiv(512, units)));
+  pl.down = !many ? 1 : M > 1024 ? 4 : 2;
+  pl.up = many ? 2 : 1;
+  pl.slots = many ? 2 : 0;
+  const int64_t down = many ? cdiv(M, 16 * pl.down) : M, up = many ? cdiv(M, 16 * pl.up) : M;
+  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), cdiv(512, down)));
   pl.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(cdiv(K, splits), 256)) * 256);
   pl.splits = static_cast<int>(cdiv(K, pl.chunk));
-  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 1024), cdiv(1024, units)));
+  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), many ? std::max<int64_t>(4, 512 / up) : cdiv(2048, up)));
   pl.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
   pl.bytes = static_cast<size_t>(pl.splits) * M * 16 * pl.rt * 4;
   return pl;
 }
 
-template <int RT, int MT>
-static void launch_adapter(const AdapterPlan &pl, const AdapterArgs &p, hipStream_t s) {
-  const unsigned units = static_cast<unsigned>(pl.by_row ? p.M : cdiv(p.M, 16 * MT));
-  hipLaunchKernelGGL((adapter_down<RT, MT>), dim3(units, static_cast<unsigned>(pl.splits)), dim3(256), 0, s, p);
-  hipLaunchKernelGGL((adapter_up<RT, MT>), dim3(units, static_cast<unsigned>(cdiv(p.N, pl.cols))), dim3(256), 0, s, p);
+static dim3 adapter_grid(const AdapterPlan &pl, const AdapterArgs &p, int tiles, int64_t y) {
+  return dim3(static_cast<unsigned>(pl.slots == 0 ? p.M : cdiv(p.M, 16 * tiles) * pl.slots), static_cast<unsigned>(y));
 }
 template <int RT>
 static void launch_adapter(const AdapterPlan &pl, const AdapterArgs &p, hipStream_t s) {
-  if (pl.mt == 2) launch_adapter<RT, 2>(pl, p, s);
-  else launch_adapter<RT, 1>(pl, p, s);
+  const dim3 down = adapter_grid(pl, p, pl.down, pl.splits), up = adapter_grid(pl, p, pl.up, cdiv(p.N, pl.cols));
+  if (pl.down == 4) hipLaunchKernelGGL((adapter_down<RT, 4>), down, dim3(256), 0, s, p);
+  else if (pl.down == 2) hipLaunchKernelGGL((adapter_down<RT, 2>), down, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((adapter_down<RT, 1>), down, dim3(256), 0, s, p);
+  if (pl.up == 2) hipLaunchKernelGGL((adapter_up<RT, 2>), up, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((adapter_up<RT, 1>), up, dim3(256), 0, s, p);
 }
 
 }  // namespace teeny
@@ -342,26 +426,28 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
   const char *nm = "adapter_add";
   TEENY_REQUIRE(M >= 0 && N >= 0 && K >= 0 && rank >= 0 && num_adapters >= 0, TEENY_ERR_SHAPE_MISMATCH,
                 "adapter_add: negative size");
-  TEENY_REQUIRE(M <= 1 << 24 && N <= 1 << 24 && K <= 1 << 24 && num_adapters <= 1 << 24, TEENY_ERR_SHAPE_MISMATCH,
-                "adapter_add: M, N, K or num_adapters exceed 2^24");
+  TEENY_REQUIRE(M <= 1 << 24 && N <= 1 << 24 && K <= 1 << 22 && num_adapters <= 1 << 24, TEENY_ERR_SHAPE_MISMATCH,
+                "adapter_add: M, N or num_adapters exceed 2^24, or K 2^22");
+  TEENY_REQUIRE(N * rank < 1 << 30, TEENY_ERR_SHAPE_MISMATCH, "adapter_add: N * rank must be below 2^30");
   TEENY_REQUIRE(K % 8 == 0, TEENY_ERR_SHAPE_MISMATCH, "adapter_add: K must be a multiple of 8");
   TEENY_REQUIRE(rank % 8 == 0 && rank <= 128, TEENY_ERR_UNSUPPORTED, "adapter_add: rank must be a multiple of 8 up to 128");
   if (M == 0 || N == 0) return TEENY_OK;
   TEENY_REQUIRE(adapters != nullptr && y != nullptr && out != nullptr, TEENY_ERR_NULL_POINTER, "adapter_add: adapters/y/out");
-  TEENY_REQUIRE(y_stride >= N && out_stride >= N, TEENY_ERR_SHAPE_MISMATCH, "adapter_add: row strides below N");
+  TEENY_REQUIRE(y_stride >= N && out_stride >= N && y_stride <= 1 << 24 && out_stride <= 1 << 24, TEENY_ERR_SHAPE_MISMATCH,
+                "adapter_add: row strides below N or above 2^24");
   TEENY_REQUIRE(y != out || y_stride == out_stride, TEENY_ERR_INVALID_ARGUMENT,
                 "adapter_add: out can be y only with the same row stride");
   if (rank == 0 || K == 0) num_adapters = 0;
   TEENY_REQUIRE(num_adapters == 0 || (x != nullptr && a != nullptr && b != nullptr), TEENY_ERR_NULL_POINTER,
                 "adapter_add: x/a/b");
-  TEENY_REQUIRE(num_adapters == 0 || x_stride >= K, TEENY_ERR_SHAPE_MISMATCH, "adapter_add: row stride below K");
+  TEENY_REQUIRE(num_adapters == 0 || (x_stride >= K && x_stride <= 1 << 24), TEENY_ERR_SHAPE_MISMATCH,
+                "adapter_add: x's row stride below K or above 2^24");
   TEENY_REQUIRE(num_adapters == 0 || (aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && x_stride % 8 == 0),
                 TEENY_ERR_MISALIGNED, "adapter_add: 16-byte aligned x, a, b and x's row stride");
   AdapterArgs p{static_cast<const bf16 *>(x), static_cast<const bf16 *>(a), static_cast<const bf16 *>(b), adapters, scale,
                 static_cast<const bf16 *>(y), static_cast<bf16 *>(out), x_stride, y_stride, out_stride,
                 static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), static_cast<int>(rank),
-                static_cast<int>(num_adapters),
-                aligned(y, 16) && aligned(out, 16) && y_stride % 8 == 0 && out_stride % 8 == 0, 0, nullptr, 1, 0, 0};
+                static_cast<int>(num_adapters), 0, nullptr, 1, 0, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const AdapterPlan pl = adapter_plan(M, N, K, rank);
   const Scratch scr = stream_scratch(s);
@@ -370,7 +456,7 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
     p.cols = pl.cols;
     p.splits = pl.splits;
     p.chunk = pl.chunk;
-    p.by_row = pl.by_row;
+    p.slots = pl.slots;
     switch (pl.rt) {
       case 1: launch_adapter<1>(pl, p, s); break;
       case 2: launch_adapter<2>(pl, p, s); break;
@@ -396,7 +482,7 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
 teeny_status teeny_adapter_add_workspace_size(int64_t M, int64_t N, int64_t K, int64_t rank, size_t *bytes) {
   TEENY_REQUIRE(bytes != nullptr, TEENY_ERR_NULL_POINTER, "adapter_add_workspace_size: bytes");
   *bytes = 0;
-  TEENY_REQUIRE(M >= 0 && N >= 0 && K >= 0 && rank >= 0 && M <= 1 << 24 && N <= 1 << 24 && K <= 1 << 24,
+  TEENY_REQUIRE(M >= 0 && N >= 0 && K >= 0 && rank >= 0 && M <= 1 << 24 && N <= 1 << 24 && K <= 1 << 22,
                 TEENY_ERR_SHAPE_MISMATCH, "adapter_add_workspace_size: sizes out of range");
   TEENY_REQUIRE(rank % 8 == 0 && rank <= 128, TEENY_ERR_UNSUPPORTED,
                 "adapter_add_workspace_size: rank must be a multiple of 8 up to 128");

@@ -122,7 +122,7 @@ def adapter_args(**kw):
     (dict(M=(1 << 24) + 1), _lib.ERR_SHAPE_MISMATCH), (dict(N=(1 << 24) + 1, y_stride=1 << 25, out_stride=1 << 25), _lib.ERR_SHAPE_MISMATCH),
     (dict(K=1 << 25, x_stride=1 << 25), _lib.ERR_SHAPE_MISMATCH), (dict(num_adapters=BIG), _lib.ERR_SHAPE_MISMATCH),
     (dict(K=60), _lib.ERR_SHAPE_MISMATCH), (dict(rank=12), _lib.ERR_UNSUPPORTED), (dict(rank=136), _lib.ERR_UNSUPPORTED),
-    (dict(x_stride=56), _lib.ERR_SHAPE_MISMATCH), (dict(y_stride=99), _lib.ERR_SHAPE_MISMATCH), (dict(out_stride=99), _lib.ERR_SHAPE_MISMATCH),
+    (dict(x_stride=(1 << 24) + 8), _lib.ERR_SHAPE_MISMATCH), (dict(x_stride=56), _lib.ERR_SHAPE_MISMATCH), (dict(y_stride=99), _lib.ERR_SHAPE_MISMATCH), (dict(out_stride=99), _lib.ERR_SHAPE_MISMATCH),
     (dict(x_stride=68), _lib.ERR_MISALIGNED), *[(dict([(n, FAKE_ODD)]), _lib.ERR_MISALIGNED) for n in "xab"],
     (dict(out=FAKE, out_stride=108), _lib.ERR_INVALID_ARGUMENT),
     *[(dict([(n, None)]), _lib.ERR_NULL_POINTER) for n in ("x", "a", "b", "adapters", "y", "out")]])
