@@ -101,8 +101,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
   const u32x4 off_bits = u32x4{0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};  // -1.5
   const bf16x8 off = __builtin_bit_cast(bf16x8, off_bits);
+  const W4Bits w4;
   bf16x8 qf[NQ][NC];
-  f32x4 q_off[NQ][NG];  // -1.5 sum of q over the group, in every row
+  // NQ = 2 has no registers to spare for q_off and p_off: the products that give them are made again where they are used
+  f32x4 q_off[NQ == 1 ? NG : 1];  // -1.5 sum of q over the group, in every row
   int vis[NQ];
   int64_t out_row[NQ];
 #pragma unroll
@@ -118,15 +120,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       raw ^= qsign;
       qf[n][j] = __builtin_bit_cast(bf16x8, raw);
     }
+    if constexpr (NQ == 1)
 #pragma unroll
-    for (int G = 0; G < NG; ++G) {
-      q_off[n][G] = mfma16(off, qf[n][2 * G], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-      q_off[n][G] = mfma16(off, qf[n][2 * G + 1], q_off[n][G]);
-    }
+      for (int G = 0; G < NG; ++G)
+        q_off[G] = mfma16(off, qf[n][2 * G + 1], mfma16(off, qf[n][2 * G], f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
   }
   const int all_see = seen(r.row0);  // all rows see the tokens below it
 
-  f32x4 acc[NQ][ND], p_off[NQ][NG];  // p_off: -1.5 sum of the weighted probabilities, in every row
+  f32x4 acc[NQ][ND], p_off[NQ == 1 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
   float m_run[NQ], l_run[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -134,15 +135,17 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     l_run[n] = 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (NQ == 1)
 #pragma unroll
-    for (int G = 0; G < NG; ++G) p_off[n][G] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int G = 0; G < NG; ++G) p_off[G] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 #pragma unroll 1
   for (; t0 < ke; t0 += STEP) {
     float ksc[NG], vsc[NG];  // of the lane group's token c
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
-      ksc[G] = static_cast<float>(ks[G]) * sc0;
+      const float k = static_cast<float>(ks[G]);
+      ksc[G] = __builtin_fmaf(k, 0.0f, k) * sc0;  // an infinity counts as NaN
       vsc[G] = static_cast<float>(vs[G]);
     }
     f32x4 s[NQ][4];
@@ -150,26 +153,30 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int G = 0; G < NG; ++G) {
-        const bf16x8 a0 = w4_values(kr[i][2 * G]), a1 = w4_values(kr[i][2 * G + 1]);
+        const bf16x8 a0 = w4.values(kr[i][2 * G]), a1 = w4.values(kr[i][2 * G + 1]);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-          const f32x4 x = mfma16(a1, qf[n][2 * G + 1], mfma16(a0, qf[n][2 * G], q_off[n][G]));
+          f32x4 x = mfma16(a1, qf[n][2 * G + 1], mfma16(a0, qf[n][2 * G], NQ == 1 ? q_off[G % (NQ == 1 ? NG : 1)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+          if constexpr (NQ > 1) x = mfma16(off, qf[n][2 * G + 1], mfma16(off, qf[n][2 * G], x));
           each16([&](auto t) {
             constexpr int T = decltype(t)::value;
             if (T >> 2 == i) {
               const float sc = row_lane<T>(ksc[G]);
-              s[n][i][T & 3] = G == 0 ? x[T & 3] * sc : __builtin_fmaf(x[T & 3], sc, s[n][i][T & 3]);
+              s[n][i][T & 3] = G == 0 ? sc * x[T & 3] : __builtin_fmaf(sc, x[T & 3], s[n][i][T & 3]);
             }
           });
         }
       }
+      // scaled here and now, or the scaling sinks below the branch, away from the lanes it takes the scales from
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) asm volatile("" : "+v"(s[n][i]));
+      __builtin_amdgcn_sched_barrier(0);
     }
     const bool more = t0 + STEP < ke;
     const bool hidden = none;
     if (more) load_k(t0 + STEP, pg);
     const bool masks = t0 + 64 > all_see || __any(hidden);
     const int at = t0 + 16 * g;  // the lane's first token
-    bf16x8 pb[NQ][NG][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       if (masks) {  // also the scores of scales that may be anything
@@ -187,8 +194,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
         l_run[n] *= alpha;
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
+        if constexpr (NQ == 1)
 #pragma unroll
-        for (int G = 0; G < NG; ++G) p_off[n][G] *= alpha;
+          for (int G = 0; G < NG; ++G) p_off[G] *= alpha;
         m_run[n] = m_new;
       }
       const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
@@ -198,8 +206,12 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
         l_run[n] += e;
         s[n][i >> 2][i & 3] = e;
       }
+    }
 #pragma unroll
-      for (int G = 0; G < NG; ++G) {
+    for (int G = 0; G < NG; ++G) {
+      bf16x8 pb[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
         float v[16];
         each16([&](auto t) {
           constexpr int T = decltype(t)::value;
@@ -213,24 +225,25 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const bf16x2 pr = cvt_pk_bf16(v[i], v[i + 1]);
-          pb[n][G][i >> 3][i & 7] = pr[0];
-          pb[n][G][i >> 3][(i & 7) + 1] = pr[1];
+          pb[n][i >> 3][i & 7] = pr[0];
+          pb[n][i >> 3][(i & 7) + 1] = pr[1];
         }
       }
-    }
-#pragma unroll
-    for (int G = 0; G < NG; ++G)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) p_off[n][G] = mfma16(off, pb[n][G][h], p_off[n][G]);
+        if constexpr (NQ == 1) p_off[G % (NQ == 1 ? NG : 1)] = mfma16(off, pb[0][h], p_off[G % (NQ == 1 ? NG : 1)]);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const bf16x8 a = w4_values(vr[2 * G + (d >> 1)][2 * (d & 1) + h]);
+          const bf16x8 a = w4.values(vr[2 * G + (d >> 1)][2 * (d & 1) + h]);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) acc[n][4 * G + d] = mfma16(a, pb[n][G][h], acc[n][4 * G + d]);
+          for (int n = 0; n < NQ; ++n) {
+            acc[n][4 * G + d] = mfma16(a, pb[n][h], acc[n][4 * G + d]);
+            if constexpr (NQ > 1) acc[n][4 * G + d] = mfma16(off, pb[n][h], acc[n][4 * G + d]);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
     if (more) {
       load_v(t0 + STEP, pg);
       pg = load_pages(t0 + 2 * STEP);
@@ -264,7 +277,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     // blocks 2 a and 2 a + 1 hold the even and odd d's of 32 a ..: the lane's are eight consecutive ones
 #pragma unroll
     for (int a = 0; a < NV; ++a) {
-      const f32x4 even = (acc[n][2 * a] + p_off[n][a >> 1]) * mul, odd = (acc[n][2 * a + 1] + p_off[n][a >> 1]) * mul;
+      f32x4 even = acc[n][2 * a], odd = acc[n][2 * a + 1];
+      if constexpr (NQ == 1) even += p_off[a >> 1], odd += p_off[a >> 1];
+      even *= mul, odd *= mul;
       float *to = red + (w * WROWS + at) * LD + 32 * a + 8 * g;
       *reinterpret_cast<f32x4 *>(to) = f32x4{even[0], odd[0], even[1], odd[1]};
       *reinterpret_cast<f32x4 *>(to + 4) = f32x4{even[2], odd[2], even[3], odd[3]};
@@ -297,10 +312,295 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   }
 }
 
+// Eight codes of a word as code / 16 times eight scales.
+template <typename S>
+__device__ __forceinline__ bf16x8 kv4_values8(uint32_t word, S scale) {
+  const uint32_t even = word ^ 0x88888888u;  // two's complement nibbles
+  uint32_t odd = even >> 4;
+  asm("" : "+v"(odd));  // a byte of it is an operand as it is, of word >> 4 a shift more
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int n = w4_nibble(j);
+    v[j] = __builtin_amdgcn_cvt_off_f32_i4(static_cast<int>((n & 1 ? odd : even) >> (8 * (n >> 1)) & 0xffu));
+  }
+  scale(v);
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bf16x2 pr = cvt_pk_bf16(v[2 * j], v[2 * j + 1]);
+    r[2 * j] = pr[0];
+    r[2 * j + 1] = pr[1];
+  }
+  return r;
+}
+
+// Many query rows (prompts in pieces): bound by the products and the work beside
+// them.  As in kv_attn_tile a workgroup of four waves, 32 rows each, turns a tile of
+// 64 tokens once into the bf16 operands of v_mfma_f32_32x32x16_bf16, in LDS in the
+// order in which lanes take them up; here code times scale, a bf16 number already
+// where the scale has five bits (other scales: rounded), so that the products need
+// no scale of their own.  The next tile is turned while one is multiplied, the codes
+// of the tile after that are in flight; one barrier a tile.
+template <int D>
+__global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
+  constexpr int RB = 128, NS = D / 16, ND = D / 32, NU = D / 64, NG = D / 64, EPW = D / 32, FR = 2 * NS + 4 * ND;
+  typedef uint32_t kvec __attribute__((ext_vector_type(EPW)));
+  typedef __bf16 svec __attribute__((ext_vector_type(NG)));
+  __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
+  __shared__ uint64_t bad[2][NG];  // tokens of a tile whose V scale is not finite (they are turned to zeros)
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
+  const int split = in_head / p.blocks, u = in_head - split * p.blocks;
+  KvRows r;
+  if (!kv_rows_sorted<RB>(p, u, r)) return;
+  auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
+  const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
+  const int kb = split * p.chunk, ke = split == p.splits - 1 ? k_end : min(k_end, kb + p.chunk);
+  if (split > 0 && kb >= k_end) return;
+  const int base = r.row0 + 32 * w;  // the wave's rows; past r.rows it only helps to turn the tiles
+
+  // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too; 16: of kv4_values8
+  const float sc = fmaxf(16.0f * fabsf(p.scale_log2), 1.17549435e-38f);
+  const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
+  const int my = min(base + c, r.rows - 1), qt = my / p.group, qh = head * p.group + my - qt * p.group;
+  const int64_t out_row = static_cast<int64_t>(r.first + qt) * p.heads + qh;
+  const int vis = seen(my), all_see = seen(min(base, r.rows - 1));
+  const int w_end = base < r.rows ? min(ke, seen(min(base + 32, r.rows) - 1)) : 0;
+  bf16x8 qf[NS];  // step i: numbers of the K word that a lane of wave 2 x + i / EPW turns into it
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int e = i % EPW, d = 64 * (e >> 1) + 16 * (2 * (i / EPW) + g) + 8 * (e & 1);
+    u32x4 raw = *reinterpret_cast<const u32x4 *>(p.q + (r.first + qt) * p.q_stride + qh * D + d);
+    raw ^= qsign;
+    qf[i] = __builtin_bit_cast(bf16x8, raw);
+  }
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = zero16();
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  // The wave's share of a tile: 16 D / 8 bytes of each K row of block w / 2, and V of d block w, tokens of both blocks
+  // (D = 64: of d block w / 2 and block w % 2).  The four pages of a tile are one load for the wave; what follows from
+  // them is the same for all lanes and is worked out in scalar registers.
+  const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
+  const int page_mask = (1 << p.shift) - 1, wb = w >> 1, vd = D == 128 ? w : wb;
+  const bool k_odd = (c >> 2) & 1, g_odd = g;
+  const int k_row = 4 * (c >> 3) + (c & 3), k_lane = k_row * (D / 2) + (D / 8) * (2 * (w & 1) + g);
+  const int v_lane = 8 * (32 * vd + c);
+  auto v_block = [&](int i) { return D == 128 ? i : w & 1; };
+  // lane l: the page of tokens 16 (l % 4) .. of a tile
+  auto load_pages = [&](int t0) { return row[min(t0 + 16 * (lane & 3), k_end - 1) >> p.shift]; };
+  kvec kr;
+  u32x2 vr[NU];
+  svec ks;
+  bf16 vs[NU];
+  bool there_v[NU], hidden_next[2];
+  auto load_codes = [&](int t0, int pg) {
+    int64_t at[4];  // tokens of the cache
+    bool there[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int page = __builtin_amdgcn_readlane(pg, j), t = t0 + 16 * j;
+      there[j] = page >= 0 && page < p.pages && t < ke;
+      at[j] = ((static_cast<int64_t>(there[j] ? page : 0) * p.kv_heads + head) << p.shift) + (t & page_mask);
+    }
+    auto pick = [&](bool odd, int64_t x, int64_t y) { return odd ? y : x; };
+    const int64_t k_at = pick(k_odd, wb ? at[2] : at[0], wb ? at[3] : at[1]);
+    kr = *reinterpret_cast<const kvec *>(p.kc + k_at * (D / 2) + k_lane);
+    ks = *reinterpret_cast<const svec *>(p.ks + (k_at + k_row) * NG);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int v = v_block(i);
+      const int64_t v_at = pick(g_odd, v ? at[2] : at[0], v ? at[3] : at[1]);
+      vr[i] = *reinterpret_cast<const u32x2 *>(p.vc + v_at * (D / 2) + v_lane);
+      vs[i] = p.vs[(v_at + (lane & 15)) * NG + (vd >> 1)];
+      there_v[i] = (g_odd ? (v ? there[3] : there[1]) : (v ? there[2] : there[0])) && t0 + 32 * v + 16 * g + (lane & 15) < ke;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) hidden_next[b] = g_odd ? !there[2 * b + 1] : !there[2 * b];
+  };
+  auto turn = [&](int buf) {
+    u32x4 *to = frag[buf];
+#pragma unroll
+    for (int e = 0; e < EPW; ++e) {
+      const float s = static_cast<float>(ks[e >> 1]);
+      to[(wb * NS + EPW * (w & 1) + e) * 64 + lane] =
+          __builtin_bit_cast(u32x4, kv4_values8(kr[e], [&](float (&v)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= s;
+          }));
+    }
+    uint64_t unfit = 0;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      float s = static_cast<float>(vs[i]);
+      const bool finite = fabsf(s) < INFINITY;
+      const uint64_t m = __ballot(there_v[i] && !finite);  // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
+      unfit |= ((m & 0xffffu) | ((m >> 32 & 0xffffu) << 16)) << (32 * v_block(i));
+      s = there_v[i] && finite ? s : 0.0f;
+      const int at = 2 * NS + (vd * 2 + v_block(i)) * 2;
+      to[at * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[i][0], [&](float (&v)[8]) {
+                                                each16([&](auto t) {
+                                                  if constexpr (t < 8) v[t] *= row_lane<t>(s);
+                                                });
+                                              }));
+      to[(at + 1) * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[i][1], [&](float (&v)[8]) {
+                                                      each16([&](auto t) {
+                                                        if constexpr (t >= 8) v[t - 8] *= row_lane<t>(s);
+                                                      });
+                                                    }));
+    }
+    if constexpr (D == 128) {
+      if ((w & 1) == 0 && lane == 0) bad[buf][w >> 1] = unfit;
+    } else {
+      if (w < 2 && lane == 0) reinterpret_cast<uint32_t *>(bad[buf])[w] = static_cast<uint32_t>(unfit >> (32 * w));
+    }
+  };
+
+  int pg = 0, buf = 0;
+  bool none[2];
+  auto take = [&]() {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) none[b] = hidden_next[b];
+  };
+  if (kb < ke) {
+    pg = load_pages(kb);
+    load_codes(kb, pg);
+    pg = load_pages(kb + 64);
+    turn(0);
+    take();
+    if (kb + 64 < ke) {
+      load_codes(kb + 64, pg);
+      pg = load_pages(kb + 128);
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t0 = kb; t0 < ke; t0 += 64) {
+    const u32x4 *now = frag[buf];
+    const bool hidden[2] = {none[0], none[1]};
+    if (t0 + 64 < ke) {
+      turn(buf ^ 1);
+      take();
+      if (t0 + 128 < ke) {
+        load_codes(t0 + 128, pg);
+        pg = load_pages(t0 + 192);
+      }
+    }
+    if (t0 < w_end) {
+      // operands are read LA products ahead, V's first ones before the exponentials; the order is kept as written
+      constexpr int LA = 4, W = LA + 1;
+      u32x4 win[W];
+      auto read = [&](int i) __attribute__((always_inline)) {
+        const int j = i - 2 * NS;  // scores: both blocks in turn; outputs: the d blocks in turn
+        const int at = i < 2 * NS ? (i & 1) * NS + (i >> 1) : 2 * NS + (j % ND) * 4 + j / ND;
+        win[i % W] = now[at * 64 + lane];
+      };
+#pragma unroll
+      for (int i = 0; i < LA; ++i) read(i);
+      f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        read(i + LA);
+        s[i & 1] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), qf[i >> 1], s[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (t0 + 64 > all_see || __any(hidden[0] || hidden[1])) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (hidden[b] || t0 + 32 * b + 16 * g + v >= vis) s[b][v] = -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int v = 1; v < 32; ++v) mx = __builtin_elementwise_maximum(mx, s[v >> 4][v & 15]);
+      mx *= sc;
+      mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+      if (__any(mx > m_run + 8.0f)) {  // rescaled rarely: p <= 2^8
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+        m_run = m_new;
+      }
+      const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+      bf16x8 pb[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          s[b][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][v], sc, neg_m));
+          l_run += s[b][v];
+        }
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+          const bf16x2 pr = cvt_pk_bf16(s[b][v], s[b][v + 1]);
+          pb[b][v >> 3][v & 7] = pr[0];
+          pb[b][v >> 3][(v & 7) + 1] = pr[1];
+        }
+      }
+      // a row that sees a token whose V is NaN: its outputs of that group are
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        const uint64_t unfit = bad[buf][G];
+        if (unfit != 0) {
+          bool sees = false;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sees |= ((unfit >> (32 * b + 16 * g + v)) & 1) && !(s[b][v] == 0.0f);
+          sees = __shfl_xor(static_cast<int>(sees), 32, 64) != 0 || sees;  // the row's other tokens
+          if (sees) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4 * ND; ++j) {
+        const int i = 2 * NS + j, d = j % ND, bh = j / ND;
+        if (j + LA < 4 * ND) read(i + LA);
+        acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), pb[bh >> 1][bh & 1], acc[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    buf ^= 1;
+    __syncthreads();
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (base + c >= r.rows) return;
+  const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
+  const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
+  const int64_t slot = (unit * p.splits + split) * RB + 32 * w + c;
+  const float mul = 16.0f * (whole ? (l_run == 0.0f ? 0.0f : 1.0f / l_run) : 1.0f);
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int at = 32 * d + 8 * a + 4 * g;
+      f32x4 o = f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]} * mul;
+      if (whole) {
+        bf16x4 o4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o4[v] = static_cast<bf16>(o[v]);
+        *reinterpret_cast<bf16x4 *>(p.o + out_row * D + at) = o4;
+      } else {
+        *reinterpret_cast<f32x4 *>(p.part + slot * D + at) = o;
+      }
+    }
+  if (g == 0 && !whole) {
+    p.part[p.ml_off + slot * 2] = m_run;
+    p.part[p.ml_off + slot * 2 + 1] = l_run;
+  } else if (g == 0 && p.l != nullptr) {
+    p.l[out_row] = (m_run + log2f(l_run)) * 0.6931471805599453f;
+  }
+}
+
 static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                 int64_t max_ctx, size_t scratch) {
-  KvAttnPlan pl = kv_attn_plan(tokens, batch, heads, kv_heads, D, std::min<int64_t>(max_q, std::max<int64_t>(1, 64 * kv_heads / heads)), max_ctx, scratch);
-  return pl;
+  return kv_attn_plan(tokens, batch, heads, kv_heads, D, max_q, max_ctx, scratch);
 }
 
 template <int D, int NQ>
@@ -314,7 +614,12 @@ static void launch_kv4_attn(const KvAttnPlan &pl, const Kv4AttnArgs &p, hipStrea
 
 template <int D>
 static void launch_kv4_attn(const KvAttnPlan &pl, const Kv4AttnArgs &p, hipStream_t s) {
-  if (pl.nq == 2) launch_kv4_attn<D, 2>(pl, p, s);
+  if (pl.tile) {
+    const int64_t units = pl.blocks * p.kv_heads, rows = static_cast<int64_t>(p.tokens) * p.heads;
+    hipLaunchKernelGGL(kv4_attn_tile<D>, dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+    if (pl.splits > 1)
+      hipLaunchKernelGGL((kv_attn_combine<D, 128>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
+  } else if (pl.nq == 2) launch_kv4_attn<D, 2>(pl, p, s);
   else launch_kv4_attn<D, 1>(pl, p, s);
 }
 

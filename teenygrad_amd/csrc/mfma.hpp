@@ -174,5 +174,18 @@ __device__ __forceinline__ bf16x8 w4_values(uint32_t word) {
   r[3] = ((word >> 9) & 0x00780078u) | 0x3F803F80u;
   return __builtin_bit_cast(bf16x8, r);
 }
+// The same with the constants in registers, where AND and OR are one instruction (it takes one literal at most).
+struct W4Bits {
+  uint32_t mask = 0x00780078u, one = 0x3F803F80u;
+  __device__ __forceinline__ W4Bits() { asm("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ bf16x8 values(uint32_t word) const {
+    u32x4 r;
+    r[0] = ((word << 3) & mask) | one;
+    r[1] = ((word >> 1) & mask) | one;
+    r[2] = ((word >> 5) & mask) | one;
+    r[3] = ((word >> 9) & mask) | one;
+    return __builtin_bit_cast(bf16x8, r);
+  }
+};
 
 }  // namespace teeny
