@@ -30,12 +30,46 @@ struct Kv4AttnArgs : KvAttnArgs {
   const bf16 *ks, *vs;
 };
 
+// Codes as fp8 (e4m3): the bytes 0 .. 15 are the numbers 0 .. 15 times 2^-9, since denormal numbers and the first
+// normal ones lie equally far apart.  So a nibble is its operand as it is, in the order of fp8_order.
+__device__ __forceinline__ int64_t w4_fp8(uint32_t word) {
+  const uint32_t even = word & 0x0f0f0f0fu, odd = (word >> 4) & 0x0f0f0f0fu;
+  return static_cast<int64_t>(static_cast<uint64_t>(odd) << 32 | even);
+}
+__device__ constexpr int fp8_order(int byte) { return (byte & 1) * 4 + (byte >> 1); }
+
+// Eight numbers as the sum of two fp8 ones each, bytes in fp8_order.  Of numbers up to 256 the first takes four bits of
+// significand, the second what is left, down to 2^-9.
+__device__ __forceinline__ void fp8_parts(const float (&v)[8], int64_t &first, int64_t &second) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  uint32_t part[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[fp8_order(4 * h + i)];
+    int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], a, true);
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+    int b = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] - lo[0], x[1] - lo[1], 0, false);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] - hi[0], x[3] - hi[1], b, true);
+    part[0][h] = a;
+    part[1][h] = b;
+  }
+  first = static_cast<int64_t>(static_cast<uint64_t>(part[0][1]) << 32 | part[0][0]);
+  second = static_cast<int64_t>(static_cast<uint64_t>(part[1][1]) << 32 | part[1][0]);
+}
+__device__ __forceinline__ f32x4 mfma16_fp8(int64_t a, int64_t b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a, b, c, 0, 0, 0);
+}
+
 // NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   constexpr int WK = 4, WROWS = 16 * NQ, RB = WROWS;
   constexpr int NC = D / 32, ND = D / 16, NG = D / 64, NV = D / 32;  // k-steps of the scores, d blocks, groups, V vectors
   constexpr int LD = D + 4;
+  constexpr bool FP8 = NQ == 1;  // keys as fp8 operands
   typedef uint32_t kvec __attribute__((ext_vector_type(2 * NG)));
   typedef __bf16 svec __attribute__((ext_vector_type(NG)));
   __shared__ __attribute__((aligned(16))) float red[WK * WROWS * LD];
@@ -97,37 +131,69 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     pg = load_pages(t0 + STEP);
   }
 
-  const float sc0 = 16.0f * fabsf(p.scale_log2);  // 16: of w4_values
   const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
   const u32x4 off_bits = u32x4{0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};  // -1.5
   const bf16x8 off = __builtin_bit_cast(bf16x8, off_bits);
   const W4Bits w4;
-  bf16x8 qf[NQ][NC];
-  // NQ = 2 has no registers to spare for q_off and p_off: the products that give them are made again where they are used
-  f32x4 q_off[NQ == 1 ? NG : 1];  // -1.5 sum of q over the group, in every row
+  bf16x8 qf[FP8 ? 1 : NQ][FP8 ? 1 : NC];
+  int64_t q8[FP8 ? NC : 1][2];
+  f32x4 q_off[FP8 ? NG : 1];  // -8 sum of q over the group (times 2^-9), in every row
+  float col[NQ];              // what the column's scores are to be multiplied with, softmax_scale among it
   int vis[NQ];
-  int64_t out_row[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int i = min(r.row0 + 16 * n + c, r.rows - 1), t = i / p.group;
     vis[n] = p.causal ? min(max(r.ctx - r.len + 1 + t, 0), r.ctx) : r.ctx;
     const int h = head * p.group + i - t * p.group;
-    out_row[n] = static_cast<int64_t>(r.first + t) * p.heads + h;
     const bf16 *at = p.q + (r.first + t) * p.q_stride + h * D;
+    u32x4 raw[NC];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      u32x4 raw = *reinterpret_cast<const u32x4 *>(at + (j >> 1) * 64 + g * 16 + (j & 1) * 8);
-      raw ^= qsign;
-      qf[n][j] = __builtin_bit_cast(bf16x8, raw);
+      raw[j] = *reinterpret_cast<const u32x4 *>(at + (j >> 1) * 64 + g * 16 + (j & 1) * 8);
+      raw[j] ^= qsign;
     }
-    if constexpr (NQ == 1)
+    float scale = 16.0f * fabsf(p.scale_log2);  // 16: of W4Bits
+    if constexpr (FP8) {
+      // the row's largest number to 128 .. 256 by a power of two; an infinity or NaN makes all of it NaN
+      uint32_t most = 0;
 #pragma unroll
-      for (int G = 0; G < NG; ++G)
-        q_off[G] = mfma16(off, qf[n][2 * G + 1], mfma16(off, qf[n][2 * G], f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, max(raw[j][e] & 0x7fffu, raw[j][e] >> 16 & 0x7fffu));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16, 64)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32, 64)));
+      const int exponent = max(static_cast<int>(most >> 7), 8);  // biased; below: numbers that lose bits beside 2^-119
+      const float up = most >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(127 + 127 + 7 - exponent) << 23);
+      scale = __builtin_ldexpf(fabsf(p.scale_log2), exponent - 134 + 9);  // over `up` and 2^-9
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] = __uint_as_float(raw[j][e] << 16) * up;
+          v[2 * e + 1] = __uint_as_float(raw[j][e] & 0xffff0000u) * up;
+        }
+        fp8_parts(v, q8[j][0], q8[j][1]);
+      }
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        q_off[G] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int64_t minus8 = static_cast<int64_t>(0x8888888888888888ull);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) q_off[G] = mfma16_fp8(minus8, q8[2 * G + j][b], q_off[G]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) qf[n][j] = __builtin_bit_cast(bf16x8, raw[j]);
+    }
+    // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too
+    col[n] = fmaxf(scale, 1.17549435e-38f);
   }
   const int all_see = seen(r.row0);  // all rows see the tokens below it
 
-  f32x4 acc[NQ][ND], p_off[NQ == 1 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
+  f32x4 acc[NQ][ND], p_off[FP8 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
   float m_run[NQ], l_run[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -135,7 +201,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     l_run[n] = 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (NQ == 1)
+    if constexpr (FP8)
 #pragma unroll
       for (int G = 0; G < NG; ++G) p_off[G] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -145,7 +211,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
       const float k = static_cast<float>(ks[G]);
-      ksc[G] = __builtin_fmaf(k, 0.0f, k) * sc0;  // an infinity counts as NaN
+      ksc[G] = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
       vsc[G] = static_cast<float>(vs[G]);
     }
     f32x4 s[NQ][4];
@@ -153,11 +219,29 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int G = 0; G < NG; ++G) {
-        const bf16x8 a0 = w4.values(kr[i][2 * G]), a1 = w4.values(kr[i][2 * G + 1]);
+        f32x4 xs[NQ];
+        if constexpr (FP8) {
+          xs[0] = q_off[G % (FP8 ? NG : 1)];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int64_t a = w4_fp8(kr[i][2 * G + j]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) xs[0] = mfma16_fp8(a, q8[(2 * G + j) % (FP8 ? NC : 1)][b], xs[0]);
+          }
+        } else {
+          // (no registers to spare for the offsets: the products that give them are made again)
+          const bf16x8 a0 = w4.values(kr[i][2 * G]), a1 = w4.values(kr[i][2 * G + 1]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            const bf16x8 *q = qf[n % (FP8 ? 1 : NQ)];
+            const int j = (2 * G) % (FP8 ? 1 : NC), k = (2 * G + 1) % (FP8 ? 1 : NC);
+            xs[n] = mfma16(a1, q[k], mfma16(a0, q[j], f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+            xs[n] = mfma16(off, q[k], mfma16(off, q[j], xs[n]));
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-          f32x4 x = mfma16(a1, qf[n][2 * G + 1], mfma16(a0, qf[n][2 * G], NQ == 1 ? q_off[G % (NQ == 1 ? NG : 1)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
-          if constexpr (NQ > 1) x = mfma16(off, qf[n][2 * G + 1], mfma16(off, qf[n][2 * G], x));
+          const f32x4 x = xs[n];
           each16([&](auto t) {
             constexpr int T = decltype(t)::value;
             if (T >> 2 == i) {
@@ -187,14 +271,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       float mx = s[n][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
-      mx = over_groups(mx, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      mx = over_groups(mx * col[n], [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
       if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
         const float m_new = fmaxf(m_run[n], mx);
         const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
         l_run[n] *= alpha;
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[n][d] *= alpha;
-        if constexpr (NQ == 1)
+        if constexpr (FP8)
 #pragma unroll
           for (int G = 0; G < NG; ++G) p_off[G] *= alpha;
         m_run[n] = m_new;
@@ -202,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(s[n][i >> 2][i & 3] + neg_m);
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], col[n], neg_m));
         l_run[n] += e;
         s[n][i >> 2][i & 3] = e;
       }
@@ -231,14 +315,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if constexpr (NQ == 1) p_off[G % (NQ == 1 ? NG : 1)] = mfma16(off, pb[0][h], p_off[G % (NQ == 1 ? NG : 1)]);
+        if constexpr (FP8) p_off[G % (FP8 ? NG : 1)] = mfma16(off, pb[0][h], p_off[G % (FP8 ? NG : 1)]);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           const bf16x8 a = w4.values(vr[2 * G + (d >> 1)][2 * (d & 1) + h]);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
             acc[n][4 * G + d] = mfma16(a, pb[n][h], acc[n][4 * G + d]);
-            if constexpr (NQ > 1) acc[n][4 * G + d] = mfma16(off, pb[n][h], acc[n][4 * G + d]);
+            if constexpr (!FP8) acc[n][4 * G + d] = mfma16(off, pb[n][h], acc[n][4 * G + d]);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -278,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
 #pragma unroll
     for (int a = 0; a < NV; ++a) {
       f32x4 even = acc[n][2 * a], odd = acc[n][2 * a + 1];
-      if constexpr (NQ == 1) even += p_off[a >> 1], odd += p_off[a >> 1];
+      if constexpr (FP8) even += p_off[(a >> 1) % (FP8 ? NG : 1)], odd += p_off[(a >> 1) % (FP8 ? NG : 1)];
       even *= mul, odd *= mul;
       float *to = red + (w * WROWS + at) * LD + 32 * a + 8 * g;
       *reinterpret_cast<f32x4 *>(to) = f32x4{even[0], odd[0], even[1], odd[1]};
@@ -289,7 +373,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
         p.part[p.ml_off + (slot + at) * 2] = m;
         p.part[p.ml_off + (slot + at) * 2 + 1] = l;
       } else if (p.l != nullptr) {
-        p.l[out_row[n]] = (m + log2f(l)) * 0.6931471805599453f;
+        const int t = (r.row0 + at) / p.group;
+        p.l[static_cast<int64_t>(r.first + t) * p.heads + head * p.group + r.row0 + at - t * p.group] = (m + log2f(l)) * 0.6931471805599453f;
       }
     }
   }

@@ -94,7 +94,8 @@ def attention(q, kc, vc, ks, vs, table, ctx, starts, scale, causal):
     """(o, lse, bound on o's error, bound on lse's) in 64 bits; q fp32 [T, Hq, D].  Rows of no sequence hold NaN.
 
     The bound: a group's scores are an fp32 sum of 64 products of q and 24 + code (16 to 31) and of 24 times q's sum, which
-    the scale multiplies; the exponents are off by as much and a few roundings; a probability times its V scale is rounded
+    the scale multiplies; where q is held as the sum of two fp8 numbers (its largest between 128 and 256, the second's last
+    bit 2^-9), it is off by 2^-10, so by 2^-17 of the largest; the exponents are off by as much and a few roundings; a probability times its V scale is rounded
     to bf16 (of the sum of p |v|), multiplies 24 + code in an fp32 sum over the tokens, less 24 times its own sum; the
     output is rounded to bf16.  A code times its scale is a bf16 number (scales of five bits): kernels may multiply that."""
     t, hq, d = q.shape
@@ -130,7 +131,8 @@ def attention(q, kc, vc, ks, vs, table, ctx, starts, scale, causal):
                 lse[rows] = (m + np.log(den))[:, 0]
                 # 2.4375 = 39 / 16: the largest operand, with that of the sum beside it
                 made = (np.abs(qq) @ (39 * np.abs(steps[0][:n]) + np.abs(k)).T).max(-1, keepdims=True) * abs(scale)
-                off_s = (64 + 16) * H32 * made + 8 * H32 * (np.abs(s).max(-1, keepdims=True) + 16)
+                made = made * (64 + 16) * H32 + np.abs(qq).max(-1, keepdims=True) * np.abs(k).sum(-1).max() * 2.0 ** -17 * abs(scale)
+                off_s = made + 8 * H32 * (np.abs(s).max(-1, keepdims=True) + 16)
                 mag, held = p @ np.abs(v) / den, p @ (39 * np.abs(steps[1][:n])) / den
                 tol[rows] = (mag * (H16 + 2 * off_s) + (mag + held) * (n + 64) * 2 * H32) * 1.01 + np.abs(o[rows]) * H16 * 1.01 + 1e-30
                 # (the rounded probabilities also multiply the offset, whose sum is taken off exactly: the same rounded ones)
