@@ -28,7 +28,45 @@ namespace teeny {
 
 struct Kv4AttnArgs : KvAttnArgs {
   const bf16 *ks, *vs;
+  int sorted;  // parts in order of their length
 };
+
+// Part u of a head, one split of one row block, the longest parts first (in eighths of a split), for up to 64 sequences:
+// a later, longer part would run on alone when the others are done.  Lane b counts its sequence's parts that are longer
+// than tau eighths; they are the first ones of the order: whole splits, then the rest of the context.
+template <int RB>
+__device__ __forceinline__ bool kv4_parts_sorted(const KvAttnArgs &p, int u, KvRows &r, int &split) {
+  const int lane = threadIdx.x & 63, b = min(lane, p.batch - 1);
+  auto start = [&](int i) { return min(max(p.starts ? p.starts[i] : i, 0), p.tokens); };
+  const int first = start(b), len = lane < p.batch ? max(start(b + 1) - first, 0) : 0;
+  const int nb = (len * p.group + RB - 1) / RB, ctx = min(max(p.ctx[b], 0), p.width << p.shift);
+  const int full = min(ctx / p.chunk, p.splits), rest = full < p.splits ? ctx - full * p.chunk : 0, eighth = p.chunk / 8;
+  auto count = [&](int tau) -> uint32_t {
+    if (tau == 0) return nb * max(full + (rest > 0), 1);
+    return nb * ((tau <= 8 ? full : 0) + (rest > (tau - 1) * eighth && tau <= 8));
+  };
+  auto total = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(v)), 63)); };
+  if (total(count(0)) <= static_cast<uint32_t>(u)) return false;
+  int lo = 0, hi = 9;  // total(count(lo)) > u >= total(count(hi)) = 0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (total(count(mid)) > static_cast<uint32_t>(u)) lo = mid;
+    else hi = mid;
+  }
+  const uint32_t above = count(hi), here = count(lo) - above, upto = wave_scan(here);
+  const uint32_t at = u - total(above);
+  const int owner = __builtin_ctzll(__ballot(upto > at));
+  auto from = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+  const int blocks = from(nb), part = from(above) + at - (from(upto) - from(here));
+  r.b = owner;
+  r.first = from(first);
+  r.len = from(len);
+  r.rows = r.len * p.group;
+  r.ctx = from(ctx);
+  split = part / blocks;
+  r.row0 = (part - split * blocks) * RB;
+  return true;
+}
 
 // Codes as fp8 (e4m3): the bytes 0 .. 15 are the numbers 0 .. 15 times 2^-9, since denormal numbers and the first
 // normal ones lie equally far apart.  So a nibble is its operand as it is, in the order of fp8_order.
@@ -79,9 +117,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   const int per_block = p.splits * p.kv_heads, first = p.walk * per_block;
   const bool beyond = static_cast<int>(blockIdx.x) >= first;
   const int id = beyond ? blockIdx.x - first : xcd_remap(blockIdx.x, first), of = beyond ? p.blocks - p.walk : p.walk;
-  const int head = id / (p.splits * of), in_head = id - head * (p.splits * of), split = in_head / of;
+  const int head = id / (p.splits * of), in_head = id - head * (p.splits * of);
+  int split = in_head / of;
   KvRows r;
-  if (!kv_rows<RB>(p, in_head - split * of + (beyond ? p.walk : 0), r)) return;
+  if (p.sorted) {
+    if (!kv4_parts_sorted<RB>(p, in_head + (beyond ? p.walk * p.splits : 0), r, split)) return;
+  } else if (!kv_rows<RB>(p, in_head - split * of + (beyond ? p.walk : 0), r)) {
+    return;
+  }
   // row i of the sequence: query i / group, head i % group of the K/V head's; it sees seen(i) tokens
   auto seen = [&](int i) { return p.causal ? min(max(r.ctx - r.len + 1 + i / p.group, 0), r.ctx) : r.ctx; };
   const int k_end = seen(min(r.row0 + RB, r.rows) - 1);
@@ -683,9 +726,45 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   }
 }
 
+// ── which form, and how many splits ─────────────────────────────────────────
+// Few rows take kv4_attn, more than 64 a sequence the shared tiles, with splits as kv_attn.hip's.  kv4_attn's splits give
+// a workgroup one round of 256 tokens where they leave CUs free, two where the device is busier, from three rounds on.
+// Several sequences, which may differ in length, take so many that there are four workgroups to a CU if all are as long
+// as the longest, of 1024 tokens or more each, and never more than 8192 tokens to
+// one (of many sequences one may be by far the longest); up to 64 of them are dealt out longest first.  us by splits, one query, 8
+// K/V heads of 128: 64 x 90 to 8000 1 / 2 / 4 / 8 72 / 68 / 67 / 72 (in the sequences' order 72 / 71 / 72 / 76), of
+// 8000 107 / 122 / 118 / 131; 32 x 100 to 8000 1 / 2 / 4 / 8 62 / 49 / 38 / 40; 64 x 90 to 4000 1 / 2 / 3 / 4 42 / 39 / 42 /
+// 41; 16 x 90 to 20000 4 / 6 / 8 / 12 59 / 47 / 45 / 46; 16 x 4000 1 / 2 / 4 / 8 31 / 24 / 22.4 / 26; 100 x 90 to 8000 1 / 2 /
+// 4 102 / 111 / 108; 4 x 2000 1 / 2 / 4 / 8 16 / 13.6 / 11 / 9.7; 1 x 2000 1 / 4 / 8 16 / 10.5 / 9.2; 1 x 30000 8 / 16 / 32 33
+// / 22.5 / 18; 8 x 1000 1 / 2 / 4 10.4 / 11.1 / 10.0; 4 heads of 64: 64 x 90 to 8000 1 / 2 / 4 / 8 39 / 33 / 31 / 35.
 static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                 int64_t max_ctx, size_t scratch) {
-  return kv_attn_plan(tokens, batch, heads, kv_heads, D, max_q, max_ctx, scratch);
+  KvAttnPlan pl;
+  const int64_t group = heads / kv_heads, rows = group * std::min(max_q, tokens);
+  if (rows > 64) return kv_attn_plan(tokens, batch, heads, kv_heads, D, max_q, max_ctx, scratch);
+  if (rows > 16) pl.nq = 2, pl.rb = 32;
+  pl.blocks = tokens * group / pl.rb + batch;
+  const int64_t there = std::max<int64_t>(1, std::min(pl.blocks, batch * cdiv(std::max<int64_t>(rows, 1), pl.rb)));
+  pl.walk = batch > kDense ? pl.blocks : there;
+  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count();
+  const int64_t busy = there * kv_heads;  // workgroups with work, unsplit
+  const int64_t least = busy <= 64 ? 256 : 512;
+  int64_t splits = 1;
+  if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
+  if (batch > 1) splits = std::max({splits, std::min((4 * cus + busy / 2) / busy, max_ctx / 1024), max_ctx / 8192});
+  // a launch has less than 2^31 threads (the limit of rows leaves room for four splits at least)
+  splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / 256 - 1) / units));
+  auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
+  auto cut = [&](int64_t n) {
+    pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), n), 256) * 256);
+    pl.splits = static_cast<int>(cdiv(std::max<int64_t>(max_ctx, 1), pl.chunk));
+    pl.bytes = size(pl.splits);
+  };
+  cut(splits);
+  pl.most = size(splits);
+  if (pl.bytes > scratch)  // as many parts as it holds
+    cut(std::max<int64_t>(1, static_cast<int64_t>(scratch / (static_cast<size_t>(units) * pl.rb * (D + 2) * 4))));
+  return pl;
 }
 
 template <int D, int NQ>
@@ -731,6 +810,7 @@ teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, con
                 "kv4_cache_attention: 4-byte aligned scales");
   p.ks = static_cast<const bf16 *>(k_scale);
   p.vs = static_cast<const bf16 *>(v_scale);
+  p.sorted = batch > 1 && batch <= 64 && pl.walk * pl.splits * kv_heads > 2 * device_cu_count();
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 64) launch_kv4_attn<64>(pl, p, s);
   else launch_kv4_attn<128>(pl, p, s);
