@@ -464,19 +464,19 @@ __device__ __forceinline__ bf16x8 kv4_values8(uint32_t word, S scale) {
 }
 
 // Many query rows (prompts in pieces): bound by the products and the work beside
-// them.  As in kv_attn_tile a workgroup of four waves, 32 rows each, turns a tile of
+// them.  As in kv_attn_tile a workgroup of eight waves, 32 rows each, turns a tile of
 // 64 tokens once into the bf16 operands of v_mfma_f32_32x32x16_bf16, in LDS in the
 // order in which lanes take them up; here code times scale, a bf16 number already
 // where the scale has five bits (other scales: rounded), so that the products need
 // no scale of their own.  The next tile is turned while one is multiplied, the codes
-// of the tile after that are in flight; one barrier a tile.
+// of the tile after that are in flight; one barrier a tile.  (Four waves and 128 rows, two workgroups on a CU: every row
+// pays for turning twice as often, 4 x 700 queries 174 us to 150.)
 template <int D>
-__global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
-  constexpr int RB = 128, NS = D / 16, ND = D / 32, NU = D / 64, NG = D / 64, EPW = D / 32, FR = 2 * NS + 4 * ND;
-  typedef uint32_t kvec __attribute__((ext_vector_type(EPW)));
-  typedef __bf16 svec __attribute__((ext_vector_type(NG)));
+__global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
+  constexpr int RB = 256, NS = D / 16, ND = D / 32, NG = D / 64, EPW = D / 32, KW = D / 64, FR = 2 * NS + 4 * ND;
+  typedef uint32_t kvec __attribute__((ext_vector_type(KW)));
   __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
-  __shared__ uint64_t bad[2][NG];  // tokens of a tile whose V scale is not finite (they are turned to zeros)
+  __shared__ uint32_t bad[2][NG][2];  // tokens of a tile whose V scale is not finite (they are turned to zeros)
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
@@ -509,22 +509,20 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   for (int d = 0; d < ND; ++d) acc[d] = zero16();
   float m_run = -INFINITY, l_run = 0.0f;
 
-  // The wave's share of a tile: 16 D / 8 bytes of each K row of block w / 2, and V of d block w, tokens of both blocks
-  // (D = 64: of d block w / 2 and block w % 2).  The four pages of a tile are one load for the wave; what follows from
-  // them is the same for all lanes and is worked out in scalar registers.
+  // The wave's share of a tile: of the K rows of block w / 2 % 2, of their chunks 2 (w % 2) and 2 (w % 2) + 1, the words of
+  // group w / 4 (D = 64: word w / 4), and of V block w % 2 of d block w / 2 (D = 64: four waves do).  The four pages of a
+  // tile are one load for the wave; what follows from them is the same for all lanes and is worked out in scalar registers.
   const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
-  const int page_mask = (1 << p.shift) - 1, wb = w >> 1, vd = D == 128 ? w : wb;
+  const int page_mask = (1 << p.shift) - 1, wb = (w >> 1) & 1, wk = w >> 2, vd = D == 128 ? w >> 1 : (w >> 1) & 1, vb = w & 1;
   const bool k_odd = (c >> 2) & 1, g_odd = g;
-  const int k_row = 4 * (c >> 3) + (c & 3), k_lane = k_row * (D / 2) + (D / 8) * (2 * (w & 1) + g);
+  const int k_row = 4 * (c >> 3) + (c & 3), k_lane = k_row * (D / 2) + (D / 8) * (2 * (w & 1) + g) + 4 * KW * wk;
   const int v_lane = 8 * (32 * vd + c);
-  auto v_block = [&](int i) { return D == 128 ? i : w & 1; };
   // lane l: the page of tokens 16 (l % 4) .. of a tile
   auto load_pages = [&](int t0) { return row[min(t0 + 16 * (lane & 3), k_end - 1) >> p.shift]; };
   kvec kr;
-  u32x2 vr[NU];
-  svec ks;
-  bf16 vs[NU];
-  bool there_v[NU], hidden_next[2];
+  u32x2 vr;
+  bf16 ks, vs;
+  bool there_v, hidden_next[2];
   auto load_codes = [&](int t0, int pg) {
     int64_t at[4];  // tokens of the cache
     bool there[4];
@@ -537,54 +535,43 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     auto pick = [&](bool odd, int64_t x, int64_t y) { return odd ? y : x; };
     const int64_t k_at = pick(k_odd, wb ? at[2] : at[0], wb ? at[3] : at[1]);
     kr = *reinterpret_cast<const kvec *>(p.kc + k_at * (D / 2) + k_lane);
-    ks = *reinterpret_cast<const svec *>(p.ks + (k_at + k_row) * NG);
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int v = v_block(i);
-      const int64_t v_at = pick(g_odd, v ? at[2] : at[0], v ? at[3] : at[1]);
-      vr[i] = *reinterpret_cast<const u32x2 *>(p.vc + v_at * (D / 2) + v_lane);
-      vs[i] = p.vs[(v_at + (lane & 15)) * NG + (vd >> 1)];
-      there_v[i] = (g_odd ? (v ? there[3] : there[1]) : (v ? there[2] : there[0])) && t0 + 32 * v + 16 * g + (lane & 15) < ke;
+    ks = p.ks[(k_at + k_row) * NG + (D == 128 ? wk : 0)];
+    const int64_t v_at = pick(g_odd, vb ? at[2] : at[0], vb ? at[3] : at[1]);
+    if (D == 128 || w < 4) {
+      vr = *reinterpret_cast<const u32x2 *>(p.vc + v_at * (D / 2) + v_lane);
+      vs = p.vs[(v_at + (lane & 15)) * NG + (vd >> 1)];
+      there_v = (g_odd ? (vb ? there[3] : there[1]) : (vb ? there[2] : there[0])) && t0 + 32 * vb + 16 * g + (lane & 15) < ke;
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) hidden_next[b] = g_odd ? !there[2 * b + 1] : !there[2 * b];
   };
   auto turn = [&](int buf) {
     u32x4 *to = frag[buf];
+    const float k_scale = static_cast<float>(ks);
 #pragma unroll
-    for (int e = 0; e < EPW; ++e) {
-      const float s = static_cast<float>(ks[e >> 1]);
-      to[(wb * NS + EPW * (w & 1) + e) * 64 + lane] =
+    for (int e = 0; e < KW; ++e)
+      to[(wb * NS + EPW * (w & 1) + KW * wk + e) * 64 + lane] =
           __builtin_bit_cast(u32x4, kv4_values8(kr[e], [&](float (&v)[8]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= s;
+            for (int j = 0; j < 8; ++j) v[j] *= k_scale;
           }));
-    }
-    uint64_t unfit = 0;
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      float s = static_cast<float>(vs[i]);
-      const bool finite = fabsf(s) < INFINITY;
-      const uint64_t m = __ballot(there_v[i] && !finite);  // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
-      unfit |= ((m & 0xffffu) | ((m >> 32 & 0xffffu) << 16)) << (32 * v_block(i));
-      s = there_v[i] && finite ? s : 0.0f;
-      const int at = 2 * NS + (vd * 2 + v_block(i)) * 2;
-      to[at * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[i][0], [&](float (&v)[8]) {
-                                                each16([&](auto t) {
-                                                  if constexpr (t < 8) v[t] *= row_lane<t>(s);
-                                                });
-                                              }));
-      to[(at + 1) * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[i][1], [&](float (&v)[8]) {
-                                                      each16([&](auto t) {
-                                                        if constexpr (t >= 8) v[t - 8] *= row_lane<t>(s);
-                                                      });
-                                                    }));
-    }
-    if constexpr (D == 128) {
-      if ((w & 1) == 0 && lane == 0) bad[buf][w >> 1] = unfit;
-    } else {
-      if (w < 2 && lane == 0) reinterpret_cast<uint32_t *>(bad[buf])[w] = static_cast<uint32_t>(unfit >> (32 * w));
-    }
+    if (D == 64 && w >= 4) return;
+    float s = static_cast<float>(vs);
+    const bool finite = fabsf(s) < INFINITY;
+    const uint64_t m = __ballot(there_v && !finite);  // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
+    s = there_v && finite ? s : 0.0f;
+    const int at = 2 * NS + (vd * 2 + vb) * 2;
+    to[at * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[0], [&](float (&v)[8]) {
+                                              each16([&](auto t) {
+                                                if constexpr (t < 8) v[t] *= row_lane<t>(s);
+                                              });
+                                            }));
+    to[(at + 1) * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[1], [&](float (&v)[8]) {
+                                                    each16([&](auto t) {
+                                                      if constexpr (t >= 8) v[t - 8] *= row_lane<t>(s);
+                                                    });
+                                                  }));
+    if ((vd & 1) == 0 && lane == 0) bad[buf][vd >> 1][vb] = static_cast<uint32_t>((m & 0xffffu) | (m >> 32 & 0xffffu) << 16);
   };
 
   int pg = 0, buf = 0;
@@ -619,12 +606,12 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     }
     if (t0 < w_end) {
       // operands are read LA products ahead, V's first ones before the exponentials; the order is kept as written
-      constexpr int LA = 4, W = LA + 1;
-      u32x4 win[W];
+      constexpr int LA = 4, WIN = LA + 1;
+      u32x4 win[WIN];
       auto read = [&](int i) __attribute__((always_inline)) {
         const int j = i - 2 * NS;  // scores: both blocks in turn; outputs: the d blocks in turn
         const int at = i < 2 * NS ? (i & 1) * NS + (i >> 1) : 2 * NS + (j % ND) * 4 + j / ND;
-        win[i % W] = now[at * 64 + lane];
+        win[i % WIN] = now[at * 64 + lane];
       };
 #pragma unroll
       for (int i = 0; i < LA; ++i) read(i);
@@ -632,7 +619,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 #pragma unroll
       for (int i = 0; i < 2 * NS; ++i) {
         read(i + LA);
-        s[i & 1] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), qf[i >> 1], s[i & 1]);
+        s[i & 1] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % WIN]), qf[i >> 1], s[i & 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (t0 + 64 > all_see || __any(hidden[0] || hidden[1])) {
@@ -674,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
       // a row that sees a token whose V is NaN: its outputs of that group are
 #pragma unroll
       for (int G = 0; G < NG; ++G) {
-        const uint64_t unfit = bad[buf][G];
+        const uint64_t unfit = bad[buf][G][0] | static_cast<uint64_t>(bad[buf][G][1]) << 32;
         if (unfit != 0) {
           bool sees = false;
 #pragma unroll
@@ -690,7 +677,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
       for (int j = 0; j < 4 * ND; ++j) {
         const int i = 2 * NS + j, d = j % ND, bh = j / ND;
         if (j + LA < 4 * ND) read(i + LA);
-        acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % W]), pb[bh >> 1][bh & 1], acc[d]);
+        acc[d] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % WIN]), pb[bh >> 1][bh & 1], acc[d]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -727,36 +714,48 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 }
 
 // ── which form, and how many splits ─────────────────────────────────────────
-// Few rows take kv4_attn, more than 64 a sequence the shared tiles, with splits as kv_attn.hip's.  kv4_attn's splits give
-// a workgroup one round of 256 tokens where they leave CUs free, two where the device is busier, from three rounds on.
-// Several sequences, which may differ in length, take so many that there are four workgroups to a CU if all are as long
-// as the longest, of 1024 tokens or more each, and never more than 8192 tokens to
-// one (of many sequences one may be by far the longest); up to 64 of them are dealt out longest first.  us by splits, one query, 8
-// K/V heads of 128: 64 x 90 to 8000 1 / 2 / 4 / 8 72 / 68 / 67 / 72 (in the sequences' order 72 / 71 / 72 / 76), of
-// 8000 107 / 122 / 118 / 131; 32 x 100 to 8000 1 / 2 / 4 / 8 62 / 49 / 38 / 40; 64 x 90 to 4000 1 / 2 / 3 / 4 42 / 39 / 42 /
-// 41; 16 x 90 to 20000 4 / 6 / 8 / 12 59 / 47 / 45 / 46; 16 x 4000 1 / 2 / 4 / 8 31 / 24 / 22.4 / 26; 100 x 90 to 8000 1 / 2 /
-// 4 102 / 111 / 108; 4 x 2000 1 / 2 / 4 / 8 16 / 13.6 / 11 / 9.7; 1 x 2000 1 / 4 / 8 16 / 10.5 / 9.2; 1 x 30000 8 / 16 / 32 33
-// / 22.5 / 18; 8 x 1000 1 / 2 / 4 10.4 / 11.1 / 10.0; 4 heads of 64: 64 x 90 to 8000 1 / 2 / 4 / 8 39 / 33 / 31 / 35.
+// Few rows take kv4_attn, more than 64 a sequence the shared tiles.  kv4_attn's splits give a workgroup one round of 256
+// tokens where they leave CUs free, two where the device is busier, from three rounds on.  Several sequences, which may
+// differ in length, take so many that there are four workgroups to a CU if all are as long as the longest, of 1024 tokens
+// or more each, and never more than 8192 tokens to one (of many sequences one may be by far the longest); up to 64 of them
+// are dealt out longest first.  us by splits, one query, 8 K/V heads of 128: 64 x 90 to 8000 1 / 2 / 4 / 8 72 / 68 / 67 / 72
+// (in the sequences' order 72 / 71 / 72 / 76), of 8000 107 / 122 / 118 / 131; 32 x 100 to 8000 1 / 2 / 4 / 8 62 / 49 / 38 / 40;
+// 64 x 90 to 4000 1 / 2 / 3 / 4 42 / 39 / 42 / 41; 16 x 90 to 20000 4 / 6 / 8 / 12 59 / 47 / 45 / 46; 16 x 4000 1 / 2 / 4 / 8 31 /
+// 24 / 22.4 / 26; 100 x 90 to 8000 1 / 2 / 4 102 / 111 / 108; 4 x 2000 1 / 2 / 4 / 8 16 / 13.6 / 11 / 9.7; 1 x 2000 1 / 4 / 8 16 /
+// 10.5 / 9.2; 1 x 30000 8 / 16 / 32 33 / 22.5 / 18; 8 x 1000 1 / 2 / 4 10.4 / 11.1 / 10.0; 4 heads of 64: 64 x 90 to 8000 1 / 2 /
+// 4 / 8 39 / 33 / 31 / 35.
+// Shared tiles (a workgroup to a CU): one to a CU where there are fewer, half as many again for several sequences; where
+// they do not fill whole rounds, long contexts take the splits whose rounds come out best, of 4000 tokens or more, since a
+// part of 256 rows is 130 KB.  8 x 100 x 300 to 8000 1 / 2 / 3 / 4 298 / 170 / 126 / 181; 16 x 40 x 1000 to 6000 1 / 2 / 3 / 4 226 /
+// 130 / 108 / 148; 4 x 700 x 1100 to 4100 1 / 2 146 / 185; 1 x 1900 x 6400 1 / 2 249 / 287; 1 x 64 x 16000 1 / 8 / 16 / 32 599 /
+// 92 / 58 / 69; 16 heads of 64: 2 x 128 x 6000 1 / 4 / 6 / 8 138 / 47 / 37 / 52; 1 x 3000 x 16000 1 / 2 / 3 / 4 / 6 425 / 428 / 406 /
+// 357 / 378.
 static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                 int64_t max_ctx, size_t scratch) {
   KvAttnPlan pl;
   const int64_t group = heads / kv_heads, rows = group * std::min(max_q, tokens);
-  if (rows > 64) return kv_attn_plan(tokens, batch, heads, kv_heads, D, max_q, max_ctx, scratch);
-  if (rows > 16) pl.nq = 2, pl.rb = 32;
+  if (rows > 64) pl.tile = true, pl.rb = 256;
+  else if (rows > 16) pl.nq = 2, pl.rb = 32;
   pl.blocks = tokens * group / pl.rb + batch;
   const int64_t there = std::max<int64_t>(1, std::min(pl.blocks, batch * cdiv(std::max<int64_t>(rows, 1), pl.rb)));
   pl.walk = batch > kDense ? pl.blocks : there;
-  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count();
+  const int64_t units = pl.blocks * kv_heads, cus = device_cu_count(), step = pl.tile ? 64 : 256;
   const int64_t busy = there * kv_heads;  // workgroups with work, unsplit
-  const int64_t least = busy <= 64 ? 256 : 512;
   int64_t splits = 1;
-  if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
-  if (batch > 1) splits = std::max({splits, std::min((4 * cus + busy / 2) / busy, max_ctx / 1024), max_ctx / 8192});
+  if (pl.tile) {
+    splits = std::max<int64_t>(1, std::min((batch > 1 && 2 * busy >= cus ? 3 : 2) * cus / (2 * busy), max_ctx / (busy < 32 ? 1024 : 768)));
+    for (int64_t n = 2; n <= 8 && max_ctx / n >= 4000; ++n)  // rounds of workgroups to a part
+      if (2 * busy > cus && cdiv(busy * n, cus) * splits < cdiv(busy * splits, cus) * n) splits = n;
+  } else {
+    const int64_t least = busy <= 64 ? 256 : 512;
+    if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
+    if (batch > 1) splits = std::max({splits, std::min((4 * cus + busy / 2) / busy, max_ctx / 1024), max_ctx / 8192});
+  }
   // a launch has less than 2^31 threads (the limit of rows leaves room for four splits at least)
-  splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / 256 - 1) / units));
+  splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / (pl.tile ? 512 : 256) - 1) / units));
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   auto cut = [&](int64_t n) {
-    pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), n), 256) * 256);
+    pl.chunk = static_cast<int>(cdiv(cdiv(std::max<int64_t>(max_ctx, 1), n), step) * step);
     pl.splits = static_cast<int>(cdiv(std::max<int64_t>(max_ctx, 1), pl.chunk));
     pl.bytes = size(pl.splits);
   };
@@ -780,9 +779,9 @@ template <int D>
 static void launch_kv4_attn(const KvAttnPlan &pl, const Kv4AttnArgs &p, hipStream_t s) {
   if (pl.tile) {
     const int64_t units = pl.blocks * p.kv_heads, rows = static_cast<int64_t>(p.tokens) * p.heads;
-    hipLaunchKernelGGL(kv4_attn_tile<D>, dim3(static_cast<unsigned>(units * pl.splits)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(kv4_attn_tile<D>, dim3(static_cast<unsigned>(units * pl.splits)), dim3(512), 0, s, p);
     if (pl.splits > 1)
-      hipLaunchKernelGGL((kv_attn_combine<D, 128>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((kv_attn_combine<D, 256>), dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(256), 0, s, p);
   } else if (pl.nq == 2) launch_kv4_attn<D, 2>(pl, p, s);
   else launch_kv4_attn<D, 1>(pl, p, s);
 }
@@ -810,7 +809,7 @@ teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, con
                 "kv4_cache_attention: 4-byte aligned scales");
   p.ks = static_cast<const bf16 *>(k_scale);
   p.vs = static_cast<const bf16 *>(v_scale);
-  p.sorted = batch > 1 && batch <= 64 && pl.walk * pl.splits * kv_heads > 2 * device_cu_count();
+  p.sorted = !pl.tile && batch > 1 && batch <= 64 && pl.walk * pl.splits * kv_heads > 2 * device_cu_count();
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 64) launch_kv4_attn<64>(pl, p, s);
   else launch_kv4_attn<128>(pl, p, s);
