@@ -71,14 +71,21 @@ __device__ __forceinline__ uint32_t over8(uint32_t v, F f) {
   return f(v, dpp<0x141>(v));
 }
 
-// Rows of q and k: D / 8 lanes a row, eight numbers each.  The angles' cosines and sines are taken once per token,
-// in 64 bits, as are the rotated keys: a code that falls on the other side of a half would be a whole step off.
+// Rows of q and k: D / 8 lanes a row, eight numbers each and their partners.  The angles' cosines and sines are taken
+// once per token, in 64 bits, as are the rotated keys: a code that falls on the other side of a half would be a whole
+// step off.
 template <int D>
 __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
-  constexpr int LPR = D / 8, NG = D / 64, PASS = 256 / LPR;
+  constexpr int LPR = D / 8, NG = D / 64, PASS = 256 / LPR, U = 4;
   __shared__ double2 turn64[4][64];
   __shared__ float2 turn32[4][64];
+  __shared__ int at_pos[4], at_slot[4];
   const int tid = threadIdx.x, part = block % p.parts, t0 = block / p.parts * p.per, n = min(p.per, p.tokens - t0);
+  if (tid < n) {
+    const int pos = p.positions[t0 + tid], slot = p.kv_heads > 0 ? p.slots[t0 + tid] : -1;
+    at_pos[tid] = pos;
+    at_slot[tid] = pos >= 0 && slot < p.limit ? slot : -1;
+  }
   if ((tid >> 6) < n && (tid & 63) < p.half) {
     const int pos = p.positions[t0 + (tid >> 6)];
     const double angle = static_cast<double>(pos) * static_cast<double>(p.inv_freq[tid & 63]);
@@ -87,77 +94,109 @@ __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
     turn64[tid >> 6][tid & 63] = cs;
     turn32[tid >> 6][tid & 63] = float2{static_cast<float>(cs.x), static_cast<float>(cs.y)};
   }
-  __syncthreads();
-  const int heads = p.q_heads + p.kv_heads, m = tid % LPR, d0 = 8 * m;
+  const int m = tid % LPR, d0 = 8 * m;
   const bool turned = d0 < 2 * p.half, upper = !p.interleaved && d0 >= p.half;
   const int f0 = p.interleaved ? d0 / 2 : upper ? d0 - p.half : d0;  // the lane's first angle
   const int other = p.interleaved || !turned ? 0 : upper ? -p.half : p.half;
-  for (int row = part * PASS + tid / LPR; row < n * heads; row += p.parts * PASS) {
-    const int i = row / heads, head = row - i * heads, t = t0 + i;
-    if (p.positions[t] < 0) continue;
-    const bool is_q = head < p.q_heads;
-    const bf16 *src = is_q ? p.q + t * p.q_stride + head * D + d0 : p.k + t * p.k_stride + (head - p.q_heads) * D + d0;
-    const int slot = is_q ? 0 : p.slots[t];
-    if (slot < 0 || (!is_q && slot >= p.limit)) continue;
-    const bf16x8 a = *reinterpret_cast<const bf16x8 *>(src), b = *reinterpret_cast<const bf16x8 *>(src + other);
-    if (is_q) {
-      bf16x8 y = a;
+  // the first two rows of k are on their way while the angles are worked out
+  auto k_row = [&](int row) {
+    const int i = row / p.kv_heads, head = row - i * p.kv_heads;
+    return p.k + (t0 + i) * p.k_stride + head * D + d0;
+  };
+  const int k_rows = n * p.kv_heads, k_step = p.parts * PASS, k_first = (p.parts - 1 - part) * PASS + tid / LPR;
+  bf16x8 ka[2], kb[2];
+  if (k_rows > 0)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bf16 *src = k_row(min(k_first + u * k_step, k_rows - 1));
+      ka[u] = *reinterpret_cast<const bf16x8 *>(src);
+      kb[u] = *reinterpret_cast<const bf16x8 *>(src + other);
+    }
+  __syncthreads();
+  for (int row = k_first, u = 0; row < k_rows; row += k_step, ++u) {
+    const int i = row / p.kv_heads, head = row - i * p.kv_heads, slot = at_slot[i];
+    bf16x8 a = ka[0], b = kb[0];
+    ka[0] = ka[1], kb[0] = kb[1];
+    if (u >= 2) {
+      const bf16 *src = k_row(row);
+      a = *reinterpret_cast<const bf16x8 *>(src);
+      b = *reinterpret_cast<const bf16x8 *>(src + other);
+    }
+    if (slot < 0) continue;
+    float y[8];
+    const double2 *turn = turn64[i] + f0;
+    if (!turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(a[e]);
+    } else if (p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double2 cs = turn[e];
+        const double x1 = static_cast<float>(a[2 * e]), x2 = static_cast<float>(a[2 * e + 1]);
+        y[2 * e] = static_cast<float>(__builtin_fma(x1, cs.x, -x2 * cs.y));
+        y[2 * e + 1] = static_cast<float>(__builtin_fma(x2, cs.x, x1 * cs.y));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double2 cs = turn[e];
+        const double x = static_cast<float>(a[e]), o = static_cast<float>(b[e]);
+        y[e] = static_cast<float>(__builtin_fma(x, cs.x, upper ? o * cs.y : -o * cs.y));
+      }
+    }
+    uint32_t key = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = __float_as_uint(y[e]);
+      key = max(key, (u << 1) | (~u >> 31));
+    }
+    key = over8(key, [](uint32_t x, uint32_t z) { return max(x, z); });
+    const float s = kv4_scale(key), inv = kv4_inverse(s);
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word |= kv4_code<2>(y[e], s, inv) << (4 * w4_nibble(e));
+    if (!(s == s)) word = 0x88888888u;
+    const int64_t token = ((static_cast<int64_t>(slot >> p.shift) * p.kv_heads + head) << p.shift) + (slot & ((1 << p.shift) - 1));
+    *reinterpret_cast<uint32_t *>(p.kc + token * (D / 2) + 4 * (NG * (m & 6) + 2 * (m >> 3) + (m & 1))) = word;
+    if ((m & 7) == 0) p.ks[token * NG + (m >> 3)] = static_cast<bf16>(s);
+  }  // U rows' loads at once
+  const int q_rows = n * p.q_heads;
+  for (int row0 = part * PASS + tid / LPR; row0 < q_rows; row0 += U * p.parts * PASS) {
+    bf16x8 a[U], b[U];
+    int at[U], head[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = min(row0 + u * p.parts * PASS, q_rows - 1);
+      at[u] = row / p.q_heads;
+      head[u] = row - at[u] * p.q_heads;
+      const bf16 *src = p.q + (t0 + at[u]) * p.q_stride + head[u] * D + d0;
+      a[u] = *reinterpret_cast<const bf16x8 *>(src);
+      b[u] = *reinterpret_cast<const bf16x8 *>(src + other);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (row0 + u * p.parts * PASS >= q_rows || at_pos[at[u]] < 0) continue;
+      bf16x8 y = a[u];
       if (turned) {
+        const float2 *turn = turn32[at[u]] + f0;
         if (p.interleaved) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 cs = turn32[i][f0 + e];
-            const float x1 = static_cast<float>(a[2 * e]), x2 = static_cast<float>(a[2 * e + 1]);
+            const float2 cs = turn[e];
+            const float x1 = static_cast<float>(a[u][2 * e]), x2 = static_cast<float>(a[u][2 * e + 1]);
             y[2 * e] = static_cast<bf16>(__builtin_fmaf(x1, cs.x, -x2 * cs.y));
             y[2 * e + 1] = static_cast<bf16>(__builtin_fmaf(x2, cs.x, x1 * cs.y));
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float2 cs = turn32[i][f0 + e];
-            const float x = static_cast<float>(a[e]), o = static_cast<float>(b[e]);
+            const float2 cs = turn[e];
+            const float x = static_cast<float>(a[u][e]), o = static_cast<float>(b[u][e]);
             y[e] = static_cast<bf16>(__builtin_fmaf(x, cs.x, upper ? o * cs.y : -o * cs.y));
           }
         }
       }
-      *reinterpret_cast<bf16x8 *>(p.q_out + (static_cast<int64_t>(t) * p.q_heads + head) * D + d0) = y;
-    } else {
-      float y[8];
-      if (!turned) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(a[e]);
-      } else if (p.interleaved) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double2 cs = turn64[i][f0 + e];
-          const double x1 = static_cast<float>(a[2 * e]), x2 = static_cast<float>(a[2 * e + 1]);
-          y[2 * e] = static_cast<float>(__builtin_fma(x1, cs.x, -x2 * cs.y));
-          y[2 * e + 1] = static_cast<float>(__builtin_fma(x2, cs.x, x1 * cs.y));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double2 cs = turn64[i][f0 + e];
-          const double x = static_cast<float>(a[e]), o = static_cast<float>(b[e]);
-          y[e] = static_cast<float>(__builtin_fma(x, cs.x, upper ? o * cs.y : -o * cs.y));
-        }
-      }
-      uint32_t key = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t u = __float_as_uint(y[e]);
-        key = max(key, (u << 1) | (~u >> 31));
-      }
-      key = over8(key, [](uint32_t x, uint32_t z) { return max(x, z); });
-      const float s = kv4_scale(key), inv = kv4_inverse(s);
-      uint32_t word = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) word |= kv4_code<2>(y[e], s, inv) << (4 * w4_nibble(e));
-      if (!(s == s)) word = 0x88888888u;
-      const int page = slot >> p.shift, h = head - p.q_heads, G = m >> 3;
-      const int64_t at = ((static_cast<int64_t>(page) * p.kv_heads + h) << p.shift) + (slot & ((1 << p.shift) - 1));
-      *reinterpret_cast<uint32_t *>(p.kc + at * (D / 2) + 4 * (NG * (m & 6) + 2 * G + (m & 1))) = word;
-      if ((m & 7) == 0) p.ks[at * NG + G] = static_cast<bf16>(s);
+      *reinterpret_cast<bf16x8 *>(p.q_out + (static_cast<int64_t>(t0 + at[u]) * p.q_heads + head[u]) * D + d0) = y;
     }
   }
 }
