@@ -33,29 +33,23 @@ __device__ __forceinline__ bf16x8 load8(const bf16 *p, bool there) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// A lane's numbers of 64 columns n ..: of a row m, the columns n + 8 g + 0..7 and 32 further on, two tiles each; so a
-// wave's access is 64 bytes of each row.  Rows may begin anywhere (global memory takes 16 bytes at any address).
-typedef u32x4 AdapterRow[2];
-__device__ __forceinline__ void adapter_load(const AdapterArgs &p, int m, int n, AdapterRow &v) {
-  const bf16 *y = p.y + m * p.y_stride + n;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) __builtin_memcpy(&v[h], y + 32 * h, 16);
+// Eight numbers of a row.  Rows may begin anywhere (global memory takes 16 bytes at any address).
+__device__ __forceinline__ u32x4 adapter_load(const AdapterArgs &p, int m, int n) {
+  u32x4 v;
+  __builtin_memcpy(&v, p.y + m * p.y_stride + n, 16);
+  return v;
 }
-__device__ __forceinline__ void adapter_store(const AdapterArgs &p, int m, int n, const AdapterRow &v, const f32x4 (&add)[4]) {
-  bf16 *out = p.out + m * p.out_stride + n;
+__device__ __forceinline__ void adapter_store(const AdapterArgs &p, int m, int n, u32x4 v, f32x4 lo, f32x4 hi) {
+  u32x4 o;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 &a = add[2 * h + (i >> 1)];
-      o[i] = __builtin_bit_cast(uint32_t, cvt_pk_bf16(__uint_as_float(v[h][i] << 16) + a[2 * (i & 1)],
-                                                      __uint_as_float(v[h][i] & 0xffff0000u) + a[2 * (i & 1) + 1]));
-    }
-    typedef u32x4 any __attribute__((aligned(2)));
-    // past the caches, which hold B (2000 rows x 11008 columns of rank 64: 36.0 -> 30.0 us)
-    __builtin_nontemporal_store(o, reinterpret_cast<any *>(out + 32 * h));
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 &a = i < 2 ? lo : hi;
+    o[i] = __builtin_bit_cast(uint32_t, cvt_pk_bf16(__uint_as_float(v[i] << 16) + a[2 * (i & 1)],
+                                                    __uint_as_float(v[i] & 0xffff0000u) + a[2 * (i & 1) + 1]));
   }
+  typedef u32x4 any __attribute__((aligned(2)));
+  // past the caches, which hold B (2000 rows x 11008 columns of rank 64: 36.0 -> 30.0 us)
+  __builtin_nontemporal_store(o, reinterpret_cast<any *>(p.out + m * p.out_stride + n));
 }
 // Where the 64 columns pass the last one: number by number; rows as offsets from m0's, so that the 16 addresses are one.
 __device__ __forceinline__ void adapter_edge(const AdapterArgs &p, int m0, int row, int n, const f32x4 (&add)[4]) {
@@ -93,15 +87,31 @@ __device__ __forceinline__ void adapter_copy(const AdapterArgs &p, int m0, uint6
 }
 __device__ __forceinline__ void adapter_add_row(const AdapterArgs &p, int m0, int row, int n, bool whole, const f32x4 (&add)[4]) {
   if (whole) {
-    AdapterRow v;
-    adapter_load(p, m0 + row, n, v);
-    adapter_store(p, m0 + row, n, v, add);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) adapter_store(p, m0 + row, n + 32 * h, adapter_load(p, m0 + row, n + 32 * h), add[2 * h], add[2 * h + 1]);
   } else {
     adapter_edge(p, m0, row, n, add);
   }
 }
-// The row of B that lane c holds for tile j of the columns n ..
+// The row of B that lane c holds for tile j of the columns n ..: a lane's products are a row's columns n + 8 g + 0..7, and 32 further on.
 __device__ __forceinline__ int adapter_col(int n, int j, int c) { return n + 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3); }
+
+// Lanes of two rows swap halves: each then has the same eight columns of both (odd lanes those 32 further on), and a wave's
+// access is 128 bytes of each row, a whole line where rows begin on one.
+__device__ __forceinline__ float dpp_swap(float v) {  // lane l has lane l ^ 1's
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), 0xb1, 0xf, 0xf, false));
+}
+__device__ __forceinline__ void adapter_swap(f32x4 (&o)[4], bool odd) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float low = o[j][i], high = o[2 + j][i];
+      const float other_low = dpp_swap(low), other_high = dpp_swap(high);
+      o[j][i] = odd ? other_high : low;
+      o[2 + j][i] = odd ? high : other_low;
+    }
+}
 
 // The rows of 16 MT ones that each adapter has: lane l's row l.  Either (slots 0) there is a workgroup for each row, which
 // takes the adapter of which the row is the first, or `slots` workgroups for each tile take its adapters in turn.
@@ -224,9 +234,6 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
   int a;
   uint64_t mine;
   while (rows.next(p, a, mine)) {
-    bool in[MT];  // the lane's rows
-#pragma unroll
-    for (int t = 0; t < MT; ++t) in[t] = (mine >> (16 * t + c)) & 1;
     if (a < 0) {
       if (p.out != p.y) adapter_copy(p, rows.m0, mine, n0, n1);
       continue;
@@ -236,7 +243,14 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
     const auto br = buffer_rsrc(p.b + static_cast<int64_t>(a) * p.N * p.rank, p.N * p.rank * 2);
     const int r0 = RT == 1 ? 8 * (gg & 1) : 8 * gg;
     u32x4 b[4][KS];
-    AdapterRow y[MT];
+    u32x4 y[MT][2];
+    const bool odd = cc & 1;
+    const int pair = cc & ~1, nn = 8 * gg + 32 * (cc & 1);  // the rows and columns that a lane has in the end
+    bool in[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) in[t][q] = (mine >> (16 * t + pair + q)) & 1;
     uint32_t b_at[KS];  // zeros past the rank
 #pragma unroll
     for (int k = 0; k < KS; ++k) b_at[k] = r0 + 32 * k < p.rank ? 2 * (r0 + 32 * k) : static_cast<uint32_t>(kOffNone);
@@ -250,7 +264,9 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
     auto load_y = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
-        if (in[t]) adapter_load(p, rows.m0 + 16 * t + cc, n + 8 * gg, y[t]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (in[t][q]) y[t][q] = adapter_load(p, rows.m0 + 16 * t + pair + q, n + nn);
     };
     auto products = [&](int t, f32x4 (&o)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -297,10 +313,13 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
         f32x4 o[4];
         products(t, o);
         if (t == MT - 1 && n + 256 < n1) load_b(n + 256);
-        if (in[t]) {
-          adapter_store(p, rows.m0 + 16 * t + cc, n + 8 * gg, y[t], o);
-          if (n + 256 < n_whole) adapter_load(p, rows.m0 + 16 * t + cc, n + 256 + 8 * gg, y[t]);
-        }
+        adapter_swap(o, odd);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (in[t][q]) {
+            adapter_store(p, rows.m0 + 16 * t + pair + q, n + nn, y[t][q], o[2 * q], o[2 * q + 1]);
+            if (n + 256 < n_whole) y[t][q] = adapter_load(p, rows.m0 + 16 * t + pair + q, n + 256 + nn);
+          }
       }
     }
     if (n < n1) {
@@ -308,7 +327,7 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
       for (int t = 0; t < MT; ++t) {
         f32x4 o[4];
         products(t, o);
-        if (in[t]) adapter_edge(p, rows.m0, 16 * t + cc, n + 8 * gg, o);
+        if ((mine >> (16 * t + cc)) & 1) adapter_edge(p, rows.m0, 16 * t + cc, n + 8 * gg, o);
       }
     }
   }
