@@ -28,11 +28,6 @@ struct AdapterArgs {
 __device__ __forceinline__ f32x4 mfma_16x16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ bf16x8 load8(const bf16 *p, bool there) {
-  const u32x4 v = there ? *reinterpret_cast<const u32x4 *>(p) : u32x4{0u, 0u, 0u, 0u};
-  return __builtin_bit_cast(bf16x8, v);
-}
-
 // Eight numbers of a row.  Rows may begin anywhere (global memory takes 16 bytes at any address).
 __device__ __forceinline__ u32x4 adapter_load(const AdapterArgs &p, int m, int n) {
   u32x4 v;
@@ -75,7 +70,7 @@ __device__ __forceinline__ void adapter_copy(const AdapterArgs &p, int m0, uint6
     const bf16 *y = p.y + m * p.y_stride;
     bf16 *out = p.out + m * p.out_stride;
 #pragma unroll 1
-    for (int n = n0 + 8 * threadIdx.x; n < n1; n += 8 * 256) {
+    for (int n = n0 + 8 * threadIdx.x; n < n1; n += 8 * blockDim.x) {
       if (n + 8 <= n1) {
         __builtin_memcpy(out + n, y + n, 16);
       } else {
@@ -83,14 +78,6 @@ __device__ __forceinline__ void adapter_copy(const AdapterArgs &p, int m0, uint6
         for (int i = n; i < n1; ++i) out[i] = y[i];
       }
     }
-  }
-}
-__device__ __forceinline__ void adapter_add_row(const AdapterArgs &p, int m0, int row, int n, bool whole, const f32x4 (&add)[4]) {
-  if (whole) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) adapter_store(p, m0 + row, n + 32 * h, adapter_load(p, m0 + row, n + 32 * h), add[2 * h], add[2 * h + 1]);
-  } else {
-    adapter_edge(p, m0, row, n, add);
   }
 }
 // The row of B that lane c holds for tile j of the columns n ..: a lane's products are a row's columns n + 8 g + 0..7, and 32 further on.
@@ -333,65 +320,109 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
   }
 }
 
-// One workgroup for 16 rows and a range of columns, without scratch: the ranks'
-// products for these rows are summed in LDS, once for each range of columns.
-template <int RT>  // 16-row tiles of the rank
-__global__ __launch_bounds__(256) void adapter_one(AdapterArgs p) {
-  constexpr int LR = 16 * RT + 4;
-  __shared__ __attribute__((aligned(16))) float part[4][16][LR];
-  __shared__ __attribute__((aligned(16))) bf16 hs[2][16][16 * RT + 24];  // [hi, lo]; k past the rank's tiles read as zeros
+// Both products in one launch, without scratch: each workgroup has the ranks' products
+// of its rows to itself, so A is read once for each range of columns.  Sixteen waves
+// share out the k's, then the columns, 16 at a time.
+template <int RT>
+__global__ __launch_bounds__(1024) void adapter_one(AdapterArgs p) {
+  constexpr int U = RT == 1 ? 4 : RT == 2 ? 2 : 1, H = RT == 8 ? 1 : 2, RP = 16 * RT, KS = RT == 1 ? 1 : RT / 2, LH = (RT == 1 ? 32 : RP) + 8, PARTS = RT == 1 ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) float sum[16][16][RP + 4];
+  __shared__ __attribute__((aligned(16))) bf16 hs[PARTS][16][LH];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.x * 16, n0 = blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
-  const int row = min(m0 + c, p.M - 1);
-  int id = m0 + c < p.M ? p.ids[row] : -1;
-  if (id < 0 || id >= p.adapters) id = -1;
-  const bool here = m0 + c < p.M;
-  if (p.out != p.y) adapter_copy(p, m0, __ballot(here && id < 0) & 0xffffu, n0, n1);
-  uint64_t left = __ballot(id >= 0) & 0xffffu;
-  while (left != 0) {
-    const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    const bool mine = id == a;
-    left &= ~__ballot(mine);
+  AdapterRows<1> rows(p, blockIdx.x);
+  const int n0 = blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
+  const int last = min(16, p.M - rows.m0) - 1;
+  const auto xr = buffer_rsrc(p.x + rows.m0 * p.x_stride, static_cast<int>((last * p.x_stride + p.K) * 2));
+  const int x_at = static_cast<int>((min(c, last) * p.x_stride + 8 * g) * 2);
+  int a;
+  uint64_t mine;
+  while (rows.next(p, a, mine)) {
+    if (a < 0) {
+      if (p.out != p.y) adapter_copy(p, rows.m0, mine, n0, n1);
+      continue;
+    }
+    const bool in = (mine >> c) & 1;
+    const auto ar = buffer_rsrc(p.a + static_cast<int64_t>(a) * p.rank * p.K, p.rank * p.K * 2);
+    const auto br = buffer_rsrc(p.b + static_cast<int64_t>(a) * p.N * p.rank, p.N * p.rank * 2);
     f32x4 acc[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const bf16 *x = p.x + row * p.x_stride;
-    for (int k = 32 * w; k < p.K; k += 128) {
-      const bool in = k + 8 * g < p.K;
-      const bf16x8 xf = load8(x + k + 8 * g, in && mine);
+    for (int r = 0; r < RT; ++r) acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 64 * w; k < p.K; k += 1024 * U) {
+#pragma unroll 1
+      for (int h0 = 0; h0 < 2; h0 += H) {
+        u32x4 xf[U][H], af[U][H][RT];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int r = 16 * t + c;
-        acc[t] = mfma_16x16(load8(p.a + (static_cast<int64_t>(a) * p.rank + r) * p.K + k + 8 * g, in && r < p.rank), xf, acc[t]);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            const int at = k + 1024 * u + 32 * (h0 + h);
+            const bool there = at + 8 * g < p.K;
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+              af[u][h][r] = buffer_load16(ar, there ? (min(16 * r + c, p.rank - 1) * p.K + at + 8 * g) * 2 : kOffNone);
+            xf[u][h] = buffer_load16(xr, there ? x_at + 2 * at : kOffNone);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+              acc[r] = mfma_16x16(__builtin_bit_cast(bf16x8, af[u][h][r]), __builtin_bit_cast(bf16x8, xf[u][h]), acc[r]);
       }
     }
-    __syncthreads();  // the last round's products have been read
+    // the first columns' operands, ahead of the sums
+    const int r0 = RT == 1 ? 8 * (g & 1) : 8 * g;
+    u32x4 b[KS];
+    auto load_b = [&](int n) __attribute__((always_inline)) {  // zeros past the rank and the columns
 #pragma unroll
-    for (int t = 0; t < RT; ++t) *reinterpret_cast<f32x4 *>(&part[w][c][16 * t + 4 * g]) = acc[t];
-    __syncthreads();
+      for (int k = 0; k < KS; ++k) 
+        b[k] = buffer_load16(br, static_cast<int>(r0 + 32 * k < p.rank ? (static_cast<uint32_t>((n + c) * p.rank) + r0 + 32 * k) * 2u : kOffNone));
+    };
+    int n = n0 + 16 * w;
+    if (n < n1) load_b(n);
     const float scale = p.scale != nullptr ? p.scale[a] : 1.0f;
-    for (int i = tid; i < 16 * (16 * RT + 16); i += 256) {
-      const int m = i / (16 * RT + 16), r = i - m * (16 * RT + 16);
-      const float h = r < 16 * RT ? scale * (part[0][m][r] + part[1][m][r] + part[2][m][r] + part[3][m][r]) : 0.0f;
+    __syncthreads();  // the last adapter's products have been read
+#pragma unroll
+    for (int r = 0; r < RT; ++r) *reinterpret_cast<f32x4 *>(&sum[w][c][16 * r + 4 * g]) = acc[r];
+    __syncthreads();
+    for (int i = tid; i < 16 * RP; i += 1024) {
+      const int m = i / RP, r = i - m * RP;
+      float h = 0.0f;
+      if ((mine >> m) & 1 && r < p.rank) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) h += sum[j][m][r];
+        h *= scale;
+      }
       const bf16 hi = static_cast<bf16>(h);
       hs[0][m][r] = hi;
-      hs[1][m][r] = fabsf(static_cast<float>(hi)) < INFINITY ? static_cast<bf16>(h - static_cast<float>(hi)) : static_cast<bf16>(0.0f);
+      hs[PARTS - 1][m][RT == 1 ? 16 + r : r] = fabsf(static_cast<float>(hi)) < INFINITY ? static_cast<bf16>(h - static_cast<float>(hi)) : static_cast<bf16>(0.0f);
     }
     __syncthreads();
-    for (int n = n0 + 64 * w; n < n1; n += 256) {
-      f32x4 o[4];
+    for (; n < n1; n += 256) {
+      f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int col = adapter_col(n, j, c);
+      for (int s = 0; s < PARTS; ++s)
 #pragma unroll
-        for (int k = 0; k < 16 * RT; k += 32) {
-          const bf16x8 bf = load8(p.b + (static_cast<int64_t>(a) * p.N + col) * p.rank + k + 8 * g, col < p.N && k + 8 * g < p.rank);
+        for (int k = 0; k < KS; ++k)
+          o = mfma_16x16(__builtin_bit_cast(bf16x8, b[k]), *reinterpret_cast<const bf16x8 *>(&hs[s][c][32 * k + 8 * g]), o);
+      if (n + 256 < n1) load_b(n + 256);
+      if (in) {
+        const bf16 *y = p.y + (rows.m0 + c) * p.y_stride + n + 4 * g;
+        bf16 *out = p.out + (rows.m0 + c) * p.out_stride + n + 4 * g;
+        if (n + 16 <= p.N) {
+          bf16 v[4];
+          __builtin_memcpy(v, y, 8);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) o[j] = mfma_16x16(bf, *reinterpret_cast<const bf16x8 *>(&hs[s][c][k + 8 * g]), o[j]);
+          for (int e = 0; e < 4; ++e) v[e] = static_cast<bf16>(static_cast<float>(v[e]) + o[e]);
+          __builtin_memcpy(out, v, 8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + 4 * g + e < p.N) out[e] = static_cast<bf16>(static_cast<float>(y[e]) + o[e]);
         }
       }
-      if (mine && here) adapter_add_row(p, m0, row - m0, n + 8 * g, n + 64 <= p.N, o);
     }
   }
 }
@@ -399,6 +430,7 @@ __global__ __launch_bounds__(256) void adapter_one(AdapterArgs p) {
 // ── which form ──────────────────────────────────────────────────────────────
 struct AdapterPlan {
   int rt = 1, down = 1, up = 1, slots = 0, splits = 1, chunk = 0, cols = 0;  // down, up: 16-row tiles of a workgroup
+  bool one = false;  // one launch
   size_t bytes = 0;
 };
 
@@ -415,7 +447,11 @@ static AdapterPlan adapter_plan(int64_t M, int64_t N, int64_t K, int64_t rank) {
   pl.splits = static_cast<int>(cdiv(K, pl.chunk));
   const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), many ? std::max<int64_t>(4, 512 / up) : cdiv(2048, up)));
   pl.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
-  pl.bytes = static_cast<size_t>(pl.splits) * M * 16 * pl.rt * 4;
+  // One launch for few small products, each workgroup having a CU to itself: a row, rank 16, 1024 -> 4096: 5.6 us against
+  // 6.4; 16 rows: 6.4 against 7.0; but every range of columns reads all of A: a row, 4096 -> 4096: 7.5 against 6.2 us
+  // (2048 -> 2048: 6.9 both); more workgroups than CUs: 64 rows, 1024 -> 4096: 22.5 against 9.0 us.
+  pl.one = 16 * pl.rt * K <= 16384 && M * cdiv(N, 256) <= 256;
+  pl.bytes = pl.one ? 0 : static_cast<size_t>(pl.splits) * M * 16 * pl.rt * 4;
   return pl;
 }
 
@@ -470,7 +506,7 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
   hipStream_t s = static_cast<hipStream_t>(stream);
   const AdapterPlan pl = adapter_plan(M, N, K, rank);
   const Scratch scr = stream_scratch(s);
-  if (num_adapters > 0 && scr.ptr != nullptr && scr.bytes >= pl.bytes) {
+  if (num_adapters > 0 && !pl.one && scr.ptr != nullptr && scr.bytes >= pl.bytes) {
     p.part = static_cast<float *>(scr.ptr);
     p.cols = pl.cols;
     p.splits = pl.splits;
@@ -484,16 +520,14 @@ teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, cons
     }
     return after_launch(nm, s);
   }
-  const int64_t tiles = cdiv(M, 16), ranges = std::min<int64_t>(cdiv(N, 256), cdiv(512, tiles));
-  p.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(cdiv(N, p.cols)));
-  switch ((rank + 15) / 16) {
-    case 0:
-    case 1: hipLaunchKernelGGL(adapter_one<1>, grid, dim3(256), 0, s, p); break;
-    case 2: hipLaunchKernelGGL(adapter_one<2>, grid, dim3(256), 0, s, p); break;
-    case 3:
-    case 4: hipLaunchKernelGGL(adapter_one<4>, grid, dim3(256), 0, s, p); break;
-    default: hipLaunchKernelGGL(adapter_one<8>, grid, dim3(256), 0, s, p); break;
+  p.slots = M <= 256 ? 0 : 1;
+  p.cols = static_cast<int>(cdiv(cdiv(N, std::max<int64_t>(1, 512 / cdiv(M, 16))), 256) * 256);
+  const dim3 grid(static_cast<unsigned>(p.slots == 0 ? M : cdiv(M, 16)), static_cast<unsigned>(cdiv(N, p.cols)));
+  switch (pl.rt) {
+    case 1: hipLaunchKernelGGL(adapter_one<1>, grid, dim3(1024), 0, s, p); break;
+    case 2: hipLaunchKernelGGL(adapter_one<2>, grid, dim3(1024), 0, s, p); break;
+    case 4: hipLaunchKernelGGL(adapter_one<4>, grid, dim3(1024), 0, s, p); break;
+    default: hipLaunchKernelGGL(adapter_one<8>, grid, dim3(1024), 0, s, p); break;
   }
   return after_launch(nm, s);
 }

@@ -64,9 +64,9 @@ IDS = {
 @pytest.mark.parametrize("rank", [8, 16, 24, 32, 64, 104, 128])
 @pytest.mark.parametrize("ids", list(IDS))
 def test_adapters(dev, ids, rank, space):
-    """Odd numbers of columns and sizes of K, rows in any order."""
+    """Odd numbers of columns and sizes of K, rows in any order; small products are one launch, with or without a workspace."""
     rng = np.random.default_rng(rank + len(ids))
-    for n, k in ((4, 8), (100, 264), (333, 1032)):
+    for n, k in ((4, 8), (100, 264), (333, 1032), (4, 2056)):
         c = case(rng, IDS[ids], n, k, rank, 40 if ids == "each its own" else 4)
         with space_for(dev, c, space):
             check_run(c, run(dev, c))
@@ -89,7 +89,8 @@ def test_larger(dev, m, n, k, rank, adapters, space):
 def test_rows_are_apart(dev, space):
     """What a row of x holds reaches that row alone, an adapter's numbers its own rows, and infinities follow the products."""
     rng = np.random.default_rng(3)
-    c = case(rng, [0, 1, 0, 2, -1, 1, 0], 70, 40, 16, 3)
+    c = case(rng, [0, 1, 0, 2, -1, 1, 0], 70, 1064 if space else 40, 16, 3)
+    assert (size_of(c) > 0) == space
     clean = kv4.adapter(c["x"], c["a"], c["b"], c["ids"], c["scale"], c["y"])
     c["x"][2, 5], c["x"][4, 1], c["a"][2, 3, 7], c["b"][1, 11, 4] = np.nan, np.inf, np.inf, np.nan
     c["x"][3] = 1.0
@@ -107,15 +108,16 @@ def test_strides(dev, space):
     """Rows of x, y and out inside wider ones, the aligned and the odd kind; nothing between them is written."""
     rng = np.random.default_rng(4)
     for n, first, row in ((64, 16, 96), (61, 3, 67), (64, 2, 70)):
-        c = case(rng, [0, 2, -1, 1, 1], n, 48, 8, 3)
+        k = 1072 if space else 48
+        c = case(rng, [0, 2, -1, 1, 1], n, k, 8, 3)
         m = 5
-        x, y, out = (np.full((m, w), 5.0, np.float32) for w in (64, row, row + 4))
-        x[:, 8:56], y[:, first:first + n] = c["x"], c["y"]
+        x, y, out = (np.full((m, w), 5.0, np.float32) for w in (k + 16, row, row + 4))
+        x[:, 8:k + 8], y[:, first:first + n] = c["x"], c["y"]
         xb, yb, ob, a, b = (up(dev, z) for z in (x, y, out, c["a"], c["b"]))
         ids, s = dev.upload(c["ids"]), dev.upload(c["scale"])
         with space_for(dev, c, space):
-            check(lib.teeny_adapter_add(xb.ptr + 16, a.ptr, b.ptr, ids.ptr, s.ptr, yb.ptr + 2 * first, ob.ptr + 2 * first, m, n, 48, 8, 3,
-                                        64, row, row + 4, None))
+            check(lib.teeny_adapter_add(xb.ptr + 16, a.ptr, b.ptr, ids.ptr, s.ptr, yb.ptr + 2 * first, ob.ptr + 2 * first, m, n, k, 8, 3,
+                                        k + 16, row, row + 4, None))
             got = from_bf16(ob.to_host())
         check_run(c, got[:, first:first + n])
         assert (np.delete(got, np.s_[first:first + n], axis=1) == 5.0).all()
@@ -138,7 +140,7 @@ def test_two_streams_and_a_graph(dev):
     rng = np.random.default_rng(6)
     streams = [Stream.create(), Stream.create()]
     ids = [[0] * 40 + [2, 1, -1] * 9, [1, 0, 2, 2, -1]]
-    cases = [case(rng, i, 300, 512, 16, 3) for i in ids]
+    cases = [case(rng, i, 300, 2048, 16, 3) for i in ids]
     bufs = [(up(dev, c["x"]), up(dev, c["a"]), up(dev, c["b"]), dev.upload(c["ids"]), up(dev, c["y"])) for c in cases]
     scales, outs = [dev.upload(c["scale"]) for c in cases], [dev.buffer(bf16, c["y"].shape) for c in cases]
     with stream_workspace(dev, size_of(cases[0]), streams[0]), stream_workspace(dev, size_of(cases[1]), streams[1]):

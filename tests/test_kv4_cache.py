@@ -139,7 +139,8 @@ def test_adapter_workspace_refusals():
     expect(f(4, 32, BIG, 16, ctypes.byref(n)), _lib.ERR_SHAPE_MISMATCH)
     assert n.value == 0
     assert f(4, 32, 0, 16, ctypes.byref(n)) == _lib.OK and n.value == 0
-    assert f(4, 32, 256, 16, ctypes.byref(n)) == _lib.OK and n.value > 0
+    assert f(4, 32, 256, 16, ctypes.byref(n)) == _lib.OK and n.value == 0  # one launch
+    assert f(4, 32, 2048, 16, ctypes.byref(n)) == _lib.OK and n.value > 0
 
 
 def test_nothing_to_adapt():
