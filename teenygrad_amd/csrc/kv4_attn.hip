@@ -511,39 +511,35 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 
   // The wave's share of a tile: of the K rows of block w / 2 % 2, of their chunks 2 (w % 2) and 2 (w % 2) + 1, the words of
   // group w / 4 (D = 64: word w / 4), and of V block w % 2 of d block w / 2 (D = 64: four waves do).  The four pages of a
-  // tile are one load for the wave; what follows from them is the same for all lanes and is worked out in scalar registers.
+  // tile are one load for the wave, from which each lane takes those of its K row and its V tokens.
   const int32_t *row = p.table + static_cast<int64_t>(r.b) * p.width;
   const int page_mask = (1 << p.shift) - 1, wb = (w >> 1) & 1, wk = w >> 2, vd = D == 128 ? w >> 1 : (w >> 1) & 1, vb = w & 1;
-  const bool k_odd = (c >> 2) & 1, g_odd = g;
-  const int k_row = 4 * (c >> 3) + (c & 3), k_lane = k_row * (D / 2) + (D / 8) * (2 * (w & 1) + g) + 4 * KW * wk;
-  const int v_lane = 8 * (32 * vd + c);
+  const int k_block = 2 * wb + ((c >> 2) & 1), v_block = 2 * vb + g;  // of 16 tokens, of the tile's four
+  const int k_token = 16 * k_block + 4 * (c >> 3) + (c & 3), v_token = 16 * v_block + (lane & 15);
+  const int8_t *k_from = p.kc + (D / 8) * (2 * (w & 1) + g) + 4 * KW * wk, *v_from = p.vc + 8 * (32 * vd + c);
+  const bf16 *ks_from = p.ks + (D == 128 ? wk : 0), *vs_from = p.vs + (vd >> 1);
   // lane l: the page of tokens 16 (l % 4) .. of a tile
   auto load_pages = [&](int t0) { return row[min(t0 + 16 * (lane & 3), k_end - 1) >> p.shift]; };
   kvec kr;
   u32x2 vr;
   bf16 ks, vs;
-  bool there_v, hidden_next[2];
+  bool there_v;
+  uint32_t here_next;  // bit j: the tile's tokens 16 j .. have a page (the first of them is below ke)
   auto load_codes = [&](int t0, int pg) {
-    int64_t at[4];  // tokens of the cache
-    bool there[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int page = __builtin_amdgcn_readlane(pg, j), t = t0 + 16 * j;
-      there[j] = page >= 0 && page < p.pages && t < ke;
-      at[j] = ((static_cast<int64_t>(there[j] ? page : 0) * p.kv_heads + head) << p.shift) + (t & page_mask);
-    }
-    auto pick = [&](bool odd, int64_t x, int64_t y) { return odd ? y : x; };
-    const int64_t k_at = pick(k_odd, wb ? at[2] : at[0], wb ? at[3] : at[1]);
-    kr = *reinterpret_cast<const kvec *>(p.kc + k_at * (D / 2) + k_lane);
-    ks = p.ks[(k_at + k_row) * NG + (D == 128 ? wk : 0)];
-    const int64_t v_at = pick(g_odd, vb ? at[2] : at[0], vb ? at[3] : at[1]);
+    const int of = t0 + 16 * (lane & 3) < ke && static_cast<uint32_t>(pg) < static_cast<uint32_t>(p.pages) ? pg : -1;
+    here_next = static_cast<uint32_t>(__ballot(of >= 0)) & 15;
+    const int k_page = __builtin_amdgcn_ds_bpermute(4 * k_block, of), v_page = __builtin_amdgcn_ds_bpermute(4 * v_block, of);
+    auto token = [&](int page, int t) __attribute__((always_inline)) {  // of the cache; page 0 where there is none
+      return ((static_cast<uint64_t>(static_cast<uint32_t>(max(page, 0))) * static_cast<uint32_t>(p.kv_heads) + head) << p.shift) + (t & page_mask);
+    };
+    const uint64_t k_at = token(k_page, t0 + k_token), v_at = token(v_page, t0 + v_token);
+    kr = *reinterpret_cast<const kvec *>(k_from + k_at * (D / 2));
+    ks = ks_from[k_at * NG];
     if (D == 128 || w < 4) {
-      vr = *reinterpret_cast<const u32x2 *>(p.vc + v_at * (D / 2) + v_lane);
-      vs = p.vs[(v_at + (lane & 15)) * NG + (vd >> 1)];
-      there_v = (g_odd ? (vb ? there[3] : there[1]) : (vb ? there[2] : there[0])) && t0 + 32 * vb + 16 * g + (lane & 15) < ke;
+      vr = *reinterpret_cast<const u32x2 *>(v_from + (v_at & ~15ull) * (D / 2));
+      vs = vs_from[v_at * NG];
+      there_v = v_page >= 0 && t0 + v_token < ke;
     }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) hidden_next[b] = g_odd ? !there[2 * b + 1] : !there[2 * b];
   };
   auto turn = [&](int buf) {
     u32x4 *to = frag[buf];
@@ -575,17 +571,13 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   };
 
   int pg = 0, buf = 0;
-  bool none[2];
-  auto take = [&]() {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) none[b] = hidden_next[b];
-  };
+  uint32_t here = 0;
   if (kb < ke) {
     pg = load_pages(kb);
     load_codes(kb, pg);
     pg = load_pages(kb + 64);
     turn(0);
-    take();
+    here = here_next;
     if (kb + 64 < ke) {
       load_codes(kb + 64, pg);
       pg = load_pages(kb + 128);
@@ -595,10 +587,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 #pragma unroll 1
   for (int t0 = kb; t0 < ke; t0 += 64) {
     const u32x4 *now = frag[buf];
-    const bool hidden[2] = {none[0], none[1]};
+    const uint32_t here_now = here;
     if (t0 + 64 < ke) {
       turn(buf ^ 1);
-      take();
+      here = here_next;
       if (t0 + 128 < ke) {
         load_codes(t0 + 128, pg);
         pg = load_pages(t0 + 192);
@@ -622,12 +614,12 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
         s[i & 1] = mfma32x32x16(__builtin_bit_cast(bf16x8, win[i % WIN]), qf[i >> 1], s[i & 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (t0 + 64 > all_see || __any(hidden[0] || hidden[1])) {
+      if (t0 + 64 > all_see || here_now != 15) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int v = 0; v < 16; ++v)
-            if (hidden[b] || t0 + 32 * b + 16 * g + v >= vis) s[b][v] = -INFINITY;
+            if (((here_now >> (2 * b + g)) & 1) == 0 || t0 + 32 * b + 16 * g + v >= vis) s[b][v] = -INFINITY;
       }
       float mx = s[0][0];
 #pragma unroll
