@@ -588,6 +588,9 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   for (int t0 = kb; t0 < ke; t0 += 64) {
     const u32x4 *now = frag[buf];
     const uint32_t here_now = here;
+    uint32_t unfit[NG][2];
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) unfit[i >> 1][i & 1] = bad[buf][i >> 1][i & 1];
     if (t0 + 64 < ke) {
       turn(buf ^ 1);
       here = here_next;
@@ -625,7 +628,8 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 #pragma unroll
       for (int v = 1; v < 32; ++v) mx = __builtin_elementwise_maximum(mx, s[v >> 4][v & 15]);
       mx *= sc;
-      mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
       if (__any(mx > m_run + 8.0f)) {  // rescaled rarely: p <= 2^8
         const float m_new = fmaxf(m_run, mx);
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
@@ -652,18 +656,22 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
       }
       // a row that sees a token whose V is NaN: its outputs of that group are
 #pragma unroll
-      for (int G = 0; G < NG; ++G) {
-        const uint64_t unfit = bad[buf][G][0] | static_cast<uint64_t>(bad[buf][G][1]) << 32;
-        if (unfit != 0) {
+      for (int G = 0; G < NG; ++G)
+        if ((unfit[G][0] | unfit[G][1]) != 0) {
           bool sees = false;
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < 2; ++b) {
+            uint32_t bits = unfit[G][b] >> (16 * g);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sees |= ((unfit >> (32 * b + 16 * g + v)) & 1) && !(s[b][v] == 0.0f);
+            for (int v = 0; v < 16; ++v) {
+              float pv = s[b][v];
+              asm volatile("" : "+v"(pv), "+v"(bits));  // or its comparison is made for every tile
+              sees |= ((bits >> v) & 1) && !(pv == 0.0f);
+            }
+          }
           sees = __shfl_xor(static_cast<int>(sees), 32, 64) != 0 || sees;  // the row's other tokens
           if (sees) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
         }
-      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 4 * ND; ++j) {
