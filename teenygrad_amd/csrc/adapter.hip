@@ -428,6 +428,20 @@ __global__ __launch_bounds__(1024) void adapter_one(AdapterArgs p) {
 }
 
 // ── which form ──────────────────────────────────────────────────────────────
+// Two launches.  Up to 256 rows, which may all have adapters of their own, there are workgroups for each row, of which those
+// that are not their adapter's first in 16 rows end at once; more rows come as runs, as a rule, and have tiles of 32 rows (down:
+// 64 past 1024), with as many workgroups as a tile may have adapters without one waiting: three, past 512 rows two.  us for
+// 4096 -> 4096 of rank 16, a workgroup a row / two / three / four a tile: 300 rows and 100 adapters 22 / 83 / 60 / 50, three runs of
+// 100 17 / 10.3 / 9.9 / 10.5; 500 rows, 20 adapters 30 / 55 / 44 / 41; three runs of 300 - / 12.6 / 15.5 / 16.0; 200 rows of their
+// own 19 / 82 / - / 46.  2000 rows in five runs, rank 64, 4096 -> 11008: tiles of 16 / 32 / 64 for the columns 51.5 / 40.6 / 53.5, of
+// 32 / 64 for the ranks 43.5 / 40.6 (800 rows: 24.5 / 26.9).
+// down: 1024 k's or more to a split, since every range of columns sums all parts, and up to 512 workgroups or four splits (us
+// for 512 k's / 1024: 64 rows and adapters of rank 64, 4096 -> 4096 21.7 / 19.2; 20 adapters, -> 11008 28.3 / 23.7; rank 16, 40
+// adapters 11.6 / 10.8; two / four splits of two runs of 100 rows 10.6 / 9.3).
+// up: ranges of columns for 768 workgroups, of which the idle ones cost little (us by 512 / 768 / 1024 / 2048 / 4096: rank 16, 64
+// rows, 40 adapters, -> 11008 11.2 / 10.8 / 10.7 / 12.0 / 13.9; 200 rows, 100 adapters 25.6 / 25.4 / 27.9 / 28.4 / 27.8), or eight
+// (two runs of 100 rows of rank 64: 4 / 6 / 10 34 / 31 / 26.5; 200 rows, 100 adapters 25.4 / 27.9 / 26.9); of many rows for 512
+// (2000 rows of rank 64, -> 11008: 256 / 512 / 1024 / 2048 47.2 / 40.6 / 41.5 / 43.7; rank 16, 11008 -> 4096 29.4 / 28.3 / 30.2 / 30.1).
 struct AdapterPlan {
   int rt = 1, down = 1, up = 1, slots = 0, splits = 1, chunk = 0, cols = 0;  // down, up: 16-row tiles of a workgroup
   bool one = false;  // one launch
@@ -440,12 +454,12 @@ static AdapterPlan adapter_plan(int64_t M, int64_t N, int64_t K, int64_t rank) {
   pl.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   pl.down = !many ? 1 : M > 1024 ? 4 : 2;
   pl.up = many ? 2 : 1;
-  pl.slots = many ? 2 : 0;
+  pl.slots = !many ? 0 : M > 512 ? 2 : 3;
   const int64_t down = many ? cdiv(M, 16 * pl.down) : M, up = many ? cdiv(M, 16 * pl.up) : M;
-  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), cdiv(512, down)));
+  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), std::max<int64_t>(many ? 1 : 4, cdiv(512, down))));
   pl.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(cdiv(K, splits), 256)) * 256);
   pl.splits = static_cast<int>(cdiv(K, pl.chunk));
-  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), many ? std::max<int64_t>(4, 512 / up) : cdiv(2048, up)));
+  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), std::max<int64_t>(many ? 4 : 8, (many ? 512 : 768) / up)));
   pl.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
   // One launch for few small products, each workgroup having a CU to itself: a row, rank 16, 1024 -> 4096: 5.6 us against
   // 6.4; 16 rows: 6.4 against 7.0; but every range of columns reads all of A: a row, 4096 -> 4096: 7.5 against 6.2 us
