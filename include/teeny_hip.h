@@ -643,7 +643,8 @@ teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t b
  * of the page keep their codes.  The new tokens of 16 slots that begin at a
  * multiple of 16 are consecutive rows at consecutive slots, as the plan lays them
  * out; otherwise V's codes of those 16 are unspecified.  rotary_dim a multiple of
- * 16 up to head_dim (0: no rotation, inv_freq may be NULL); at most 2^24 tokens;
+ * 16 up to head_dim (0: no rotation, inv_freq may be NULL); at most 2^24 tokens,
+ * and n_tokens / 4 + n_tokens / 32 * kv_heads below 2^23;
  * q_heads 0: no queries; 16-byte aligned tensors. */
 teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v, const int32_t *positions,
                                     const int32_t *slots, const float *inv_freq, void *q_out, int8_t *k_cache,
@@ -654,8 +655,10 @@ teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v,
 
 /* Attention over the 4-bit cache: arguments, results, hints and workspace as
  * teeny_kv_cache_attention's (its size: teeny_kv4_cache_attention_workspace_size).
- * Scales may have either sign, and any bf16 value.  An infinity in a row of q
- * gives NaN in that row and head.  Scales 4-byte aligned. */
+ * Scales may have either sign, and any bf16 value; an infinite one counts as NaN,
+ * and NaN reaches the rows that see its token: of K's all of the row and head, of
+ * V's the 64 numbers of its group.  An infinity in a row of q gives NaN in that row
+ * and head.  Scales 4-byte aligned. */
 teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const void *k_scale,
                                        const void *v_scale, const int32_t *block_table, const int32_t *context_lens,
                                        const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,

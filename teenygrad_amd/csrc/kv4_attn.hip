@@ -14,13 +14,21 @@
 // token's K row, or of two of V's d's over 16 tokens, so codes come straight from
 // memory, each byte to one lane: no LDS and no barrier in the loop.
 //
-// Codes become the bf16 values (24 + code) / 16 with two instructions a pair
-// (w4_values), exact.  The 24/16 too much is -1.5 times the sum of q, which the
-// scores start from, and -1.5 times the sum of the weighted probabilities, one more
-// product with a constant operand.  Scales are applied in fp32: K's to the group's
-// scores, V's to the probability before its rounding to bf16 (the one rounding on
-// the way, as in kv_attn).  Lane c of a group holds the scale of the group's token
-// c, and the multiplication fetches it across the 16 lanes (row_newbcast).
+// The codes' way to operands, of which there are more than bytes from memory, is
+// what it takes beside the reading.  Of up to 16 rows the keys are fp8 operands,
+// where a nibble is a number as it stands (w4_fp8), and a query is the sum of two
+// fp8 ones, which leaves an error of 2^-17 of its row's largest number; the 8 too
+// much is -8 times the sum of q, which the scores start from.  Values, and keys of 17
+// to 64 rows, become the bf16 numbers (24 + code) / 16 with two instructions a pair
+// (W4Bits), exact; the 24/16 too much is -1.5 times the sum of what they are
+// multiplied with, one more product with a constant operand.  Scales are applied in
+// fp32: K's to the group's scores, V's to the probability before its rounding to bf16
+// (the one rounding on the way, as in kv_attn).  Lane c of a group holds the scale of
+// the group's token c, and the multiplication fetches it across the 16 lanes
+// (row_newbcast).  For 64 tokens of 128 numbers a wave reads 8.7 KB and issues 360
+// vector instructions and 52 products.  One query to each of 64 contexts of 8000
+// tokens, 32 heads over 8 of 128: 107 us, 5.2 TB/s, the rate of a copy; 90 to 8000
+// tokens: 68 us, 4.1 TB/s, for want of waves at the end.
 #include "kv4.hpp"
 #include "kv_attn.hpp"
 
@@ -469,8 +477,12 @@ __device__ __forceinline__ bf16x8 kv4_values8(uint32_t word, S scale) {
 // order in which lanes take them up; here code times scale, a bf16 number already
 // where the scale has five bits (other scales: rounded), so that the products need
 // no scale of their own.  The next tile is turned while one is multiplied, the codes
-// of the tile after that are in flight; one barrier a tile.  (Four waves and 128 rows, two workgroups on a CU: every row
-// pays for turning twice as often, 4 x 700 queries 174 us to 150.)
+// of the tile after that are in flight; one barrier a tile.  Bound by the vector instructions, 290 a wave and tile, 32 of
+// them exponentials, beside 32 products of 32 cycles: 4 requests of 700 queries and
+// 1100 to 4100 tokens, 32 heads of 128 over 8: 130 us, 717 TFLOP/s; 1900 queries of
+// 6400: 209 us, 813.  (Four waves and 128 rows, two workgroups on a CU: every row pays
+// for turning twice as often, 174 us to 150.  Two groups of waves half a tile apart: 175
+// to 150.  Turning and exponentials between the products: 134 to 140.)
 template <int D>
 __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   constexpr int RB = 256, NS = D / 16, ND = D / 32, NG = D / 64, EPW = D / 32, KW = D / 64, FR = 2 * NS + 4 * ND;
@@ -543,7 +555,7 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   };
   auto turn = [&](int buf) {
     u32x4 *to = frag[buf];
-    const float k_scale = static_cast<float>(ks);
+    const float k = static_cast<float>(ks), k_scale = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
 #pragma unroll
     for (int e = 0; e < KW; ++e)
       to[(wb * NS + EPW * (w & 1) + KW * wk + e) * 64 + lane] =
@@ -654,23 +666,18 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
           pb[b][v >> 3][(v & 7) + 1] = pr[1];
         }
       }
-      // a row that sees a token whose V is NaN: its outputs of that group are
+      // a row that sees a token whose V is NaN: its outputs of that group are, whatever the token's weight
 #pragma unroll
       for (int G = 0; G < NG; ++G)
         if ((unfit[G][0] | unfit[G][1]) != 0) {
-          bool sees = false;
+          uint32_t sees = 0;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            uint32_t bits = unfit[G][b] >> (16 * g);
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              float pv = s[b][v];
-              asm volatile("" : "+v"(pv), "+v"(bits));  // or its comparison is made for every tile
-              sees |= ((bits >> v) & 1) && !(pv == 0.0f);
-            }
+            const int n = min(max(vis - (t0 + 32 * b + 16 * g), 0), 16);  // of the lane's 16 tokens
+            sees |= unfit[G][b] >> (16 * g) & ((1u << n) - 1);
           }
-          sees = __shfl_xor(static_cast<int>(sees), 32, 64) != 0 || sees;  // the row's other tokens
-          if (sees) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
+          sees |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(sees), 32, 64));  // the row's other tokens
+          if (sees != 0) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
         }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

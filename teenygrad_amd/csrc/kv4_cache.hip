@@ -29,7 +29,7 @@ struct Kv4AppendArgs {
   bf16 *ks, *vs;
   int tokens, q_heads, kv_heads, limit, shift;  // limit: slots of the cache
   int half, interleaved;                        // rotated pairs of a head
-  int per, parts, rows_grid;                    // tokens per workgroup of rows, workgroups per tokens, workgroups of rows
+  int per, rows_grid;                           // tokens per workgroup of rows, workgroups of rows
   int share;                                    // workgroups to 64 tokens' V of a head
 };
 
@@ -73,14 +73,15 @@ __device__ __forceinline__ uint32_t over8(uint32_t v, F f) {
 
 // Rows of q and k: D / 8 lanes a row, eight numbers each and their partners.  The angles' cosines and sines are taken
 // once per token, in 64 bits, as are the rotated keys: a code that falls on the other side of a half would be a whole
-// step off.
+// step off.  Keys are first, with the loads of the next rows of queries ahead of the work of this one's.  Bound by memory
+// where there are many tokens: 8000 of 32 and 8 heads of 128 move 173 MB in 44 us, 3.9 TB/s.
 template <int D>
 __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
   constexpr int LPR = D / 8, NG = D / 64, PASS = 256 / LPR, U = 4;
   __shared__ double2 turn64[4][64];
   __shared__ float2 turn32[4][64];
   __shared__ int at_pos[4], at_slot[4];
-  const int tid = threadIdx.x, part = block % p.parts, t0 = block / p.parts * p.per, n = min(p.per, p.tokens - t0);
+  const int tid = threadIdx.x, t0 = block * p.per, n = min(p.per, p.tokens - t0);
   if (tid < n) {
     const int pos = p.positions[t0 + tid], slot = p.kv_heads > 0 ? p.slots[t0 + tid] : -1;
     at_pos[tid] = pos;
@@ -103,17 +104,17 @@ __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
     const int i = row / p.kv_heads, head = row - i * p.kv_heads;
     return p.k + (t0 + i) * p.k_stride + head * D + d0;
   };
-  const int k_rows = n * p.kv_heads, k_step = p.parts * PASS, k_first = (p.parts - 1 - part) * PASS + tid / LPR;
+  const int k_rows = n * p.kv_heads, k_first = tid / LPR;
   bf16x8 ka[2], kb[2];
   if (k_rows > 0)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const bf16 *src = k_row(min(k_first + u * k_step, k_rows - 1));
+      const bf16 *src = k_row(min(k_first + u * PASS, k_rows - 1));
       ka[u] = *reinterpret_cast<const bf16x8 *>(src);
       kb[u] = *reinterpret_cast<const bf16x8 *>(src + other);
     }
   __syncthreads();
-  for (int row = k_first, u = 0; row < k_rows; row += k_step, ++u) {
+  for (int row = k_first, u = 0; row < k_rows; row += PASS, ++u) {
     const int i = row / p.kv_heads, head = row - i * p.kv_heads, slot = at_slot[i];
     bf16x8 a = ka[0], b = kb[0];
     ka[0] = ka[1], kb[0] = kb[1];
@@ -159,14 +160,14 @@ __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
     const int64_t token = ((static_cast<int64_t>(slot >> p.shift) * p.kv_heads + head) << p.shift) + (slot & ((1 << p.shift) - 1));
     *reinterpret_cast<uint32_t *>(p.kc + token * (D / 2) + 4 * (NG * (m & 6) + 2 * (m >> 3) + (m & 1))) = word;
     if ((m & 7) == 0) p.ks[token * NG + (m >> 3)] = static_cast<bf16>(s);
-  }  // U rows' loads at once
+  }
   const int q_rows = n * p.q_heads;
-  for (int row0 = part * PASS + tid / LPR; row0 < q_rows; row0 += U * p.parts * PASS) {
+  for (int row0 = tid / LPR; row0 < q_rows; row0 += U * PASS) {  // U rows' loads at once
     bf16x8 a[U], b[U];
     int at[U], head[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int row = min(row0 + u * p.parts * PASS, q_rows - 1);
+      const int row = min(row0 + u * PASS, q_rows - 1);
       at[u] = row / p.q_heads;
       head[u] = row - at[u] * p.q_heads;
       const bf16 *src = p.q + (t0 + at[u]) * p.q_stride + head[u] * D + d0;
@@ -175,7 +176,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AppendArgs &p, int block) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (row0 + u * p.parts * PASS >= q_rows || at_pos[at[u]] < 0) continue;
+      if (row0 + u * PASS >= q_rows || at_pos[at[u]] < 0) continue;
       bf16x8 y = a[u];
       if (turned) {
         const float2 *turn = turn32[at[u]] + f0;
@@ -346,12 +347,15 @@ teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v,
                   k_stride, v_stride, positions, slots, inv_freq, static_cast<bf16 *>(q_out), k_cache, v_cache,
                   static_cast<bf16 *>(k_scale), static_cast<bf16 *>(v_scale), static_cast<int>(n_tokens),
                   static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(num_pages << shift), shift,
-                  static_cast<int>(rotary_dim / 2), interleaved != 0, 1, 1, 0, 1};
-  const int64_t pass = 256 / (head_dim / 8);
+                  static_cast<int>(rotary_dim / 2), interleaved != 0, 1, 0, 1};
+  // Workgroups of rows take a token, of more than 512 tokens four, which share the angles' work (1 / 4 tokens, 32 and 8 heads of
+  // 128: 300 tokens 6.4 / 7.4 us, 900 11.0 / 9.1, 8000 56 / 44).  V's 64 tokens of a head may be 64 runs, in a decode step, or
+  // four: workgroups to them by the number of tokens (4 / 8 / 16 of them: 64 tokens of their own 10.4 / 6.5 / 4.5 us, 256
+  // 12.3 / 8.4 / 6.7, 80 in runs of five, 16 heads of 64 4.8 / 5.0 / 5.5; 1 / 2 / 4 / 8: 8000 tokens 44.3 / 44.3 / 46 / 51, 500
+  // 8 / 16 9.8 / 11.0).
   p.per = n_tokens > 512 ? 4 : 1;
-  p.parts = static_cast<int>(n_tokens > 512 ? 1 : cdiv(q_heads + kv_heads, pass));
   p.share = n_tokens <= 256 ? 16 : n_tokens <= 1024 ? 8 : 2;
-  const int64_t rows = cdiv(n_tokens, p.per) * p.parts, all = rows + cdiv(n_tokens, 64) * p.share * kv_heads;
+  const int64_t rows = cdiv(n_tokens, p.per), all = rows + cdiv(n_tokens, 64) * p.share * kv_heads;
   TEENY_REQUIRE(all < int64_t{1} << 23, TEENY_ERR_SHAPE_MISMATCH, "kv4_cache_append: too many rows for a launch");
   p.rows_grid = static_cast<int>(rows);
   hipStream_t s = static_cast<hipStream_t>(stream);

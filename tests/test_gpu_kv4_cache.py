@@ -410,6 +410,28 @@ def test_attention_unseen_tokens(dev, new, d):
     assert (np.abs(o - ref)[:-1] <= tol[:-1]).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_scales_that_are_no_numbers(dev, new, d):
+    """An infinite scale counts as NaN; a token that a row sees counts however little it weighs, early or late in the context."""
+    rng = np.random.default_rng(new)
+    for where in (3, 90, 195):
+        for value in (np.nan, np.inf, -np.inf):
+            c = attn_case(rng, [300], [new], 4, 2, d, 16)
+            c["q"][...] = 30.0  # the token's score lies some hundreds below the others'
+            ks, vs = c["cache"][2:]
+            page, at = c["table"][0, where // 16], where % 16
+            k_codes = c["cache"][0]
+            k_codes[page, 0, at] = 0x11  # codes of -7
+            ks[page, 0, at] = 0.5
+            vs[page, 0, at, 0] = value
+            o, _ = run_attn(dev, c)
+            assert np.isnan(o[:, :2, :64]).all() and np.isfinite(o[:, :2, 64:]).all() and np.isfinite(o[:, 2:]).all()
+            ks[page, 1, at, 0] = value
+            o, _ = run_attn(dev, c)
+            assert np.isnan(o[:, 2:]).all() and np.isfinite(o[:, :2, 64:]).all()
+
+
 def test_attention_of_infinite_queries(dev):
     """An infinity or NaN in one row and head of q reaches that one alone."""
     rng = np.random.default_rng(5)
