@@ -575,8 +575,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile(Kv8AttnArgs p) {
 // on a busy device get half as many again, since contexts seldom are of one length:
 // 16 x 40 x 1000 to 6000 2 / 3 / 4 133 / 101 / 125, of 4000 104 / 116 / 110; 20 x
 // 40 x 300 to 4000 1 / 2 125 / 97, of 2000 88 / 98.
-KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
-                        int64_t max_ctx, size_t scratch) {
+static KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
+                               int64_t max_ctx, size_t scratch) {
   KvAttnPlan pl;
   const int64_t group = heads / kv_heads, rows = group * std::min(max_q, tokens);
   if (rows > 64) pl.tile = true, pl.rb = 128;

@@ -224,9 +224,6 @@ inline teeny_status kv_attn_sizes(const char *nm, int64_t n_tokens, int64_t batc
   return TEENY_OK;
 }
 
-KvAttnPlan kv_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
-                        int64_t max_ctx, size_t scratch);
-
 using KvAttnPlanFn = KvAttnPlan (*)(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                     int64_t max_ctx, size_t scratch);
 
