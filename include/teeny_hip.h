@@ -154,7 +154,8 @@ teeny_status teeny_hip_stream_sync(teeny_stream stream);
  * too small to fill the device, the space-to-depth copy of stride-2 NHWC
  * convs whose C_IN is not a multiple of 8, the bf16 copy of the int8
  * weights of W8A16 3x3 convs that run on the band-tiled kernel, that of 4-bit
- * weights for many rows, and the parts of attention over the paged cache -- run
+ * weights for many rows, the parts of attention over the paged caches, and the
+ * ranks' products of adapters -- run
  * only when the stream's workspace is large enough (sizes from
  * teeny_linear_workspace_size, teeny_conv2d_workspace_size and the other
  * teeny_*_workspace_size), and otherwise the operator takes a path that
@@ -794,10 +795,10 @@ teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t
  * [num_adapters] or NULL (1), y (the shared layer's output) and out (which may be
  * y) bf16 [M,N]; rows of x, y and out x_stride, y_stride and out_stride elements
  * apart.  With a stream workspace of teeny_adapter_add_workspace_size bytes the
- * ranks' products are worked out once, shared out over the device; without it
- * again by each workgroup.  Rows of an adapter need not lie together, but are faster so.  fp32 sums,
- * the rank's products held in two bf16 parts (2^-17) for the second product; out
- * is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
+ * ranks' products are worked out once, shared out over the device; without it, and
+ * where the size is 0, again by each workgroup.  Rows of an adapter need not lie
+ * together, but are faster so.  fp32 sums, the rank's products held in two bf16
+ * parts (2^-17) for the second product; out is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
  * zeros), N * rank below 2^30; K a multiple of 8 up to 2^22, x_stride up to 2^24; x,
  * a, b and x's rows 16-byte aligned. */
 teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, const int32_t *adapters, const float *scale,

@@ -48,7 +48,7 @@ __device__ __forceinline__ void adapter_store(const AdapterArgs &p, int m, int n
 }
 // Where the 64 columns pass the last one: number by number; rows as offsets from m0's, so that the 16 addresses are one.
 __device__ __forceinline__ void adapter_edge(const AdapterArgs &p, int m0, int row, int n, const f32x4 (&add)[4]) {
-  const int extent = static_cast<int>(min(p.M - m0, 64) - 1);
+  const int extent = min(p.M - m0, 32) - 1;  // of a workgroup's rows, two tiles at most
   const auto yr = buffer_rsrc(p.y + m0 * p.y_stride, static_cast<int>((extent * p.y_stride + p.N) * 2));
   const auto outr = buffer_rsrc(p.out + m0 * p.out_stride, static_cast<int>((extent * p.out_stride + p.N) * 2));
   const int y_at = static_cast<int>((row * p.y_stride + n) * 2), out_at = static_cast<int>((row * p.out_stride + n) * 2);

@@ -86,6 +86,19 @@ def test_larger(dev, m, n, k, rank, adapters, space):
 
 
 @pytest.mark.parametrize("space", [False, True])
+@pytest.mark.parametrize("ordered", [False, True])
+@pytest.mark.parametrize("m,n,k,rank", [(257, 70, 264, 16), (513, 333, 40, 32), (601, 36, 1032, 64), (1025, 300, 520, 8), (1090, 66, 136, 128)])
+def test_many_rows(dev, m, n, k, rank, ordered, space):
+    """Tiles of several adapters, more of them than workgroups take at once, and a last tile that is not whole."""
+    rng = np.random.default_rng(m)
+    ids = rng.integers(-1, 9, m)
+    c = case(rng, np.sort(ids) if ordered else ids, n, k, rank, 9)
+    with space_for(dev, c, space):
+        check_run(c, run(dev, c))
+        check_run(c, run(dev, c, in_place=True))
+
+
+@pytest.mark.parametrize("space", [False, True])
 def test_rows_are_apart(dev, space):
     """What a row of x holds reaches that row alone, an adapter's numbers its own rows, and infinities follow the products."""
     rng = np.random.default_rng(3)
