@@ -141,7 +141,9 @@ struct AdapterRows {
 // part[split] = A[a] x over the split's k's.  Four waves share them out in turn, 64 at
 // a time, and meet in LDS; all of a wave's share is in flight at once (a k past the
 // split's end loads zeros).  Rows of other adapters are multiplied too and not
-// written; rows of A past the rank repeat the last one and are not read again.
+// written; rows of A past the rank repeat the last one and are not read again.  Bound
+// by latency: ids, operands, the meeting, in turn.  64 requests, 40 adapters of rank
+// 16, K 4096: 5 us; 2000 rows of rank 64: 12 us, 35 MB read.
 template <int RT, int MT>
 __global__ __launch_bounds__(256) void adapter_down(AdapterArgs p) {
   constexpr int U = RT * MT >= 8 ? 2 : 4, RP = 16 * RT;
@@ -210,7 +212,10 @@ __global__ __launch_bounds__(256) void adapter_down(AdapterArgs p) {
 // out = y + B[a] (scale part).  A wave takes 64 columns a time.  The ranks' products
 // are two bf16 parts of an fp32 number; at a rank of 16 or less both are the k's of
 // one product.  The next columns' operands are loaded as soon as this one's have
-// been multiplied, the first ones ahead of the ranks' sums.
+// been multiplied, the first ones ahead of the ranks' sums.  Those 64 requests with
+// 11008 columns: 6 us, ids, parts and B in turn; 2000 rows of rank 64: 28 us, 88 MB of
+// y and out at 3.1 TB/s.  (With an XCD's workgroups on one range of columns, so that
+// each reads its part of B alone: 46 us for both launches to 40.6.)
 template <int RT, int MT>
 __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT >= 4 || MT == 2 ? 3 : 4) void adapter_up(AdapterArgs p) {
   constexpr int RP = 16 * RT, KS = RT == 1 ? 1 : RT / 2, LH = (RT == 1 ? 32 : RP) + 8, PARTS = RT == 1 ? 1 : 2;
