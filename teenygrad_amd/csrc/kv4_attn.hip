@@ -479,8 +479,8 @@ __device__ __forceinline__ bf16x8 kv4_values8(uint32_t word, S scale) {
 // no scale of their own.  The next tile is turned while one is multiplied, the codes
 // of the tile after that are in flight; one barrier a tile.  Bound by the vector instructions, 290 a wave and tile, 32 of
 // them exponentials, beside 32 products of 32 cycles: 4 requests of 700 queries and
-// 1100 to 4100 tokens, 32 heads of 128 over 8: 130 us, 717 TFLOP/s; 1900 queries of
-// 6400: 209 us, 813.  (Four waves and 128 rows, two workgroups on a CU: every row pays
+// 1100 to 4100 tokens, 32 heads of 128 over 8: 122 to 130 us, 717 TFLOP/s and more;
+// 1900 queries of 6400: 203 us, 835.  (Four waves and 128 rows, two workgroups on a CU: every row pays
 // for turning twice as often, 174 us to 150.  Two groups of waves half a tile apart: 175
 // to 150.  Turning and exponentials between the products: 134 to 140.)
 template <int D>
@@ -733,10 +733,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
 // 4 / 8 39 / 33 / 31 / 35.
 // Shared tiles (a workgroup to a CU): one to a CU where there are fewer, half as many again for several sequences; where
 // they do not fill whole rounds, long contexts take the splits whose rounds come out best, of 4000 tokens or more, since a
-// part of 256 rows is 130 KB.  8 x 100 x 300 to 8000 1 / 2 / 3 / 4 298 / 170 / 126 / 181; 16 x 40 x 1000 to 6000 1 / 2 / 3 / 4 226 /
-// 130 / 108 / 148; 4 x 700 x 1100 to 4100 1 / 2 146 / 185; 1 x 1900 x 6400 1 / 2 249 / 287; 1 x 64 x 16000 1 / 8 / 16 / 32 599 /
-// 92 / 58 / 69; 16 heads of 64: 2 x 128 x 6000 1 / 4 / 6 / 8 138 / 47 / 37 / 52; 1 x 3000 x 16000 1 / 2 / 3 / 4 / 6 425 / 428 / 406 /
-// 357 / 378.
+// part of 256 rows is 130 KB.  8 x 100 x 300 to 8000 1 / 2 / 3 / 4 237 / 138 / 106 / 150; 16 x 40 x 1000 to 6000 1 / 2 / 3 / 4 179 /
+// 107 / 91 / 116; 4 x 700 x 1100 to 4100 1 / 2 122 / 161; 1 x 1900 x 6400 1 / 2 203 / 240; 1 x 64 x 16000 1 / 8 / 16 / 32 470 /
+// 75 / 49 / 60; 16 heads of 64: 2 x 128 x 6000 1 / 4 / 6 / 8 113 / 41 / 33 / 46; 1 x 3000 x 16000 1 / 2 / 3 / 4 / 6 350 / 357 / 338 /
+// 301 / 318.
 static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                 int64_t max_ctx, size_t scratch) {
   KvAttnPlan pl;
