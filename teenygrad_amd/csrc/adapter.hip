@@ -434,12 +434,16 @@ __global__ __launch_bounds__(1024) void adapter_one(AdapterArgs p) {
 
 // ── which form ──────────────────────────────────────────────────────────────
 // Two launches.  Up to 256 rows, which may all have adapters of their own, there are workgroups for each row, of which those
-// that are not their adapter's first in 16 rows end at once; more rows come as runs, as a rule, and have tiles of 32 rows (down:
-// 64 past 1024), with as many workgroups as a tile may have adapters without one waiting: three, past 512 rows two.  us for
-// 4096 -> 4096 of rank 16, a workgroup a row / two / three / four a tile: 300 rows and 100 adapters 22 / 83 / 60 / 50, three runs of
-// 100 17 / 10.3 / 9.9 / 10.5; 500 rows, 20 adapters 30 / 55 / 44 / 41; three runs of 300 - / 12.6 / 15.5 / 16.0; 200 rows of their
-// own 19 / 82 / - / 46.  2000 rows in five runs, rank 64, 4096 -> 11008: tiles of 16 / 32 / 64 for the columns 51.5 / 40.6 / 53.5, of
-// 32 / 64 for the ranks 43.5 / 40.6 (800 rows: 24.5 / 26.9).
+// that are not their adapter's first in 16 rows end at once.  More rows come as runs, as a rule, or as many requests' single
+// tokens: tiles of rows, each with some workgroups that take its adapters in turn, and end if there are not as many.  Up to 512
+// rows, where the rank is 16 or less: tiles of 16 rows with four; else of 32 (down: 64 past 1024) with three, past 512 rows two.
+// us for 4096 -> 4096 of rank 16, 16 rows and four / 32 and three: 300 rows and 100 adapters 36 / 60 (a workgroup a row: 22),
+// 500 rows of their own 46 / 74, runs of 100 rows, three 10.7 / 9.9 (17), five 13.2 / 10.8; past 512, 32 and two: 900 rows and 100
+// adapters 63 / 114, but three runs of 300 14.9 / 12.9, five of 200, -> 11008, 23.2 / 17.6; of rank 64, 4096 -> 11008: five runs
+// of 100 31 / 24.9, 500 rows and ten adapters 94 / 76.
+// 2000 rows in five runs, rank 64, 4096 -> 11008: tiles of 16 / 32 / 64 for the columns 51.5 / 40.6 / 53.5, of 32 / 64 for the
+// ranks 43.5 / 40.6 (800 rows: 24.5 / 26.9); 300 rows and 100 adapters, two / three / four workgroups to 32: 83 / 60 / 50, three
+// runs of 300 12.6 / 15.5 / 16.0.
 // down: 1024 k's or more to a split, since every range of columns sums all parts, and up to 512 workgroups or four splits (us
 // for 512 k's / 1024: 64 rows and adapters of rank 64, 4096 -> 4096 21.7 / 19.2; 20 adapters, -> 11008 28.3 / 23.7; rank 16, 40
 // adapters 11.6 / 10.8; two / four splits of two runs of 100 rows 10.6 / 9.3).
@@ -457,14 +461,15 @@ static AdapterPlan adapter_plan(int64_t M, int64_t N, int64_t K, int64_t rank) {
   AdapterPlan pl;
   const bool many = M > 256;
   pl.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
-  pl.down = !many ? 1 : M > 1024 ? 4 : 2;
-  pl.up = many ? 2 : 1;
-  pl.slots = !many ? 0 : M > 512 ? 2 : 3;
+  const bool small = !many || (pl.rt == 1 && M <= 512);  // tiles
+  pl.down = small ? 1 : M > 1024 ? 4 : 2;
+  pl.up = small ? 1 : 2;
+  pl.slots = !many ? 0 : small ? 4 : M > 512 ? 2 : 3;
   const int64_t down = many ? cdiv(M, 16 * pl.down) : M, up = many ? cdiv(M, 16 * pl.up) : M;
-  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), std::max<int64_t>(many ? 1 : 4, cdiv(512, down))));
+  const int64_t splits = std::max<int64_t>(1, std::min(cdiv(K, 1024), std::max<int64_t>(small ? 4 : 1, cdiv(512, down))));
   pl.chunk = static_cast<int>(std::max<int64_t>(1, cdiv(cdiv(K, splits), 256)) * 256);
   pl.splits = static_cast<int>(cdiv(K, pl.chunk));
-  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), std::max<int64_t>(many ? 4 : 8, (many ? 512 : 768) / up)));
+  const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), std::max<int64_t>(small ? 8 : 4, (many ? 512 : 768) / up)));
   pl.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
   // One launch for few small products, each workgroup having a CU to itself: a row, rank 16, 1024 -> 4096: 5.6 us against
   // 6.4; 16 rows: 6.4 against 7.0; but every range of columns reads all of A: a row, 4096 -> 4096: 7.5 against 6.2 us

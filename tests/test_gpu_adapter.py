@@ -87,7 +87,7 @@ def test_larger(dev, m, n, k, rank, adapters, space):
 
 @pytest.mark.parametrize("space", [False, True])
 @pytest.mark.parametrize("ordered", [False, True])
-@pytest.mark.parametrize("m,n,k,rank", [(257, 70, 264, 16), (513, 333, 40, 32), (601, 36, 1032, 64), (1025, 300, 520, 8), (1090, 66, 136, 128)])
+@pytest.mark.parametrize("m,n,k,rank", [(257, 70, 264, 16), (400, 130, 520, 16), (777, 130, 520, 16), (513, 333, 40, 32), (601, 36, 1032, 64), (1025, 300, 520, 8), (1090, 66, 136, 128)])
 def test_many_rows(dev, m, n, k, rank, ordered, space):
     """Tiles of several adapters, more of them than workgroups take at once, and a last tile that is not whole."""
     rng = np.random.default_rng(m)
