@@ -514,6 +514,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     const int e = i % EPW, d = 64 * (e >> 1) + 16 * (2 * (i / EPW) + g) + 8 * (e & 1);
     u32x4 raw = *reinterpret_cast<const u32x4 *>(p.q + (r.first + qt) * p.q_stride + qh * D + d);
     raw ^= qsign;
+    // an infinity is NaN, or a row whose scores are all -inf would count as one that sees nothing
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      raw[j] |= ((raw[j] & 0x7f80u) == 0x7f80u ? 0x40u : 0u) | ((raw[j] & 0x7f800000u) == 0x7f800000u ? 0x400000u : 0u);
     qf[i] = __builtin_bit_cast(bf16x8, raw);
   }
   f32x16 acc[ND];

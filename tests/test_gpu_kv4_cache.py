@@ -446,6 +446,26 @@ def test_attention_of_infinite_queries(dev):
         assert np.isnan(o[bad]).all() and (np.abs(o - ref)[~bad] <= tol[~bad]).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_infinite_queries_whose_scores_are_all_low(dev, new, d):
+    """An infinity is NaN also where every token that the row sees gives -inf: nothing tells it from a row that sees none."""
+    rng = np.random.default_rng(new + d)
+    for ctx, causal in ((3, False), (new, True)):
+        c = attn_case(rng, [ctx], [new], 4, 2, d, 16)
+        c["cache"][0][...] = 0x33  # codes of -5
+        c["cache"][2] = np.abs(c["cache"][2])
+        ref, lse, tol, ltol = oracle(c, causal=causal)
+        for scale, value in ((None, np.inf), (-1 / math.sqrt(d), -np.inf)):
+            q = c["q"] * (1 if scale is None else -1)
+            q[0, 1, 5] = value
+            o, low = run_attn(dev, dict(c, q=q), scale=scale, causal=causal)
+            bad = np.zeros(o.shape[:2], bool)
+            bad[0, 1] = True
+            assert np.isnan(o[bad]).all() and np.isnan(low[bad]).all()
+            assert (np.abs(o - ref)[~bad] <= tol[~bad]).all() and (np.abs(low - lse)[~bad] <= ltol[~bad]).all()
+
+
 def test_attention_empty_tables(dev):
     """No page at all, and tables of unfilled rows."""
     rng = np.random.default_rng(6)
