@@ -658,8 +658,9 @@ teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v,
  * teeny_kv_cache_attention's (its size: teeny_kv4_cache_attention_workspace_size).
  * Scales may have either sign, and any bf16 value; an infinite one counts as NaN,
  * and NaN reaches the rows that see its token: of K's all of the row and head, of
- * V's the 64 numbers of its group.  An infinity in a row of q gives NaN in that row
- * and head.  Scales 4-byte aligned. */
+ * V's the 64 numbers of its group.  Beside a V scale of 2^80 or more, of a token
+ * that the row or one near it sees, numbers of V below 2^-70 may count as 0.  An
+ * infinity in a row of q gives NaN in that row and head.  Scales 4-byte aligned. */
 teeny_status teeny_kv4_cache_attention(const void *q, const int8_t *k_cache, const int8_t *v_cache, const void *k_scale,
                                        const void *v_scale, const int32_t *block_table, const int32_t *context_lens,
                                        const int32_t *q_starts, void *o, float *l, int64_t n_tokens, int64_t batch,

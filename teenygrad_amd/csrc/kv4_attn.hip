@@ -109,6 +109,12 @@ __device__ __forceinline__ f32x4 mfma16_fp8(int64_t a, int64_t b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a, b, c, 0, 0, 0);
 }
 
+// V scales from kVast on could overflow the sums of p v, where p is up to 2^8 and there may be 2^30 tokens.  Once a wave
+// meets one that a row of its block sees, the exponents' reference lies kRaise above the scores' maximum: p, l and the sums
+// are all by 2^-kRaise smaller, and every join of parts goes by that reference.  (Beside such a scale, values below 2^-70
+// fall below bf16's and fp32's smallest numbers.)
+constexpr float kVast = 0x1p80f, kRaise = 48.0f;
+
 // NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
@@ -245,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   const int all_see = seen(r.row0);  // all rows see the tokens below it
 
   f32x4 acc[NQ][ND], p_off[FP8 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
-  float m_run[NQ], l_run[NQ];
+  float m_run[NQ], l_run[NQ], raise = 0.0f;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     m_run[n] = -INFINITY;
@@ -265,6 +271,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       ksc[G] = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
       vsc[G] = static_cast<float>(vs[G]);
     }
+    const bool vast = fmaxf(fabsf(vsc[0]), fabsf(vsc[NG - 1])) >= kVast;
+    if (__any(vast) && __any(vast && !none && t0 + 16 * g + c < k_end)) raise = kRaise;
     f32x4 s[NQ][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       float mx = s[n][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
-      mx = over_groups(mx * col[n], [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      mx = over_groups(__builtin_fmaf(mx, col[n], raise), [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
       if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
         const float m_new = fmaxf(m_run[n], mx);
         const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
@@ -489,6 +497,7 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   typedef uint32_t kvec __attribute__((ext_vector_type(KW)));
   __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
   __shared__ uint32_t bad[2][NG][2];  // tokens of a tile whose V scale is not finite (they are turned to zeros)
+  __shared__ int vast_from;           // the first token turned whose V scale is kVast or more
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
@@ -557,7 +566,7 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
       there_v = v_page >= 0 && t0 + v_token < ke;
     }
   };
-  auto turn = [&](int buf) {
+  auto turn = [&](int buf, int t0) {
     u32x4 *to = frag[buf];
     const float k = static_cast<float>(ks), k_scale = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
 #pragma unroll
@@ -571,6 +580,7 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     float s = static_cast<float>(vs);
     const bool finite = fabsf(s) < INFINITY;
     const uint64_t m = __ballot(there_v && !finite);  // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
+    const uint64_t vast = __ballot(there_v && fabsf(s) >= kVast);
     s = there_v && finite ? s : 0.0f;
     const int at = 2 * NS + (vd * 2 + vb) * 2;
     to[at * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[0], [&](float (&v)[8]) {
@@ -583,16 +593,22 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
                                                       if constexpr (t >= 8) v[t - 8] *= row_lane<t>(s);
                                                     });
                                                   }));
-    if ((vd & 1) == 0 && lane == 0) bad[buf][vd >> 1][vb] = static_cast<uint32_t>((m & 0xffffu) | (m >> 32 & 0xffffu) << 16);
+    auto tokens = [](uint64_t v) { return static_cast<uint32_t>((v & 0xffffu) | (v >> 32 & 0xffffu) << 16); };
+    if ((vd & 1) == 0 && lane == 0) {
+      bad[buf][vd >> 1][vb] = tokens(m);
+      if (vast != 0) atomicMin(&vast_from, t0 + 32 * vb + __builtin_ctz(tokens(vast)));
+    }
   };
 
   int pg = 0, buf = 0;
   uint32_t here = 0;
+  if (threadIdx.x == 0) vast_from = 0x7fffffff;
+  if (kb < ke) pg = load_pages(kb);
+  __syncthreads();
   if (kb < ke) {
-    pg = load_pages(kb);
     load_codes(kb, pg);
     pg = load_pages(kb + 64);
-    turn(0);
+    turn(0, kb);
     here = here_next;
     if (kb + 64 < ke) {
       load_codes(kb + 64, pg);
@@ -607,8 +623,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     uint32_t unfit[NG][2];
 #pragma unroll
     for (int i = 0; i < 2 * NG; ++i) unfit[i >> 1][i & 1] = bad[buf][i >> 1][i & 1];
+    // (the next tile's turning, which may be under way, does not change which side of this tile's end it lies on)
+    const int vast_at = vast_from;
     if (t0 + 64 < ke) {
-      turn(buf ^ 1);
+      turn(buf ^ 1, t0 + 64);
       here = here_next;
       if (t0 + 128 < ke) {
         load_codes(t0 + 128, pg);
@@ -643,7 +661,8 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
       float mx = s[0][0];
 #pragma unroll
       for (int v = 1; v < 32; ++v) mx = __builtin_elementwise_maximum(mx, s[v >> 4][v & 15]);
-      mx *= sc;
+      const float raise = vast_at < min(t0 + 64, w_end) ? kRaise : 0.0f;  // once above 0 it stays
+      mx = __builtin_fmaf(mx, sc, raise);
       const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
       mx = __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
       if (__any(mx > m_run + 8.0f)) {  // rescaled rarely: p <= 2^8

@@ -1,5 +1,6 @@
 """The 4-bit paged K/V cache on the GPU: appends, attention, and a step of them with plan, 4-bit layers and adapters,
 against the plain forms of kv4_cases.py."""
+import contextlib
 import math
 
 import numpy as np
@@ -464,6 +465,45 @@ def test_attention_of_infinite_queries_whose_scores_are_all_low(dev, new, d):
             bad[0, 1] = True
             assert np.isnan(o[bad]).all() and np.isnan(low[bad]).all()
             assert (np.abs(o - ref)[~bad] <= tol[~bad]).all() and (np.abs(low - lse)[~bad] <= ltol[~bad]).all()
+
+
+@pytest.mark.parametrize("space", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_vast_values(dev, new, d, space):
+    """V scales near bf16's largest number, of all tokens, of late ones, of one: outputs are finite, so is every sum on the way.
+    The bounds are relative (a power of two on V's scales changes no rounding)."""
+    rng = np.random.default_rng(new + d)
+    hint = (new, 2100)
+    for tokens in (slice(None), slice(700, None), slice(1203, 1204), slice(40, 60)):
+        c = attn_case(rng, [2100, 130], [new, new], 4, 2, d, 16)
+        vs = c["cache"][3]
+        at = np.arange(2100)[tokens]
+        where = c["table"][0, at // 16], slice(None), at % 16, 0
+        vs[where] = np.abs(vs[where]) * np.float32(2.0 ** 126)  # below 0.12 * 2^126, so the values below 2^126
+        ref = oracle(c)
+        with stream_workspace(dev, K.kv4_cache_attention_workspace_size(2 * new, 2, 4, 2, d, *hint)) if space else contextlib.nullcontext():
+            check_attn(c, run_attn(dev, c, hint=hint), ref=ref)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_small_values_beside_unseen_vast_ones(dev, new, d):
+    """Scales behind the context and on pages that are none change no bit, however large."""
+    rng = np.random.default_rng(new + d)
+    c = attn_case(rng, [200, 130], [new, new], 4, 2, d, 16, extra=6)
+    ks, vs = c["cache"][2:]
+    vs *= np.float32(2.0 ** -86)
+    c["table"][0, 2] = -1
+    spare = np.setdiff1d(np.arange(len(ks)), c["table"])
+    want = run_attn(dev, c)
+    assert (want[0] != 0).any()
+    for value in (2.0 ** 120, np.inf):
+        for s in (ks, vs):
+            s[spare] = value
+            s[c["table"][0, 12], :, 8:], s[c["table"][1, 8], :, 2:] = value, -value
+        for g, w in zip(run_attn(dev, c), want):
+            np.testing.assert_array_equal(g, w)
 
 
 def test_attention_empty_tables(dev):
