@@ -271,8 +271,21 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       ksc[G] = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
       vsc[G] = static_cast<float>(vs[G]);
     }
-    const bool vast = fmaxf(fabsf(vsc[0]), fabsf(vsc[NG - 1])) >= kVast;
-    if (__any(vast) && __any(vast && !none && t0 + 16 * g + c < k_end)) raise = kRaise;
+    const float v_most = fmaxf(fabsf(vsc[0]), fabsf(vsc[NG - 1])), k_most = FP8 ? fmaxf(fabsf(ksc[0]), fabsf(ksc[NG - 1])) : 0.0f;
+    float up = 1.0f;
+    if (__any(fmaxf(v_most, k_most) >= kVast)) {
+      const bool there = !none && t0 + 16 * g + c < k_end;
+      if (__any(there && v_most >= kVast)) raise = kRaise;
+      // beside queries of up to 256 they could overflow scores before `col` (where that is as large, all overflows)
+      if (FP8 && __any(there && k_most >= kVast) && !__any(col[0] >= 0x1p79f)) {
+        up = 0x1p48f;
+#pragma unroll
+        for (int G = 0; G < NG; ++G) ksc[G] *= 0x1p-48f;
+      }
+    }
+    float mul[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) mul[n] = FP8 ? col[n] * up : col[n];
     f32x4 s[NQ][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -330,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       float mx = s[n][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
-      mx = over_groups(__builtin_fmaf(mx, col[n], raise), [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      mx = over_groups(__builtin_fmaf(mx, mul[n], raise), [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
       if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
         const float m_new = fmaxf(m_run[n], mx);
         const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
@@ -345,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], col[n], neg_m));
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], mul[n], neg_m));
         l_run[n] += e;
         s[n][i >> 2][i & 3] = e;
       }

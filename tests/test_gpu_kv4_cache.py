@@ -488,6 +488,20 @@ def test_attention_of_vast_values(dev, new, d, space):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_vast_keys(dev, new, d):
+    """K scales near bf16's largest number and small queries: scores of ordinary size."""
+    rng = np.random.default_rng(new + d)
+    for tokens in (slice(None), slice(700, None), slice(1203, 1204)):
+        c = attn_case(rng, [1500, 130], [new, new], 4, 2, d, 16, low=1.0, high=1.9)
+        c["q"] *= np.float32(2.0 ** -117)
+        ks = c["cache"][2]
+        at = np.arange(1500)[tokens]
+        ks[c["table"][0, at // 16], :, at % 16] *= np.float32(2.0 ** 124)
+        check_attn(c, run_attn(dev, c, scale=2.0 ** -8), scale=2.0 ** -8)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
 def test_attention_of_small_values_beside_unseen_vast_ones(dev, new, d):
     """Scales behind the context and on pages that are none change no bit, however large."""
     rng = np.random.default_rng(new + d)
