@@ -790,8 +790,8 @@ teeny_status teeny_w4a16_linear_workspace_size(int64_t M, int64_t N, int64_t K, 
 teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t K, teeny_stream stream);
 
 /* Low-rank adapters of many requests beside a linear layer that they share:
- * out[m] = y[m] + scale[a] B[a] (A[a] x[m]) with a = adapters[m]; out[m] = y[m]
- * where that is negative or num_adapters or more.  x bf16 [M,K], a bf16
+ * out[m] = y[m] + B[a] (scale[a] (A[a] x[m])) with a = adapters[m]; out[m] = y[m]
+ * where that is negative or num_adapters or more; infinities and NaN follow it.  x bf16 [M,K], a bf16
  * [num_adapters, rank, K], b bf16 [num_adapters, N, rank], scale fp32
  * [num_adapters] or NULL (1), y (the shared layer's output) and out (which may be
  * y) bf16 [M,N]; rows of x, y and out x_stride, y_stride and out_stride elements

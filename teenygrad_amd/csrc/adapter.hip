@@ -1,6 +1,6 @@
 // Low-rank adapters of many requests beside a projection that they share:
 //
-//   out[m] = y[m] + scale[a] B[a] (A[a] x[m]),  a = adapters[m] (none: out[m] = y[m])
+//   out[m] = y[m] + B[a] (scale[a] A[a] x[m]),  a = adapters[m] (none: out[m] = y[m])
 //
 // x bf16 [M, K], A bf16 [adapters, rank, K], B bf16 [adapters, N, rank], y and out
 // bf16 [M, N].  The reference has no such operator; the shared projection is
@@ -79,6 +79,13 @@ __device__ __forceinline__ void adapter_copy(const AdapterArgs &p, int m0, uint6
       }
     }
   }
+}
+// Whether one of a lane's sums is NaN.  An infinity in B gives NaN beside a second part that is 0 or of the other sign,
+// where the first part alone gives what the whole number does: those sums are made again without the second part.
+__device__ __forceinline__ bool adapter_nan(f32x4 o) { return __builtin_isunordered(o[0], o[1]) | __builtin_isunordered(o[2], o[3]); }
+__device__ __forceinline__ void adapter_mend(f32x4 &o, f32x4 first) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = o[i] == o[i] ? o[i] : first[i];
 }
 // The row of B that lane c holds for tile j of the columns n ..: a lane's products are a row's columns n + 8 g + 0..7, and 32 further on.
 __device__ __forceinline__ int adapter_col(int n, int j, int c) { return n + 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3); }
@@ -271,6 +278,18 @@ __global__ __launch_bounds__(256, RT * MT >= 16 ? 1 : RT * MT >= 8 ? 2 : RT * MT
             o[j] = mfma_16x16(__builtin_bit_cast(bf16x8, b[j][k]),
                               *reinterpret_cast<const bf16x8 *>(&hs[s][16 * t + cc][32 * k + 8 * gg]), o[j]);
       }
+      if (__builtin_expect(__any(adapter_nan(o[0]) | adapter_nan(o[1]) | adapter_nan(o[2]) | adapter_nan(o[3])), 0)) {
+        const u32x4 zero = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 first = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            first = mfma_16x16(__builtin_bit_cast(bf16x8, RT > 1 || gg < 2 ? b[j][k] : zero),
+                               *reinterpret_cast<const bf16x8 *>(&hs[0][16 * t + cc][32 * k + 8 * gg]), first);
+          adapter_mend(o[j], first);
+        }
+      }
     };
     int n = n0 + 64 * w;
     asm volatile("" : "+s"(n));  // or the loop over adapters carries every address along
@@ -412,6 +431,15 @@ __global__ __launch_bounds__(1024) void adapter_one(AdapterArgs p) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
           o = mfma_16x16(__builtin_bit_cast(bf16x8, b[k]), *reinterpret_cast<const bf16x8 *>(&hs[s][c][32 * k + 8 * g]), o);
+      if (__builtin_expect(__any(adapter_nan(o)), 0)) {
+        const u32x4 zero = {};
+        f32x4 first = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          first = mfma_16x16(__builtin_bit_cast(bf16x8, RT > 1 || g < 2 ? b[k] : zero),
+                             *reinterpret_cast<const bf16x8 *>(&hs[0][c][32 * k + 8 * g]), first);
+        adapter_mend(o, first);
+      }
       if (n + 256 < n1) load_b(n + 256);
       if (in) {
         const bf16 *y = p.y + (rows.m0 + c) * p.y_stride + n + 4 * g;

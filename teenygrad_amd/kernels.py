@@ -1769,7 +1769,7 @@ def adapter_dims(x_shape, a_shape, b_shape, n_ids, y_shape, scale_shape=None) ->
 
 def adapter_add(x: Buffer, a: Buffer, b: Buffer, adapters: Buffer, y: Buffer, scale: Optional[Buffer] = None,
                 out: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
-    """Low-rank adapters of many requests beside a linear layer that all share: out[m] = y[m] + scale[i] b[i] (a[i] x[m]),
+    """Low-rank adapters of many requests beside a linear layer that all share: out[m] = y[m] + b[i] (scale[i] a[i] x[m]),
     i = adapters[m] (int32; negative: out[m] = y[m]).  x bf16 [M, K], y the shared layer's output on x, bf16 [M, N], a bf16
     [adapters, rank, K], b bf16 [adapters, N, rank], scale fp32 [adapters] (None: 1).  out=y updates in place."""
     m, n, k, rank, count = adapter_dims(x.shape, a.shape, b.shape, adapters.numel, y.shape,

@@ -117,6 +117,31 @@ def test_rows_are_apart(dev, space):
 
 
 @pytest.mark.parametrize("space", [False, True])
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(7, 70, 1064), (9, 333, 40), (300, 520, 264), (600, 130, 264)])
+def test_infinities_in_b(dev, m, n, k, rank, space):
+    """An infinity in B gives the infinity or NaN of the formula, whatever the sign and size of the ranks' second part."""
+    rng = np.random.default_rng(m + rank)
+    c = case(rng, np.sort(rng.integers(-1, 3, m)) if m > 9 else [0, 1, 0, 2, -1, 1, 0, 2, 2][:m], n, k, rank, 3)
+    # each product of the ranks is one number of x times one of A: its sign is in no doubt, and some have a second part of 0
+    c["x"][:, 1:] = 0
+    c["x"][:, 0] = np.where(np.arange(m) % 2, 2.0 ** rng.integers(-3, 4, m), rounded(rng.uniform(0.5, 2, m))) * rng.choice([-1, 1], m)
+    c["a"][:, ::2, 0] = 1
+    c["scale"][0] = 1
+    c["b"][0, 11, 4], c["b"][0, 12, 7], c["b"][1, 3, 5], c["b"][2, 69, 6] = np.inf, -np.inf, np.inf, np.inf
+    c["b"][0, 20, :2] = np.inf, -np.inf
+    c["b"][1, 40, 1] = np.nan
+    with np.errstate(all="ignore"):
+        ref, tol = kv4.adapter(c["x"], c["a"], c["b"], c["ids"], c["scale"], c["y"])
+    with space_for(dev, c, space):
+        got = run(dev, c)
+    fin = np.isfinite(ref)
+    assert np.isinf(ref).any() and np.isnan(ref).any()
+    np.testing.assert_array_equal(got[~fin], ref[~fin].astype(np.float32))
+    assert (np.abs(got[fin] - ref[fin]) <= tol[fin]).all()
+
+
+@pytest.mark.parametrize("space", [False, True])
 def test_strides(dev, space):
     """Rows of x, y and out inside wider ones, the aligned and the odd kind; nothing between them is written."""
     rng = np.random.default_rng(4)
