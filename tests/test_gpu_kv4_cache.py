@@ -346,6 +346,21 @@ def test_attention_of_many_sequences(dev, new, batch):
         check_attn(c, run_attn(dev, c, hint=hint, pad=2), ref=ref)
 
 
+def test_attention_of_many_sequences_in_tiles(dev):
+    """5000 sequences of 32 heads of their own under a hint of many queries: near the limit of rows."""
+    rng = np.random.default_rng(71)
+    batch, heads = 5000, 32
+    c = attn_case(rng, [int(n) for n in rng.integers(0, 40, batch)], [1] * batch, heads, heads, 64, 16)
+    o, lse = run_attn(dev, c, hint=(100, 40), pad=2)
+    assert (o[:batch] != 123.0).all() and (o[batch:] == 123.0).all() and (lse[batch:] == 55.0).all()
+    some = np.concatenate([[0, batch - 1], rng.choice(batch, 40, replace=False)])  # for the oracle
+    table = c["table"][some]
+    pages = np.unique(table[table >= 0])
+    table = np.where(table >= 0, np.searchsorted(pages, table), -1)
+    part = dict(q=c["q"][some], cache=[a[pages] for a in c["cache"]], table=table, ctx=c["ctx"][some], starts=np.arange(len(some) + 1))
+    check_attn(part, (o[some], lse[some]))
+
+
 @pytest.mark.parametrize("new", [1, 30, 90])
 def test_attention_rows_of_no_sequence(dev, new):
     """Rows before the first sequence stay as they were, as those past the last one do."""

@@ -110,6 +110,22 @@ def test_attention_splits_fit_a_launch(batch, hq, hkv, d, longest, context):
     assert splits > 1 and units * splits < (1 << 31) // 256
 
 
+LIMIT = 1 << 25  # of n_tokens * q_heads + 128 * batch * kv_heads
+
+
+@pytest.mark.parametrize("tokens,batch,hq,hkv,longest", [
+    (5000, 5000, 32, 32, 100), (LIMIT // 8 - 200, 1, 8, 1, 100), (LIMIT // 32 // 129 - 1, LIMIT // 32 // 129 - 1, 32, 32, 65),
+    (LIMIT // 136 - 1, LIMIT // 136 - 1, 8, 1, 1), (LIMIT // 160 - 1, LIMIT // 160 - 1, 32, 1, 1)])
+def test_attention_rows_within_the_limit(tokens, batch, hq, hkv, longest):
+    """Calls within the documented limit are not refused for their rows, whichever form they take: the one thing that is wrong
+    with these, and found later, are their scales' addresses.  32 times the rows are refused."""
+    assert tokens * hq + 128 * batch * hkv < LIMIT
+    a = dict(n_tokens=tokens, batch=batch, q_heads=hq, kv_heads=hkv, max_q_len=longest, q_stride=hq * 128, k_scale=FAKE_ODD)
+    expect(lib.teeny_kv4_cache_attention(*attn_args(**a)), _lib.ERR_MISALIGNED)
+    a.update(n_tokens=32 * tokens, batch=32 * batch if batch > 1 else 1)
+    expect(lib.teeny_kv4_cache_attention(*attn_args(**a)), _lib.ERR_SHAPE_MISMATCH)
+
+
 def adapter_args(**kw):
     a = dict(x=FAKE, a=FAKE, b=FAKE, adapters=FAKE, scale=None, y=FAKE, out=2 * FAKE, M=4, N=100, K=64, rank=16, num_adapters=3, x_stride=64,
              y_stride=100, out_stride=100)
