@@ -336,6 +336,17 @@ teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v,
   TEENY_REQUIRE((q_heads == 0 || q_stride >= q_heads * head_dim) &&
                     (kv_heads == 0 || (k_stride >= kv_heads * head_dim && v_stride >= kv_heads * head_dim)),
                 TEENY_ERR_SHAPE_MISMATCH, "kv4_cache_append: token strides below heads * head_dim");
+  // Workgroups of rows take a token, of more than 512 tokens four, which share the angles' work (1 / 4 tokens, 32 and 8 heads of
+  // 128: 300 tokens 6.4 / 7.4 us, 900 11.0 / 9.1, 8000 56 / 44).  V's 64 tokens of a head may be 64 runs, in a decode step, or
+  // four: workgroups to them by the number of tokens (4 / 8 / 16 of them: 64 tokens of their own 10.4 / 6.5 / 4.5 us, 256
+  // 12.3 / 8.4 / 6.7, 80 in runs of five, 16 heads of 64 4.8 / 5.0 / 5.5; 1 / 2 / 4 / 8: 8000 tokens 44.3 / 44.3 / 46 / 51, 500
+  // 8 / 16 9.8 / 11.0).
+  const int per = n_tokens > 512 ? 4 : 1;
+  int share = n_tokens <= 256 ? 16 : n_tokens <= 1024 ? 8 : 2;
+  const int64_t rows = cdiv(n_tokens, per), values = cdiv(n_tokens, 64) * kv_heads, most = int64_t{1} << 23;
+  while (share > 1 && rows + values * share >= most) share /= 2;  // thousands of heads
+  const int64_t all = rows + values * share;
+  TEENY_REQUIRE(all < most, TEENY_ERR_SHAPE_MISMATCH, "kv4_cache_append: too many rows for a launch");
   TEENY_REQUIRE(aligned(q, 16) && aligned(q_out, 16) && aligned(k, 16) && aligned(v, 16) && aligned(k_cache, 16) &&
                     aligned(v_cache, 16) && (q_heads == 0 || q_stride % 8 == 0) &&
                     (kv_heads == 0 || (k_stride % 8 == 0 && v_stride % 8 == 0)),
@@ -348,15 +359,8 @@ teeny_status teeny_kv4_cache_append(const void *q, const void *k, const void *v,
                   static_cast<bf16 *>(k_scale), static_cast<bf16 *>(v_scale), static_cast<int>(n_tokens),
                   static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(num_pages << shift), shift,
                   static_cast<int>(rotary_dim / 2), interleaved != 0, 1, 0, 1};
-  // Workgroups of rows take a token, of more than 512 tokens four, which share the angles' work (1 / 4 tokens, 32 and 8 heads of
-  // 128: 300 tokens 6.4 / 7.4 us, 900 11.0 / 9.1, 8000 56 / 44).  V's 64 tokens of a head may be 64 runs, in a decode step, or
-  // four: workgroups to them by the number of tokens (4 / 8 / 16 of them: 64 tokens of their own 10.4 / 6.5 / 4.5 us, 256
-  // 12.3 / 8.4 / 6.7, 80 in runs of five, 16 heads of 64 4.8 / 5.0 / 5.5; 1 / 2 / 4 / 8: 8000 tokens 44.3 / 44.3 / 46 / 51, 500
-  // 8 / 16 9.8 / 11.0).
-  p.per = n_tokens > 512 ? 4 : 1;
-  p.share = n_tokens <= 256 ? 16 : n_tokens <= 1024 ? 8 : 2;
-  const int64_t rows = cdiv(n_tokens, p.per), all = rows + cdiv(n_tokens, 64) * p.share * kv_heads;
-  TEENY_REQUIRE(all < int64_t{1} << 23, TEENY_ERR_SHAPE_MISMATCH, "kv4_cache_append: too many rows for a launch");
+  p.per = per;
+  p.share = share;
   p.rows_grid = static_cast<int>(rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(all));

@@ -44,6 +44,18 @@ def test_append_refusals(kw, code):
     expect(lib.teeny_kv4_cache_append(*append_args(**kw)), code)
 
 
+@pytest.mark.parametrize("tokens,kv_heads", [(1024, 65535), (961, 65535), (4000, 65535), (1 << 20, 247), (1 << 24, 7), (513, 65535), (1, 65535)])
+def test_append_within_the_limit(tokens, kv_heads):
+    """Calls within the documented limit are not refused for their size: the one thing that is wrong with these, and found
+    later, is the cache's address."""
+    assert tokens / 4 + tokens / 32 * kv_heads < 1 << 23
+    row = kv_heads * 64
+    a = dict(n_tokens=tokens, kv_heads=kv_heads, head_dim=64, rotary_dim=64, k_stride=row, v_stride=row, v_cache=FAKE_ODD)
+    expect(lib.teeny_kv4_cache_append(*append_args(**a)), _lib.ERR_MISALIGNED)
+    a.update(n_tokens=1 << 24, kv_heads=65535, k_stride=1 << 23, v_stride=1 << 23)
+    expect(lib.teeny_kv4_cache_append(*append_args(**a)), _lib.ERR_SHAPE_MISMATCH)
+
+
 def test_nothing_to_append():
     none = dict(q=None, k=None, v=None, positions=None, slots=None, inv_freq=None, q_out=None)
     assert lib.teeny_kv4_cache_append(*append_args(n_tokens=0, **none)) == _lib.OK
