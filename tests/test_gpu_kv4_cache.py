@@ -346,6 +346,29 @@ def test_attention_of_many_sequences(dev, new, batch):
         check_attn(c, run_attn(dev, c, hint=hint, pad=2), ref=ref)
 
 
+@pytest.mark.parametrize("d,batch,hkv,new,causal", [(64, 40, 16, 1, True), (128, 40, 16, 1, True), (64, 64, 9, 3, False), (64, 24, 16, 20, True),
+                                                    (128, 24, 16, 20, False)])
+def test_attention_of_many_parts(dev, d, batch, hkv, new, causal):
+    """Up to 64 sequences with more parts than the device takes at once, which go out longest first: empty contexts, sequences
+    without queries, contexts past all splits and rows past the hinted ones among them."""
+    rng = np.random.default_rng(batch + hkv + new)
+    ctx, lens = rng.integers(0, 900, batch), rng.integers(0, new + 1, batch)
+    ctx[[0, 5, 17, batch - 1]], lens[[0, 3, 5, batch - 1]] = [0, 5000, 1290, 2100], [new, 0, new, new]
+    if new == 1:
+        lens[:] = 1
+    c = attn_case(rng, [int(n) for n in ctx], [int(n) for n in lens], 2 * hkv, hkv, d, 16)
+    t, ref = int(c["starts"][-1]), oracle(c, causal=causal)
+    block = 32 if new > 8 else 16
+    walk = min(t * 2 // block + batch, batch * -(-2 * new // block))
+    assert walk * hkv > 2 * dev.info()["compute_units"], "few parts go out in the sequences' order"
+    for hint in ((new, 5000), (new, 2100), (1, 2100), (new, 1)):
+        check_attn(c, run_attn(dev, c, causal=causal, hint=hint, pad=2), ref=ref)
+        size = K.kv4_cache_attention_workspace_size(t + 2, batch, 2 * hkv, hkv, d, *hint)
+        assert (size > 0) == (hint[1] > 1)
+        with stream_workspace(dev, max(size, 4096)):
+            check_attn(c, run_attn(dev, c, causal=causal, hint=hint, pad=2), ref=ref)
+
+
 def test_attention_of_many_sequences_in_tiles(dev):
     """5000 sequences of 32 heads of their own under a hint of many queries: near the limit of rows."""
     rng = np.random.default_rng(71)
