@@ -122,6 +122,21 @@ def test_attention_splits_fit_a_launch(batch, hq, hkv, d, longest, context):
     assert splits > 1 and units * splits < (1 << 31) // 256
 
 
+@pytest.mark.parametrize("tokens,batch,hq,hkv,d,longest,context", [
+    ((1 << 22) - 1000, 1, 8, 1, 128, 10, 1 << 30), ((1 << 20) - 1000, 1, 32, 2, 64, 8, 1 << 28), (1 << 19, 2, 32, 1, 64, 3, 1 << 29)])
+def test_attention_splits_of_tiles_fit_a_launch(tokens, batch, hq, hkv, d, longest, context):
+    """Many more rows than the hint stands for: as many splits as a launch of 512 threads a workgroup holds."""
+    assert hq // hkv * longest > 64, "shared tiles, of 256 rows"
+    units = (tokens * (hq // hkv) // 256 + batch) * hkv
+    n = ctypes.c_size_t(0)
+    assert lib.teeny_kv4_cache_attention_workspace_size(tokens, batch, hq, hkv, d, longest, context, ctypes.byref(n)) == _lib.OK
+    splits = n.value // (units * 256 * (d + 2) * 4)
+    assert n.value == splits * units * 256 * (d + 2) * 4
+    most = ((1 << 31) // 512 - 1) // units
+    assert 1 < splits <= most
+    assert splits == most, "the launch is what bounds it"
+
+
 LIMIT = 1 << 25  # of n_tokens * q_heads + 128 * batch * kv_heads
 
 
