@@ -784,3 +784,41 @@ def test_step_in_a_graph(dev):
                 np.testing.assert_array_equal(a.to_host(), b.to_host(), err_msg=f"replay {i}")
         assert nets[0].seq.to_host().tolist() == [n + 20 for n in lens]
         graph.destroy()
+
+
+class WideLayer(Layer):
+    """Adapters of a rank that takes two launches, the ranks' products by way of the workspace that the step's other operators use."""
+
+    def __init__(self, dev, rng, *args):
+        super().__init__(dev, rng, *args)
+        loaded, rank = 3, 128
+        for name, (codes, scale, _, _, s) in list(self.w.items()):
+            n, k = codes.shape
+            a, b = rounded(rng.standard_normal((loaded, rank, k)) / 16), rounded(rng.standard_normal((loaded, n, rank)) * 0.05)
+            self.w[name] = codes, scale, a, b, s
+            self.parts[name] = *self.parts[name][:2], up(dev, a), up(dev, b), self.parts[name][4]
+
+    def workspace(self, longest):
+        """The largest of the step's operators'."""
+        context = self.width * self.page
+        adapters = [K.adapter_add_workspace_size(self.rows, c.shape[0], c.shape[1], 128) for c, *_ in self.w.values()]
+        attention = K.kv4_cache_attention_workspace_size(self.rows, self.seq.numel, self.hq, self.hkv, self.d, longest, context)
+        layers = [K.w4a16_linear_workspace_size(self.rows, *c.shape, 64) for c, *_ in self.w.values()]
+        assert min(adapters) > 0
+        return max(*adapters, *layers, attention)
+
+
+def test_steps_with_one_workspace(dev, monkeypatch):
+    """The steps of test_steps_together, with prompts: the adapters' two launches and the 4-bit layers on one workspace."""
+    monkeypatch.setitem(globals(), "Layer", WideLayer)
+    with stream_workspace(dev, WideLayer(dev, np.random.default_rng(0), 4, 200, 40, 12).workspace(100)):
+        test_steps_together(dev)
+
+
+def test_step_with_one_workspace_in_a_graph(dev, monkeypatch):
+    """The replays of test_step_in_a_graph, with those adapters and split attention: its workspace holds every operator's part."""
+    monkeypatch.setitem(globals(), "Layer", WideLayer)
+    net = WideLayer(dev, np.random.default_rng(0), 3, 3, 90, 40)
+    size = K.kv4_cache_attention_workspace_size(3, 3, net.hq, net.hkv, net.d, 1, 40 * 16)
+    assert size > 0 and net.workspace(1) <= size + (1 << 20)
+    test_step_in_a_graph(dev)
