@@ -115,6 +115,14 @@ __device__ __forceinline__ f32x4 mfma16_fp8(int64_t a, int64_t b, f32x4 c) {
 // fall below bf16's and fp32's smallest numbers.)
 constexpr float kVast = 0x1p80f, kRaise = 48.0f;
 
+// Whether one of a token's V scales is kVast or more, or no number: by its bits.
+template <int NG, typename S>
+__device__ __forceinline__ bool kv4_vast(S scales) {
+  constexpr uint32_t vast = 0x6780;  // 2^80
+  if constexpr (NG == 1) return (__builtin_bit_cast(uint16_t, scales) & 0x7fffu) >= vast;
+  else return (__builtin_bit_cast(uint32_t, scales) & 0x7fffffffu) >= vast << 16 || (__builtin_bit_cast(uint32_t, scales) & 0x7fffu) >= vast;
+}
+
 // NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
@@ -248,6 +256,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
     // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too
     col[n] = fmaxf(scale, 1.17549435e-38f);
   }
+  // Beside a query of up to 256 K scales near the largest number could overflow the scores, before `col`: they are taken
+  // 2^-12 of.  (Where `col` is so large that it could not make up for it, such scores overflow anyway.)
+  const float down = FP8 && !__any(col[0] >= 0x1p100f) ? 0x1p-12f : 1.0f;
+  col[0] *= 1.0f / down;
   const int all_see = seen(r.row0);  // all rows see the tokens below it
 
   f32x4 acc[NQ][ND], p_off[FP8 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
@@ -264,28 +276,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
   }
 #pragma unroll 1
   for (; t0 < ke; t0 += STEP) {
+    if (__any(kv4_vast<NG>(vs)) && __any(kv4_vast<NG>(vs) && !none && t0 + 16 * g + c < k_end)) raise = kRaise;
     float ksc[NG], vsc[NG];  // of the lane group's token c
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
       const float k = static_cast<float>(ks[G]);
-      ksc[G] = __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
+      ksc[G] = FP8 ? __builtin_fmaf(k, down, k * 0.0f) : __builtin_fmaf(k, 0.0f, k);  // an infinity counts as NaN
       vsc[G] = static_cast<float>(vs[G]);
     }
-    const float v_most = fmaxf(fabsf(vsc[0]), fabsf(vsc[NG - 1])), k_most = FP8 ? fmaxf(fabsf(ksc[0]), fabsf(ksc[NG - 1])) : 0.0f;
-    float up = 1.0f;
-    if (__any(fmaxf(v_most, k_most) >= kVast)) {
-      const bool there = !none && t0 + 16 * g + c < k_end;
-      if (__any(there && v_most >= kVast)) raise = kRaise;
-      // beside queries of up to 256 they could overflow scores before `col` (where that is as large, all overflows)
-      if (FP8 && __any(there && k_most >= kVast) && !__any(col[0] >= 0x1p79f)) {
-        up = 0x1p48f;
-#pragma unroll
-        for (int G = 0; G < NG; ++G) ksc[G] *= 0x1p-48f;
-      }
-    }
-    float mul[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) mul[n] = FP8 ? col[n] * up : col[n];
     f32x4 s[NQ][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -343,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       float mx = s[n][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, s[n][i >> 2][i & 3]);
-      mx = over_groups(__builtin_fmaf(mx, mul[n], raise), [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      mx = over_groups(__builtin_fmaf(mx, col[n], raise), [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
       if (__any(mx > m_run[n] + 8.0f)) {  // rescaled rarely: p <= 2^8
         const float m_new = fmaxf(m_run[n], mx);
         const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == -INFINITY ? 0.0f : m_new));
@@ -358,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
       const float neg_m = m_run[n] == -INFINITY ? 0.0f : -m_run[n];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], mul[n], neg_m));
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], col[n], neg_m));
         l_run[n] += e;
         s[n][i >> 2][i & 3] = e;
       }
