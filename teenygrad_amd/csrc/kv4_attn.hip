@@ -115,6 +115,10 @@ __device__ __forceinline__ f32x4 mfma16_fp8(int64_t a, int64_t b, f32x4 c) {
 // fall below bf16's and fp32's smallest numbers.)
 constexpr float kVast = 0x1p80f, kRaise = 48.0f;
 
+// The least that scores are multiplied with, so that a masked -inf gives p = 0 under a zero scale too.  (It is the smallest
+// number: times the largest score it is 2^-21, where FLT_MIN gave 4.)
+constexpr float kLeast = 0x1p-149f;
+
 // Whether one of a token's V scales is kVast or more, or no number: by its bits.
 template <int NG, typename S>
 __device__ __forceinline__ bool kv4_vast(S scales) {
@@ -253,13 +257,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn(Kv4AttnArgs p) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) qf[n][j] = __builtin_bit_cast(bf16x8, raw[j]);
     }
-    // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too
-    col[n] = fmaxf(scale, 1.17549435e-38f);
+    col[n] = scale;
   }
   // Beside a query of up to 256 K scales near the largest number could overflow the scores, before `col`: they are taken
   // 2^-12 of.  (Where `col` is so large that it could not make up for it, such scores overflow anyway.)
   const float down = FP8 && !__any(col[0] >= 0x1p100f) ? 0x1p-12f : 1.0f;
   col[0] *= 1.0f / down;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) col[n] = fmaxf(col[n], kLeast);
   const int all_see = seen(r.row0);  // all rows see the tokens below it
 
   f32x4 acc[NQ][ND], p_off[FP8 ? NG : 1];  // p_off: -1.5 sum of the weighted probabilities, in every row
@@ -521,8 +526,7 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   if (split > 0 && kb >= k_end) return;
   const int base = r.row0 + 32 * w;  // the wave's rows; past r.rows it only helps to turn the tiles
 
-  // at least FLT_MIN, so that a masked -inf gives p = 0 under a zero scale too; 16: of kv4_values8
-  const float sc = fmaxf(16.0f * fabsf(p.scale_log2), 1.17549435e-38f);
+  const float sc = fmaxf(16.0f * fabsf(p.scale_log2), kLeast);  // 16: of kv4_values8
   const uint32_t qsign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale's sign goes to Q
   const int my = min(base + c, r.rows - 1), qt = my / p.group, qh = head * p.group + my - qt * p.group;
   const int64_t out_row = static_cast<int64_t>(r.first + qt) * p.heads + qh;

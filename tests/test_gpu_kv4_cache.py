@@ -540,6 +540,18 @@ def test_attention_of_vast_keys(dev, new, d):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_of_vast_keys_under_a_scale_of_zero(dev, new, d):
+    """Every token that a row sees counts alike, whatever its keys."""
+    rng = np.random.default_rng(new + d)
+    c = attn_case(rng, [700, 130], [new, new], 4, 2, d, 16, low=1.0, high=1.9)
+    c["q"] *= np.float32(0.25)
+    clean = oracle(c, scale=0.0)
+    c["cache"][2] *= np.float32(2.0 ** 124)
+    check_attn(c, run_attn(dev, c, scale=0.0), ref=clean)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 20, 80])
 def test_attention_of_small_values_beside_unseen_vast_ones(dev, new, d):
     """Scales behind the context and on pages that are none change no bit, however large."""
     rng = np.random.default_rng(new + d)
