@@ -512,8 +512,9 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   constexpr int RB = 256, NS = D / 16, ND = D / 32, NG = D / 64, EPW = D / 32, KW = D / 64, FR = 2 * NS + 4 * ND;
   typedef uint32_t kvec __attribute__((ext_vector_type(KW)));
   __shared__ __attribute__((aligned(16))) u32x4 frag[2][FR * 64];  // K [block][step], then V [d block][block][half]
-  __shared__ uint32_t bad[2][NG][2];  // tokens of a tile whose V scale is not finite (they are turned to zeros)
-  __shared__ int vast_from;           // the first token turned whose V scale is kVast or more
+  // of the tokens turned the first whose V scale is not finite (it is turned to zeros), for each group, and the first whose is
+  // kVast or more: a row sees it or later ones at most
+  __shared__ int nan_from[NG], vast_from;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int head = id / (p.splits * p.blocks), in_head = id - head * (p.splits * p.blocks);
@@ -594,8 +595,8 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
     if (D == 64 && w >= 4) return;
     float s = static_cast<float>(vs);
     const bool finite = fabsf(s) < INFINITY;
-    const uint64_t m = __ballot(there_v && !finite);  // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
-    const uint64_t vast = __ballot(there_v && fabsf(s) >= kVast);
+    // lanes 0 .. 15: tokens 0 .. 15 of the block, 32 .. 47: the others
+    const uint64_t odd = __ballot(there_v && !(fabsf(s) < kVast)), fit = __ballot(finite);
     s = there_v && finite ? s : 0.0f;
     const int at = 2 * NS + (vd * 2 + vb) * 2;
     to[at * 64 + lane] = __builtin_bit_cast(u32x4, kv4_values8(vr[0], [&](float (&v)[8]) {
@@ -608,16 +609,17 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
                                                       if constexpr (t >= 8) v[t - 8] *= row_lane<t>(s);
                                                     });
                                                   }));
-    auto tokens = [](uint64_t v) { return static_cast<uint32_t>((v & 0xffffu) | (v >> 32 & 0xffffu) << 16); };
-    if ((vd & 1) == 0 && lane == 0) {
-      bad[buf][vd >> 1][vb] = tokens(m);
-      if (vast != 0) atomicMin(&vast_from, t0 + 32 * vb + __builtin_ctz(tokens(vast)));
+    if (odd != 0) {
+      auto note = [&](int *from, uint64_t m) {
+        if (m != 0) atomicMin(from, t0 + 32 * vb + __builtin_ctz(static_cast<uint32_t>((m & 0xffffu) | (m >> 32 & 0xffffu) << 16)));
+      };
+      if ((vd & 1) == 0 && lane == 0) note(&nan_from[vd >> 1], odd & ~fit), note(&vast_from, odd & fit);
     }
   };
 
   int pg = 0, buf = 0;
   uint32_t here = 0;
-  if (threadIdx.x == 0) vast_from = 0x7fffffff;
+  if (threadIdx.x == 0) vast_from = nan_from[0] = nan_from[NG - 1] = 0x7fffffff;
   if (kb < ke) pg = load_pages(kb);
   __syncthreads();
   if (kb < ke) {
@@ -635,9 +637,6 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   for (int t0 = kb; t0 < ke; t0 += 64) {
     const u32x4 *now = frag[buf];
     const uint32_t here_now = here;
-    uint32_t unfit[NG][2];
-#pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) unfit[i >> 1][i & 1] = bad[buf][i >> 1][i & 1];
     // (the next tile's turning, which may be under way, does not change which side of this tile's end it lies on)
     const int vast_at = vast_from;
     if (t0 + 64 < ke) {
@@ -704,19 +703,6 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
           pb[b][v >> 3][(v & 7) + 1] = pr[1];
         }
       }
-      // a row that sees a token whose V is NaN: its outputs of that group are, whatever the token's weight
-#pragma unroll
-      for (int G = 0; G < NG; ++G)
-        if ((unfit[G][0] | unfit[G][1]) != 0) {
-          uint32_t sees = 0;
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int n = min(max(vis - (t0 + 32 * b + 16 * g), 0), 16);  // of the lane's 16 tokens
-            sees |= unfit[G][b] >> (16 * g) & ((1u << n) - 1);
-          }
-          sees |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(sees), 32, 64));  // the row's other tokens
-          if (sees != 0) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
-        }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 4 * ND; ++j) {
@@ -731,6 +717,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   }
   l_run += __shfl_xor(l_run, 32, 64);
   if (base + c >= r.rows) return;
+  // a row that sees a token whose V is NaN: its outputs of that group are, whatever the token's weight
+#pragma unroll
+  for (int G = 0; G < NG; ++G)
+    if (nan_from[G] < vis) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
   const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
   const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
   const int64_t slot = (unit * p.splits + split) * RB + 32 * w + c;
