@@ -638,9 +638,11 @@ teeny_status teeny_kv_cache_attention_workspace_size(int64_t n_tokens, int64_t b
  * at `positions` (negative: the row is skipped).  Numbers i and i + rotary_dim / 2
  * of a head of q and k (interleaved: 2 i and 2 i + 1) are rotated by the angle
  * position * inv_freq[i] (fp32 [rotary_dim / 2]; the product, its cosine and sine
- * in 64 bits), further numbers stay.  Rotated q goes to q_out (dense, rounded once;
- * may be q where q is dense), k (rotated in 64 bits, rounded to fp32) and v into
- * the slots (negative or beyond the cache: only q's row is written).  Other tokens
+ * in 64 bits), further numbers stay.  Rotated q (with cosine and sine rounded to
+ * fp32 and fp32 products: within 2^-22 of the pair's larger number, then rounded to
+ * bf16) goes to q_out (dense; may be q where q is dense), k (rotated in 64 bits,
+ * rounded to fp32) and v into the slots (negative or beyond the cache: only q's row
+ * is written).  Other tokens
  * of the page keep their codes.  The new tokens of 16 slots that begin at a
  * multiple of 16 are consecutive rows at consecutive slots, as the plan lays them
  * out; otherwise V's codes of those 16 are unspecified.  rotary_dim a multiple of
@@ -799,9 +801,10 @@ teeny_status teeny_pack_int4(const int8_t *q, int8_t *packed, int64_t N, int64_t
  * ranks' products are worked out once, shared out over the device; without it, and
  * where the size is 0, again by each workgroup.  Rows of an adapter need not lie
  * together, but are faster so.  fp32 sums, the rank's products held in two bf16
- * parts (2^-17) for the second product; out is rounded once.  rank a multiple of 8 up to 128 (smaller ones are filled up with
- * zeros), N * rank below 2^30; K a multiple of 8 up to 2^22, x_stride up to 2^24; x,
- * a, b and x's rows 16-byte aligned. */
+ * parts (2^-17) for the second product; out is rounded once.  rank a multiple of 8
+ * up to 128 (smaller ones are filled up with zeros), N * rank below 2^30; K a
+ * multiple of 8 up to 2^22; M, N, num_adapters and the strides up to 2^24; x, a, b
+ * and x's rows 16-byte aligned. */
 teeny_status teeny_adapter_add(const void *x, const void *a, const void *b, const int32_t *adapters, const float *scale,
                                const void *y, void *out, int64_t M, int64_t N, int64_t K, int64_t rank,
                                int64_t num_adapters, int64_t x_stride, int64_t y_stride, int64_t out_stride,

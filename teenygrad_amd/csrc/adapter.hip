@@ -467,7 +467,7 @@ __global__ __launch_bounds__(1024) void adapter_one(AdapterArgs p) {
 // rows, where the rank is 16 or less: tiles of 16 rows with four; else of 32 (down: 64 past 1024) with three, past 512 rows two.
 // us for 4096 -> 4096 of rank 16, 16 rows and four / 32 and three: 300 rows and 100 adapters 36 / 60 (a workgroup a row: 22),
 // 500 rows of their own 46 / 74, runs of 100 rows, three 10.7 / 9.9 (17), five 13.2 / 10.8; past 512, 32 and two: 900 rows and 100
-// adapters 63 / 114, but three runs of 300 14.9 / 12.9, five of 200, -> 11008, 23.2 / 17.6; of rank 64, 4096 -> 11008: five runs
+// adapters 63 / 118, but three runs of 300 14.9 / 12.9, five of 200, -> 11008, 23.2 / 17.6; of rank 64, 4096 -> 11008: five runs
 // of 100 31 / 24.9, 500 rows and ten adapters 94 / 76.
 // 2000 rows in five runs, rank 64, 4096 -> 11008: tiles of 16 / 32 / 64 for the columns 51.5 / 40.6 / 53.5, of 32 / 64 for the
 // ranks 43.5 / 40.6 (800 rows: 24.5 / 26.9); 300 rows and 100 adapters, two / three / four workgroups to 32: 83 / 60 / 50, three
@@ -500,7 +500,7 @@ static AdapterPlan adapter_plan(int64_t M, int64_t N, int64_t K, int64_t rank) {
   const int64_t ranges = std::max<int64_t>(1, std::min(cdiv(N, 256), std::max<int64_t>(small ? 8 : 4, (many ? 512 : 768) / up)));
   pl.cols = static_cast<int>(cdiv(cdiv(N, ranges), 256) * 256);
   // One launch for few small products, each workgroup having a CU to itself: a row, rank 16, 1024 -> 4096: 5.6 us against
-  // 6.4; 16 rows: 6.4 against 7.0; but every range of columns reads all of A: a row, 4096 -> 4096: 7.5 against 6.2 us
+  // 6.4; 16 rows: 6.4 against 7.0; but every range of columns reads all of A: a row, 4096 -> 4096: 7.5 against 6.4 us
   // (2048 -> 2048: 6.9 both); more workgroups than CUs: 64 rows, 1024 -> 4096: 22.5 against 9.0 us.
   pl.one = 16 * pl.rt * K <= 16384 && M * cdiv(N, 256) <= 256;
   pl.bytes = pl.one ? 0 : static_cast<size_t>(pl.splits) * M * 16 * pl.rt * 4;

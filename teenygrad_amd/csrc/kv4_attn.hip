@@ -26,9 +26,14 @@
 // (the one rounding on the way, as in kv_attn).  Lane c of a group holds the scale of
 // the group's token c, and the multiplication fetches it across the 16 lanes
 // (row_newbcast).  For 64 tokens of 128 numbers a wave reads 8.7 KB and issues 360
-// vector instructions and 52 products.  One query to each of 64 contexts of 8000
-// tokens, 32 heads over 8 of 128: 107 us, 5.2 TB/s, the rate of a copy; 90 to 8000
-// tokens: 68 us, 4.1 TB/s, for want of waves at the end.
+// vector instructions and 52 products.  One query to each of 64 contexts of 90 to
+// 8000 tokens, 32 heads over 8 of 128: 68 us, 4.1 TB/s, for want of waves at the end;
+// of 8000 tokens each 122 us, 4.6 TB/s, in the two splits that serve ragged contexts
+// (unsplit 107 us, 5.2 TB/s, the rate of a copy).  17 to 64 rows: five queries to each
+// of 16 contexts of 3000 tokens, 64 heads over 8 of 128, 39.5 us, 1.4 TB/s: two blocks of
+// rows read and unpack the cache each, with 128 products for 64 tokens; vector
+// instructions take 59 % of the SIMDs' cycles and products 34 %, with 1.7 waves (of two
+// that 242 registers allow) to do one beside the other.
 #include "kv4.hpp"
 #include "kv_attn.hpp"
 
@@ -123,8 +128,12 @@ constexpr float kLeast = 0x1p-149f;
 template <int NG, typename S>
 __device__ __forceinline__ bool kv4_vast(S scales) {
   constexpr uint32_t vast = 0x6780;  // 2^80
-  if constexpr (NG == 1) return (__builtin_bit_cast(uint16_t, scales) & 0x7fffu) >= vast;
-  else return (__builtin_bit_cast(uint32_t, scales) & 0x7fffffffu) >= vast << 16 || (__builtin_bit_cast(uint32_t, scales) & 0x7fffu) >= vast;
+  if constexpr (NG == 1) {
+    return (__builtin_bit_cast(uint16_t, scales) & 0x7fffu) >= vast;
+  } else {
+    const uint32_t both = __builtin_bit_cast(uint32_t, scales);
+    return (both & 0x7fffffffu) >= vast << 16 || (both & 0x7fffu) >= vast;
+  }
 }
 
 // NQ: 16-row column blocks; the four waves share out the tokens, 64 a time.
@@ -502,9 +511,9 @@ __device__ __forceinline__ bf16x8 kv4_values8(uint32_t word, S scale) {
 // where the scale has five bits (other scales: rounded), so that the products need
 // no scale of their own.  The next tile is turned while one is multiplied, the codes
 // of the tile after that are in flight; one barrier a tile.  Bound by the vector instructions, 290 a wave and tile, 32 of
-// them exponentials, beside 32 products of 32 cycles: 4 requests of 700 queries and
-// 1100 to 4100 tokens, 32 heads of 128 over 8: 122 to 130 us, 717 TFLOP/s and more;
-// 1900 queries of 6400: 203 us, 835.  (Four waves and 128 rows, two workgroups on a CU: every row pays
+// them exponentials (62 % of the SIMDs' cycles), beside 32 products of 32 cycles (44 %): 4 requests of 700 queries and
+// 1100 to 4100 tokens, 32 heads of 128 over 8: 122 to 132 us, 705 to 764 TFLOP/s;
+// 1900 queries of 6400: 203 to 210 us, 806 to 836.  (Four waves and 128 rows, two workgroups on a CU: every row pays
 // for turning twice as often, 174 us to 150.  Two groups of waves half a tile apart: 175
 // to 150.  Turning and exponentials between the products: 134 to 140.)
 template <int D>
@@ -720,7 +729,10 @@ __global__ __launch_bounds__(512, 2) void kv4_attn_tile(Kv4AttnArgs p) {
   // a row that sees a token whose V is NaN: its outputs of that group are, whatever the token's weight
 #pragma unroll
   for (int G = 0; G < NG; ++G)
-    if (nan_from[G] < vis) acc[2 * G] = acc[2 * G] * __uint_as_float(0x7fc00000u), acc[2 * G + 1] = acc[2 * G + 1] * __uint_as_float(0x7fc00000u);
+    if (nan_from[G] < vis) {
+      acc[2 * G] *= __uint_as_float(0x7fc00000u);
+      acc[2 * G + 1] *= __uint_as_float(0x7fc00000u);
+    }
   const bool whole = p.part == nullptr || k_end <= p.chunk;  // no other split has a part of these rows
   const int64_t unit = static_cast<int64_t>(head) * p.blocks + r.number<RB>(p);
   const int64_t slot = (unit * p.splits + split) * RB + 32 * w + c;

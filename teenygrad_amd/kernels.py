@@ -1548,7 +1548,8 @@ def kv4_cache_append(q: Optional[Buffer], k: Buffer, v: Buffer, positions: Buffe
     q_heads, head_dim], or None) rotated by `positions` times inv_freq (fp32 [rotary_dim / 2]; None: not rotated): numbers
     i and i + rotary_dim / 2 of a head, or 2 i and 2 i + 1 (interleaved).  slots and positions as ``kv_cache_plan`` gives
     them; a row of a negative position is skipped, one of a negative slot gives its q alone.  Returns the rotated q
-    (q_out, which may be q; a skipped row is left as it was)."""
+    (q_out, which may be q; a skipped row is left as it was).  Rows that are parts of wider ones (of one projection's
+    output) go to ``teeny_kv4_cache_append``, which takes their strides."""
     pages, heads, size, d = _need_cache4(k_cache, v_cache, k_scale, v_scale)
     t = slots.numel
     if not k.shape == v.shape == (t, heads, d):
@@ -1770,7 +1771,7 @@ def adapter_dims(x_shape, a_shape, b_shape, n_ids, y_shape, scale_shape=None) ->
 def adapter_add(x: Buffer, a: Buffer, b: Buffer, adapters: Buffer, y: Buffer, scale: Optional[Buffer] = None,
                 out: Optional[Buffer] = None, stream: Optional[Stream] = None) -> Buffer:
     """Low-rank adapters of many requests beside a linear layer that all share: out[m] = y[m] + b[i] (scale[i] a[i] x[m]),
-    i = adapters[m] (int32; negative: out[m] = y[m]).  x bf16 [M, K], y the shared layer's output on x, bf16 [M, N], a bf16
+    i = adapters[m] (int32; none of the adapters: out[m] = y[m]).  x bf16 [M, K], y the shared layer's output on x, bf16 [M, N], a bf16
     [adapters, rank, K], b bf16 [adapters, N, rank], scale fp32 [adapters] (None: 1).  out=y updates in place."""
     m, n, k, rank, count = adapter_dims(x.shape, a.shape, b.shape, adapters.numel, y.shape,
                                         scale.shape if scale is not None else None)
