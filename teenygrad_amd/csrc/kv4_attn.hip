@@ -798,7 +798,7 @@ static KvAttnPlan kv4_attn_plan(int64_t tokens, int64_t batch, int64_t heads, in
     if (max_ctx > 2 * least) splits = std::min((busy < 32 ? cus : 2 * cus) / busy, cdiv(max_ctx, least));
     if (batch > 1) splits = std::max({splits, std::min((4 * cus + busy / 2) / busy, max_ctx / 1024), max_ctx / 8192});
   }
-  // a launch has less than 2^31 threads (the limit of rows leaves room for three splits at least)
+  // a launch has less than 2^31 threads (the limit of rows leaves room for four splits at least)
   splits = std::max<int64_t>(1, std::min(splits, ((int64_t{1} << 31) / (pl.tile ? 512 : 256) - 1) / units));
   auto size = [&](int64_t n) { return n > 1 ? static_cast<size_t>(units) * n * pl.rb * (D + 2) * 4 : 0; };
   auto cut = [&](int64_t n) {

@@ -261,7 +261,7 @@ inline teeny_status kv_attn_open(const char *nm, KvAttnPlanFn plan, const void *
   max_context = std::min(std::max<int64_t>(max_context, 1), std::max<int64_t>(max_pages * page_size, 1));
   pl = plan(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, max_context, scr.ptr ? scr.bytes : 0);
   const int64_t units = pl.blocks * kv_heads;
-  // a join has 64 threads for each row; row blocks of up to 512 threads leave room for three splits and more
+  // a join has 64 threads for each row; 256 threads to a row block, 512 to one of 256 rows, leave room for four splits
   TEENY_REQUIRE(units * std::min(pl.rb, 128) < (int64_t{1} << 31) / 64 && n_tokens * q_heads < (int64_t{1} << 31) / 64,
                 TEENY_ERR_SHAPE_MISMATCH, at("too many rows for a launch"));
   p.q = static_cast<const bf16 *>(q);
