@@ -611,6 +611,22 @@ def test_attention_of_any_scale(dev):
         check_attn(c, run_attn(dev, c), ref=(o, lse, tol + most[1] * (2 * off[..., None] + H16), ltol + 2 * off))
 
 
+@pytest.mark.parametrize("new", [1, 20, 80])
+def test_attention_repeats(dev, new):
+    """The same call gives the same bits, split or not, also where scales are vast or no numbers."""
+    rng = np.random.default_rng(new)
+    c = attn_case(rng, [2100, 130], [new, new], 8, 2, 128, 16)
+    for value in (None, 2.0 ** 120, np.nan):
+        if value is not None:
+            c["cache"][3][c["table"][0, 70], 0, 3:9, 1] = value
+        for size in (4096, K.kv4_cache_attention_workspace_size(2 * new, 2, 8, 2, 128, new, 2100)):
+            with stream_workspace(dev, size):
+                runs = [run_attn(dev, c, hint=(new, 2100)) for _ in range(4)]
+            for o, lse in runs[1:]:
+                np.testing.assert_array_equal(o, runs[0][0])
+                np.testing.assert_array_equal(lse, runs[0][1])
+
+
 # ── together ────────────────────────────────────────────────────────────────
 
 
